@@ -263,6 +263,58 @@ int tuna_quantize(const void *w, const void *code, void *q, void *absmax, int m,
 /* The same with the NF4 levels, which are also written to code_out fp32 [16]: nothing to upload. */
 int tuna_quantize_nf4(const void *w, void *q, void *absmax, void *code_out, int m, int k, void *stream);
 
+/*
+ * Microscaled 4-bit matrices (OCP MXFP4).  No counterpart in the reference, whose one 4-bit format is the codebook of the
+ * calls above; this is the one that the tensor cores of sm_100a multiply themselves, both operands in 4 bits.
+ *   numbers  code e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives; bit 3 is the sign) x scale 2^(byte - 127); 32 columns
+ *            of a row share a scale byte, and byte 255 makes them NaN
+ *   q        u8 [ceil(k/256), rows, 128]  codes in chunks of 256 columns: byte j of a chunk's row holds column 2j in its
+ *                                         LOW and 2j+1 in its HIGH nibble
+ *   s        u8 [ceil(k/128), rows, 4]    scale bytes in words of 128 columns
+ * k is a multiple of 32; what lies behind column k in the last chunk or word is zero, and has to be.  A set of `batch` or
+ * `experts` matrices has them one after another.
+ */
+typedef enum tuna_type { TUNA_FP16 = 0, TUNA_BF16 = 1, TUNA_FP32 = 2, TUNA_MXFP4 = 3 } tuna_type;
+#define TUNA_MX_MAX_EXPERTS 1024
+
+/*
+ * Quantizer: x [batch, rows, k] of x_type (fp16, bf16 or fp32), rows row_stride elements apart (>= k; the matrices of a
+ * batch follow one another at rows * row_stride), 16-byte aligned rows -> q and s.  The scale of a block is
+ * 2^(floor(log2(largest magnitude)) - 2), not below 2^-127; codes are its numbers over the scale, rounded to nearest with ties
+ * to even, saturating at 6.  A block that holds an infinity or NaN gets scale byte 255.
+ */
+int tuna_mx_quantize(const void *x, int x_type, long long row_stride, void *q, void *s, int rows, int k, int batch, void *stream);
+
+/* o [batch, rows, k] of o_type (fp16, bf16 or fp32) = the numbers of q and s, rounded once. */
+int tuna_mx_dequant(const void *q, const void *s, void *o, int o_type, int rows, int k, int batch, void *stream);
+
+/*
+ * o[n, m] (fp16, bf16 or fp32) = x[n, k] * w[m, k]^T, w given by q and s, fp32 accumulation, one rounding; results are
+ * bit-identical from run to run.  x_type TUNA_MXFP4: x and xs are codes and scales of the tokens.  TUNA_FP16 or TUNA_BF16: x is
+ * [n, k] of that type, xs is not read, and the call quantizes x as tuna_mx_quantize does.  m a multiple of 8, k of 32, any
+ * n >= 1.  Alignment: x, q, s, o, workspace 16 bytes; xs 4.  Ordinary stream order for everything.
+ * Workspace: tuna_mx_workspace_bytes (with experts = 1), its first tuna_mx_workspace_zero_bytes() bytes ZERO before
+ * the first call; every call leaves them so, and one allocation of the largest size serves consecutive calls of any shapes on a
+ * stream.  Calls that overlap on the device need separate ones, and so do graphs that are replayed side by side.
+ */
+int tuna_mx_matmul(const void *x, int x_type, const void *xs, const void *q, const void *s, void *o, int o_type, int m, int n, int k, void *workspace,
+                   size_t workspace_bytes, void *stream);
+
+/*
+ * The same for the experts of a mixture (1 to TUNA_MX_MAX_EXPERTS), the tokens lying expert by expert: row t of x with
+ * offsets[e] <= t < offsets[e + 1] is multiplied with matrix e of q [experts, ..] and s [experts, ..].  `offsets` (int32,
+ * experts + 1, not decreasing) is in DEVICE memory, as a router leaves it: nothing is read back.  n counts the rows of x and o,
+ * which may be more than offsets[experts] (0: nothing to do): rows before offsets[0] or behind offsets[experts] of o are left as they were.  Offsets outside
+ * 0 .. n are taken as the nearest of these; of experts whose ranges overlap any one may have written the rows in common.
+ */
+int tuna_mx_matmul_grouped(const void *x, int x_type, const void *xs, const void *q, const void *s, const void *offsets, void *o, int o_type, int m, int n,
+                           int k, int experts, void *workspace, size_t workspace_bytes, void *stream);
+size_t tuna_mx_workspace_bytes(int m, int n, int k, int experts, int x_type);
+size_t tuna_mx_workspace_zero_bytes(void);
+
+/* A number for the CUDA graph capture that `stream` is part of, different for each; 0 outside of one. */
+unsigned long long tuna_stream_capture_id(void *stream);
+
 const char *tuna_status_string(int status);
 
 /* Library / table identification: ABI version and number of table entries. */

@@ -1,0 +1,344 @@
+"""Products of microscaled matrices on the GPU against sums in 64 bits, with the bound that mx_util derives."""
+
+import numpy as np
+import pytest
+import torch
+
+import tuna_b200
+from tests.gpu_util import Guarded
+from tests.mx_util import check_product, random_packed
+from oracle import mx_oracle as mxo
+from tuna_b200 import _lib
+
+pytestmark = pytest.mark.gpu
+TYPES = [torch.float16, torch.bfloat16, torch.float32]
+
+
+def dev(*arrays):
+    return [torch.from_numpy(a).cuda() for a in arrays]
+
+
+def finish():
+    torch.cuda.synchronize()
+    assert _lib.load().tuna_check_device_status(torch.cuda.current_stream().cuda_stream) == 0
+
+
+def product(m, n, k, seed=0, dtype=torch.float32, spread=3):
+    (xq, xs), x = random_packed(n, k, 2 * seed + 1, spread)
+    (wq, ws), w = random_packed(m, k, 2 * seed + 2, spread)
+    hold = Guarded(n * m * dtype.itemsize, dtype, (n, m))
+    tuna_b200.mx_matmul(*dev(xq, xs), *dev(wq, ws), hold.view, m, n, k)
+    finish()
+    assert hold.guards_intact()
+    check_product(hold.view, x, w)
+    return hold.view
+
+
+@pytest.mark.parametrize("k", [32, 64, 96, 128, 160, 256, 288, 512, 4096])
+def test_one_token(k):
+    product(128, 1, k, seed=k)
+
+
+@pytest.mark.parametrize("m", [8, 16, 120, 128, 136, 1000, 4096])
+def test_output_features(m):
+    product(m, 3, 544, seed=m)
+
+
+@pytest.mark.parametrize("n", [1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 200, 255, 256, 257, 300, 513])
+def test_tokens(n):
+    product(264, n, 800, seed=n, dtype=torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("m,n,k", [(4096, 1, 4096), (1000, 43, 4128), (6144, 256, 1024), (520, 130, 14336), (20000, 16, 512), (2048, 700, 2048), (40, 2000, 96)])
+def test_sizes_and_types(m, n, k, dtype):
+    product(m, n, k, seed=m + n, dtype=dtype)
+
+
+def test_single_products_are_exact():
+    """One column of x is not zero: the outputs are w's numbers, so no row, column or scale is taken for another."""
+    m, n, k = 384, 40, 1056
+    rng = np.random.default_rng(5)
+    (wq, ws), w = random_packed(m, k, 6, spread=8)
+    codes = np.zeros((n, k), dtype=np.uint8)
+    at = rng.permutation(k)[:n]
+    codes[np.arange(n), at] = 2  # 1.0
+    scales = rng.integers(120, 135, (n, k // 32), dtype=np.uint8)
+    o = torch.full((n, m), float("nan"), device="cuda")
+    tuna_b200.mx_matmul(*dev(*mxo.pack(codes, scales)), *dev(wq, ws), o, m, n, k)
+    finish()
+    want = w[:, at].T * 2.0 ** (scales[np.arange(n), at // 32].astype(float) - 127)[:, None]
+    assert np.array_equal(o.double().cpu().numpy(), want)
+
+
+def test_scales_of_every_size_and_nan():
+    """Scales from 2^-60 to 2^60 on either side; a NaN scale spoils its own row's or token's outputs and no others."""
+    m, n, k = 256, 20, 512
+    (xq, xs), x = random_packed(n, k, 1, spread=60)
+    (wq, ws), w = random_packed(m, k, 2, spread=0)
+    xs[2, 7, 1] = 255
+    x[7, 9 * 32:10 * 32] = np.nan
+    o = torch.empty(n, m, device="cuda")
+    tuna_b200.mx_matmul(*dev(xq, xs), *dev(wq, ws), o, m, n, k)
+    finish()
+    check_product(o, x, w)
+    ws[3, 100, 3] = 255
+    w[100, 15 * 32:] = np.nan
+    tuna_b200.mx_matmul(*dev(xq, xs), *dev(wq, ws), o, m, n, k)
+    finish()
+    check_product(o, x, w)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("m,n,k", [(128, 1, 32), (512, 5, 2080), (1024, 40, 4096), (256, 300, 768)])
+def test_tokens_in_16_bits_are_quantized_by_the_call(m, n, k, dtype):
+    x = torch.randn(n, k, device="cuda").to(dtype)
+    x[:, 3] *= 30
+    (wq, ws), w = random_packed(m, k, 4)
+    o = torch.empty(n, m, device="cuda", dtype=dtype)
+    q, s = dev(wq, ws)
+    tuna_b200.mx_matmul(x, None, q, s, o, m, n, k)
+    finish()
+    codes, scales = mxo.quantize(x.double().cpu().numpy())
+    check_product(o, mxo.decode(codes, scales), w)
+    o2 = torch.empty_like(o)
+    tuna_b200.mx_matmul(*tuna_b200.mx_quantize(x), q, s, o2, m, n, k)
+    assert torch.equal(o, o2)
+
+
+def test_runs_agree_bit_for_bit_and_leave_the_workspace_clean():
+    m, n, k = 2000, 24, 8192
+    (xq, xs), _ = random_packed(n, k, 1)
+    (wq, ws), _ = random_packed(m, k, 2)
+    args = dev(xq, xs, wq, ws)
+    need = _lib.load().tuna_mx_workspace_bytes(m, n, k, 1, 3)
+    zero = _lib.load().tuna_mx_workspace_zero_bytes()
+    work = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    outs = []
+    for _ in range(5):
+        o = torch.full((n, m), float("nan"), device="cuda")
+        tuna_b200.mx_matmul(*args, o, m, n, k, workspace=work)
+        outs.append(o)
+    finish()
+    assert not work[:zero].any()
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
+# ------------------------------------------------------------------ experts
+
+def grouped(counts, m, k, *, before=0, behind=0, dtype=torch.float32, seed=0, quantized=True, offsets=None):
+    e, n = len(counts), before + sum(counts) + behind
+    ends = before + np.cumsum([0] + list(counts))
+    mats = [random_packed(m, k, 100 * seed + i) for i in range(e)]
+    q, s = dev(np.stack([p[0][0] for p in mats]), np.stack([p[0][1] for p in mats]))
+    hold = Guarded(n * m * dtype.itemsize, dtype, (n, m))
+    hold.view.fill_(7.0)
+    off = torch.from_numpy(ends.astype(np.int32)).cuda()
+    if quantized:
+        (xq, xs), x = random_packed(n, k, 100 * seed + 99)
+        tuna_b200.mx_matmul_grouped(*dev(xq, xs), q, s, off, hold.view, m, n, k)
+    else:
+        t = torch.randn(n, k, device="cuda", dtype=torch.bfloat16)
+        x = mxo.decode(*mxo.quantize(t.double().cpu().numpy()))
+        tuna_b200.mx_matmul_grouped(t, None, q, s, off, hold.view, m, n, k)
+    finish()
+    assert hold.guards_intact()
+    for i in range(e):
+        if counts[i]:
+            check_product(hold.view[ends[i]:ends[i + 1]], x[ends[i]:ends[i + 1]], mats[i][1])
+    assert (hold.view[:before] == 7).all() and (hold.view[ends[-1]:] == 7).all(), "rows of no expert are left as they were"
+
+
+@pytest.mark.parametrize("counts", [[1], [0, 1], [5, 0, 3], [0, 0, 0, 9], [1] * 40, [17, 16, 15, 1, 0, 33], [200, 3, 0, 129, 64], [0, 0], [700, 1]], ids=str)
+def test_experts(counts):
+    grouped(counts, 264, 544, seed=len(counts))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("quantized", [True, False])
+def test_experts_in_a_larger_buffer(dtype, quantized):
+    grouped([3, 0, 21, 7], 136, 416, before=5, behind=9, dtype=dtype, quantized=quantized)
+
+
+def test_many_experts():
+    rng = np.random.default_rng(0)
+    grouped(list(rng.integers(0, 4, 1024)), 16, 96, seed=3)
+
+
+def test_odd_numbers_of_tokens_shift_every_experts_rows():
+    grouped([1, 2, 3, 5, 7, 11, 13], 1000, 1056, before=1, seed=4)
+
+
+def test_experts_without_tokens_at_all():
+    (wq, ws), _ = random_packed(128, 256, 1)
+    q, s = dev(wq[None], ws[None])
+    tuna_b200.mx_matmul_grouped(torch.empty(0, 256, device="cuda", dtype=torch.bfloat16), None, q, s, torch.zeros(2, dtype=torch.int32, device="cuda"),
+                                torch.empty(0, 128, device="cuda"), 128, 0, 256)
+    finish()
+
+
+@pytest.mark.parametrize("offsets", [[0, 99, 20], [-5, 3, 8], [4, 2, 6], [-2147483648, 0, 2147483647]], ids=str)
+def test_offsets_outside_the_tokens_stay_inside_the_output(offsets):
+    m, n, k = 128, 8, 256
+    mats = [random_packed(m, k, i) for i in range(2)]
+    q, s = dev(np.stack([p[0][0] for p in mats]), np.stack([p[0][1] for p in mats]))
+    (xq, xs), x = random_packed(n, k, 9)
+    hold = Guarded(n * m * 4, torch.float32, (n, m))
+    hold.view.fill_(7.0)
+    tuna_b200.mx_matmul_grouped(*dev(xq, xs), q, s, torch.tensor(offsets, dtype=torch.int32, device="cuda"), hold.view, m, n, k)
+    finish()
+    assert hold.guards_intact()
+    clamped = np.clip(offsets, 0, n)
+    covered = np.zeros(n, dtype=bool)
+    for e in range(2):
+        covered[clamped[e]:max(clamped[e], clamped[e + 1])] = True
+    assert (hold.view[torch.from_numpy(~covered).cuda()] == 7).all()
+    only = [r for r in range(n) if sum(clamped[e] <= r < clamped[e + 1] for e in range(2)) == 1]
+    for r in only:
+        e = next(e for e in range(2) if clamped[e] <= r < clamped[e + 1])
+        check_product(hold.view[r:r + 1], x[r:r + 1], mats[e][1])
+
+
+# ------------------------------------------------------------------ streams, graphs, devices, a layer
+
+def test_a_mixture_layer_from_activations_to_outputs():
+    """Tokens sorted by expert -> gate+up -> gated activation -> down: every call as a program makes it, one after another."""
+    experts, hidden, inter, tokens = 6, 512, 768, 50
+    rng = np.random.default_rng(1)
+    choice = np.sort(rng.integers(0, experts, tokens))
+    off = torch.from_numpy(np.searchsorted(choice, np.arange(experts + 1)).astype(np.int32)).cuda()
+    up = tuna_b200.mx_quantize(torch.randn(experts, 2 * inter, hidden, device="cuda") * hidden ** -0.5)
+    down = tuna_b200.mx_quantize(torch.randn(experts, hidden, inter, device="cuda") * inter ** -0.5)
+    x = torch.randn(tokens, hidden, device="cuda", dtype=torch.bfloat16)
+    h = torch.empty(tokens, 2 * inter, device="cuda", dtype=torch.bfloat16)
+    o = torch.empty(tokens, hidden, device="cuda", dtype=torch.bfloat16)
+    tuna_b200.mx_matmul_grouped(x, None, *up, off, h, 2 * inter, tokens, hidden)
+    a = torch.nn.functional.silu(h[:, :inter].float()) * h[:, inter:].float()
+    a = a.to(torch.bfloat16)
+    tuna_b200.mx_matmul_grouped(a, None, *down, off, o, hidden, tokens, inter)
+    finish()
+
+    def numbers(t):
+        return mxo.decode(*mxo.quantize(t.double().cpu().numpy()))
+
+    def matrix(pair, e, rows, k):
+        w = torch.empty(rows, k, device="cuda")
+        tuna_b200.mx_dequant(pair[0][e], pair[1][e], w, rows, k)
+        return w.double().cpu().numpy()
+
+    for e in range(experts):
+        rows = np.flatnonzero(choice == e)
+        if len(rows):
+            check_product(h[rows], numbers(x[rows]), matrix(up, e, 2 * inter, hidden))
+            check_product(o[rows], numbers(a[rows]), matrix(down, e, hidden, inter))
+
+
+def test_two_graphs_of_one_stream_replayed_side_by_side():
+    m, n, k = 1024, 16, 8192
+    cases = []
+    for i in range(2):
+        (xq, xs), x = random_packed(n, k, 10 + i)
+        (wq, ws), w = random_packed(m, k, 20 + i)
+        cases.append((dev(xq, xs, wq, ws), torch.zeros(n, m, device="cuda"), x, w))
+    graphs = []
+    side = torch.cuda.Stream()
+    for args, o, _, _ in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            for _ in range(3):
+                tuna_b200.mx_matmul(*args, o, m, n, k)
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(30):
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    finish()
+    for _, o, x, w in cases:
+        check_product(o, x, w)
+
+
+def test_calls_on_two_streams_at_once():
+    m, n, k = 1024, 16, 4096
+    (xq, xs), x = random_packed(n, k, 1)
+    (wq, ws), w = random_packed(m, k, 2)
+    args = dev(xq, xs, wq, ws)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    outs = [torch.zeros(n, m, device="cuda") for _ in streams]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for st, o in zip(streams, outs):
+            with torch.cuda.stream(st):
+                tuna_b200.mx_matmul(*args, o, m, n, k)
+    finish()
+    for o in outs:
+        check_product(o, x, w)
+
+
+def test_dependent_calls_without_a_wait_in_between():
+    """Weights and tokens quantized right before the product, overwritten right after it, over and over on one stream."""
+    m, n, k = 768, 33, 2048
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    pairs = [(torch.randn(m, k, generator=gen, device="cuda"), torch.randn(n, k, generator=gen, device="cuda", dtype=torch.float16)) for _ in range(4)]
+    want = []
+    for w, x in pairs:
+        o = torch.empty(n, m, device="cuda")
+        torch.cuda.synchronize()
+        q, s = tuna_b200.mx_quantize(w)
+        torch.cuda.synchronize()
+        tuna_b200.mx_matmul(x, None, q, s, o, m, n, k)
+        torch.cuda.synchronize()
+        want.append(o)
+    wbuf, xbuf = torch.empty(m, k, device="cuda"), torch.empty(n, k, device="cuda", dtype=torch.float16)
+    got = [torch.empty(n, m, device="cuda") for _ in range(20)]
+    for i, o in enumerate(got):
+        wbuf.copy_(pairs[i % 4][0])
+        xbuf.copy_(pairs[i % 4][1])
+        q, s = tuna_b200.mx_quantize(wbuf)
+        if i % 2:
+            tuna_b200.mx_matmul(xbuf, None, q, s, o, m, n, k)
+        else:
+            tuna_b200.mx_matmul(*tuna_b200.mx_quantize(xbuf), q, s, o, m, n, k)
+        q.zero_()
+    finish()
+    for i, o in enumerate(got):
+        assert torch.equal(o, want[i % 4])
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+def test_a_device_that_is_not_the_current_one():
+    m, n, k = 256, 5, 512
+    (xq, xs), x = random_packed(n, k, 1)
+    (wq, ws), w = random_packed(m, k, 2)
+    o = torch.empty(n, m, device="cuda:1")
+    tuna_b200.mx_matmul(*(t.to("cuda:1") for t in dev(xq, xs, wq, ws)), o, m, n, k)
+    torch.cuda.synchronize(1)
+    check_product(o, x, w)
+
+
+def test_refusals():
+    m, n, k = 128, 4, 256
+    (xq, xs), _ = random_packed(n, k, 1)
+    (wq, ws), _ = random_packed(m, k, 2)
+    xq, xs, wq, ws = dev(xq, xs, wq, ws)
+    o = torch.empty(n, m, device="cuda")
+    off = torch.zeros(2, dtype=torch.int32, device="cuda")
+    for bad in ((xq, xs, wq, ws, o, m, n, 480), (xq, xs, wq, ws, o, m, n + 1, k), (xq, xs, wq, ws[:1], o, m, n, k), (xq, xs, wq, ws, o.t(), m, n, k),
+                (xq, xs, wq, ws, o.cpu(), m, n, k), (xq, xs[:, :, ::2], wq, ws, o, m, n, k)):
+        with pytest.raises(ValueError):
+            tuna_b200.mx_matmul(*bad)
+    with pytest.raises(TypeError):
+        tuna_b200.mx_matmul(xq, xs, wq, ws, o.double(), m, n, k)
+    with pytest.raises(TypeError):
+        tuna_b200.mx_matmul(torch.empty(n, k, device="cuda"), None, wq, ws, o, m, n, k)
+    with pytest.raises(tuna_b200.TunaError):
+        tuna_b200.mx_matmul(xq, xs, wq, ws, o, m, n, k, workspace=torch.zeros(64, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(ValueError):
+        tuna_b200.mx_matmul_grouped(xq, xs, wq, ws, off, o, m, n, k)  # no leading dimension
+    with pytest.raises(TypeError):
+        tuna_b200.mx_matmul_grouped(xq, xs, wq[None], ws[None], off.long(), o, m, n, k)
+    with pytest.raises(ValueError):
+        tuna_b200.mx_matmul_grouped(xq, xs, wq[None], ws[None], off[:1], o, m, n, k)
+    with pytest.raises(ValueError):
+        tuna_b200.mx_matmul_grouped(xq, xs, wq[None], ws[None], off.cpu(), o, m, n, k)

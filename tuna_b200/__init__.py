@@ -8,9 +8,11 @@ implementation behind them.
 """
 
 from .ops import Exchange, HostPipeline, HostSequence, MatmulSequence, ReduceSequence, dequant, matmul, matmul_batched, matmul_sequence, quantize, workspace_for, lookup_config  # noqa: F401
+from .mx import mx_dequant, mx_matmul, mx_matmul_grouped, mx_pack, mx_quantize  # noqa: F401
 from ._lib import TunaConfig, TunaError, PATH_AUTO, PATH_STREAM, PATH_UMMA, PATH_TSTREAM  # noqa: F401
 
 __all__ = [
     "matmul", "matmul_batched", "matmul_sequence", "MatmulSequence", "ReduceSequence", "Exchange", "HostSequence", "dequant", "quantize", "HostPipeline", "workspace_for", "lookup_config",
+    "mx_quantize", "mx_dequant", "mx_matmul", "mx_matmul_grouped", "mx_pack",
     "TunaConfig", "TunaError", "PATH_AUTO", "PATH_STREAM", "PATH_UMMA", "PATH_TSTREAM",
 ]

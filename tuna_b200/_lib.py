@@ -6,7 +6,7 @@ import ctypes
 import functools
 import sysconfig
 import warnings
-from ctypes import c_char_p, c_int, c_int32, c_size_t, c_void_p
+from ctypes import c_char_p, c_int, c_int32, c_longlong, c_size_t, c_ulonglong, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libtuna_b200.so"
@@ -77,6 +77,13 @@ SYMBOLS = {
     "tuna_dequant": (c_int, [c_void_p] * 4 + [c_int] * 2 + [c_void_p]),
     "tuna_quantize": (c_int, [c_void_p] * 4 + [c_int] * 2 + [c_void_p]),
     "tuna_quantize_nf4": (c_int, [c_void_p] * 4 + [c_int] * 2 + [c_void_p]),
+    "tuna_mx_quantize": (c_int, [c_void_p, c_int, c_longlong, c_void_p, c_void_p] + [c_int] * 3 + [c_void_p]),
+    "tuna_mx_dequant": (c_int, [c_void_p] * 3 + [c_int] * 4 + [c_void_p]),
+    "tuna_mx_matmul": (c_int, [c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 4 + [c_void_p, c_size_t, c_void_p]),
+    "tuna_mx_matmul_grouped": (c_int, [c_void_p, c_int] + [c_void_p] * 5 + [c_int] * 5 + [c_void_p, c_size_t, c_void_p]),
+    "tuna_mx_workspace_bytes": (c_size_t, [c_int] * 5),
+    "tuna_mx_workspace_zero_bytes": (c_size_t, []),
+    "tuna_stream_capture_id": (c_ulonglong, [c_void_p]),
     "tuna_check_device_status": (c_int, [c_void_p]),
     "tuna_selftest_bounded_wait": (c_int, [c_void_p]),
     "tuna_status_string": (c_char_p, [c_int]),

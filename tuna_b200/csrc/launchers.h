@@ -35,6 +35,8 @@ struct GemmArgs {
 constexpr size_t kMaxPartialSlotBytes = 192 * 1024;
 inline size_t partial_region_bytes(int sm_count) { return 2 * (size_t)sm_count * kMaxPartialSlotBytes; }
 
+int device_sm_count();  // of the current device
+
 struct DeviceStatus;
 // One zero-initialised status word per device; bounded in-kernel waits report into it.
 DeviceStatus *device_status_word();
@@ -93,5 +95,21 @@ constexpr int kExFlagStrideWords = 32;
 size_t exchange_region_bytes(const tuna_gemm_desc *d, int count, int world);
 int launch_exchange_reduce(const tuna_exchange &ex, const tuna_gemm_desc *d, const long long *slab0_off, int count, int tile_tok,
                            long long region_bytes, cudaStream_t stream);
+
+// Microscaled 4-bit matrices.  Types are tuna_type's; workspace: counters, zero before the first use and left zero, then partial sums.
+struct MxGemmArgs {
+    const void *x, *xs, *q, *s;
+    const void *offsets;  // device, experts + 1 of them; nullptr: one matrix
+    void *o;
+    int m, n, k, experts, o_type;
+    void *workspace;
+    cudaStream_t stream;
+    int sm_count;
+};
+constexpr size_t kMxCounterBytes = 4096;
+cudaError_t launch_mx_quantize(const void *x, int type, long long row_stride, void *q, void *s, int rows, int k, int batch, cudaStream_t stream);
+cudaError_t launch_mx_dequant(const void *q, const void *s, void *o, int type, int rows, int k, int batch, cudaStream_t stream);
+int launch_mx_gemm(const MxGemmArgs &a);
+size_t mx_gemm_workspace_bytes(int m, int n, int k, int experts, int sm_count);
 
 }  // namespace tuna

@@ -33,7 +33,7 @@ static int token_bucket(int n)
     return 2048;
 }
 
-static int device_sm_count()
+int device_sm_count()
 {
     static int cached[64];
     static std::once_flag once;

@@ -1,0 +1,167 @@
+"""Microscaled 4-bit (OCP MXFP4) matrices: quantizer, its inverse, and products in which both operands have 4 bits.
+
+A matrix `[rows, k]` (k a multiple of 32) is a pair of uint8 tensors: codes `q` `[ceil(k/256), rows, 128]`, column 2j of a
+256-column chunk in the low nibble of byte j and 2j+1 in the high one, and scales `s` `[ceil(k/128), rows, 4]`, a byte
+(exponent plus 127; 255 is NaN) for every 32 columns.  What lies behind column k in the last chunk is zero.  A set of
+experts' matrices has a leading dimension.  Column ranges that start at a multiple of 256 are views of the leading dimension.
+
+The reference has no counterpart: its one 4-bit format is the codebook of `matmul`.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._lib import check
+from .ops import _expect, _on_device, _stream_ptr
+
+_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_MXFP4 = 3
+_workspaces: dict = {}
+
+
+def _code_shape(rows: int, k: int):
+    return (-(-k // 256), rows, 128)
+
+
+def _scale_shape(rows: int, k: int):
+    return (-(-k // 128), rows, 4)
+
+
+def _numel(shape) -> int:
+    return shape[0] * shape[1] * shape[2]
+
+
+def _expect_codes(q, s, names, rows, k, device=None, matrices=1):
+    _expect(q, names[0], torch.uint8, matrices * _numel(_code_shape(rows, k)), device)
+    _expect(s, names[1], torch.uint8, matrices * _numel(_scale_shape(rows, k)), q.device)
+
+
+def _expect_output(o, numel, device):
+    if not isinstance(o, torch.Tensor):
+        raise TypeError("o must be a torch.Tensor")
+    if o.dtype not in _TYPES:
+        raise TypeError(f"o must be torch.float16, torch.bfloat16 or torch.float32, got {o.dtype}")
+    _expect(o, "o", o.dtype, numel, device)
+
+
+def _workspace(need: int, device) -> torch.Tensor:
+    """The workspace of `device`'s current stream.  A graph that is being captured gets one of its own, from its own pool, whose
+    counters it zeroes at every replay: graphs may be replayed side by side, and beside calls on the stream that captured them."""
+    stream = _stream_ptr(device)
+    lib = _lib.load()
+    capture = int(lib.tuna_stream_capture_id(stream))
+    key = (device.index, stream, capture)
+    ws = _workspaces.get(key)
+    if ws is None or ws.numel() < need:
+        if capture:  # those of finished captures stay reserved in their graphs' pools without a reference from here
+            for old in [k for k in _workspaces if k[0] == device.index and k[2] not in (0, capture)]:
+                _workspaces.pop(old, None)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        ws[:int(lib.tuna_mx_workspace_zero_bytes())].zero_()
+        _workspaces[key] = ws
+    return ws
+
+
+def mx_quantize(x):
+    """`x` (fp16, bf16 or fp32; `[rows, k]`, whose rows may lie apart, or contiguous `[matrices, rows, k]`) -> codes and scales
+    `(q, s)`.  A block's scale is 2^(floor(log2(largest magnitude)) - 2), not below 2^-127; numbers over the scale are
+    rounded to nearest with ties to even and saturate at 6.  A block with an infinity or NaN reads back as NaN."""
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ValueError("x must be a CUDA tensor (there is no CPU path)")
+    if x.dtype not in _TYPES:
+        raise TypeError(f"x must be torch.float16, torch.bfloat16 or torch.float32, got {x.dtype}")
+    if x.dim() not in (2, 3) or x.numel() == 0:
+        raise ValueError("x must be a [rows, k] or [matrices, rows, k] tensor with at least one row")
+    rows, k = x.shape[-2:]
+    if k % 32:
+        raise ValueError(f"k must be a multiple of 32, got {k}")
+    stride = k
+    if x.dim() == 3 or rows == 1:
+        if not x.is_contiguous():
+            raise ValueError("x must be contiguous")
+    elif x.stride(1) != 1 or x.stride(0) < k:
+        raise ValueError("the columns of x must be contiguous and its rows must not overlap")
+    else:
+        stride = x.stride(0)
+    lead = tuple(x.shape[:-2])
+    q = torch.empty(lead + _code_shape(rows, k), dtype=torch.uint8, device=x.device)
+    s = torch.empty(lead + _scale_shape(rows, k), dtype=torch.uint8, device=x.device)
+    with _on_device(x.device):
+        check(_lib.load().tuna_mx_quantize(x.data_ptr(), _TYPES[x.dtype], stride, q.data_ptr(), s.data_ptr(), rows, k, lead[0] if lead else 1, _stream_ptr(x.device)))
+    return q, s
+
+
+def mx_dequant(q, s, o, m: int, k: int) -> None:
+    """The numbers of codes and scales, rounded once to o's type: o fp16, bf16 or fp32 `[m, k]`.  With a leading dimension of q, s
+    and o, all its matrices."""
+    dev = q.device if isinstance(q, torch.Tensor) else None
+    matrices = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() == 4 else 1
+    _expect_codes(q, s, ("q", "s"), m, k, dev, matrices)
+    _expect_output(o, matrices * m * k, dev)
+    with _on_device(dev):
+        check(_lib.load().tuna_mx_dequant(q.data_ptr(), s.data_ptr(), o.data_ptr(), _TYPES[o.dtype], m, k, matrices, _stream_ptr(dev)))
+
+
+def _tokens(x, xs, n, k):
+    """The library's type of the tokens, checked."""
+    if xs is not None:
+        _expect_codes(x, xs, ("x", "xs"), n, k)
+        return _MXFP4
+    if not isinstance(x, torch.Tensor):
+        raise TypeError("x must be a torch.Tensor")
+    if x.dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"x must be torch.float16 or torch.bfloat16, or codes with their scales xs, got {x.dtype}")
+    _expect(x, "x", x.dtype, n * k)
+    return _TYPES[x.dtype]
+
+
+def mx_matmul(x, xs, q, s, o, m: int, n: int, k: int, *, workspace=None) -> None:
+    """o `[n, m]` (fp16, bf16 or fp32, overwritten) = x `[n, k]` times the transposed matrix of `(q, s)` `[m, k]`, fp32 accumulation,
+    one rounding.  x is codes with their scales `xs`, or fp16 or bf16 with `xs=None`: the call quantizes it as
+    `mx_quantize` does.  m a multiple of 8, k of 32.  Enqueued on the current stream of x's device."""
+    kind = _tokens(x, xs, n, k)
+    dev = x.device
+    _expect_codes(q, s, ("q", "s"), m, k, dev)
+    _expect_output(o, n * m, dev)
+    lib = _lib.load()
+    with _on_device(dev):
+        ws = workspace if workspace is not None else _workspace(int(lib.tuna_mx_workspace_bytes(m, n, k, 1, kind)), dev)
+        check(lib.tuna_mx_matmul(x.data_ptr(), kind, 0 if xs is None else xs.data_ptr(), q.data_ptr(), s.data_ptr(), o.data_ptr(), _TYPES[o.dtype], m, n, k,
+                                 ws.data_ptr(), ws.numel() * ws.element_size(), _stream_ptr(dev)))
+
+
+def mx_matmul_grouped(x, xs, q, s, offsets, o, m: int, n: int, k: int, *, workspace=None) -> None:
+    """`mx_matmul` for the experts of a mixture, whose tokens lie expert by expert: rows offsets[e] up to offsets[e + 1] of x are
+    multiplied with matrix e of `q` `[experts, ceil(k/256), m, 128]` and `s`.  `offsets` int32 `[experts + 1]`, not decreasing, stays on
+    the device (a router's cumulative counts): nothing waits for it on the host.  x and o have n rows, which may be more than
+    offsets[experts]: rows of o that no expert has are left as they were.  n = 0 is nothing to do."""
+    if not isinstance(q, torch.Tensor) or q.dim() != 4:
+        raise ValueError("q must be a [experts, ceil(k/256), m, 128] tensor")
+    experts = q.shape[0]
+    kind = _tokens(x, xs, n, k)
+    dev = x.device
+    _expect_codes(q, s, ("q", "s"), m, k, dev, experts)
+    _expect(offsets, "offsets", torch.int32, experts + 1, dev)
+    _expect_output(o, n * m, dev)
+    if n == 0:
+        return
+    lib = _lib.load()
+    with _on_device(dev):
+        ws = workspace if workspace is not None else _workspace(int(lib.tuna_mx_workspace_bytes(m, n, k, experts, kind)), dev)
+        check(lib.tuna_mx_matmul_grouped(x.data_ptr(), kind, 0 if xs is None else xs.data_ptr(), q.data_ptr(), s.data_ptr(), offsets.data_ptr(), o.data_ptr(),
+                                         _TYPES[o.dtype], m, n, k, experts, ws.data_ptr(), ws.numel() * ws.element_size(), _stream_ptr(dev)))
+
+
+def mx_pack(codes, scales):
+    """Row-major codes uint8 `[.., rows, k/2]` (column 2j in the low nibble of byte j) and scale bytes uint8 `[.., rows, k/32]`, as
+    checkpoints have them, in this package's layout: `(q, s)`.  On any device."""
+    for t, name in ((codes, "codes"), (scales, "scales")):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.uint8 or t.dim() not in (2, 3):
+            raise ValueError(f"{name} must be a uint8 [rows, ..] or [matrices, rows, ..] tensor")
+    if codes.shape[:-1] != scales.shape[:-1] or codes.shape[-1] != 16 * scales.shape[-1]:
+        raise ValueError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are not of one matrix: 16 bytes of codes go with a byte of scales")
+    q = torch.nn.functional.pad(codes, (0, -codes.shape[-1] % 128)).unflatten(-1, (-1, 128)).transpose(-3, -2).contiguous()
+    s = torch.nn.functional.pad(scales, (0, -scales.shape[-1] % 4)).unflatten(-1, (-1, 4)).transpose(-3, -2).contiguous()
+    return q, s
