@@ -13,35 +13,78 @@ constexpr int kMxChunk = 256;      // columns of a chunk of codes: 128 bytes, on
 constexpr int kMxScaleCols = 128;  // columns of a word of scales
 constexpr int kMxChunkBytes = kMxChunk / 2;
 
-// Eight numbers of type T from 16 (32) bytes, as fp32.
-__device__ __forceinline__ void mx_load8(const __half *p, float (&v)[8])
-{
-    const uint4 r = ldg_stream_u4(p);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
+// Eight numbers of type T as they lie in memory, their largest magnitude and their values.
+template <typename T>
+struct Mx8;
+template <>
+struct Mx8<__half> {
+    uint4 r;
+    __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void load(const __half *p) { r = ldg_stream_u4(p); }
+    __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w; }
+    __device__ __forceinline__ __half2 pair(int i) const { const uint32_t w = word(i); return *reinterpret_cast<const __half2 *>(&w); }
+    // Bits (fp32) of the largest magnitude of the four lanes' 32 numbers; NaN's if there is one.
+    __device__ __forceinline__ uint32_t largest() const
+    {
+        __half2 m = __hmax2_nan(__hmax2_nan(__habs2(pair(0)), __habs2(pair(1))), __hmax2_nan(__habs2(pair(2)), __habs2(pair(3))));
+        m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        return __float_as_uint(__half2float(__hmax_nan(__low2half(m), __high2half(m)))) & 0x7fffffffu;
     }
-}
-__device__ __forceinline__ void mx_load8(const __nv_bfloat16 *p, float (&v)[8])
-{
-    const uint4 r = ldg_stream_u4(p);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+    __device__ __forceinline__ void values(float (&v)[8]) const
+    {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(pair(i));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
     }
-}
-__device__ __forceinline__ void mx_load8(const float *p, float (&v)[8])
-{
-    const uint4 a = ldg_stream_u4(p), b = ldg_stream_u4(p + 4);
-    const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+};
+template <>
+struct Mx8<__nv_bfloat16> {
+    uint4 r;
+    __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { r = ldg_stream_u4(p); }
+    __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w; }
+    __device__ __forceinline__ __nv_bfloat162 pair(int i) const { const uint32_t w = word(i); return *reinterpret_cast<const __nv_bfloat162 *>(&w); }
+    __device__ __forceinline__ uint32_t largest() const
+    {
+        __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(__habs2(pair(0)), __habs2(pair(1))), __hmax2_nan(__habs2(pair(2)), __habs2(pair(3))));
+        m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        return ((uint32_t)__bfloat16_as_ushort(__hmax_nan(__low2bfloat16(m), __high2bfloat16(m))) & 0x7fffu) << 16;
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const
+    {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
-}
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(word(i) << 16);
+            v[2 * i + 1] = __uint_as_float(word(i) & 0xffff0000u);
+        }
+    }
+};
+template <>
+struct Mx8<float> {
+    uint4 r, t;
+    __device__ __forceinline__ void zero() { r = t = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void load(const float *p) { r = ldg_stream_u4(p); t = ldg_stream_u4(p + 4); }
+    __device__ __forceinline__ uint32_t largest() const
+    {
+        const uint32_t w[8] = {r.x, r.y, r.z, r.w, t.x, t.y, t.z, t.w};
+        uint32_t m = 0;  // magnitudes compare as their bits do, NaN above infinity
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, w[i] & 0x7fffffffu);
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const
+    {
+        const uint32_t w[8] = {r.x, r.y, r.z, r.w, t.x, t.y, t.z, t.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+    }
+};
 
 // The scale of a block whose largest magnitude has the bits `largest` (fp32): floor(log2(largest)) - 2, so that the largest
 // lies between 4 and 8 times the scale (what is above 6 saturates), not below 2^-127.  Infinity or NaN: a NaN scale.

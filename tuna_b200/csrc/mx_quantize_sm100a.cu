@@ -10,66 +10,71 @@
 namespace tuna {
 
 constexpr int kMxqWarps = 4;
+constexpr int kMxqRows = 4;
+
+// The warps of a CTA take neighbouring chunks, 1 << log_c of them, of as many row groups as that leaves; grid (row groups, chunks).
+struct MxqPlace {
+    int c, matrix, row0;
+    bool any;
+};
+template <int ROWS>
+__device__ __forceinline__ MxqPlace mxq_place(int rows, int chunks, int batch, int log_c)
+{
+    const int warp = threadIdx.x >> 5, groups = div_up(rows, ROWS);
+    MxqPlace l;
+    l.c = (int)(blockIdx.y << log_c) + (warp & ((1 << log_c) - 1));
+    const long long g = ((long long)blockIdx.x << (2 - log_c)) + (warp >> log_c);
+    l.matrix = batch == 1 ? 0 : (int)(g / groups);
+    const int group = (int)(g - (long long)l.matrix * groups);
+    l.row0 = group * ROWS;
+    l.any = l.c < chunks && l.matrix < batch && group < groups;
+    return l;
+}
 
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(kMxqWarps * 32)
-mx_quantize_kernel(const T *__restrict__ x, long long row_stride, uint8_t *__restrict__ q, uint32_t *__restrict__ s, int rows, int k, int chunks,
-                   long long items)
+mx_quantize_kernel(const T *__restrict__ x, long long row_stride, uint8_t *__restrict__ q, uint32_t *__restrict__ s, int rows, int k, int chunks, int batch,
+                   int log_c)
 {
     const int lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * kMxqWarps + (threadIdx.x >> 5);
-    if (item >= items) return;
-    const int words = div_up(k, kMxScaleCols);
-    const int groups = div_up(rows, ROWS);
-    const int c = (int)(item % chunks);
-    const long long g = item / chunks;
-    const int matrix = (int)(g / groups), row0 = (int)(g - (long long)matrix * groups) * ROWS;
-    const int col = c * kMxChunk + lane * 8;
-    const T *src = x + ((long long)matrix * rows + row0) * row_stride + col;
-    uint8_t *dst = q + (((long long)matrix * chunks + c) * rows + row0) * kMxChunkBytes + lane * 4;
+    const MxqPlace l = mxq_place<ROWS>(rows, chunks, batch, log_c);
+    if (!l.any) return;
+    const int col = l.c * kMxChunk + lane * 8;
+    const T *src = x + ((long long)l.matrix * rows + l.row0) * row_stride + col;
+    uint8_t *dst = q + (((long long)l.matrix * chunks + l.c) * rows + l.row0) * kMxChunkBytes + lane * 4;
 
-    float v[ROWS][8];
+    Mx8<T> v[ROWS];
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-        if (col < k && row0 + r < rows) {
-            mx_load8(src + r * row_stride, v[r]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[r][i] = 0.f;
-        }
+        if (col < k && l.row0 + r < rows) v[r].load(src + r * row_stride);
+        else v[r].zero();
     }
-    uint32_t mine = 0;  // the word of scales of row (lane % 16), columns 128 (lane / 16) .. + 127 of the chunk
+    uint32_t mine = 0;  // the scale of row lane % ROWS
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-        uint32_t largest = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) largest = max(largest, __float_as_uint(v[r][i]) & 0x7fffffffu);
-        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-        largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
-        const uint32_t e = mx_scale(largest);
+        const uint32_t e = mx_scale(v[r].largest());
         const float inverse = mx_inverse(e);
+        float f[8];
+        v[r].values(f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[r][i] *= inverse;
-        const uint32_t codes = e == 255u ? 0u : mx_encode8(v[r]);
-        if (row0 + r < rows) *reinterpret_cast<uint32_t *>(dst + (size_t)r * kMxChunkBytes) = codes;
-        uint32_t w = e << (8 * ((lane >> 2) & 3));
-        w |= __shfl_xor_sync(0xffffffffu, w, 4);
-        w |= __shfl_xor_sync(0xffffffffu, w, 8);
-        if ((lane & 15) == r) mine = w;
+        for (int i = 0; i < 8; ++i) f[i] *= inverse;
+        const uint32_t codes = e == 255u ? 0u : mx_encode8(f);
+        if (l.row0 + r < rows) *reinterpret_cast<uint32_t *>(dst + (size_t)r * kMxChunkBytes) = codes;
+        if (r == 0 || (lane & 3) == r) mine = e;
     }
-    const int r = lane & 15, word = 2 * c + (lane >> 4);
-    if (r < ROWS && row0 + r < rows && word < words) s[((long long)matrix * words + word) * rows + row0 + r] = mine;
+    // a block's four lanes have the scales of one row each; the word of a row is what four neighbouring blocks have of it
+    mine <<= 8 * ((lane >> 2) & 3);
+    mine |= __shfl_xor_sync(0xffffffffu, mine, 4);
+    mine |= __shfl_xor_sync(0xffffffffu, mine, 8);
+    const int r = lane & 15, words = div_up(k, kMxScaleCols), word = 2 * l.c + (lane >> 4);
+    if (r < ROWS && l.row0 + r < rows && word < words) s[((long long)l.matrix * words + word) * rows + l.row0 + r] = mine;
 }
 
-template <typename T>
-__device__ __forceinline__ void mx_store8(T *p, const float (&v)[8]);
-template <>
-__device__ __forceinline__ void mx_store8<__half>(__half *p, const float (&v)[8])
+__device__ __forceinline__ void mx_store8(__half *p, const float (&v)[8])
 {
     *reinterpret_cast<uint4 *>(p) = make_uint4(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]), pack_half2(v[4], v[5]), pack_half2(v[6], v[7]));
 }
-template <>
-__device__ __forceinline__ void mx_store8<__nv_bfloat16>(__nv_bfloat16 *p, const float (&v)[8])
+__device__ __forceinline__ void mx_store8(__nv_bfloat16 *p, const float (&v)[8])
 {
     uint32_t w[4];
 #pragma unroll
@@ -79,89 +84,107 @@ __device__ __forceinline__ void mx_store8<__nv_bfloat16>(__nv_bfloat16 *p, const
     }
     *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
-template <>
-__device__ __forceinline__ void mx_store8<float>(float *p, const float (&v)[8])
-{
-    reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
 
-// o = code * scale in fp32 (exact: three significant bits, exponents of fp32's range), rounded once to T.
+// o = code * scale in fp32 (exact: three significant bits, exponents of fp32's range), rounded once to T.  Results of two bytes: a
+// lane has eight columns side by side, 16 bytes; of four: four columns of each half of the chunk, 16 bytes each.
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(kMxqWarps * 32)
-mx_dequant_kernel(const uint8_t *__restrict__ q, const uint32_t *__restrict__ s, T *__restrict__ o, int rows, int k, int chunks, long long items)
+mx_dequant_kernel(const uint8_t *__restrict__ q, const uint32_t *__restrict__ s, T *__restrict__ o, int rows, int k, int chunks, int batch, int log_c)
 {
+    constexpr bool kWide = sizeof(T) == 4;
     const int lane = threadIdx.x & 31;
-    const long long item = (long long)blockIdx.x * kMxqWarps + (threadIdx.x >> 5);
-    if (item >= items) return;
+    const MxqPlace l = mxq_place<ROWS>(rows, chunks, batch, log_c);
+    if (!l.any) return;
     const int words = div_up(k, kMxScaleCols);
-    const int groups = div_up(rows, ROWS);
-    const int c = (int)(item % chunks);
-    const long long g = item / chunks;
-    const int matrix = (int)(g / groups), row0 = (int)(g - (long long)matrix * groups) * ROWS;
-    const int col = c * kMxChunk + lane * 8;
-    const uint8_t *src = q + (((long long)matrix * chunks + c) * rows + row0) * kMxChunkBytes + lane * 4;
+    const int col = l.c * kMxChunk + lane * (kWide ? 4 : 8);
+    const uint8_t *src = q + (((long long)l.matrix * chunks + l.c) * rows + l.row0) * kMxChunkBytes;
+    T *dst = o + ((long long)l.matrix * rows + l.row0) * k + col;
 
-    const int wr = lane & 15, word = 2 * c + (lane >> 4);
+    const int wr = lane & 15, word = 2 * l.c + (lane >> 4);
     uint32_t codes[ROWS], scales = 0;
-    if (wr < ROWS && row0 + wr < rows && word < words) scales = __ldg(s + ((long long)matrix * words + word) * rows + row0 + wr);
-#pragma unroll
-    for (int r = 0; r < ROWS; ++r)
-        codes[r] = row0 + r < rows ? __ldg(reinterpret_cast<const uint32_t *>(src + (size_t)r * kMxChunkBytes)) : 0u;
+    if (wr < ROWS && l.row0 + wr < rows && word < words) scales = __ldg(s + ((long long)l.matrix * words + word) * rows + l.row0 + wr);
 #pragma unroll
     for (int r = 0; r < ROWS; ++r) {
-        const uint32_t e = (__shfl_sync(0xffffffffu, scales, (lane & 16) | r) >> (8 * ((lane >> 2) & 3))) & 255u;
-        const float scale = mx_scale_value(e);
+        codes[r] = 0;
+        if (l.row0 + r < rows) {
+            if (kWide) {
+                const uint16_t *p = reinterpret_cast<const uint16_t *>(src + (size_t)r * kMxChunkBytes) + lane;
+                codes[r] = (uint32_t)__ldg(p) | ((uint32_t)__ldg(p + 32) << 16);
+            } else {
+                codes[r] = __ldg(reinterpret_cast<const uint32_t *>(src + (size_t)r * kMxChunkBytes) + lane);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        float scale[2];  // of the first and the last four columns
+        if (kWide) {
+            scale[0] = mx_scale_value((__shfl_sync(0xffffffffu, scales, r) >> (8 * (lane >> 3))) & 255u);
+            scale[1] = mx_scale_value((__shfl_sync(0xffffffffu, scales, 16 | r) >> (8 * (lane >> 3))) & 255u);
+        } else {
+            scale[0] = scale[1] = mx_scale_value((__shfl_sync(0xffffffffu, scales, (lane & 16) | r) >> (8 * ((lane >> 2) & 3))) & 255u);
+        }
         uint32_t h[4];
         mx_decode8(codes[r], h);
         float v[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
-            v[2 * i] = f.x * scale;
-            v[2 * i + 1] = f.y * scale;
+            v[2 * i] = f.x * scale[i >> 1];
+            v[2 * i + 1] = f.y * scale[i >> 1];
         }
-        if (col < k && row0 + r < rows) mx_store8<T>(o + ((long long)matrix * rows + row0 + r) * k + col, v);
+        if (l.row0 + r >= rows) continue;
+        T *p = dst + (size_t)r * k;
+        if constexpr (kWide) {
+            if (col < k) *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]);
+            if (col + 128 < k) *reinterpret_cast<float4 *>(p + 128) = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            if (col < k) mx_store8(p, v);
+        }
     }
 }
 
-static long long mx_items(int rows, int k, int batch, int rows_per_warp) { return (long long)batch * div_up(rows, rows_per_warp) * div_up(k, kMxChunk); }
+// Row groups and chunks of a launch: a CTA's four warps side by side along the columns as far as there are chunks.
+template <typename Kernel>
+static cudaError_t mxq_launch(int rows, int k, int batch, int rows_per_warp, Kernel kernel)
+{
+    const int chunks = div_up(k, kMxChunk), log_c = chunks >= 4 ? 2 : chunks >= 2 ? 1 : 0;
+    const long long groups = (long long)batch * div_up(rows, rows_per_warp);
+    kernel(dim3((unsigned)div_up_ll(groups, 4 >> log_c), (unsigned)div_up(chunks, 1 << log_c)), chunks, log_c);
+    return cudaGetLastError();
+}
 
-template <typename T>
+template <typename T, int ROWS>
 static cudaError_t quantize_as(const void *x, long long row_stride, void *q, void *s, int rows, int k, int batch, cudaStream_t stream)
 {
-    const int chunks = div_up(k, kMxChunk);
-    const long long items = mx_items(rows, k, batch, 8);
-    mx_quantize_kernel<T, 8><<<(unsigned)div_up_ll(items, kMxqWarps), kMxqWarps * 32, 0, stream>>>((const T *)x, row_stride, (uint8_t *)q, (uint32_t *)s,
-                                                                                                  rows, k, chunks, items);
-    return cudaGetLastError();
+    return mxq_launch(rows, k, batch, ROWS, [&](dim3 grid, int chunks, int log_c) {
+        mx_quantize_kernel<T, ROWS><<<grid, kMxqWarps * 32, 0, stream>>>((const T *)x, row_stride, (uint8_t *)q, (uint32_t *)s, rows, k, chunks, batch, log_c);
+    });
 }
 
 cudaError_t launch_mx_quantize(const void *x, int type, long long row_stride, void *q, void *s, int rows, int k, int batch, cudaStream_t stream)
 {
     switch (type) {
-        case TUNA_FP16: return quantize_as<__half>(x, row_stride, q, s, rows, k, batch, stream);
-        case TUNA_BF16: return quantize_as<__nv_bfloat16>(x, row_stride, q, s, rows, k, batch, stream);
-        default: return quantize_as<float>(x, row_stride, q, s, rows, k, batch, stream);
+        case TUNA_FP16: return quantize_as<__half, kMxqRows>(x, row_stride, q, s, rows, k, batch, stream);
+        case TUNA_BF16: return quantize_as<__nv_bfloat16, kMxqRows>(x, row_stride, q, s, rows, k, batch, stream);
+        default: return quantize_as<float, kMxqRows>(x, row_stride, q, s, rows, k, batch, stream);
     }
 }
 
-template <typename T>
+template <typename T, int ROWS>
 static cudaError_t dequant_as(const void *q, const void *s, void *o, int rows, int k, int batch, cudaStream_t stream)
 {
-    const int chunks = div_up(k, kMxChunk);
-    const long long items = mx_items(rows, k, batch, 8);
-    mx_dequant_kernel<T, 8><<<(unsigned)div_up_ll(items, kMxqWarps), kMxqWarps * 32, 0, stream>>>((const uint8_t *)q, (const uint32_t *)s, (T *)o, rows, k,
-                                                                                                 chunks, items);
-    return cudaGetLastError();
+    return mxq_launch(rows, k, batch, ROWS, [&](dim3 grid, int chunks, int log_c) {
+        mx_dequant_kernel<T, ROWS><<<grid, kMxqWarps * 32, 0, stream>>>((const uint8_t *)q, (const uint32_t *)s, (T *)o, rows, k, chunks, batch, log_c);
+    });
 }
 
 cudaError_t launch_mx_dequant(const void *q, const void *s, void *o, int type, int rows, int k, int batch, cudaStream_t stream)
 {
     switch (type) {
-        case TUNA_FP16: return dequant_as<__half>(q, s, o, rows, k, batch, stream);
-        case TUNA_BF16: return dequant_as<__nv_bfloat16>(q, s, o, rows, k, batch, stream);
-        default: return dequant_as<float>(q, s, o, rows, k, batch, stream);
+        case TUNA_FP16: return dequant_as<__half, 8>(q, s, o, rows, k, batch, stream);
+        case TUNA_BF16: return dequant_as<__nv_bfloat16, 8>(q, s, o, rows, k, batch, stream);
+        default: return dequant_as<float, 8>(q, s, o, rows, k, batch, stream);
     }
 }
 
