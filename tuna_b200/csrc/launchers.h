@@ -101,7 +101,7 @@ struct MxGemmArgs {
     const void *x, *xs, *q, *s;
     const void *offsets;  // device, experts + 1 of them; nullptr: one matrix
     void *o;
-    int m, n, k, experts, o_type;
+    int m, n, k, experts, x_type, o_type;
     void *workspace;
     cudaStream_t stream;
     int sm_count;
@@ -110,6 +110,7 @@ constexpr size_t kMxCounterBytes = 4096;
 cudaError_t launch_mx_quantize(const void *x, int type, long long row_stride, void *q, void *s, int rows, int k, int batch, cudaStream_t stream);
 cudaError_t launch_mx_dequant(const void *q, const void *s, void *o, int type, int rows, int k, int batch, cudaStream_t stream);
 int launch_mx_gemm(const MxGemmArgs &a);
+bool mx_gemm_takes(int m, int n, int k, int experts, int x_type, bool grouped, int sm_count);
 size_t mx_gemm_workspace_bytes(int m, int n, int k, int experts, int sm_count);
 
 }  // namespace tuna

@@ -12,7 +12,7 @@ static int type_bytes(int t) { return t == TUNA_FP32 ? 4 : 2; }
 static int check_matrix(int rows, int k, int batch)
 {
     if (rows < 1 || k < 1 || batch < 1 || k % kMxBlock) return TUNA_ERR_BAD_SHAPE;
-    if ((double)rows * k * batch > (double)(1ll << 41)) return TUNA_ERR_TOO_LARGE;
+    if ((double)rows * k * batch > (double)(1ll << 41) || (double)rows * batch > (double)(1ll << 31)) return TUNA_ERR_TOO_LARGE;
     return TUNA_OK;
 }
 
@@ -48,9 +48,10 @@ static int mx_product(const void *x, int x_type, const void *xs, const void *q, 
     if (!workspace || workspace_bytes < w.total) return TUNA_ERR_WORKSPACE;
     MxGemmArgs a;
     a.x = x; a.xs = xs; a.q = q; a.s = s; a.offsets = offsets; a.o = o;
-    a.m = m; a.n = n; a.k = k; a.experts = experts; a.o_type = o_type;
+    a.m = m; a.n = n; a.k = k; a.experts = experts; a.x_type = x_type; a.o_type = o_type;
     a.workspace = workspace; a.stream = (cudaStream_t)stream; a.sm_count = sms;
-    if (!packed) {
+    if (!mx_gemm_takes(m, n, k, experts, x_type, offsets != nullptr, sms)) {
+        a.x_type = TUNA_MXFP4;
         a.x = (uint8_t *)workspace + w.codes;
         a.xs = (uint8_t *)workspace + w.scales;
         if (launch_mx_quantize(x, x_type, k, (uint8_t *)workspace + w.codes, (uint8_t *)workspace + w.scales, n, k, 1, a.stream) != cudaSuccess) return TUNA_ERR_LAUNCH;

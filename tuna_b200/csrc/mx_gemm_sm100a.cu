@@ -3,29 +3,36 @@
 // that the device knows.
 //
 // The tensor cores multiply e2m1 codes and apply both blocks' scales themselves (tcgen05.mma kind::mxf4, scale_vec::2X), so
-// there is nothing to dequantize: per 256 columns a tile's codes and scales are copied to shared memory, the scales go on
-// to tensor memory (tcgen05.cp), and four MMAs of 64 columns add to fp32 accumulators.  Weights are operand A (128 rows),
-// tokens operand B (N columns): few tokens cost few columns.
+// there is nothing to dequantize: per 256 columns a tile's codes are copied to shared memory and its scales written to tensor
+// memory, and four MMAs of 64 columns add to fp32 accumulators.  Weights are operand A (128 rows), tokens operand B (N
+// columns): few tokens cost few columns.
 //
-// Persistent CTAs of 8 warps:
-//   warp 0     MMA issue (one elected lane): the stage's scales to tensor memory, then its MMAs
-//   warp 1     TMA producer: codes and scales of the weights, codes of the tokens
-//   warp 2     scales of the tokens.  Tiles start at any token, so these words are 4-byte copies (cp.async) that put each
-//              one where tcgen05.cp wants it: row t at lane t % 32, word t / 32
-//   warp 3     tensor-memory allocation
-//   warps 4-7  epilogue: tensor memory -> registers -> output type -> shared memory -> one bulk copy per token
+// Persistent CTAs, or pairs of CTAs (cta_group::2: 256 weight rows, every CTA stages its own 128 and half of the tokens), of 12 warps:
+//   warp 0     MMA issue (one elected lane; in a pair the first CTA's)
+//   warp 1     TMA producer of the weights' codes and scales
+//   warp 2     TMA producer of the tokens' codes
+//   warp 3     tensor-memory allocation; words of the tokens' scales, 4-byte copies (cp.async), since tiles start at any token
+//   warps 4-7  epilogue: tensor memory -> registers -> output type -> memory, of more than 16 tokens by way of shared memory
+//              and one bulk copy per token
+//   warps 8-11 scales, one warp per lane quarter: a word of scales is four blocks (128 columns) of one row or token, and the MMAs want that of
+//              row r at lane r % 32, column r / 32, in every quarter.  So each warp reads all words of a stage from shared memory and
+//              writes them to its quarter (tcgen05.st).  Copies by the tensor pipe (tcgen05.cp) take its time: 57344x8192 at 4096
+//              tokens 923 us with them, 756 without.
+// RESIDENT: up to 16 tokens in 16 bits are quantized by the CTA itself before its first MMA, all of K, and stay in shared memory:
+// no launch before this one.
 //
-// A tile's weight rows are permuted so that its scales need no such copies: 128 consecutive words in shared memory are, to
-// tcgen05.cp, lane i's words 4i .. 4i+3, the scales of MMA rows i, 32 + i, 64 + i and 96 + i.  MMA row 32 j + i therefore
-// is weight row 4 i + j (the copy's box walks rows 0, 4, .., 124, 1, 5, ..), and so are the accumulator's lanes.
-//
-// Work split.  Tiles are numbered expert by expert.  Whole waves go out one tile per CTA; what is left over (everything, if
-// there are fewer tiles than CTAs) is cut evenly along K.  A cut tile is finished by the CTA that arrives last, which
-// adds the fp32 partial sums in K order: the result does not depend on the order of arrival.
+// Work split.  Tiles are numbered expert by expert.  With few tokens one matrix may be cut into row tiles of equal height, a multiple
+// of 8 up to 128, a whole number of them for every CTA: the MMAs compute 128 rows whatever the height, which costs nothing where
+// the weights' bytes are the bound, and no sum is cut.  Otherwise tiles have 128 rows (256 for a pair); whole waves of them
+// go out one tile per worker, and what is left over (everything, if there are fewer tiles than workers) may be cut evenly along
+// K.  A cut tile is finished by the CTA that arrives last, which adds the fp32 partial sums in K order: the result does not
+// depend on the order of arrival.
 //
 // Every wait is bounded, as in the other pipeline kernels.
 #include <algorithm>
 #include <cstring>
+#include <cstdio>
+#include <cstdlib>
 #include <mutex>
 #include "launchers.h"
 #include "mx_format.cuh"
@@ -34,18 +41,18 @@
 
 namespace tuna {
 
-constexpr int kMxWarps = 8;
+constexpr int kMxWarps = 12;
 constexpr int kMxEpilogueWarp0 = 4;
-constexpr int kMxMaxStages = 10;
-constexpr int kMxScaleDepth = 3;       // stages of token scales in flight; fewer than there are stages
-constexpr int kMxStageTokens = 32;     // tokens of an output staging buffer
-constexpr int kMxTmemCols = 512;
-constexpr uint32_t kMxWeightBytes = kBlockRows * kMxChunkBytes;
-constexpr uint32_t kMxAtomBytes = 512;  // scales of 128 rows x 128 columns
-constexpr int kMxSmemMax = 227 * 1024 - 2048;  // dynamic part: 1 KB alignment, 1 KB static
+constexpr int kMxScaleWarp0 = 8;
+constexpr int kMxMaxStages = 12;
+constexpr int kMxStageTokens = 32;      // tokens of an output staging buffer
+constexpr int kMxDirectTokens = 16;     // tiles of up to so many tokens are stored from registers
+constexpr int kMxAheadTokens = 64;      // one matrix: up to here weights are read ahead of the dependency wait
+constexpr uint32_t kMxScaleBytes = 2 * kBlockRows * 4;  // of the weights' scales in a stage
+constexpr int kMxSmemMax = 227 * 1024;  // of a CTA alone on its SM, static part included
 
 struct MxParams {
-    const uint32_t *xs;   // words of the tokens' scales [words][tokens]
+    const uint32_t *xs;   // words of the tokens' scales [words][n]
     const int *offsets;   // first token of each expert, and the end; nullptr: one matrix, all tokens
     void *o;
     float *partials;
@@ -56,7 +63,14 @@ struct MxParams {
     int tile_tok;   // N
     int chunks;     // ceil(k / 256)
     int words;      // ceil(k / 128)
-    int row_tiles;  // ceil(m / 128)
+    int row_tiles;
+    int w_bytes;    // of the weights in a stage
+    int x_rows;     // tokens in a stage of a CTA
+    int flex;       // row tiles of equal height: tile t has the groups of 8 rows t * groups / row_tiles up to the next tile's
+    int groups;     // m / 8
+    int x_bf16;     // RESIDENT: type of the tokens
+    const void *x;  // RESIDENT: the tokens [n][k]
+    int cut;        // tiles may be cut along K
     int last_steps; // MMAs of the last chunk: 64 columns each
     int stages;
     int nd;         // accumulator buffers
@@ -69,11 +83,11 @@ struct MxSplit {
     int tiles, sk_tiles, sk_workers, sk_q, sk_r;
 };
 
-__device__ __forceinline__ MxSplit mx_split(int tiles, int chunks, int workers)
+__device__ __forceinline__ MxSplit mx_split(int tiles, int chunks, int workers, int cut)
 {
     MxSplit s = {tiles, 0, 0, 1, 0};
     const int rest = tiles % workers;
-    if (rest == 0) return s;
+    if (rest == 0 || !cut) return s;
     const int ctas = min(workers, rest * chunks / 2);  // two chunks at least
     if (ctas <= rest) return s;
     s.sk_tiles = rest;
@@ -133,41 +147,46 @@ struct MxSegs {
     __device__ int total_units() const { return (u_end - u) + (dp < tiles ? ((tiles - 1 - dp) / dp_step + 1) * chunks : 0); }
 };
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, int c3, uint32_t bar)
+// One lane's words to COUNT columns of this warp's lanes.
+__device__ __forceinline__ void tc_st_words(uint32_t taddr, const uint32_t (&v)[1])
 {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
-        ::"r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
-        : "memory");
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(v[0]) : "memory");
 }
-
-// Four bytes, or zeros where `have` is false.
-__device__ __forceinline__ void cp_async_word(uint32_t dst, const uint32_t *src, bool have)
+__device__ __forceinline__ void tc_st_words(uint32_t taddr, const uint32_t (&v)[4])
 {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(have ? 4 : 0) : "memory");
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
-
-// 32 rows of 16 bytes -> 4 columns of 32 lanes, the same in all four lane quarters.
-__device__ __forceinline__ void tc_copy_scales(uint32_t taddr, uint64_t desc)
+__device__ __forceinline__ void tc_st_words(uint32_t taddr, const uint32_t (&v)[8])
 {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+                 "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
 }
 
 // D[tmem] (+)= (A * scale A) (B * scale B), 64 columns of e2m1 with a scale per 32
+template <int CG>
 __device__ __forceinline__ void tc_mma_mx(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate)
 {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
+    if (CG == 1)
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+            " tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}"
+            ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+            " tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n}"
+            ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
 }
 
 // Instruction descriptor, kind::mxf4: A and B e2m1 (1 at bits 7-9 and 10-11), both K-major, N >> 3 at bits 17-22, e8m0 scales
 // (bit 23), M >> 7 at bits 27-28, which half of a scale word A and B use (0 or 2) at bits 29-30 and 4-5.
+template <int CG>
 __host__ __device__ constexpr uint32_t mx_idesc(int cols, int half)
 {
-    return (1u << 7) | (1u << 10) | ((uint32_t)(cols >> 3) << 17) | (1u << 23) | (1u << 27) | ((uint32_t)(2 * half) << 29) | ((uint32_t)(2 * half) << 4);
+    return (1u << 7) | (1u << 10) | ((uint32_t)(cols >> 3) << 17) | (1u << 23) | ((uint32_t)CG << 27) | ((uint32_t)(2 * half) << 29) | ((uint32_t)(2 * half) << 4);
 }
 
 template <typename T>
@@ -180,53 +199,112 @@ __device__ __forceinline__ void mx_store_shared(uint32_t a, __half v) { asm vola
 __device__ __forceinline__ void mx_store_shared(uint32_t a, __nv_bfloat16 v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(__bfloat16_as_ushort(v)) : "memory"); }
 __device__ __forceinline__ void mx_store_shared(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
 
-__host__ __device__ constexpr uint32_t mx_scale_atoms(int tile_tok) { return (uint32_t)((tile_tok + 127) / 128); }
-__host__ __device__ constexpr uint32_t mx_stage_bytes(int tile_tok)
-{
-    return kMxWeightBytes + (uint32_t)tile_tok * kMxChunkBytes + 2 * kMxAtomBytes + 2 * mx_scale_atoms(tile_tok) * kMxAtomBytes;
-}
-// Tensor-memory columns of a stage's scales: two atoms of four columns for the weights, as many per 128 tokens.
-__host__ __device__ constexpr uint32_t mx_scale_cols(int tile_tok) { return 8 + 8 * mx_scale_atoms(tile_tok); }
+// Words of a half (128 columns) of the tokens' scales that a lane holds: one up to 32 tokens of a tile, else four per 128.
+__host__ __device__ constexpr int mx_token_words(int tile_tok) { return tile_tok <= 32 ? 1 : tile_tok <= 128 ? 4 : 8; }
+// Tensor-memory columns of a stage's scales: four per half for the weights, four per half and 128 tokens.
+__host__ __device__ constexpr uint32_t mx_scale_cols(int token_words) { return 8 + 2 * (token_words < 4 ? 4 : token_words); }
 
-template <typename OT>
-__global__ void __launch_bounds__(32 * kMxWarps, 1)
-mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_ws,
-               const __grid_constant__ CUtensorMap tmap_x)
+// First row of row block b (a CTA's share of a tile).
+__device__ __forceinline__ int mx_row(const MxParams &p, int b) { return p.flex ? 8 * (int)((long long)b * p.groups / p.row_tiles) : b * kBlockRows; }
+
+// Four bytes of global memory; the barrier counts the thread's copies in when they have landed.
+__device__ __forceinline__ void cp_async_word(uint32_t dst, const uint32_t *src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
+
+// Quantizes the tokens' numbers, all of K: warp `w` of `warps` takes every warps-th (chunk, token).  Codes as TMA would have put
+// them (128-byte swizzle), scale words [chunk][half][32 tokens].
+template <typename T>
+__device__ __forceinline__ void mx_quantize_resident(const MxParams &p, int w, int warps, int lane, uint32_t codes_at, uint32_t x_bytes, uint32_t words_at)
+{
+    constexpr int R = 4;  // loads in flight
+    const int items = p.chunks * p.n;
+    for (int i0 = w; i0 < items; i0 += R * warps) {
+        Mx8<T> v[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int i = i0 + r * warps, c = i / p.n, t = i - c * p.n, col = c * kMxChunk + lane * 8;
+            if (i < items && col < p.k) v[r].load(static_cast<const T *>(p.x) + (size_t)t * p.k + col);
+            else v[r].zero();
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int i = i0 + r * warps, c = i / p.n, t = i - c * p.n;
+            if (i >= items) break;
+            uint32_t e = mx_scale(v[r].largest());
+            const float inverse = mx_inverse(e);
+            float f[8];
+            v[r].values(f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] *= inverse;
+            const uint32_t codes = e == 255u ? 0u : mx_encode8(f);
+            // 16-byte piece lane / 4 of the token's 128 bytes, XORed with the token's number mod 8
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(codes_at + (uint32_t)c * x_bytes + (uint32_t)t * kMxChunkBytes + ((((uint32_t)lane >> 2) ^ ((uint32_t)t & 7u)) << 4) + ((uint32_t)lane & 3u) * 4u),
+                         "r"(codes)
+                         : "memory");
+            e <<= 8 * ((lane >> 2) & 3);  // four neighbouring blocks make a word
+            e |= __shfl_xor_sync(0xffffffffu, e, 4);
+            e |= __shfl_xor_sync(0xffffffffu, e, 8);
+            if ((lane & 15) == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(words_at + (uint32_t)c * 256u + (uint32_t)(lane >> 4) * 128u + (uint32_t)t * 4u), "r"(e) : "memory");
+        }
+    }
+}
+
+// CG: CTAs of a worker (1 or 2).  NW: mx_token_words.  RESIDENT: the tokens are numbers in 16 bits and quantized here.
+// Tiles of up to 32 tokens leave room for a second CTA on the SM: that of the next launch, which copies its first weights meanwhile.
+template <int CG, int NW, bool RESIDENT, typename OT>
+__global__ void __launch_bounds__(32 * kMxWarps, NW == 1 ? 2 : 1)
+mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_w2,
+               const __grid_constant__ CUtensorMap tmap_ws, const __grid_constant__ CUtensorMap tmap_x)
 {
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ __align__(8) uint64_t bars[2 * kMxMaxStages + 4];
+    __shared__ __align__(8) uint64_t bars[3 * kMxMaxStages + 4];
     __shared__ uint32_t s_tmem_base;
     __shared__ int s_abort, s_last;
     __shared__ MxSplit s_split;
 
+    constexpr uint32_t kTmemCols = NW == 1 ? 256 : 512;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int rank = CG == 1 ? 0 : (int)cluster_ctarank();
+    const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
     const int N = p.tile_tok, S = p.stages;
-    const uint32_t base = (smem_u32(smem) + 1023u) & ~1023u;
-    const uint32_t stage_bytes = mx_stage_bytes(N);
-    const uint32_t x_off = kMxWeightBytes, ws_off = x_off + (uint32_t)N * kMxChunkBytes, xs_off = ws_off + 2 * kMxAtomBytes;
-    const uint32_t staging = base + (uint32_t)S * stage_bytes;
+    // [stages of weights][of tokens][of the weights' scales][of the tokens' scales][staging buffers][tables]; the MMAs read 128
+    // rows, in low tiles past their stage's end.  RESIDENT: of tokens, as many as there are chunks.
+    const int x_stages = RESIDENT ? p.chunks : S;
+    const uint32_t base = smem_u32(smem), w_bytes = (uint32_t)p.w_bytes, x_bytes = (uint32_t)p.x_rows * kMxChunkBytes;
+    const uint32_t x_ring = base + (uint32_t)S * w_bytes, ws_ring = x_ring + (uint32_t)x_stages * x_bytes, xs_ring = ws_ring + (uint32_t)S * kMxScaleBytes;
+    const uint32_t staging = xs_ring + (uint32_t)x_stages * (256u * NW);
     constexpr uint32_t kTokBytes = kBlockRows * (uint32_t)sizeof(OT);
     constexpr uint32_t kStagingBytes = kMxStageTokens * kTokBytes;
-    int *tables = reinterpret_cast<int *>(smem + (base - smem_u32(smem)) + (size_t)S * stage_bytes + 2 * kStagingBytes);
+    int *tables = reinterpret_cast<int *>(smem + (staging - base) + (N > kMxDirectTokens ? 2 * kStagingBytes : 0));
 
-    const uint32_t full = smem_u32(&bars[0]), empty = full + 8 * kMxMaxStages, d_full = empty + 8 * kMxMaxStages, d_empty = d_full + 16;
+    // landed: a stage's copies; full: its scales are written as well; empty: its MMAs are done
+    const uint32_t landed = smem_u32(&bars[0]), full = landed + 8 * kMxMaxStages, empty = full + 8 * kMxMaxStages, d_full = empty + 8 * kMxMaxStages, d_empty = d_full + 16;
     volatile int *abort_flag = &s_abort;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 1) {
-        auto count = [](int i) { return i < kMxMaxStages ? 2 : i < 2 * kMxMaxStages + 2 ? 1 : 4; };  // full: the copies and the scales; d_empty: four warps
-        for (int i = lane; i < 2 * kMxMaxStages + 4; i += 32) mbar_init(full + 8 * i, count(i));
+        auto count = [&](int i) {
+            if (i < kMxMaxStages) return RESIDENT ? 1 : 34;     // landed: weights, tokens, the lanes that copy their scales
+            if (i < 2 * kMxMaxStages) return 4 * CG;            // full: the scale warps of each CTA
+            return i < 3 * kMxMaxStages + 2 ? 1 : 4 * CG;       // empty, d_full: a commit; d_empty: the epilogue warps of each CTA
+        };
+        for (int i = lane; i < 3 * kMxMaxStages + 4; i += 32) mbar_init(landed + 8 * i, count(i));
         if (lane == 0) s_abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (elect_one_sync()) {
             prefetch_map(&tmap_w);
             prefetch_map(&tmap_ws);
-            prefetch_map(&tmap_x);
+            if (!RESIDENT) prefetch_map(&tmap_x);
         }
     }
     if (warp == 3) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)), "r"(kMxTmemCols) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (CG == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)), "r"(kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)), "r"(kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
     }
     auto depend = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
     if (warp == 0) {  // the experts' tiles: first token, tokens, tiles before
@@ -259,123 +337,200 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
         }
         if (lane == 0) {
             tables[3 * p.experts] = before;
-            s_split = mx_split(before, p.chunks, gridDim.x);
+            s_split = mx_split(before, p.chunks, workers, p.cut);
         }
     }
     tc_fence_before();
     __syncthreads();
+    if (CG == 2) cluster_sync_all();  // the other CTA's barriers are there
     tc_fence_after();
     const uint32_t tmem = s_tmem_base;
-    const uint32_t sf_col = (uint32_t)(p.nd * N), sf_cols = mx_scale_cols(N);
+    const uint32_t sf_col = (uint32_t)(p.nd * N);
+    constexpr uint32_t kScaleCols = mx_scale_cols(NW), kTokenCols = NW < 4 ? 4 : NW;  // of a stage, and of a half of its tokens
     MxSegs segs;
-    segs.init(p, s_split, blockIdx.x, gridDim.x, tables);
+    segs.init(p, s_split, worker, workers, tables);
     const int total = segs.total_units();
+    auto tile_cols = [&] { return (segs.valid + 8 * CG - 1) & -(8 * CG); };  // tokens that the tile's MMAs cover
 
+    if (RESIDENT && warp != 1) {  // the weights are on their way meanwhile
+        depend();
+        const int w = warp == 0 ? 0 : warp - 1;
+        if (p.x_bf16) mx_quantize_resident<__nv_bfloat16>(p, w, kMxWarps - 1, lane, x_ring, x_bytes, xs_ring);
+        else mx_quantize_resident<__half>(p, w, kMxWarps - 1, lane, x_ring, x_bytes, xs_ring);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the MMAs read the codes
+        asm volatile("bar.sync 2, %0;" ::"n"(32 * (kMxWarps - 1)) : "memory");
+    }
+    // Whoever makes a bounded wait that ends only after the kernels before this one waits for those first.
     if (warp == 0) {
-        // ------------------------------------------------------------------ MMA issue
-        constexpr uint64_t sw128 = ((uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29))) << 32;  // 8-row groups 1024 bytes apart, version 1, 128-byte swizzle
-        constexpr uint64_t plain = ((uint64_t)((128u >> 4) | (1u << 14))) << 32;                // 8-row groups of 16 bytes a row, 128 bytes apart, no swizzle
-        Ring ru, rd;
-        bool ok = true;
-        while (ok && segs.next()) {
-            const int cols = (segs.valid + 15) & ~15;
-            ok = mbar_wait_warp(d_empty + 8 * rd.idx, rd.phase ^ 1, abort_flag, p.status, 203);
-            const uint32_t d = tmem + (uint32_t)(rd.idx * N);
-            for (int c = segs.c0; ok && c < segs.c1; ++c) {
-                ok = mbar_wait_warp(full + 8 * ru.idx, ru.phase, abort_flag, p.status, 204);
-                if (!ok) break;
-                tc_fence_after();
-                if (elect_one_sync()) {
-                    const uint32_t at = base + (uint32_t)ru.idx * stage_bytes;
-                    const uint32_t sfa = tmem + sf_col + (uint32_t)ru.idx * sf_cols, sfb = sfa + 8, atoms = mx_scale_atoms(N);
-                    auto desc = [](uint64_t kind, uint32_t addr) { return kind | (uint64_t)((addr & 0x3FFFFu) >> 4); };
-                    for (uint32_t h = 0; h < 2; ++h) {
-                        tc_copy_scales(sfa + 4 * h, desc(plain, at + ws_off + h * kMxAtomBytes));
-                        for (uint32_t a = 0; a < atoms; ++a)
-                            tc_copy_scales(sfb + 4 * (h * atoms + a), desc(plain, at + xs_off + (h * atoms + a) * kMxAtomBytes));
+        if (CG == 1 || rank == 0) {
+            depend();
+            Ring ru, rd;
+            bool ok = true;
+            // -------------------------------------------------------------- MMA issue
+            constexpr uint64_t sw128 = ((uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29))) << 32;  // 8-row groups 1024 bytes apart, version 1, 128-byte swizzle
+            while (ok && segs.next()) {
+                const uint32_t idesc = mx_idesc<CG>(tile_cols(), 0);
+                constexpr uint32_t kHalf = mx_idesc<CG>(0, 1) ^ mx_idesc<CG>(0, 0);
+                ok = mbar_wait_warp(d_empty + 8 * rd.idx, rd.phase ^ 1, abort_flag, p.status, 203);
+                const uint32_t d = tmem + (uint32_t)(rd.idx * N);
+                for (int c = segs.c0; ok && c < segs.c1; ++c) {
+                    ok = mbar_wait_warp(full + 8 * ru.idx, ru.phase, abort_flag, p.status, 204);
+                    if (!ok) break;
+                    tc_fence_after();
+                    if (elect_one_sync()) {
+                        const uint64_t a = sw128 | (uint64_t)(((base + (uint32_t)ru.idx * w_bytes) & 0x3FFFFu) >> 4);
+                        const uint64_t b = sw128 | (uint64_t)(((x_ring + (uint32_t)(RESIDENT ? c : ru.idx) * x_bytes) & 0x3FFFFu) >> 4);
+                        const uint32_t sfa = tmem + sf_col + (uint32_t)ru.idx * kScaleCols, sfb = sfa + 8;
+                        const int steps = c + 1 == p.chunks ? p.last_steps : 4;
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            if (kk < steps)
+                                tc_mma_mx<CG>(d, a + 2 * kk, b + 2 * kk, (kk & 1) ? idesc ^ kHalf : idesc, sfa + 4 * (kk >> 1), sfb + kTokenCols * (kk >> 1),
+                                              c == segs.c0 && kk == 0 ? 0u : 1u);
+                        if (CG == 1) {
+                            tc_commit(empty + 8 * ru.idx);
+                            if (c + 1 == segs.c1) tc_commit(d_full + 8 * rd.idx);
+                        } else {
+                            tc_commit_pair(empty + 8 * ru.idx);
+                            if (c + 1 == segs.c1) tc_commit_pair(d_full + 8 * rd.idx);
+                        }
                     }
-                    const int steps = c + 1 == p.chunks ? p.last_steps : 4;
-                    for (int kk = 0; kk < steps; ++kk)
-                        tc_mma_mx(d, desc(sw128, at + 32 * kk), desc(sw128, at + x_off + 32 * kk), mx_idesc(cols, kk & 1), sfa + 4 * (kk >> 1),
-                                  sfb + 4 * atoms * (kk >> 1), c == segs.c0 && kk == 0 ? 0u : 1u);
-                    tc_commit(empty + 8 * ru.idx);
-                    if (c + 1 == segs.c1) tc_commit(d_full + 8 * rd.idx);
+                    __syncwarp();
+                    ru.advance(S);
                 }
-                __syncwarp();
-                ru.advance(S);
+                rd.advance(p.nd);
             }
-            rd.advance(p.nd);
         }
     } else if (warp == 1) {
-        // ------------------------------------------------------------------ weights and tokens' codes
+        // ------------------------------------------------------------------ weights
         Ring ru;
         bool ok = true;
-        depend();
+        int issued = 0;
+        if (!p.ahead) depend();
         while (ok && segs.next()) {
+            const int block = CG * segs.rt + rank, row = mx_row(p, block), rows = mx_row(p, block + 1) - row;
+            const CUtensorMap *map = !p.flex || rows * kMxChunkBytes == p.w_bytes ? &tmap_w : &tmap_w2;  // boxes of the taller and of the lower tiles
             for (int c = segs.c0; c < segs.c1; ++c, ru.advance(S)) {
+                if (issued++ == S) depend();
                 ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 200);
                 if (!ok) break;
                 if (elect_one_sync()) {
-                    const uint32_t at = base + (uint32_t)ru.idx * stage_bytes, bar = full + 8 * ru.idx;
-                    mbar_expect_tx(bar, kMxWeightBytes + (uint32_t)N * kMxChunkBytes + 2 * kMxAtomBytes);
-                    tma_load_4d(at, &tmap_w, 0, segs.rt * (kBlockRows / 4), 0, segs.e * p.chunks + c, bar);
-                    tma_load_2d(at + ws_off, &tmap_ws, segs.rt * kBlockRows, segs.e * p.words + 2 * c, bar);
-                    tma_load_3d(at + x_off, &tmap_x, 0, segs.tok0, c, bar);
+                    const uint32_t bar = landed + 8 * ru.idx;
+                    mbar_expect_tx(bar, (uint32_t)rows * kMxChunkBytes + kMxScaleBytes);
+                    tma_load_3d(base + (uint32_t)ru.idx * w_bytes, map, 0, row, segs.e * p.chunks + c, bar);
+                    tma_load_2d(ws_ring + (uint32_t)ru.idx * kMxScaleBytes, &tmap_ws, row, segs.e * p.words + 2 * c, bar);
                 }
                 __syncwarp();
             }
         }
         // The MMAs' commits have arrived at every stage in use before the CTA leaves.
+        depend();
         if (total < S) ru = Ring();
         for (int i = min(S, total); ok && i > 0; --i, ru.advance(S)) ok = mbar_wait_warp(empty + 8 * ru.idx, total < S ? 0u : ru.phase ^ 1, abort_flag, p.status, 210);
-    } else if (warp == 2) {
-        // ------------------------------------------------------------------ tokens' scales
-        Ring ru, ra;
-        int flying = 0;
+    } else if (warp == 2 && !RESIDENT) {
+        // ------------------------------------------------------------------ tokens' codes
+        Ring ru;
         bool ok = true;
-        auto arrive = [&] {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // what cp.async wrote is read by tcgen05.cp
-            __syncwarp();
-            if (lane == 0) mbar_arrive(full + 8 * ra.idx);
-            ra.advance(S);
-        };
         depend();
         while (ok && segs.next()) {
-            const int rows = min(N, p.n - segs.tok0);
+            const int tok = segs.tok0 + rank * (tile_cols() / CG);
+            for (int c = segs.c0; c < segs.c1; ++c, ru.advance(S)) {
+                ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 211);
+                if (!ok) break;
+                if (elect_one_sync()) {
+                    mbar_expect_tx(landed + 8 * ru.idx, x_bytes);
+                    tma_load_3d(x_ring + (uint32_t)ru.idx * x_bytes, &tmap_x, 0, tok, c, landed + 8 * ru.idx);
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == 3 && !RESIDENT) {
+        // ------------------------------------------------------------------ tokens' scales
+        Ring ru;
+        bool ok = true;
+        depend();
+        while (ok && segs.next()) {
             for (int c = segs.c0; c < segs.c1; ++c, ru.advance(S)) {
                 ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 201);
                 if (!ok) break;
-                const uint32_t at = base + (uint32_t)ru.idx * stage_bytes + xs_off, half = mx_scale_atoms(N) * kMxAtomBytes;
+                const uint32_t to = xs_ring + (uint32_t)ru.idx * (256u * NW) + 4u * lane;
+                const uint32_t *src = p.xs + (size_t)(2 * c) * p.n + segs.tok0 + lane;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int word = min(2 * c + h, p.words - 1);  // behind the last word of an odd number of them nothing is multiplied
-                    const uint32_t *src = p.xs + (size_t)word * p.n + segs.tok0;
-                    for (int t = lane; t < N; t += 32)
-                        cp_async_word(at + h * half + (uint32_t)(t >> 7) * kMxAtomBytes + (uint32_t)((t & 31) * 16 + ((t >> 5) & 3) * 4), src + min(t, rows - 1), t < rows);
+                for (int j = 0; j < NW; ++j) {
+                    if (32 * j + lane >= segs.valid) continue;  // whatever lies there scales columns that nobody reads
+                    cp_async_word(to + 128u * j, src + 32 * j);
+                    if (2 * c + 1 < p.words) cp_async_word(to + 128u * (NW + j), src + p.n + 32 * j);
                 }
-                asm volatile("cp.async.commit_group;" ::: "memory");
-                if (++flying > kMxScaleDepth) {
-                    asm volatile("cp.async.wait_group %0;" ::"n"(kMxScaleDepth) : "memory");
-                    arrive();
-                    --flying;
+                cp_async_arrive(landed + 8 * ru.idx);
+            }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+    } else if (warp >= kMxScaleWarp0) {
+        // ------------------------------------------------------------------ scales to tensor memory
+        const int quarter = warp - kMxScaleWarp0;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + sf_col;
+        const uint32_t leader_full = CG == 1 ? full : map_to_rank(full, 0);
+        Ring ru;
+        bool ok = true;
+        if (!RESIDENT) depend();
+        auto words = [&](auto &v, uint32_t at) {
+#pragma unroll
+            for (int i = 0; i < (int)(sizeof(v) / 4); ++i) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[i]) : "r"(at + 128u * i + 4u * lane));
+        };
+        while (ok && segs.next()) {
+            for (int c = segs.c0; c < segs.c1; ++c, ru.advance(S)) {
+                // a stage's copies have landed, so its MMAs of the round before are done, and its scales may be overwritten
+                ok = mbar_wait_warp(landed + 8 * ru.idx, ru.phase, abort_flag, p.status, 212);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t to = lanes + (uint32_t)ru.idx * kScaleCols, x_at = xs_ring + (uint32_t)(RESIDENT ? c : ru.idx) * (256u * NW);
+                uint32_t w[8];
+                words(w, ws_ring + (uint32_t)ru.idx * kMxScaleBytes);
+                if constexpr (NW == 1) {
+                    uint32_t x0[1], x1[1];
+                    words(x0, x_at);
+                    words(x1, x_at + 128);
+                    tc_st_words(to + 8, x0);
+                    tc_st_words(to + 8 + kTokenCols, x1);
+                } else {
+                    uint32_t x[2 * NW];
+                    words(x, x_at);
+                    if constexpr (NW == 4) tc_st_words(to + 8, x);
+                    else tc_st_x16(to + 8, x);
+                }
+                tc_st_words(to, w);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (CG == 1) mbar_arrive(full + 8 * ru.idx);
+                    else mbar_arrive_cluster(leader_full + 8 * ru.idx);
                 }
             }
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        for (; flying > 0; --flying) arrive();
     } else if (warp >= kMxEpilogueWarp0) {
         // ------------------------------------------------------------------ epilogue
         const int quarter = warp & 3, thread = threadIdx.x - 32 * kMxEpilogueWarp0;
-        const int row = 4 * lane + quarter;  // of the tile: see the head of the file
         const uint32_t tmem_q = tmem + ((uint32_t)(32 * quarter) << 16);
         const size_t slot_floats = (size_t)kBlockRows * N;
         OT *o = static_cast<OT *>(p.o);
         Ring rd;
         uint32_t buf = 0;
         depend();
-        // Rows of `valid` tokens, 16 at a time from `get`, through the staging buffers to memory.
+        // Rows of `valid` tokens, 16 at a time from `get`, to memory: from registers, or through the staging buffers.
         auto store_tile = [&](auto get) {
-            const uint32_t bytes = (uint32_t)min(kBlockRows, p.m - segs.rt * kBlockRows) * (uint32_t)sizeof(OT);
+            const int row0 = mx_row(p, CG * segs.rt + rank), rows = min(mx_row(p, CG * segs.rt + rank + 1), p.m) - row0;
+            if (N <= kMxDirectTokens) {
+                float v[16];
+                get(0, v);
+                OT *to = o + (size_t)segs.tok0 * p.m + row0 + thread;
+                if (thread < rows) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (i < segs.valid) to[(size_t)i * p.m] = mx_convert<OT>(v[i]);
+                }
+                return;
+            }
             for (int t0 = 0; t0 < segs.valid; t0 += kMxStageTokens, buf ^= 1) {
                 const uint32_t to = staging + buf * kStagingBytes;
                 if (lane < 8) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the buffer's previous tokens have left it
@@ -386,18 +541,27 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                     float v[16];
                     get(t0 + h, v);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) mx_store_shared(to + (uint32_t)(h + i) * kTokBytes + (uint32_t)row * (uint32_t)sizeof(OT), mx_convert<OT>(v[i]));
+                    for (int i = 0; i < 16; ++i) mx_store_shared(to + (uint32_t)(h + i) * kTokBytes + (uint32_t)thread * (uint32_t)sizeof(OT), mx_convert<OT>(v[i]));
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (lane < 8) {
                     const int t = 8 * quarter + lane;
-                    if (t0 + t < segs.valid)
-                        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(o + (size_t)(segs.tok0 + t0 + t) * p.m + segs.rt * kBlockRows),
-                                     "r"(to + (uint32_t)t * kTokBytes), "r"(bytes)
+                    if (t0 + t < segs.valid && rows > 0)
+                        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(o + (size_t)(segs.tok0 + t0 + t) * p.m + row0),
+                                     "r"(to + (uint32_t)t * kTokBytes), "r"((uint32_t)rows * (uint32_t)sizeof(OT))
                                      : "memory");
                     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
                 }
+            }
+        };
+        const uint32_t leader_d_empty = CG == 1 ? d_empty : map_to_rank(d_empty, 0);
+        auto drained = [&] {  // the accumulator may be overwritten
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (CG == 1) mbar_arrive(d_empty + 8 * rd.idx);
+                else mbar_arrive_cluster(leader_d_empty + 8 * rd.idx);
             }
         };
         while (segs.next()) {
@@ -407,21 +571,17 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
             const uint32_t d = tmem_q + (uint32_t)(rd.idx * N);
             if (segs.c0 == 0 && segs.c1 == p.chunks) {
                 store_tile([&](int t, float (&v)[16]) { tc_ld_x16(d + t, v); });
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(d_empty + 8 * rd.idx);
+                drained();
             } else {
                 // [4-token group][128 lanes] float4: a warp store is 512 contiguous bytes
-                float4 *dst = reinterpret_cast<float4 *>(p.partials + (size_t)(2 * blockIdx.x + (segs.c0 == 0 ? 1 : 0)) * slot_floats) + 32 * quarter + lane;
+                float4 *dst = reinterpret_cast<float4 *>(p.partials + (size_t)(2 * blockIdx.x + (segs.c0 == 0 ? 1 : 0)) * slot_floats) + thread;
                 for (int t0 = 0; t0 < segs.valid; t0 += 16) {
                     float v[16];
                     tc_ld_x16(d + t0, v);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) dst[(size_t)(t0 / 4 + i) * kBlockRows] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(d_empty + 8 * rd.idx);
+                drained();
                 auto worker_of = [&](int unit) {
                     const int big = s_split.sk_r * (s_split.sk_q + 1);
                     return unit < big ? unit / (s_split.sk_q + 1) : s_split.sk_r + (unit - big) / s_split.sk_q;
@@ -431,9 +591,9 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                 if (thread == 0) {
                     unsigned int old;
                     // releases the four warps' partials (ordered before it by the barrier) and acquires the others'
-                    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(p.counters + segs.tile) : "memory");
+                    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(p.counters + CG * segs.tile + rank) : "memory");
                     s_last = old == (unsigned)nseg - 1;
-                    if (s_last) p.counters[segs.tile] = 0;  // left clean for the next call
+                    if (s_last) p.counters[CG * segs.tile + rank] = 0;  // left clean for the next call
                 }
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (s_last) {
@@ -441,7 +601,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
 #pragma unroll
                         for (int i = 0; i < 16; ++i) v[i] = 0.f;
                         for (int s = 0; s < nseg; ++s) {
-                            const float4 *src = reinterpret_cast<const float4 *>(p.partials + (size_t)(2 * (first + s) + (s == 0 ? 1 : 0)) * slot_floats) + (size_t)(t / 4) * kBlockRows + 32 * quarter + lane;
+                            const float4 *src = reinterpret_cast<const float4 *>(p.partials + (size_t)(2 * (CG * (first + s) + rank) + (s == 0 ? 1 : 0)) * slot_floats) + (size_t)(t / 4) * kBlockRows + thread;
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const float4 w = __ldcg(src + i * kBlockRows);
@@ -460,41 +620,91 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if (CG == 2) cluster_sync_all();
     if (warp == 3) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kMxTmemCols) : "memory");
+        if (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
     }
 }
 
 // ------------------------------------------------------------------ host side
 
 struct MxPlan {
-    int tile_tok, stages, nd;
+    int cg, tile_tok, stages, nd;
+    bool resident;
+    int flex, row_tiles, cut, w_bytes, x_rows;
+    int workers;
     size_t smem;
 };
 
-static MxPlan mx_plan(int n, int experts, int o_type)
+static MxPlan mx_plan(int m, int n, int k, int experts, int x_type, int o_type, bool grouped, int sm_count)
 {
-    MxPlan l;
-    const int each = div_up(n, experts);
-    l.tile_tok = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : 128;
-    const size_t tail = 2 * (size_t)kMxStageTokens * kBlockRows * (o_type == TUNA_FP32 ? 4 : 2) + (3 * (size_t)experts + 1) * 4;
-    const size_t room = kMxSmemMax - tail;
-    l.stages = (int)std::min<size_t>(kMxMaxStages, room / mx_stage_bytes(l.tile_tok));
-    l.nd = 2;
-    l.smem = (size_t)l.stages * mx_stage_bytes(l.tile_tok) + tail + 1024;
+    MxPlan l = {};
+    const int each = div_up(n, experts), chunks = div_up(k, kMxChunk);
+    (void)chunks;
+    l.cg = each > 128 ? 2 : 1;
+    l.tile_tok = std::min(l.cg == 2 ? 256 : 128, div_up(each, 16) * 16);
+    if (grouped) l.tile_tok = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : each <= 128 ? 128 : 256;
+    l.cut = 1;
+    if (!grouped && l.cg == 1) l.flex = 1;
+    int rt = 0;
+    if (const char *env = getenv("MXPLAN")) {  // cg,N,flex[,row tiles]
+        sscanf(env, "%d,%d,%d,%d", &l.cg, &l.tile_tok, &l.flex, &rt);
+        if (l.cg == 2) l.flex = 0;
+    }
+    l.row_tiles = div_up(m, kBlockRows * l.cg);
+    l.w_bytes = kBlockRows * kMxChunkBytes;
+    if (l.flex) {
+        const int waves = div_up(m, kBlockRows * sm_count);
+        l.row_tiles = std::min(div_up(m, 32), waves * sm_count);
+        if (rt >= div_up(m, kBlockRows) && rt <= m / 8) l.row_tiles = rt;
+        l.cut = 0;
+        l.w_bytes = 8 * div_up(m / 8, l.row_tiles) * kMxChunkBytes;
+    }
+    l.workers = sm_count / l.cg;
+    const int words = mx_token_words(l.tile_tok);
+    const size_t room = words == 1 ? 111 * 1024 : kMxSmemMax - 2048;
+    const size_t tail = (l.tile_tok > kMxDirectTokens ? 2 * (size_t)kMxStageTokens * kBlockRows * (o_type == TUNA_FP32 ? 4 : 2) : 0) + (3 * (size_t)experts + 1) * 4;
+    l.x_rows = l.tile_tok / l.cg;
+    const size_t w_stage = (size_t)l.w_bytes + kMxScaleBytes;
+    size_t x_stage = (size_t)l.x_rows * kMxChunkBytes + 256 * words;
+    // tokens' codes that stay in shared memory: what is left has to hold stages enough
+    const size_t resident = (size_t)chunks * (div_up(n, 8) * 8 * kMxChunkBytes + 256);
+    l.resident = x_type != TUNA_MXFP4 && !grouped && n <= 16 && l.flex && resident + 4 * w_stage + tail <= room && resident + 60 * 1024 <= room;
+    size_t fixed = tail;
+    if (l.resident) {
+        l.x_rows = div_up(n, 8) * 8;
+        fixed += resident;
+        x_stage = 0;
+    }
+    l.stages = (int)std::min<size_t>(kMxMaxStages, (room - fixed) / (w_stage + x_stage));
+    const int tmem_cols = words == 1 ? 256 : 512, scales = l.stages * (int)mx_scale_cols(words);
+    l.nd = 2 * l.tile_tok + scales <= tmem_cols ? 2 : 1;
+    // the last stage's MMAs read 128 rows
+    l.smem = std::max((size_t)l.stages * (w_stage + x_stage) + fixed, (size_t)(l.stages - 1) * l.w_bytes + kBlockRows * kMxChunkBytes);
     return l;
+}
+
+// Whether the product quantizes tokens of this type itself; otherwise it wants their codes and scales.
+bool mx_gemm_takes(int m, int n, int k, int experts, int x_type, bool grouped, int sm_count)
+{
+    return x_type == TUNA_MXFP4 || mx_plan(m, n, k, experts, x_type, TUNA_FP16, grouped, sm_count).resident;
 }
 
 size_t mx_gemm_workspace_bytes(int m, int n, int k, int experts, int sm_count)
 {
-    (void)m; (void)k;
-    const MxPlan l = mx_plan(n, experts, TUNA_FP32);
-    return kMxCounterBytes + 2 * (size_t)sm_count * kBlockRows * l.tile_tok * 4;
+    size_t floats = 0;  // of the plan for one matrix and the one for experts
+    for (int grouped = 0; grouped < 2; ++grouped) floats = std::max(floats, (size_t)kBlockRows * mx_plan(m, n, k, experts, TUNA_MXFP4, TUNA_FP16, grouped, sm_count).tile_tok);
+    return kMxCounterBytes + 2 * (size_t)sm_count * floats * 4;
 }
 
-template <typename OT>
-static int launch_mx(const MxParams &p, const CUtensorMap &mw, const CUtensorMap &ms, const CUtensorMap &mx, int ctas, size_t smem, cudaStream_t stream)
+struct MxMaps {
+    CUtensorMap w, w2, ws, x;
+};
+
+template <int CG, int NW, bool RESIDENT, typename OT>
+static int launch_mx(const MxParams &p, const MxMaps &maps, int ctas, size_t smem, cudaStream_t stream)
 {
     static bool attr_set[64] = {false};
     static std::mutex mu;
@@ -503,7 +713,7 @@ static int launch_mx(const MxParams &p, const CUtensorMap &mw, const CUtensorMap
     {
         std::lock_guard<std::mutex> lock(mu);
         if (!attr_set[dev]) {
-            if (cudaFuncSetAttribute(mx_gemm_kernel<OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMxSmemMax + 1024) != cudaSuccess) return TUNA_ERR_NO_DEVICE;
+            if (cudaFuncSetAttribute(mx_gemm_kernel<CG, NW, RESIDENT, OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMxSmemMax - 2048) != cudaSuccess) return TUNA_ERR_NO_DEVICE;
             attr_set[dev] = true;
         }
     }
@@ -512,52 +722,64 @@ static int launch_mx(const MxParams &p, const CUtensorMap &mw, const CUtensorMap
     lc.blockDim = dim3(32 * kMxWarps);
     lc.dynamicSmemBytes = smem;
     lc.stream = stream;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = CG;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     lc.attrs = attr;
-    lc.numAttrs = 1;
-    return cudaLaunchKernelEx(&lc, mx_gemm_kernel<OT>, p, mw, ms, mx) == cudaSuccess ? TUNA_OK : TUNA_ERR_LAUNCH;
+    lc.numAttrs = CG == 1 ? 1 : 2;
+    return cudaLaunchKernelEx(&lc, mx_gemm_kernel<CG, NW, RESIDENT, OT>, p, maps.w, maps.w2, maps.ws, maps.x) == cudaSuccess ? TUNA_OK : TUNA_ERR_LAUNCH;
+}
+
+template <typename OT>
+static int launch_mx_as(const MxPlan &l, const MxParams &p, const MxMaps &maps, int ctas, cudaStream_t stream)
+{
+    const int words = mx_token_words(l.tile_tok);
+    if (l.cg == 2) return words <= 4 ? launch_mx<2, 4, false, OT>(p, maps, ctas, l.smem, stream) : launch_mx<2, 8, false, OT>(p, maps, ctas, l.smem, stream);
+    if (words == 4) return launch_mx<1, 4, false, OT>(p, maps, ctas, l.smem, stream);
+    return l.resident ? launch_mx<1, 1, true, OT>(p, maps, ctas, l.smem, stream) : launch_mx<1, 1, false, OT>(p, maps, ctas, l.smem, stream);
 }
 
 int launch_mx_gemm(const MxGemmArgs &a)
 {
-    const MxPlan l = mx_plan(a.n, a.experts, a.o_type);
+    const MxPlan l = mx_plan(a.m, a.n, a.k, a.experts, a.x_type, a.o_type, a.offsets != nullptr, a.sm_count);
     MxParams p;
     std::memset(&p, 0, sizeof(p));
-    p.xs = (const uint32_t *)a.xs; p.offsets = (const int *)a.offsets; p.o = a.o;
+    p.xs = (const uint32_t *)a.xs; p.x = a.x; p.offsets = (const int *)a.offsets; p.o = a.o;
     p.m = a.m; p.n = a.n; p.k = a.k; p.experts = a.experts;
+    p.x_bf16 = a.x_type == TUNA_BF16;
     p.tile_tok = l.tile_tok;
     p.chunks = div_up(a.k, kMxChunk);
     p.words = div_up(a.k, kMxScaleCols);
-    p.row_tiles = div_up(a.m, kBlockRows);
     p.last_steps = div_up(a.k - (p.chunks - 1) * kMxChunk, 64);
-    p.stages = l.stages;
-    p.nd = l.nd;
+    p.row_tiles = l.row_tiles; p.w_bytes = l.w_bytes; p.x_rows = l.x_rows; p.flex = l.flex; p.groups = a.m / 8; p.cut = l.cut;
+    p.stages = l.stages; p.nd = l.nd;
+    p.ahead = a.offsets == nullptr && a.n <= kMxAheadTokens;
     p.counters = (unsigned int *)a.workspace;
     p.partials = (float *)((uint8_t *)a.workspace + kMxCounterBytes);
     p.status = device_status_word();
     if (!p.status) return TUNA_ERR_NO_DEVICE;
     const long long tiles = ((long long)div_up(a.n, l.tile_tok) + a.experts - 1) * p.row_tiles;  // at most
-    if (tiles >= 1ll << 30 || (tiles / a.sm_count + 2) * p.chunks >= 1ll << 30 || (long long)a.sm_count * p.chunks >= 1ll << 30 || (long long)a.experts * p.words >= 1ll << 30) return TUNA_ERR_TOO_LARGE;
+    if (tiles >= 1ll << 30 || (tiles / l.workers + 2) * p.chunks >= 1ll << 30 || (long long)a.sm_count * p.chunks >= 1ll << 30 || (long long)a.experts * p.words >= 1ll << 30) return TUNA_ERR_TOO_LARGE;
 
-    CUtensorMap mw, ms, mx;
-    {
-        const uint64_t dims[4] = {kMxChunkBytes, (uint64_t)a.m / 4, 4, (uint64_t)a.experts * p.chunks};
-        const uint64_t strides[3] = {4 * kMxChunkBytes, kMxChunkBytes, (uint64_t)a.m * kMxChunkBytes};
-        const uint32_t box[4] = {kMxChunkBytes, kBlockRows / 4, 4, 1};
-        if (!make_tensor_map_nd(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.q, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)) return TUNA_ERR_NO_DEVICE;
-    }
-    if (!make_tensor_map_2d(&ms, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.s, (uint64_t)a.m, (uint64_t)a.experts * p.words, (uint64_t)a.m * 4, kBlockRows, 2, CU_TENSOR_MAP_SWIZZLE_NONE))
+    MxMaps maps;
+    auto tiles_of = [](CUtensorMap *map, const void *at, uint64_t rows, uint64_t chunks, uint32_t box_rows) {  // [chunks][rows][128 bytes]
+        return make_tensor_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, at, kMxChunkBytes, rows, chunks, kMxChunkBytes, rows * kMxChunkBytes, kMxChunkBytes, box_rows, 1,
+                                  CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    if (!tiles_of(&maps.w, a.q, (uint64_t)a.m, (uint64_t)a.experts * p.chunks, (uint32_t)l.w_bytes / kMxChunkBytes)) return TUNA_ERR_NO_DEVICE;
+    maps.w2 = maps.x = maps.w;
+    if (l.flex && p.groups % l.row_tiles && !tiles_of(&maps.w2, a.q, (uint64_t)a.m, (uint64_t)p.chunks, 8u * (uint32_t)(p.groups / l.row_tiles))) return TUNA_ERR_NO_DEVICE;
+    if (!l.resident && !tiles_of(&maps.x, a.x, (uint64_t)a.n, (uint64_t)p.chunks, (uint32_t)l.x_rows)) return TUNA_ERR_NO_DEVICE;
+    if (!make_tensor_map_2d(&maps.ws, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.s, (uint64_t)a.m, (uint64_t)a.experts * p.words, (uint64_t)a.m * 4, kBlockRows, 2, CU_TENSOR_MAP_SWIZZLE_NONE))
         return TUNA_ERR_NO_DEVICE;
-    if (!make_tensor_map_3d(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.x, kMxChunkBytes, (uint64_t)a.n, (uint64_t)p.chunks, kMxChunkBytes, (uint64_t)a.n * kMxChunkBytes,
-                            kMxChunkBytes, (uint32_t)l.tile_tok, 1, CU_TENSOR_MAP_SWIZZLE_128B))
-        return TUNA_ERR_NO_DEVICE;
-    const int ctas = a.sm_count;
+    const int ctas = l.workers * l.cg;
     switch (a.o_type) {
-        case TUNA_FP16: return launch_mx<__half>(p, mw, ms, mx, ctas, l.smem, a.stream);
-        case TUNA_BF16: return launch_mx<__nv_bfloat16>(p, mw, ms, mx, ctas, l.smem, a.stream);
-        default: return launch_mx<float>(p, mw, ms, mx, ctas, l.smem, a.stream);
+        case TUNA_FP16: return launch_mx_as<__half>(l, p, maps, ctas, a.stream);
+        case TUNA_BF16: return launch_mx_as<__nv_bfloat16>(l, p, maps, ctas, a.stream);
+        default: return launch_mx_as<float>(l, p, maps, ctas, a.stream);
     }
 }
 
