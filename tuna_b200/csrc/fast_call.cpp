@@ -1,5 +1,6 @@
-// The argument checks and the launch of `ops.matmul` in one native call.  In Python they take 8 us of host time, more than the
-// kernel of a small layer (4096x4096 at 1 token 6.8 us), so a decode step's small GEMMs waited for the host.
+// The argument checks and the launch of `ops.matmul` and of the microscaled operators of mx.py in one native call.  In Python they take
+// 8 us of host time, more than the kernel of a small layer (4096x4096 at 1 token 6.8 us), so a decode step's small GEMMs waited
+// for the host.
 //
 // matmul(x, q, s, c, o, m, n, k) answers True when the GEMM was launched and False when anything is not as the
 // common case has it - a wrong type, device, layout or size, no workspace yet, one too small.  Nothing has been launched
@@ -7,6 +8,7 @@
 // library is the answer itself: a call of several launches may have made some of them, and is not made again.
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include "../../include/tuna_b200.h"
@@ -23,10 +25,10 @@ PyObject *g_workspaces = nullptr;  // the dict (device, stream) -> tensor that o
 // place while this one is in use.  Null where there is none.
 struct Workspace {
     PyObject *tensor = nullptr;
-    Workspace(int device, void *stream)
+    Workspace(int device, void *stream) : Workspace(g_workspaces, Py_BuildValue("(iK)", device, (unsigned long long)stream)) {}
+    Workspace(PyObject *workspaces, PyObject *key)  // takes the reference to `key`
     {
-        PyObject *key = Py_BuildValue("(iK)", device, (unsigned long long)stream);
-        PyObject *found = key ? PyDict_GetItemWithError(g_workspaces, key) : nullptr;
+        PyObject *found = key ? PyDict_GetItemWithError(workspaces, key) : nullptr;
         Py_XDECREF(key);
         if (found && THPVariable_Check(found)) tensor = Py_NewRef(found);
         PyErr_Clear();
@@ -85,6 +87,162 @@ int launch(PyObject *const *args)
     return st == TUNA_ERR_WORKSPACE ? kPythonWay : st;
 }
 
+// ---- the microscaled operators (mx.py): the same answers
+
+struct {
+    int (*quantize)(const void *x, int x_type, long long row_stride, void *q, void *s, int rows, int k, int batch, void *stream);
+    int (*dequant)(const void *q, const void *s, void *o, int o_type, int rows, int k, int batch, void *stream);
+    int (*matmul)(const void *x, int x_type, const void *xs, const void *q, const void *s, void *o, int o_type, int m, int n, int k, void *workspace,
+                  size_t workspace_bytes, void *stream);
+    int (*matmul_grouped)(const void *x, int x_type, const void *xs, const void *q, const void *s, const void *offsets, void *o, int o_type, int m, int n, int k,
+                          int experts, void *workspace, size_t workspace_bytes, void *stream);
+    unsigned long long (*capture_id)(void *stream);
+} g_mx = {};
+PyObject *g_mx_workspaces = nullptr;  // (device, stream, capture) -> tensor
+
+int type_of(at::ScalarType t) { return t == at::kHalf ? TUNA_FP16 : t == at::kBFloat16 ? TUNA_BF16 : t == at::kFloat ? TUNA_FP32 : -1; }
+
+// A size argument: positive and of 32 bits, else 0.
+long long size_of(PyObject *o)
+{
+    if (!PyLong_CheckExact(o)) return 0;
+    int overflow = 0;
+    const long long v = PyLong_AsLongLongAndOverflow(o, &overflow);
+    return overflow || v <= 0 || v > 0x7fffffff ? 0 : v;
+}
+
+// A plain contiguous tensor of one of the number types (`type` says which), else null.
+const at::Tensor *numbers(PyObject *o, int64_t numel, int device, int *type)
+{
+    if (!THPVariable_CheckExact(o)) return nullptr;
+    const at::Tensor &t = THPVariable_Unpack(o);
+    if (!t.defined()) return nullptr;
+    *type = type_of(t.scalar_type());
+    return *type < 0 ? nullptr : plain(o, t.scalar_type(), numel, device);
+}
+
+int64_t code_bytes(int64_t rows, int64_t k) { return (k + 255) / 256 * rows * 128; }
+int64_t scale_bytes(int64_t rows, int64_t k) { return (k + 127) / 128 * rows * 4; }
+
+// x, xs, q, s, [offsets,] o, m, n, k
+int launch_mx_product(PyObject *const *args, bool grouped)
+{
+    PyObject *const *tail = args + (grouped ? 5 : 4);
+    const long long m = size_of(tail[1]), n = size_of(tail[2]), k = size_of(tail[3]);
+    if (!m || !n || !k) return kPythonWay;
+    int x_type = TUNA_MXFP4, o_type;
+    const bool packed = args[1] != Py_None;
+    const at::Tensor *x = packed ? plain(args[0], at::kByte, code_bytes(n, k), -1) : numbers(args[0], n * k, -1, &x_type);
+    if (!x) return kPythonWay;
+    const int device = x->get_device();
+    const at::Tensor *xs = packed ? plain(args[1], at::kByte, scale_bytes(n, k), device) : nullptr;
+    if ((packed && !xs) || x_type == TUNA_FP32 || device != c10::cuda::current_device()) return kPythonWay;
+    long long experts = 1;
+    const at::Tensor *offsets = nullptr;
+    if (grouped) {
+        if (!THPVariable_CheckExact(args[2])) return kPythonWay;
+        const at::Tensor &q = THPVariable_Unpack(args[2]);
+        if (!q.defined() || q.dim() != 4 || q.size(0) < 1 || q.size(0) > TUNA_MX_MAX_EXPERTS) return kPythonWay;
+        experts = q.size(0);
+        offsets = plain(args[4], at::kInt, experts + 1, device);
+        if (!offsets) return kPythonWay;
+    }
+    const at::Tensor *q = plain(args[2], at::kByte, experts * code_bytes(m, k), device), *s = plain(args[3], at::kByte, experts * scale_bytes(m, k), device),
+                     *o = numbers(tail[0], n * m, device, &o_type);
+    if (!q || !s || !o) return kPythonWay;
+    void *stream = c10::cuda::getCurrentCUDAStream(device).stream();
+    const Workspace ws(g_mx_workspaces, Py_BuildValue("(iKK)", device, (unsigned long long)stream, g_mx.capture_id(stream)));
+    if (!ws.tensor) return kPythonWay;
+    const void *xp = x->const_data_ptr(), *xsp = xs ? xs->const_data_ptr() : nullptr, *qp = q->const_data_ptr(), *sp = s->const_data_ptr(),
+               *fp = offsets ? offsets->const_data_ptr() : nullptr;
+    void *op = o->mutable_data_ptr(), *wp = ws.ptr();
+    const size_t bytes = ws.bytes();
+    const auto f = g_mx;
+    const Unlocked unlocked;
+    const int st = grouped ? f.matmul_grouped(xp, x_type, xsp, qp, sp, fp, op, o_type, (int)m, (int)n, (int)k, (int)experts, wp, bytes, stream)
+                           : f.matmul(xp, x_type, xsp, qp, sp, op, o_type, (int)m, (int)n, (int)k, wp, bytes, stream);
+    return st == TUNA_ERR_WORKSPACE ? kPythonWay : st;
+}
+
+// q, s, o, m, k
+int launch_mx_dequant(PyObject *const *args)
+{
+    const long long m = size_of(args[3]), k = size_of(args[4]);
+    int o_type;
+    if (!m || !k || !THPVariable_CheckExact(args[0])) return kPythonWay;
+    const at::Tensor &t = THPVariable_Unpack(args[0]);
+    if (!t.defined() || t.dim() != 3) return kPythonWay;  // one matrix
+    const at::Tensor *q = plain(args[0], at::kByte, code_bytes(m, k), -1);
+    if (!q) return kPythonWay;
+    const int device = q->get_device();
+    const at::Tensor *s = plain(args[1], at::kByte, scale_bytes(m, k), device), *o = numbers(args[2], m * k, device, &o_type);
+    if (!s || !o || device != c10::cuda::current_device()) return kPythonWay;
+    void *stream = c10::cuda::getCurrentCUDAStream(device).stream();
+    const void *qp = q->const_data_ptr(), *sp = s->const_data_ptr();
+    void *op = o->mutable_data_ptr();
+    const auto f = g_mx.dequant;
+    const Unlocked unlocked;
+    return f(qp, sp, op, o_type, (int)m, (int)k, 1, stream);
+}
+
+// x [rows, k] -> (q, s) in `out`; a status
+int launch_mx_quantize(PyObject *x, at::Tensor (&out)[2])
+{
+    if (!THPVariable_CheckExact(x)) return kPythonWay;
+    const at::Tensor &t = THPVariable_Unpack(x);
+    if (!t.defined() || t.dim() != 2 || t.numel() == 0) return kPythonWay;
+    const int64_t rows = t.size(0), k = t.size(1);
+    int type;
+    if (!numbers(x, t.numel(), -1, &type) || rows > 0x7fffffff || k > 0x7fffffff || k % 32 || t.get_device() != c10::cuda::current_device()) return kPythonWay;
+    void *stream = c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
+    const auto bytes = t.options().dtype(at::kByte).requires_grad(false);
+    out[0] = at::empty({(k + 255) / 256, rows, 128}, bytes);
+    out[1] = at::empty({(k + 127) / 128, rows, 4}, bytes);
+    const void *xp = t.const_data_ptr();
+    void *qp = out[0].mutable_data_ptr(), *sp = out[1].mutable_data_ptr();
+    const auto f = g_mx.quantize;
+    const Unlocked unlocked;
+    return f(xp, type, k, qp, sp, (int)rows, (int)k, 1, stream);
+}
+
+PyObject *answer(int st) { return st == TUNA_OK || st == kPythonWay ? PyBool_FromLong(st == TUNA_OK) : PyLong_FromLong(st); }
+
+template <int NARGS, typename Launch>
+PyObject *guarded(Py_ssize_t nargs, Launch launch)
+{
+    int st = kPythonWay;
+    try {
+        if (nargs == NARGS && g_mx.matmul) st = launch();
+    } catch (...) {
+    }
+    return answer(st);
+}
+PyObject *fast_mx_matmul(PyObject *, PyObject *const *args, Py_ssize_t nargs) { return guarded<8>(nargs, [&] { return launch_mx_product(args, false); }); }
+PyObject *fast_mx_matmul_grouped(PyObject *, PyObject *const *args, Py_ssize_t nargs) { return guarded<9>(nargs, [&] { return launch_mx_product(args, true); }); }
+PyObject *fast_mx_dequant(PyObject *, PyObject *const *args, Py_ssize_t nargs) { return guarded<5>(nargs, [&] { return launch_mx_dequant(args); }); }
+
+// The pair of tensors, or the answers of the others
+PyObject *fast_mx_quantize(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    at::Tensor out[2];
+    PyObject *st = guarded<1>(nargs, [&] { return launch_mx_quantize(args[0], out); });
+    if (st != Py_True) return st;
+    Py_DECREF(st);
+    PyObject *q = THPVariable_Wrap(out[0]), *s = THPVariable_Wrap(out[1]);
+    return q && s ? Py_BuildValue("(NN)", q, s) : nullptr;
+}
+
+// bind_mx(addresses of the five functions, dict of the workspaces)
+PyObject *bind_mx(PyObject *, PyObject *args)
+{
+    unsigned long long f[5];
+    PyObject *workspaces;
+    if (!PyArg_ParseTuple(args, "KKKKKO!", &f[0], &f[1], &f[2], &f[3], &f[4], &PyDict_Type, &workspaces)) return nullptr;
+    g_mx = {(decltype(g_mx.quantize))f[0], (decltype(g_mx.dequant))f[1], (decltype(g_mx.matmul))f[2], (decltype(g_mx.matmul_grouped))f[3], (decltype(g_mx.capture_id))f[4]};
+    Py_XSETREF(g_mx_workspaces, Py_NewRef(workspaces));
+    Py_RETURN_NONE;
+}
+
 PyObject *fast_matmul(PyObject *, PyObject *const *args, Py_ssize_t nargs)
 {
     int st = kPythonWay;
@@ -92,7 +250,7 @@ PyObject *fast_matmul(PyObject *, PyObject *const *args, Py_ssize_t nargs)
         if (nargs == 8 && g_matmul) st = launch(args);
     } catch (...) {  // a tensor without storage of its own (vmap, a trace): the Python way says what is wrong
     }
-    return st == TUNA_OK || st == kPythonWay ? PyBool_FromLong(st == TUNA_OK) : PyLong_FromLong(st);
+    return answer(st);
 }
 
 // workspace(device, stream) -> (address, bytes) of the one that a launch there uses, or None
@@ -120,6 +278,11 @@ PyObject *bind(PyObject *, PyObject *args)
 
 PyMethodDef methods[] = {
     {"matmul", (PyCFunction)(void (*)(void))fast_matmul, METH_FASTCALL, nullptr},
+    {"mx_quantize", (PyCFunction)(void (*)(void))fast_mx_quantize, METH_FASTCALL, nullptr},
+    {"mx_dequant", (PyCFunction)(void (*)(void))fast_mx_dequant, METH_FASTCALL, nullptr},
+    {"mx_matmul", (PyCFunction)(void (*)(void))fast_mx_matmul, METH_FASTCALL, nullptr},
+    {"mx_matmul_grouped", (PyCFunction)(void (*)(void))fast_mx_matmul_grouped, METH_FASTCALL, nullptr},
+    {"bind_mx", bind_mx, METH_VARARGS, nullptr},
     {"workspace", workspace, METH_VARARGS, nullptr},
     {"bind", bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -107,7 +107,8 @@ struct MxGemmArgs {
     int sm_count;
 };
 constexpr size_t kMxCounterBytes = 4096;
-cudaError_t launch_mx_quantize(const void *x, int type, long long row_stride, void *q, void *s, int rows, int k, int batch, cudaStream_t stream);
+// chained: right before the product that reads q and s
+cudaError_t launch_mx_quantize(const void *x, int type, long long row_stride, void *q, void *s, int rows, int k, int batch, cudaStream_t stream, bool chained = false);
 cudaError_t launch_mx_dequant(const void *q, const void *s, void *o, int type, int rows, int k, int batch, cudaStream_t stream);
 int launch_mx_gemm(const MxGemmArgs &a);
 bool mx_gemm_takes(int m, int n, int k, int experts, int x_type, bool grouped, int sm_count);

@@ -54,7 +54,7 @@ static int mx_product(const void *x, int x_type, const void *xs, const void *q, 
         a.x_type = TUNA_MXFP4;
         a.x = (uint8_t *)workspace + w.codes;
         a.xs = (uint8_t *)workspace + w.scales;
-        if (launch_mx_quantize(x, x_type, k, (uint8_t *)workspace + w.codes, (uint8_t *)workspace + w.scales, n, k, 1, a.stream) != cudaSuccess) return TUNA_ERR_LAUNCH;
+        if (launch_mx_quantize(x, x_type, k, (uint8_t *)workspace + w.codes, (uint8_t *)workspace + w.scales, n, k, 1, a.stream, true) != cudaSuccess) return TUNA_ERR_LAUNCH;
     }
     return launch_mx_gemm(a);
 }
@@ -110,6 +110,9 @@ extern "C" unsigned long long tuna_stream_capture_id(void *stream)
 {
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
     unsigned long long id = 0;
-    if (cudaStreamGetCaptureInfo((cudaStream_t)stream, &status, &id) != cudaSuccess || status != cudaStreamCaptureStatusActive) return 0;
-    return id;
+    if (cudaStreamGetCaptureInfo((cudaStream_t)stream, &status, &id) != cudaSuccess) {
+        cudaGetLastError();  // the legacy stream beside a capture elsewhere: an answer, not a failure
+        return 0;
+    }
+    return status == cudaStreamCaptureStatusActive ? id : 0;
 }

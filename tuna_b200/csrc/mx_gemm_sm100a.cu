@@ -45,8 +45,9 @@ constexpr int kMxWarps = 12;
 constexpr int kMxEpilogueWarp0 = 4;
 constexpr int kMxScaleWarp0 = 8;
 constexpr int kMxMaxStages = 12;
-constexpr int kMxStageTokens = 32;      // tokens of an output staging buffer
+__host__ __device__ constexpr int mx_stage_tokens(int token_words) { return token_words == 1 ? 32 : 64; }  // of an output staging buffer
 constexpr int kMxDirectTokens = 16;     // tiles of up to so many tokens are stored from registers
+constexpr uint32_t kMxFoldBytes = kMxDirectTokens * kBlockRows * 4;  // where the parts of a folded tile are added up
 constexpr int kMxAheadTokens = 64;      // one matrix: up to here weights are read ahead of the dependency wait
 constexpr uint32_t kMxScaleBytes = 2 * kBlockRows * 4;  // of the weights' scales in a stage
 constexpr int kMxSmemMax = 227 * 1024;  // of a CTA alone on its SM, static part included
@@ -62,6 +63,8 @@ struct MxParams {
     int experts;
     int tile_tok;   // N
     int chunks;     // ceil(k / 256)
+    int units;      // stages of a tile: ceil(chunks / fold)
+    int fold_log;   // log2(fold): chunks side by side in a stage
     int words;      // ceil(k / 128)
     int row_tiles;
     int w_bytes;    // of the weights in a stage
@@ -73,7 +76,10 @@ struct MxParams {
     int cut;        // tiles may be cut along K
     int last_steps; // MMAs of the last chunk: 64 columns each
     int stages;
-    int nd;         // accumulator buffers
+    int nd;         // accumulators that are free of one another
+    int d_cols;     // tensor-memory columns of an accumulator: tokens of a tile times fold
+    int d_step;     // where the second one starts; nd = 1: 0, or where it overlaps the first
+    int sf_col;     // where the scales start
     int ahead;      // weights are taken from before the dependency wait
 };
 
@@ -99,7 +105,7 @@ __device__ __forceinline__ MxSplit mx_split(int tiles, int chunks, int workers, 
 
 // The segments of a worker in order, and where each lies.
 struct MxSegs {
-    int u, u_end, dp, dp_step, tiles, chunks, row_tiles, tile_tok;
+    int u, u_end, dp, dp_step, tiles, chunks, row_tiles, tile_tok;  // chunks: a tile's stages
     const int *first_tile, *begin, *count;  // per expert (shared memory)
     int e;
     int tile, c0, c1;     // the segment
@@ -112,7 +118,7 @@ struct MxSegs {
         dp = s.sk_tiles + worker;
         dp_step = workers;
         tiles = s.tiles;
-        chunks = p.chunks;
+        chunks = p.units;
         row_tiles = p.row_tiles;
         tile_tok = p.tile_tok;
         begin = tables;
@@ -195,6 +201,15 @@ template <> __device__ __forceinline__ __half mx_convert<__half>(float v) { retu
 template <> __device__ __forceinline__ __nv_bfloat16 mx_convert<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ float mx_convert<float>(float v) { return v; }
 
+template <typename T>
+__device__ __forceinline__ uint32_t mx_pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t mx_pack2<__half>(float lo, float hi) { return pack_half2(lo, hi); }
+template <> __device__ __forceinline__ uint32_t mx_pack2<__nv_bfloat16>(float lo, float hi)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
 __device__ __forceinline__ void mx_store_shared(uint32_t a, __half v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(__half_as_ushort(v)) : "memory"); }
 __device__ __forceinline__ void mx_store_shared(uint32_t a, __nv_bfloat16 v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(__bfloat16_as_ushort(v)) : "memory"); }
 __device__ __forceinline__ void mx_store_shared(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
@@ -207,17 +222,20 @@ __host__ __device__ constexpr uint32_t mx_scale_cols(int token_words) { return 8
 // First row of row block b (a CTA's share of a tile).
 __device__ __forceinline__ int mx_row(const MxParams &p, int b) { return p.flex ? 8 * (int)((long long)b * p.groups / p.row_tiles) : b * kBlockRows; }
 
-// Four bytes of global memory; the barrier counts the thread's copies in when they have landed.
-__device__ __forceinline__ void cp_async_word(uint32_t dst, const uint32_t *src) { asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory"); }
+// Four bytes of global memory, or zeros; the barrier counts the thread's copies in when they have landed.
+__device__ __forceinline__ void cp_async_word(uint32_t dst, const uint32_t *src, bool have)
+{
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(have ? 4 : 0) : "memory");
+}
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
 
 // Quantizes the tokens' numbers, all of K: warp `w` of `warps` takes every warps-th (chunk, token).  Codes as TMA would have put
-// them (128-byte swizzle), scale words [chunk][half][32 tokens].
+// them (128-byte swizzle), scale words [stage][half][token of a chunk of the stage].
 template <typename T>
-__device__ __forceinline__ void mx_quantize_resident(const MxParams &p, int w, int warps, int lane, uint32_t codes_at, uint32_t x_bytes, uint32_t words_at)
+__device__ __forceinline__ void mx_quantize_resident(const MxParams &p, int w, int warps, int lane, uint32_t codes_at, uint32_t words_at)
 {
     constexpr int R = 4;  // loads in flight
-    const int items = p.chunks * p.n;
+    const int items = (p.units << p.fold_log) * p.n;  // chunks behind the last one are zeros
     for (int i0 = w; i0 < items; i0 += R * warps) {
         Mx8<T> v[R];
 #pragma unroll
@@ -238,13 +256,14 @@ __device__ __forceinline__ void mx_quantize_resident(const MxParams &p, int w, i
             for (int k = 0; k < 8; ++k) f[k] *= inverse;
             const uint32_t codes = e == 255u ? 0u : mx_encode8(f);
             // 16-byte piece lane / 4 of the token's 128 bytes, XORed with the token's number mod 8
-            asm volatile("st.shared.u32 [%0], %1;" ::"r"(codes_at + (uint32_t)c * x_bytes + (uint32_t)t * kMxChunkBytes + ((((uint32_t)lane >> 2) ^ ((uint32_t)t & 7u)) << 4) + ((uint32_t)lane & 3u) * 4u),
+            asm volatile("st.shared.u32 [%0], %1;" ::"r"(codes_at + ((uint32_t)c * p.x_rows + (uint32_t)t) * kMxChunkBytes + ((((uint32_t)lane >> 2) ^ ((uint32_t)t & 7u)) << 4) + ((uint32_t)lane & 3u) * 4u),
                          "r"(codes)
                          : "memory");
+            const int unit = c >> p.fold_log, at = (c - (unit << p.fold_log)) * p.x_rows + t;
             e <<= 8 * ((lane >> 2) & 3);  // four neighbouring blocks make a word
             e |= __shfl_xor_sync(0xffffffffu, e, 4);
             e |= __shfl_xor_sync(0xffffffffu, e, 8);
-            if ((lane & 15) == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(words_at + (uint32_t)c * 256u + (uint32_t)(lane >> 4) * 128u + (uint32_t)t * 4u), "r"(e) : "memory");
+            if ((lane & 15) == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(words_at + (uint32_t)unit * 256u + (uint32_t)(lane >> 4) * 128u + (uint32_t)at * 4u), "r"(e) : "memory");
         }
     }
 }
@@ -268,14 +287,15 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
     const int N = p.tile_tok, S = p.stages;
     // [stages of weights][of tokens][of the weights' scales][of the tokens' scales][staging buffers][tables]; the MMAs read 128
-    // rows, in low tiles past their stage's end.  RESIDENT: of tokens, as many as there are chunks.
-    const int x_stages = RESIDENT ? p.chunks : S;
-    const uint32_t base = smem_u32(smem), w_bytes = (uint32_t)p.w_bytes, x_bytes = (uint32_t)p.x_rows * kMxChunkBytes;
+    // rows, in low tiles past their stage's end.  RESIDENT: of tokens, all of a tile's stages.
+    const int x_stages = RESIDENT ? p.units : S;
+    const uint32_t base = smem_u32(smem), w_bytes = (uint32_t)p.w_bytes, x_bytes = (uint32_t)(p.x_rows << p.fold_log) * kMxChunkBytes;
     const uint32_t x_ring = base + (uint32_t)S * w_bytes, ws_ring = x_ring + (uint32_t)x_stages * x_bytes, xs_ring = ws_ring + (uint32_t)S * kMxScaleBytes;
     const uint32_t staging = xs_ring + (uint32_t)x_stages * (256u * NW);
-    constexpr uint32_t kTokBytes = kBlockRows * (uint32_t)sizeof(OT);
-    constexpr uint32_t kStagingBytes = kMxStageTokens * kTokBytes;
-    int *tables = reinterpret_cast<int *>(smem + (staging - base) + (N > kMxDirectTokens ? 2 * kStagingBytes : 0));
+    constexpr int kStageTokens = mx_stage_tokens(NW);
+    constexpr uint32_t kTokPitch = kBlockRows * (uint32_t)sizeof(OT) + (sizeof(OT) == 2 ? 16 : 0);  // 16-bit results: 16 bytes more, so that a column of 8 tokens meets all banks
+    constexpr uint32_t kStagingBytes = kStageTokens * kTokPitch;
+    int *tables = reinterpret_cast<int *>(smem + (staging - base) + (N > kMxDirectTokens ? 2 * kStagingBytes : p.fold_log ? kMxFoldBytes : 0));
 
     // landed: a stage's copies; full: its scales are written as well; empty: its MMAs are done
     const uint32_t landed = smem_u32(&bars[0]), full = landed + 8 * kMxMaxStages, empty = full + 8 * kMxMaxStages, d_full = empty + 8 * kMxMaxStages, d_empty = d_full + 16;
@@ -337,7 +357,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
         }
         if (lane == 0) {
             tables[3 * p.experts] = before;
-            s_split = mx_split(before, p.chunks, workers, p.cut);
+            s_split = mx_split(before, p.units, workers, p.cut);
         }
     }
     tc_fence_before();
@@ -345,7 +365,8 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     if (CG == 2) cluster_sync_all();  // the other CTA's barriers are there
     tc_fence_after();
     const uint32_t tmem = s_tmem_base;
-    const uint32_t sf_col = (uint32_t)(p.nd * N);
+    const uint32_t sf_col = (uint32_t)p.sf_col;
+    const int fold = 1 << p.fold_log, part = kBlockRows >> p.fold_log;  // rows of a part
     constexpr uint32_t kScaleCols = mx_scale_cols(NW), kTokenCols = NW < 4 ? 4 : NW;  // of a stage, and of a half of its tokens
     MxSegs segs;
     segs.init(p, s_split, worker, workers, tables);
@@ -355,8 +376,8 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     if (RESIDENT && warp != 1) {  // the weights are on their way meanwhile
         depend();
         const int w = warp == 0 ? 0 : warp - 1;
-        if (p.x_bf16) mx_quantize_resident<__nv_bfloat16>(p, w, kMxWarps - 1, lane, x_ring, x_bytes, xs_ring);
-        else mx_quantize_resident<__half>(p, w, kMxWarps - 1, lane, x_ring, x_bytes, xs_ring);
+        if (p.x_bf16) mx_quantize_resident<__nv_bfloat16>(p, w, kMxWarps - 1, lane, x_ring, xs_ring);
+        else mx_quantize_resident<__half>(p, w, kMxWarps - 1, lane, x_ring, xs_ring);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the MMAs read the codes
         asm volatile("bar.sync 2, %0;" ::"n"(32 * (kMxWarps - 1)) : "memory");
     }
@@ -366,13 +387,15 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
             depend();
             Ring ru, rd;
             bool ok = true;
+            int second = 0;  // which accumulator
             // -------------------------------------------------------------- MMA issue
             constexpr uint64_t sw128 = ((uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29))) << 32;  // 8-row groups 1024 bytes apart, version 1, 128-byte swizzle
             while (ok && segs.next()) {
-                const uint32_t idesc = mx_idesc<CG>(tile_cols(), 0);
+                const uint32_t idesc = mx_idesc<CG>(p.fold_log ? p.d_cols : tile_cols(), 0);
                 constexpr uint32_t kHalf = mx_idesc<CG>(0, 1) ^ mx_idesc<CG>(0, 0);
                 ok = mbar_wait_warp(d_empty + 8 * rd.idx, rd.phase ^ 1, abort_flag, p.status, 203);
-                const uint32_t d = tmem + (uint32_t)(rd.idx * N);
+                const uint32_t d = tmem + (uint32_t)(second * p.d_step);
+                second ^= 1;
                 for (int c = segs.c0; ok && c < segs.c1; ++c) {
                     ok = mbar_wait_warp(full + 8 * ru.idx, ru.phase, abort_flag, p.status, 204);
                     if (!ok) break;
@@ -381,7 +404,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                         const uint64_t a = sw128 | (uint64_t)(((base + (uint32_t)ru.idx * w_bytes) & 0x3FFFFu) >> 4);
                         const uint64_t b = sw128 | (uint64_t)(((x_ring + (uint32_t)(RESIDENT ? c : ru.idx) * x_bytes) & 0x3FFFFu) >> 4);
                         const uint32_t sfa = tmem + sf_col + (uint32_t)ru.idx * kScaleCols, sfb = sfa + 8;
-                        const int steps = c + 1 == p.chunks ? p.last_steps : 4;
+                        const int steps = c + 1 == p.units && !p.fold_log ? p.last_steps : 4;
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
                             if (kk < steps)
@@ -409,16 +432,19 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
         if (!p.ahead) depend();
         while (ok && segs.next()) {
             const int block = CG * segs.rt + rank, row = mx_row(p, block), rows = mx_row(p, block + 1) - row;
-            const CUtensorMap *map = !p.flex || rows * kMxChunkBytes == p.w_bytes ? &tmap_w : &tmap_w2;  // boxes of the taller and of the lower tiles
+            const CUtensorMap *map = !p.flex || rows == 8 * div_up(p.groups, p.row_tiles) ? &tmap_w : &tmap_w2;  // boxes of the taller and of the lower tiles
             for (int c = segs.c0; c < segs.c1; ++c, ru.advance(S)) {
                 if (issued++ == S) depend();
                 ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 200);
                 if (!ok) break;
                 if (elect_one_sync()) {
                     const uint32_t bar = landed + 8 * ru.idx;
-                    mbar_expect_tx(bar, (uint32_t)rows * kMxChunkBytes + kMxScaleBytes);
-                    tma_load_3d(base + (uint32_t)ru.idx * w_bytes, map, 0, row, segs.e * p.chunks + c, bar);
-                    tma_load_2d(ws_ring + (uint32_t)ru.idx * kMxScaleBytes, &tmap_ws, row, segs.e * p.words + 2 * c, bar);
+                    mbar_expect_tx(bar, (uint32_t)(rows << p.fold_log) * kMxChunkBytes + kMxScaleBytes);
+                    for (int f = 0; f < fold; ++f) {  // chunks behind the last one read as zeros
+                        const int chunk = (c << p.fold_log) + f;
+                        tma_load_3d(base + (uint32_t)ru.idx * w_bytes + (uint32_t)(f * part) * kMxChunkBytes, map, 0, row, segs.e * p.chunks + chunk, bar);
+                        tma_load_2d(ws_ring + (uint32_t)ru.idx * kMxScaleBytes + (uint32_t)(f * part) * 8u, &tmap_ws, row, segs.e * p.words + 2 * chunk, bar);
+                    }
                 }
                 __syncwarp();
             }
@@ -439,7 +465,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                 if (!ok) break;
                 if (elect_one_sync()) {
                     mbar_expect_tx(landed + 8 * ru.idx, x_bytes);
-                    tma_load_3d(x_ring + (uint32_t)ru.idx * x_bytes, &tmap_x, 0, tok, c, landed + 8 * ru.idx);
+                    tma_load_3d(x_ring + (uint32_t)ru.idx * x_bytes, &tmap_x, 0, tok, c << p.fold_log, landed + 8 * ru.idx);
                 }
                 __syncwarp();
             }
@@ -454,12 +480,23 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                 ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 201);
                 if (!ok) break;
                 const uint32_t to = xs_ring + (uint32_t)ru.idx * (256u * NW) + 4u * lane;
-                const uint32_t *src = p.xs + (size_t)(2 * c) * p.n + segs.tok0 + lane;
+                if (NW > 1 || !p.fold_log) {
+                    const uint32_t *src = p.xs + (size_t)(2 * c) * p.n + segs.tok0 + lane;
 #pragma unroll
-                for (int j = 0; j < NW; ++j) {
-                    if (32 * j + lane >= segs.valid) continue;  // whatever lies there scales columns that nobody reads
-                    cp_async_word(to + 128u * j, src + 32 * j);
-                    if (2 * c + 1 < p.words) cp_async_word(to + 128u * (NW + j), src + p.n + 32 * j);
+                    for (int j = 0; j < NW; ++j) {
+                        if (32 * j + lane >= segs.valid) continue;  // whatever lies there scales columns that nobody reads
+                        cp_async_word(to + 128u * j, src + 32 * j, true);
+                        if (2 * c + 1 < p.words) cp_async_word(to + 128u * (NW + j), src + p.n + 32 * j, true);
+                    }
+                } else {  // token t of the stage's chunk f: zeros behind the last word, where the codes are zeros too
+                    const int f = lane / p.x_rows, t = lane - f * p.x_rows;
+                    if (f < fold && t < segs.valid) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int word = 2 * ((c << p.fold_log) + f) + h;
+                            cp_async_word(to + 128u * h, p.xs + (size_t)min(word, p.words - 1) * p.n + segs.tok0 + t, word < p.words);
+                        }
+                    }
                 }
                 cp_async_arrive(landed + 8 * ru.idx);
             }
@@ -484,8 +521,12 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                 if (!ok) break;
                 tc_fence_after();
                 const uint32_t to = lanes + (uint32_t)ru.idx * kScaleCols, x_at = xs_ring + (uint32_t)(RESIDENT ? c : ru.idx) * (256u * NW);
-                uint32_t w[8];
-                words(w, ws_ring + (uint32_t)ru.idx * kMxScaleBytes);
+                uint32_t w[8];  // of half i / 4: MMA row 32 (i % 4) + lane is row `of` of part f
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int row = 32 * (i & 3) + lane, f = row >> (7 - p.fold_log), of = row & (part - 1);
+                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(ws_ring + (uint32_t)ru.idx * kMxScaleBytes + (uint32_t)((2 * f + (i >> 2)) * part + of) * 4u));
+                }
                 if constexpr (NW == 1) {
                     uint32_t x0[1], x1[1];
                     words(x0, x_at);
@@ -517,41 +558,56 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
         Ring rd;
         uint32_t buf = 0;
         depend();
-        // Rows of `valid` tokens, 16 at a time from `get`, to memory: from registers, or through the staging buffers.
-        auto store_tile = [&](auto get) {
-            const int row0 = mx_row(p, CG * segs.rt + rank), rows = min(mx_row(p, CG * segs.rt + rank + 1), p.m) - row0;
-            if (N <= kMxDirectTokens) {
-                float v[16];
-                get(0, v);
-                OT *to = o + (size_t)segs.tok0 * p.m + row0 + thread;
-                if (thread < rows) {
+        int row0 = 0, rows = 0;
+        // Up to 16 tokens of this thread's row, from registers.
+        auto store_direct = [&](const float (&v)[16]) {
+            OT *to = o + (size_t)segs.tok0 * p.m + row0 + thread;
+            if (thread < rows) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (i < segs.valid) to[(size_t)i * p.m] = mx_convert<OT>(v[i]);
-                }
-                return;
+                for (int i = 0; i < 16; ++i)
+                    if (i < segs.valid) to[(size_t)i * p.m] = mx_convert<OT>(v[i]);
             }
-            for (int t0 = 0; t0 < segs.valid; t0 += kMxStageTokens, buf ^= 1) {
-                const uint32_t to = staging + buf * kStagingBytes;
-                if (lane < 8) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the buffer's previous tokens have left it
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+        };
+        // Tokens t0 .. t0 + 63 through a staging buffer: fill(t, at) puts 32 tokens from t on to `at`; one bulk copy per token.
+        auto store_block = [&](int t0, auto fill) {
+            const uint32_t to = staging + buf * kStagingBytes;
+            buf ^= 1;
+            if (lane < kStageTokens / 4) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the buffer's previous tokens have left it
+            asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll
-                for (int h = 0; h < kMxStageTokens; h += 16) {
-                    if (t0 + h >= segs.valid) break;
+            for (int h = 0; h < kStageTokens; h += 32)
+                if (t0 + h < segs.valid) fill(t0 + h, to + h * kTokPitch);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (lane < kStageTokens / 4) {
+                const int t = kStageTokens / 4 * quarter + lane;
+                if (t0 + t < segs.valid && rows > 0)
+                    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(o + (size_t)(segs.tok0 + t0 + t) * p.m + row0),
+                                 "r"(to + (uint32_t)t * kTokPitch), "r"((uint32_t)rows * (uint32_t)sizeof(OT))
+                                 : "memory");
+                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+        };
+        // 32 tokens of the accumulator at `d`, columns from t on.
+        auto fill_from = [&](uint32_t d, int t, uint32_t at) {
+            if constexpr (sizeof(OT) == 2) {
+                // Fragments of 8 rows x 8 tokens, packed, are written transposed (stmatrix): 16 bytes = 8 rows of one token.
+                uint32_t lo[16], hi[16];
+                tc_ld_16x256b_x4(d + t, lo);
+                tc_ld_16x256b_x4(d + (16u << 16) + t, hi);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                const uint32_t to = at + (uint32_t)(lane & 7) * kTokPitch + (uint32_t)(4 * quarter + (lane >> 3)) * 16u;
+                auto pack = [](uint32_t a, uint32_t b) { return mx_pack2<OT>(__uint_as_float(a), __uint_as_float(b)); };
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    stmatrix_x4_trans(to + 8u * i * kTokPitch, pack(lo[4 * i], lo[4 * i + 1]), pack(lo[4 * i + 2], lo[4 * i + 3]), pack(hi[4 * i], hi[4 * i + 1]), pack(hi[4 * i + 2], hi[4 * i + 3]));
+            } else {
+#pragma unroll
+                for (int h = 0; h < 32; h += 16) {
                     float v[16];
-                    get(t0 + h, v);
+                    tc_ld_x16(d + t + h, v);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) mx_store_shared(to + (uint32_t)(h + i) * kTokBytes + (uint32_t)thread * (uint32_t)sizeof(OT), mx_convert<OT>(v[i]));
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                if (lane < 8) {
-                    const int t = 8 * quarter + lane;
-                    if (t0 + t < segs.valid && rows > 0)
-                        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(o + (size_t)(segs.tok0 + t0 + t) * p.m + row0),
-                                     "r"(to + (uint32_t)t * kTokBytes), "r"((uint32_t)rows * (uint32_t)sizeof(OT))
-                                     : "memory");
-                    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+                    for (int i = 0; i < 16; ++i) asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + (uint32_t)(h + i) * kTokPitch + (uint32_t)thread * 4u), "f"(v[i]) : "memory");
                 }
             }
         };
@@ -564,14 +620,49 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                 else mbar_arrive_cluster(leader_d_empty + 8 * rd.idx);
             }
         };
-        while (segs.next()) {
+        int second = 0;
+        for (; segs.next(); second ^= 1) {
             const bool ok = mbar_wait_warp(d_full + 8 * rd.idx, rd.phase, abort_flag, p.status, 206);
             if (bar_any(1, 128, !ok)) break;  // the four warps go on together or not at all
             tc_fence_after();
-            const uint32_t d = tmem_q + (uint32_t)(rd.idx * N);
-            if (segs.c0 == 0 && segs.c1 == p.chunks) {
-                store_tile([&](int t, float (&v)[16]) { tc_ld_x16(d + t, v); });
+            const uint32_t d = tmem_q + (uint32_t)(second * p.d_step);
+            row0 = mx_row(p, CG * segs.rt + rank);
+            rows = min(mx_row(p, CG * segs.rt + rank + 1), p.m) - row0;
+            if (p.fold_log) {
+                // Part f's sums of row i are lane part * f + i, columns x_rows * f ..: added up in the order of the parts.
+                const int f = thread >> (7 - p.fold_log);
+                float v[16];
+                tc_ld_x16(d + f * p.x_rows, v);
                 drained();
+                float *sums = reinterpret_cast<float *>(smem + (staging - base));
+#pragma unroll
+                for (int t = 0; t < 16; ++t)
+                    if (t < segs.valid) sums[t * kBlockRows + thread] = v[t];
+                asm volatile("bar.sync 1, 128;" ::: "memory");
+                const int i = thread & (part - 1);
+                for (int t = f; t < segs.valid && i < rows; t += fold) {
+                    float sum = sums[t * kBlockRows + i];
+                    for (int g = 1; g < fold; ++g) sum += sums[t * kBlockRows + g * part + i];
+                    o[(size_t)(segs.tok0 + t) * p.m + row0 + i] = mx_convert<OT>(sum);
+                }
+                asm volatile("bar.sync 1, 128;" ::: "memory");  // they have been read
+            } else if (segs.c0 == 0 && segs.c1 == p.units) {
+                if (N <= kMxDirectTokens) {
+                    float v[16];
+                    tc_ld_x16(d, v);
+                    drained();
+                    store_direct(v);
+                } else {
+                    // Of two accumulators that overlap, the columns they share first: then the other one may be written.
+                    const bool shared = p.nd == 1 && p.d_step;
+                    const int turn = shared && second == 0 ? p.d_step : 0;
+                    for (int b = 0; b < N; b += kStageTokens) {
+                        const int t0 = b + turn < N ? b + turn : b + turn - N;
+                        if (t0 < segs.valid) store_block(t0, [&](int t, uint32_t at) { fill_from(d, t, at); });
+                        if (shared && b + kStageTokens == N - p.d_step) drained();
+                    }
+                    if (!shared) drained();
+                }
             } else {
                 // [4-token group][128 lanes] float4: a warp store is 512 contiguous bytes
                 float4 *dst = reinterpret_cast<float4 *>(p.partials + (size_t)(2 * blockIdx.x + (segs.c0 == 0 ? 1 : 0)) * slot_floats) + thread;
@@ -586,7 +677,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                     const int big = s_split.sk_r * (s_split.sk_q + 1);
                     return unit < big ? unit / (s_split.sk_q + 1) : s_split.sk_r + (unit - big) / s_split.sk_q;
                 };
-                const int first = worker_of(segs.tile * p.chunks), nseg = worker_of((segs.tile + 1) * p.chunks - 1) - first + 1;
+                const int first = worker_of(segs.tile * p.units), nseg = worker_of((segs.tile + 1) * p.units - 1) - first + 1;
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (thread == 0) {
                     unsigned int old;
@@ -597,7 +688,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                 }
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (s_last) {
-                    store_tile([&](int t, float (&v)[16]) {
+                    auto sum16 = [&](int t, float (&v)[16]) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) v[i] = 0.f;
                         for (int s = 0; s < nseg; ++s) {
@@ -608,13 +699,28 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                                 v[4 * i] += w.x; v[4 * i + 1] += w.y; v[4 * i + 2] += w.z; v[4 * i + 3] += w.w;
                             }
                         }
-                    });
+                    };
+                    if (N <= kMxDirectTokens) {
+                        float v[16];
+                        sum16(0, v);
+                        store_direct(v);
+                    } else {
+                        for (int t0 = 0; t0 < segs.valid; t0 += kStageTokens)
+                            store_block(t0, [&](int t, uint32_t at) {
+                                for (int h = 0; h < 32 && t + h < segs.valid; h += 16) {
+                                    float v[16];
+                                    sum16(t + h, v);
+#pragma unroll
+                                    for (int i = 0; i < 16; ++i) mx_store_shared(at + (uint32_t)(h + i) * kTokPitch + (uint32_t)thread * (uint32_t)sizeof(OT), mx_convert<OT>(v[i]));
+                                }
+                            });
+                    }
                 }
                 asm volatile("bar.sync 1, 128;" ::: "memory");  // s_last has been read
             }
             rd.advance(p.nd);
         }
-        if (lane < 8) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        if (lane < kStageTokens / 4) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 
     __syncwarp();
@@ -631,9 +737,9 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
 // ------------------------------------------------------------------ host side
 
 struct MxPlan {
-    int cg, tile_tok, stages, nd;
+    int cg, tile_tok, stages, nd, d_cols, d_step, sf_col;
     bool resident;
-    int flex, row_tiles, cut, w_bytes, x_rows;
+    int flex, fold_log, row_tiles, cut, w_bytes, x_rows;
     int workers;
     size_t smem;
 };
@@ -642,36 +748,40 @@ static MxPlan mx_plan(int m, int n, int k, int experts, int x_type, int o_type, 
 {
     MxPlan l = {};
     const int each = div_up(n, experts), chunks = div_up(k, kMxChunk);
-    (void)chunks;
     l.cg = each > 128 ? 2 : 1;
     l.tile_tok = std::min(l.cg == 2 ? 256 : 128, div_up(each, 16) * 16);
     if (grouped) l.tile_tok = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : each <= 128 ? 128 : 256;
-    l.cut = 1;
     if (!grouped && l.cg == 1) l.flex = 1;
-    int rt = 0;
-    if (const char *env = getenv("MXPLAN")) {  // cg,N,flex[,row tiles]
-        sscanf(env, "%d,%d,%d,%d", &l.cg, &l.tile_tok, &l.flex, &rt);
+    int rt = 0, fl = -1;
+    if (const char *env = getenv("MXPLAN")) {  // cg,N,flex[,row tiles,fold]
+        sscanf(env, "%d,%d,%d,%d,%d", &l.cg, &l.tile_tok, &l.flex, &rt, &fl);
         if (l.cg == 2) l.flex = 0;
     }
+    l.cut = l.cg == 1;
     l.row_tiles = div_up(m, kBlockRows * l.cg);
     l.w_bytes = kBlockRows * kMxChunkBytes;
     if (l.flex) {
         const int waves = div_up(m, kBlockRows * sm_count);
-        l.row_tiles = std::min(div_up(m, 32), waves * sm_count);
+        l.row_tiles = std::min(m / 8, waves * sm_count);
         if (rt >= div_up(m, kBlockRows) && rt <= m / 8) l.row_tiles = rt;
         l.cut = 0;
-        l.w_bytes = 8 * div_up(m / 8, l.row_tiles) * kMxChunkBytes;
+        const int height = 8 * div_up(m / 8, l.row_tiles);
+        if (n <= 16) l.fold_log = height <= 32 && n <= 8 ? 2 : height <= 64 ? 1 : 0;
+        if (fl >= 0) l.fold_log = std::min(l.fold_log, fl);
+        if (!l.fold_log) l.w_bytes = height * kMxChunkBytes;
     }
     l.workers = sm_count / l.cg;
-    const int words = mx_token_words(l.tile_tok);
+    const int words = mx_token_words(l.tile_tok), fold = 1 << l.fold_log;
     const size_t room = words == 1 ? 111 * 1024 : kMxSmemMax - 2048;
-    const size_t tail = (l.tile_tok > kMxDirectTokens ? 2 * (size_t)kMxStageTokens * kBlockRows * (o_type == TUNA_FP32 ? 4 : 2) : 0) + (3 * (size_t)experts + 1) * 4;
-    l.x_rows = l.tile_tok / l.cg;
+    const size_t pitch = kBlockRows * (o_type == TUNA_FP32 ? 4 : 2) + (o_type == TUNA_FP32 ? 0 : 16);
+    const size_t tail = (l.tile_tok > kMxDirectTokens ? 2 * mx_stage_tokens(words) * pitch : l.fold_log ? kMxFoldBytes : 0) + (3 * (size_t)experts + 1) * 4;
+    l.x_rows = l.fold_log ? div_up(n, 8) * 8 : l.tile_tok / l.cg;
+    l.d_cols = l.fold_log ? l.x_rows * fold : l.tile_tok;
     const size_t w_stage = (size_t)l.w_bytes + kMxScaleBytes;
-    size_t x_stage = (size_t)l.x_rows * kMxChunkBytes + 256 * words;
+    size_t x_stage = (size_t)l.x_rows * fold * kMxChunkBytes + 256 * words;
     // tokens' codes that stay in shared memory: what is left has to hold stages enough
-    const size_t resident = (size_t)chunks * (div_up(n, 8) * 8 * kMxChunkBytes + 256);
-    l.resident = x_type != TUNA_MXFP4 && !grouped && n <= 16 && l.flex && resident + 4 * w_stage + tail <= room && resident + 60 * 1024 <= room;
+    const size_t resident = (size_t)div_up(chunks, fold) * (div_up(n, 8) * 8 * fold * kMxChunkBytes + 256);
+    l.resident = x_type != TUNA_MXFP4 && !grouped && n <= 4 && l.flex && resident + 4 * w_stage + tail <= room && resident + 60 * 1024 <= room;
     size_t fixed = tail;
     if (l.resident) {
         l.x_rows = div_up(n, 8) * 8;
@@ -679,8 +789,16 @@ static MxPlan mx_plan(int m, int n, int k, int experts, int x_type, int o_type, 
         x_stage = 0;
     }
     l.stages = (int)std::min<size_t>(kMxMaxStages, (room - fixed) / (w_stage + x_stage));
-    const int tmem_cols = words == 1 ? 256 : 512, scales = l.stages * (int)mx_scale_cols(words);
-    l.nd = 2 * l.tile_tok + scales <= tmem_cols ? 2 : 1;
+    const int tmem_cols = words == 1 ? 256 : 512, scale_cols = (int)mx_scale_cols(words);
+    l.nd = 2 * l.d_cols + l.stages * scale_cols <= tmem_cols ? 2 : 1;
+    l.d_step = l.nd == 2 ? l.d_cols : 0;
+    // two accumulators of which the columns in the middle are shared, where two whole ones do not fit
+    if (l.nd == 1 && l.cg == 2 && l.d_cols % (2 * mx_stage_tokens(words)) == 0) {
+        l.d_step = l.d_cols / 2;
+        l.stages = std::min(l.stages, (tmem_cols - l.d_cols - l.d_step) / scale_cols);
+    }
+    l.sf_col = l.d_cols + l.d_step;
+    l.stages = std::min(l.stages, (tmem_cols - l.sf_col) / scale_cols);
     // the last stage's MMAs read 128 rows
     l.smem = std::max((size_t)l.stages * (w_stage + x_stage) + fixed, (size_t)(l.stages - 1) * l.w_bytes + kBlockRows * kMxChunkBytes);
     return l;
@@ -754,8 +872,9 @@ int launch_mx_gemm(const MxGemmArgs &a)
     p.chunks = div_up(a.k, kMxChunk);
     p.words = div_up(a.k, kMxScaleCols);
     p.last_steps = div_up(a.k - (p.chunks - 1) * kMxChunk, 64);
+    p.units = div_up(p.chunks, 1 << l.fold_log); p.fold_log = l.fold_log;
     p.row_tiles = l.row_tiles; p.w_bytes = l.w_bytes; p.x_rows = l.x_rows; p.flex = l.flex; p.groups = a.m / 8; p.cut = l.cut;
-    p.stages = l.stages; p.nd = l.nd;
+    p.stages = l.stages; p.nd = l.nd; p.d_cols = l.d_cols; p.d_step = l.d_step; p.sf_col = l.sf_col;
     p.ahead = a.offsets == nullptr && a.n <= kMxAheadTokens;
     p.counters = (unsigned int *)a.workspace;
     p.partials = (float *)((uint8_t *)a.workspace + kMxCounterBytes);
@@ -765,15 +884,15 @@ int launch_mx_gemm(const MxGemmArgs &a)
     if (tiles >= 1ll << 30 || (tiles / l.workers + 2) * p.chunks >= 1ll << 30 || (long long)a.sm_count * p.chunks >= 1ll << 30 || (long long)a.experts * p.words >= 1ll << 30) return TUNA_ERR_TOO_LARGE;
 
     MxMaps maps;
-    auto tiles_of = [](CUtensorMap *map, const void *at, uint64_t rows, uint64_t chunks, uint32_t box_rows) {  // [chunks][rows][128 bytes]
-        return make_tensor_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, at, kMxChunkBytes, rows, chunks, kMxChunkBytes, rows * kMxChunkBytes, kMxChunkBytes, box_rows, 1,
+    auto tiles_of = [](CUtensorMap *map, const void *at, uint64_t rows, uint64_t chunks, uint32_t box_rows, uint32_t box_chunks) {  // [chunks][rows][128 bytes]
+        return make_tensor_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, at, kMxChunkBytes, rows, chunks, kMxChunkBytes, rows * kMxChunkBytes, kMxChunkBytes, box_rows, box_chunks,
                                   CU_TENSOR_MAP_SWIZZLE_128B);
     };
-    if (!tiles_of(&maps.w, a.q, (uint64_t)a.m, (uint64_t)a.experts * p.chunks, (uint32_t)l.w_bytes / kMxChunkBytes)) return TUNA_ERR_NO_DEVICE;
+    if (!tiles_of(&maps.w, a.q, (uint64_t)a.m, (uint64_t)a.experts * p.chunks, l.flex ? 8u * (uint32_t)div_up(p.groups, l.row_tiles) : kBlockRows, 1)) return TUNA_ERR_NO_DEVICE;
     maps.w2 = maps.x = maps.w;
-    if (l.flex && p.groups % l.row_tiles && !tiles_of(&maps.w2, a.q, (uint64_t)a.m, (uint64_t)p.chunks, 8u * (uint32_t)(p.groups / l.row_tiles))) return TUNA_ERR_NO_DEVICE;
-    if (!l.resident && !tiles_of(&maps.x, a.x, (uint64_t)a.n, (uint64_t)p.chunks, (uint32_t)l.x_rows)) return TUNA_ERR_NO_DEVICE;
-    if (!make_tensor_map_2d(&maps.ws, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.s, (uint64_t)a.m, (uint64_t)a.experts * p.words, (uint64_t)a.m * 4, kBlockRows, 2, CU_TENSOR_MAP_SWIZZLE_NONE))
+    if (l.flex && p.groups % l.row_tiles && !tiles_of(&maps.w2, a.q, (uint64_t)a.m, (uint64_t)p.chunks, 8u * (uint32_t)(p.groups / l.row_tiles), 1)) return TUNA_ERR_NO_DEVICE;
+    if (!l.resident && !tiles_of(&maps.x, a.x, (uint64_t)a.n, (uint64_t)p.chunks, (uint32_t)l.x_rows, 1u << l.fold_log)) return TUNA_ERR_NO_DEVICE;
+    if (!make_tensor_map_2d(&maps.ws, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.s, (uint64_t)a.m, (uint64_t)a.experts * p.words, (uint64_t)a.m * 4, (uint32_t)kBlockRows >> l.fold_log, 2, CU_TENSOR_MAP_SWIZZLE_NONE))
         return TUNA_ERR_NO_DEVICE;
     const int ctas = l.workers * l.cg;
     switch (a.o_type) {

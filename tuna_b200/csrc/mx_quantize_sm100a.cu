@@ -34,8 +34,13 @@ __device__ __forceinline__ MxqPlace mxq_place(int rows, int chunks, int batch, i
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(kMxqWarps * 32)
 mx_quantize_kernel(const T *__restrict__ x, long long row_stride, uint8_t *__restrict__ q, uint32_t *__restrict__ s, int rows, int k, int chunks, int batch,
-                   int log_c)
+                   int log_c, int chained)
 {
+    // Chained: part of a product, which may start (and read its weights, not this kernel's) while this one runs.
+    if (chained) {
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+    }
     const int lane = threadIdx.x & 31;
     const MxqPlace l = mxq_place<ROWS>(rows, chunks, batch, log_c);
     if (!l.any) return;
@@ -150,24 +155,32 @@ static cudaError_t mxq_launch(int rows, int k, int batch, int rows_per_warp, Ker
 {
     const int chunks = div_up(k, kMxChunk), log_c = chunks >= 4 ? 2 : chunks >= 2 ? 1 : 0;
     const long long groups = (long long)batch * div_up(rows, rows_per_warp);
-    kernel(dim3((unsigned)div_up_ll(groups, 4 >> log_c), (unsigned)div_up(chunks, 1 << log_c)), chunks, log_c);
-    return cudaGetLastError();
+    return kernel(dim3((unsigned)div_up_ll(groups, 4 >> log_c), (unsigned)div_up(chunks, 1 << log_c)), chunks, log_c);
 }
 
 template <typename T, int ROWS>
-static cudaError_t quantize_as(const void *x, long long row_stride, void *q, void *s, int rows, int k, int batch, cudaStream_t stream)
+static cudaError_t quantize_as(const void *x, long long row_stride, void *q, void *s, int rows, int k, int batch, bool chained, cudaStream_t stream)
 {
     return mxq_launch(rows, k, batch, ROWS, [&](dim3 grid, int chunks, int log_c) {
-        mx_quantize_kernel<T, ROWS><<<grid, kMxqWarps * 32, 0, stream>>>((const T *)x, row_stride, (uint8_t *)q, (uint32_t *)s, rows, k, chunks, batch, log_c);
+        cudaLaunchConfig_t lc = {};
+        lc.gridDim = grid;
+        lc.blockDim = dim3(kMxqWarps * 32);
+        lc.stream = stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        lc.attrs = attr;
+        lc.numAttrs = chained ? 1 : 0;
+        return cudaLaunchKernelEx(&lc, mx_quantize_kernel<T, ROWS>, (const T *)x, row_stride, (uint8_t *)q, (uint32_t *)s, rows, k, chunks, batch, log_c, (int)chained);
     });
 }
 
-cudaError_t launch_mx_quantize(const void *x, int type, long long row_stride, void *q, void *s, int rows, int k, int batch, cudaStream_t stream)
+cudaError_t launch_mx_quantize(const void *x, int type, long long row_stride, void *q, void *s, int rows, int k, int batch, cudaStream_t stream, bool chained)
 {
     switch (type) {
-        case TUNA_FP16: return quantize_as<__half, kMxqRows>(x, row_stride, q, s, rows, k, batch, stream);
-        case TUNA_BF16: return quantize_as<__nv_bfloat16, kMxqRows>(x, row_stride, q, s, rows, k, batch, stream);
-        default: return quantize_as<float, kMxqRows>(x, row_stride, q, s, rows, k, batch, stream);
+        case TUNA_FP16: return quantize_as<__half, kMxqRows>(x, row_stride, q, s, rows, k, batch, chained, stream);
+        case TUNA_BF16: return quantize_as<__nv_bfloat16, kMxqRows>(x, row_stride, q, s, rows, k, batch, chained, stream);
+        default: return quantize_as<float, kMxqRows>(x, row_stride, q, s, rows, k, batch, chained, stream);
     }
 }
 
@@ -176,6 +189,7 @@ static cudaError_t dequant_as(const void *q, const void *s, void *o, int rows, i
 {
     return mxq_launch(rows, k, batch, ROWS, [&](dim3 grid, int chunks, int log_c) {
         mx_dequant_kernel<T, ROWS><<<grid, kMxqWarps * 32, 0, stream>>>((const uint8_t *)q, (const uint32_t *)s, (T *)o, rows, k, chunks, batch, log_c);
+        return cudaGetLastError();
     });
 }
 

@@ -10,6 +10,9 @@ The reference has no counterpart: its one 4-bit format is the codebook of `matmu
 
 from __future__ import annotations
 
+import ctypes
+import functools
+
 import torch
 
 from . import _lib
@@ -19,6 +22,35 @@ from .ops import _expect, _on_device, _stream_ptr
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _MXFP4 = 3
 _workspaces: dict = {}
+
+
+class _NoFront:
+    """Where the native front is missing every call is checked here."""
+
+    @staticmethod
+    def _python_way(*args):
+        return False
+
+    mx_quantize = mx_dequant = mx_matmul = mx_matmul_grouped = _python_way
+
+
+@functools.lru_cache(maxsize=None)
+def _front():
+    """The native front (csrc/fast_call.cpp), which checks and launches the common calls, bound to the library."""
+    front = _lib.load_fast_call()
+    if front is None:
+        return _NoFront
+    lib = _lib.load()
+    front.bind_mx(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in
+                    ("tuna_mx_quantize", "tuna_mx_dequant", "tuna_mx_matmul", "tuna_mx_matmul_grouped", "tuna_stream_capture_id")), _workspaces)
+    return front
+
+
+def _launched(done) -> bool:
+    """Whether the front has made the call; an error of the launch itself is raised."""
+    if done is not False and done is not True:
+        check(done)
+    return done is True
 
 
 def _code_shape(rows: int, k: int):
@@ -68,6 +100,10 @@ def mx_quantize(x):
     """`x` (fp16, bf16 or fp32; `[rows, k]`, whose rows may lie apart, or contiguous `[matrices, rows, k]`) -> codes and scales
     `(q, s)`.  A block's scale is 2^(floor(log2(largest magnitude)) - 2), not below 2^-127; numbers over the scale are
     rounded to nearest with ties to even and saturate at 6.  A block with an infinity or NaN reads back as NaN."""
+    done = _front().mx_quantize(x)
+    if isinstance(done, tuple):
+        return done
+    _launched(done)
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError("x must be a CUDA tensor (there is no CPU path)")
     if x.dtype not in _TYPES:
@@ -96,6 +132,8 @@ def mx_quantize(x):
 def mx_dequant(q, s, o, m: int, k: int) -> None:
     """The numbers of codes and scales, rounded once to o's type: o fp16, bf16 or fp32 `[m, k]`.  With a leading dimension of q, s
     and o, all its matrices."""
+    if _launched(_front().mx_dequant(q, s, o, m, k)):
+        return
     dev = q.device if isinstance(q, torch.Tensor) else None
     matrices = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() == 4 else 1
     _expect_codes(q, s, ("q", "s"), m, k, dev, matrices)
@@ -121,6 +159,8 @@ def mx_matmul(x, xs, q, s, o, m: int, n: int, k: int, *, workspace=None) -> None
     """o `[n, m]` (fp16, bf16 or fp32, overwritten) = x `[n, k]` times the transposed matrix of `(q, s)` `[m, k]`, fp32 accumulation,
     one rounding.  x is codes with their scales `xs`, or fp16 or bf16 with `xs=None`: the call quantizes it as
     `mx_quantize` does.  m a multiple of 8, k of 32.  Enqueued on the current stream of x's device."""
+    if workspace is None and _launched(_front().mx_matmul(x, xs, q, s, o, m, n, k)):
+        return
     kind = _tokens(x, xs, n, k)
     dev = x.device
     _expect_codes(q, s, ("q", "s"), m, k, dev)
@@ -137,6 +177,8 @@ def mx_matmul_grouped(x, xs, q, s, offsets, o, m: int, n: int, k: int, *, worksp
     multiplied with matrix e of `q` `[experts, ceil(k/256), m, 128]` and `s`.  `offsets` int32 `[experts + 1]`, not decreasing, stays on
     the device (a router's cumulative counts): nothing waits for it on the host.  x and o have n rows, which may be more than
     offsets[experts]: rows of o that no expert has are left as they were.  n = 0 is nothing to do."""
+    if workspace is None and _launched(_front().mx_matmul_grouped(x, xs, q, s, offsets, o, m, n, k)):
+        return
     if not isinstance(q, torch.Tensor) or q.dim() != 4:
         raise ValueError("q must be a [experts, ceil(k/256), m, 128] tensor")
     experts = q.shape[0]
