@@ -45,9 +45,10 @@ constexpr int kMxWarps = 12;
 constexpr int kMxEpilogueWarp0 = 4;
 constexpr int kMxScaleWarp0 = 8;
 constexpr int kMxMaxStages = 12;
-__host__ __device__ constexpr int mx_stage_tokens(int token_words) { return token_words == 1 ? 32 : 64; }  // of an output staging buffer
+__host__ __device__ constexpr int mx_stage_tokens(int token_words) { return token_words == 2 ? 32 : 64; }  // of an output staging buffer
 constexpr int kMxDirectTokens = 16;     // tiles of up to so many tokens are stored from registers
-constexpr uint32_t kMxFoldBytes = kMxDirectTokens * kBlockRows * 4;  // where the parts of a folded tile are added up
+constexpr int kMxFoldTokens = 32;
+constexpr uint32_t kMxFoldBytes = kMxFoldTokens * kBlockRows * 4;  // where the parts of a folded tile are added up
 constexpr int kMxAheadTokens = 64;      // one matrix: up to here weights are read ahead of the dependency wait
 constexpr uint32_t kMxScaleBytes = 2 * kBlockRows * 4;  // of the weights' scales in a stage
 constexpr int kMxSmemMax = 227 * 1024;  // of a CTA alone on its SM, static part included
@@ -154,13 +155,9 @@ struct MxSegs {
 };
 
 // One lane's words to COUNT columns of this warp's lanes.
-__device__ __forceinline__ void tc_st_words(uint32_t taddr, const uint32_t (&v)[1])
+__device__ __forceinline__ void tc_st_words(uint32_t taddr, const uint32_t (&v)[2])
 {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(v[0]) : "memory");
-}
-__device__ __forceinline__ void tc_st_words(uint32_t taddr, const uint32_t (&v)[4])
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(taddr), "r"(v[0]), "r"(v[1]) : "memory");
 }
 __device__ __forceinline__ void tc_st_words(uint32_t taddr, const uint32_t (&v)[8])
 {
@@ -214,8 +211,8 @@ __device__ __forceinline__ void mx_store_shared(uint32_t a, __half v) { asm vola
 __device__ __forceinline__ void mx_store_shared(uint32_t a, __nv_bfloat16 v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(__bfloat16_as_ushort(v)) : "memory"); }
 __device__ __forceinline__ void mx_store_shared(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
 
-// Words of a half (128 columns) of the tokens' scales that a lane holds: one up to 32 tokens of a tile, else four per 128.
-__host__ __device__ constexpr int mx_token_words(int tile_tok) { return tile_tok <= 32 ? 1 : tile_tok <= 128 ? 4 : 8; }
+// Words of a half (128 columns) of the tokens' scales that a lane holds, for so many columns of an accumulator.
+__host__ __device__ constexpr int mx_token_words(int cols) { return cols <= 64 ? 2 : cols <= 128 ? 4 : 8; }
 // Tensor-memory columns of a stage's scales: four per half for the weights, four per half and 128 tokens.
 __host__ __device__ constexpr uint32_t mx_scale_cols(int token_words) { return 8 + 2 * (token_words < 4 ? 4 : token_words); }
 
@@ -263,15 +260,15 @@ __device__ __forceinline__ void mx_quantize_resident(const MxParams &p, int w, i
             e <<= 8 * ((lane >> 2) & 3);  // four neighbouring blocks make a word
             e |= __shfl_xor_sync(0xffffffffu, e, 4);
             e |= __shfl_xor_sync(0xffffffffu, e, 8);
-            if ((lane & 15) == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(words_at + (uint32_t)unit * 256u + (uint32_t)(lane >> 4) * 128u + (uint32_t)at * 4u), "r"(e) : "memory");
+            if ((lane & 15) == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(words_at + (uint32_t)unit * 512u + (uint32_t)(lane >> 4) * 256u + (uint32_t)at * 4u), "r"(e) : "memory");
         }
     }
 }
 
 // CG: CTAs of a worker (1 or 2).  NW: mx_token_words.  RESIDENT: the tokens are numbers in 16 bits and quantized here.
-// Tiles of up to 32 tokens leave room for a second CTA on the SM: that of the next launch, which copies its first weights meanwhile.
+// Tiles of up to 64 tokens leave room for a second CTA on the SM: that of the next launch, which copies its first weights meanwhile.
 template <int CG, int NW, bool RESIDENT, typename OT>
-__global__ void __launch_bounds__(32 * kMxWarps, NW == 1 ? 2 : 1)
+__global__ void __launch_bounds__(32 * kMxWarps, NW == 2 ? 2 : 1)
 mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_w2,
                const __grid_constant__ CUtensorMap tmap_ws, const __grid_constant__ CUtensorMap tmap_x)
 {
@@ -281,7 +278,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     __shared__ int s_abort, s_last;
     __shared__ MxSplit s_split;
 
-    constexpr uint32_t kTmemCols = NW == 1 ? 256 : 512;
+    constexpr uint32_t kTmemCols = NW == 2 ? 256 : 512;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = CG == 1 ? 0 : (int)cluster_ctarank();
     const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
@@ -295,7 +292,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     constexpr int kStageTokens = mx_stage_tokens(NW);
     constexpr uint32_t kTokPitch = kBlockRows * (uint32_t)sizeof(OT) + (sizeof(OT) == 2 ? 16 : 0);  // 16-bit results: 16 bytes more, so that a column of 8 tokens meets all banks
     constexpr uint32_t kStagingBytes = kStageTokens * kTokPitch;
-    int *tables = reinterpret_cast<int *>(smem + (staging - base) + (N > kMxDirectTokens ? 2 * kStagingBytes : p.fold_log ? kMxFoldBytes : 0));
+    int *tables = reinterpret_cast<int *>(smem + (staging - base) + (p.fold_log ? kMxFoldBytes : N > kMxDirectTokens ? 2 * kStagingBytes : 0));
 
     // landed: a stage's copies; full: its scales are written as well; empty: its MMAs are done
     const uint32_t landed = smem_u32(&bars[0]), full = landed + 8 * kMxMaxStages, empty = full + 8 * kMxMaxStages, d_full = empty + 8 * kMxMaxStages, d_empty = d_full + 16;
@@ -480,7 +477,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                 ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 201);
                 if (!ok) break;
                 const uint32_t to = xs_ring + (uint32_t)ru.idx * (256u * NW) + 4u * lane;
-                if (NW > 1 || !p.fold_log) {
+                if (NW > 2 || !p.fold_log) {
                     const uint32_t *src = p.xs + (size_t)(2 * c) * p.n + segs.tok0 + lane;
 #pragma unroll
                     for (int j = 0; j < NW; ++j) {
@@ -489,12 +486,14 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                         if (2 * c + 1 < p.words) cp_async_word(to + 128u * (NW + j), src + p.n + 32 * j, true);
                     }
                 } else {  // token t of the stage's chunk f: zeros behind the last word, where the codes are zeros too
-                    const int f = lane / p.x_rows, t = lane - f * p.x_rows;
-                    if (f < fold && t < segs.valid) {
+#pragma unroll
+                    for (int j = 0; j < NW; ++j) {
+                        const int f = (32 * j + lane) / p.x_rows, t = 32 * j + lane - f * p.x_rows;
+                        if (f >= fold || t >= segs.valid) continue;
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             const int word = 2 * ((c << p.fold_log) + f) + h;
-                            cp_async_word(to + 128u * h, p.xs + (size_t)min(word, p.words - 1) * p.n + segs.tok0 + t, word < p.words);
+                            cp_async_word(to + 128u * (NW * h + j), p.xs + (size_t)min(word, p.words - 1) * p.n + segs.tok0 + t, word < p.words);
                         }
                     }
                 }
@@ -527,10 +526,10 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                     const int row = 32 * (i & 3) + lane, f = row >> (7 - p.fold_log), of = row & (part - 1);
                     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(ws_ring + (uint32_t)ru.idx * kMxScaleBytes + (uint32_t)((2 * f + (i >> 2)) * part + of) * 4u));
                 }
-                if constexpr (NW == 1) {
-                    uint32_t x0[1], x1[1];
+                if constexpr (NW == 2) {
+                    uint32_t x0[2], x1[2];
                     words(x0, x_at);
-                    words(x1, x_at + 128);
+                    words(x1, x_at + 256);
                     tc_st_words(to + 8, x0);
                     tc_st_words(to + 8 + kTokenCols, x1);
                 } else {
@@ -631,13 +630,15 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
             if (p.fold_log) {
                 // Part f's sums of row i are lane part * f + i, columns x_rows * f ..: added up in the order of the parts.
                 const int f = thread >> (7 - p.fold_log);
-                float v[16];
-                tc_ld_x16(d + f * p.x_rows, v);
-                drained();
                 float *sums = reinterpret_cast<float *>(smem + (staging - base));
+                for (int t0 = 0; t0 < segs.valid; t0 += 16) {
+                    float v[16];
+                    tc_ld_x16(d + f * p.x_rows + t0, v);
 #pragma unroll
-                for (int t = 0; t < 16; ++t)
-                    if (t < segs.valid) sums[t * kBlockRows + thread] = v[t];
+                    for (int t = 0; t < 16; ++t)
+                        if (t0 + t < segs.valid) sums[(t0 + t) * kBlockRows + thread] = v[t];
+                }
+                drained();
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 const int i = thread & (part - 1);
                 for (int t = f; t < segs.valid && i < rows; t += fold) {
@@ -737,7 +738,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
 // ------------------------------------------------------------------ host side
 
 struct MxPlan {
-    int cg, tile_tok, stages, nd, d_cols, d_step, sf_col;
+    int cg, tile_tok, words, stages, nd, d_cols, d_step, sf_col;
     bool resident;
     int flex, fold_log, row_tiles, cut, w_bytes, x_rows;
     int workers;
@@ -766,22 +767,23 @@ static MxPlan mx_plan(int m, int n, int k, int experts, int x_type, int o_type, 
         if (rt >= div_up(m, kBlockRows) && rt <= m / 8) l.row_tiles = rt;
         l.cut = 0;
         const int height = 8 * div_up(m / 8, l.row_tiles);
-        if (n <= 16) l.fold_log = height <= 32 && n <= 8 ? 2 : height <= 64 ? 1 : 0;
+        l.fold_log = height <= 32 && n <= 16 ? 2 : height <= 64 && n <= kMxFoldTokens ? 1 : 0;
         if (fl >= 0) l.fold_log = std::min(l.fold_log, fl);
         if (!l.fold_log) l.w_bytes = height * kMxChunkBytes;
     }
     l.workers = sm_count / l.cg;
-    const int words = mx_token_words(l.tile_tok), fold = 1 << l.fold_log;
-    const size_t room = words == 1 ? 111 * 1024 : kMxSmemMax - 2048;
-    const size_t pitch = kBlockRows * (o_type == TUNA_FP32 ? 4 : 2) + (o_type == TUNA_FP32 ? 0 : 16);
-    const size_t tail = (l.tile_tok > kMxDirectTokens ? 2 * mx_stage_tokens(words) * pitch : l.fold_log ? kMxFoldBytes : 0) + (3 * (size_t)experts + 1) * 4;
+    const int fold = 1 << l.fold_log;
     l.x_rows = l.fold_log ? div_up(n, 8) * 8 : l.tile_tok / l.cg;
     l.d_cols = l.fold_log ? l.x_rows * fold : l.tile_tok;
+    const int words = l.words = std::max(mx_token_words(l.d_cols), 2 * l.cg);
+    const size_t room = words == 2 ? 111 * 1024 : kMxSmemMax - 2048;
+    const size_t pitch = kBlockRows * (o_type == TUNA_FP32 ? 4 : 2) + (o_type == TUNA_FP32 ? 0 : 16);
+    const size_t tail = (l.fold_log ? kMxFoldBytes : l.tile_tok > kMxDirectTokens ? 2 * mx_stage_tokens(words) * pitch : 0) + (3 * (size_t)experts + 1) * 4;
     const size_t w_stage = (size_t)l.w_bytes + kMxScaleBytes;
     size_t x_stage = (size_t)l.x_rows * fold * kMxChunkBytes + 256 * words;
     // tokens' codes that stay in shared memory: what is left has to hold stages enough
-    const size_t resident = (size_t)div_up(chunks, fold) * (div_up(n, 8) * 8 * fold * kMxChunkBytes + 256);
-    l.resident = x_type != TUNA_MXFP4 && !grouped && n <= 4 && l.flex && resident + 4 * w_stage + tail <= room && resident + 60 * 1024 <= room;
+    const size_t resident = (size_t)div_up(chunks, fold) * (div_up(n, 8) * 8 * fold * kMxChunkBytes + 512);
+    l.resident = x_type != TUNA_MXFP4 && !grouped && n * div_up(chunks, fold) * fold <= 4 * (kMxWarps - 1) && l.flex && resident + 4 * w_stage + tail <= room && resident + 60 * 1024 <= room;
     size_t fixed = tail;
     if (l.resident) {
         l.x_rows = div_up(n, 8) * 8;
@@ -789,7 +791,7 @@ static MxPlan mx_plan(int m, int n, int k, int experts, int x_type, int o_type, 
         x_stage = 0;
     }
     l.stages = (int)std::min<size_t>(kMxMaxStages, (room - fixed) / (w_stage + x_stage));
-    const int tmem_cols = words == 1 ? 256 : 512, scale_cols = (int)mx_scale_cols(words);
+    const int tmem_cols = words == 2 ? 256 : 512, scale_cols = (int)mx_scale_cols(words);
     l.nd = 2 * l.d_cols + l.stages * scale_cols <= tmem_cols ? 2 : 1;
     l.d_step = l.nd == 2 ? l.d_cols : 0;
     // two accumulators of which the columns in the middle are shared, where two whole ones do not fit
@@ -854,10 +856,12 @@ static int launch_mx(const MxParams &p, const MxMaps &maps, int ctas, size_t sme
 template <typename OT>
 static int launch_mx_as(const MxPlan &l, const MxParams &p, const MxMaps &maps, int ctas, cudaStream_t stream)
 {
-    const int words = mx_token_words(l.tile_tok);
-    if (l.cg == 2) return words <= 4 ? launch_mx<2, 4, false, OT>(p, maps, ctas, l.smem, stream) : launch_mx<2, 8, false, OT>(p, maps, ctas, l.smem, stream);
-    if (words == 4) return launch_mx<1, 4, false, OT>(p, maps, ctas, l.smem, stream);
-    return l.resident ? launch_mx<1, 1, true, OT>(p, maps, ctas, l.smem, stream) : launch_mx<1, 1, false, OT>(p, maps, ctas, l.smem, stream);
+    switch (10 * l.cg + l.words) {
+        case 12: return l.resident ? launch_mx<1, 2, true, OT>(p, maps, ctas, l.smem, stream) : launch_mx<1, 2, false, OT>(p, maps, ctas, l.smem, stream);
+        case 14: return launch_mx<1, 4, false, OT>(p, maps, ctas, l.smem, stream);
+        case 28: return launch_mx<2, 8, false, OT>(p, maps, ctas, l.smem, stream);
+        default: return launch_mx<2, 4, false, OT>(p, maps, ctas, l.smem, stream);
+    }
 }
 
 int launch_mx_gemm(const MxGemmArgs &a)
