@@ -98,7 +98,7 @@ def _build_fast_call(force: bool) -> None:
     include = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include", sysconfig.get_paths()["include"]]
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            f'-DFAST_CALL_STAMP="{_lib.fast_call_stamp()}"', *(f"-I{p}" for p in include), str(CSRC / "fast_call.cpp"), "-o", str(FAST_CALL),
-           f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+           f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode:  # no Python headers, say: the library is complete without it
         FAST_CALL.unlink(missing_ok=True)
