@@ -292,7 +292,7 @@ int tuna_mx_dequant(const void *q, const void *s, void *o, int o_type, int rows,
  * o[n, m] (fp16, bf16 or fp32) = x[n, k] * w[m, k]^T, w given by q and s, fp32 accumulation, one rounding; results are
  * bit-identical from run to run.  x_type TUNA_MXFP4: x and xs are codes and scales of the tokens.  TUNA_FP16 or TUNA_BF16: x is
  * [n, k] of that type, xs is not read, and the call quantizes x as tuna_mx_quantize does.  m a multiple of 8, k of 32, any
- * n >= 1.  Alignment: x, q, s, o, workspace 16 bytes; xs 4.  Ordinary stream order for everything.
+ * n >= 1.  Alignment: 16 bytes.  Ordinary stream order for everything.
  * Workspace: tuna_mx_workspace_bytes (with experts = 1), its first tuna_mx_workspace_zero_bytes() bytes ZERO before
  * the first call; every call leaves them so, and one allocation of the largest size serves consecutive calls of any shapes on a
  * stream.  Calls that overlap on the device need separate ones, and so do graphs that are replayed side by side.

@@ -94,7 +94,7 @@ def test_argument_validation_needs_no_gpu(tuna_lib):
     assert mm(x=None) == -1 and mm(xs=None) == -1 and mm(q=None) == -1 and mm(s=None) == -1 and mm(o=None) == -1
     assert mm(m=60) == -2 and mm(n=0) == -2 and mm(k=48) == -2 and mm(k=0) == -2 and mm(m=-8) == -2
     assert mm(x_type=2) == -5 and mm(x_type=4) == -5 and mm(o_type=3) == -5
-    assert mm(x=odd) == -3 and mm(q=odd) == -3 and mm(s=odd) == -3 and mm(o=odd) == -3 and mm(ws=odd) == -3
+    assert mm(x=odd) == -3 and mm(xs=odd) == -3 and mm(q=odd) == -3 and mm(s=odd) == -3 and mm(o=odd) == -3 and mm(ws=odd) == -3
     assert mm(ws=None) == -4 and mm(ws_bytes=16) == -4
     assert mm(x_type=0, ws_bytes=tuna_lib.tuna_mx_workspace_bytes(64, 1, 64, 1, 3)) == -4  # no room for the tokens' codes
 

@@ -10,8 +10,11 @@
 // Persistent CTAs, or pairs of CTAs (cta_group::2: 256 weight rows, every CTA stages its own 128 and half of the tokens), of 12 warps:
 //   warp 0     MMA issue (one elected lane; in a pair the first CTA's)
 //   warp 1     TMA producer of the weights' codes and scales
-//   warp 2     TMA producer of the tokens' codes
-//   warp 3     tensor-memory allocation; words of the tokens' scales, 4-byte copies (cp.async), since tiles start at any token
+//   warp 2     TMA producer of the tokens' codes and, in wide tiles, their scales.  A tile starts at any token, a copy at a multiple
+//              of four words: the scales' copies start up to three words early, and the readers skip those
+//   warp 3     tensor-memory allocation; scales of the tokens in tiles of up to 64 columns, as 4-byte copies (cp.async).  In wide
+//              tiles this warp would set the pace (0.30 us per 256 columns of a 256-token tile before any other work), in narrow
+//              ones the small TMA copies would (4096x4096 at 1 token 7.3 us, so 4.5)
 //   warps 4-7  epilogue: tensor memory -> registers -> output type -> memory, of more than 16 tokens by way of shared memory
 //              and one bulk copy per token
 //   warps 8-11 scales, one warp per lane quarter: a word of scales is four blocks (128 columns) of one row or token, and the MMAs want that of
@@ -47,6 +50,7 @@ constexpr int kMxScaleWarp0 = 8;
 constexpr int kMxMaxStages = 12;
 __host__ __device__ constexpr int mx_stage_tokens(int token_words) { return token_words == 2 ? 32 : 64; }  // of an output staging buffer
 constexpr int kMxDirectTokens = 16;     // tiles of up to so many tokens are stored from registers
+constexpr int kMxSlackBytes = 1024;     // of shared memory at the end: scales of columns that a tile does not have are read from behind its own
 constexpr int kMxFoldTokens = 32;
 constexpr uint32_t kMxFoldBytes = kMxFoldTokens * kBlockRows * 4;  // where the parts of a folded tile are added up
 constexpr int kMxAheadTokens = 64;      // one matrix: up to here weights are read ahead of the dependency wait
@@ -70,6 +74,8 @@ struct MxParams {
     int row_tiles;
     int w_bytes;    // of the weights in a stage
     int x_rows;     // tokens in a stage of a CTA
+    int xs_pitch;   // bytes between the copies of a stage's token scales
+    int xs_bytes;   // of all of them
     int flex;       // row tiles of equal height: tile t has the groups of 8 rows t * groups / row_tiles up to the next tile's
     int groups;     // m / 8
     int x_bf16;     // RESIDENT: type of the tokens
@@ -153,6 +159,11 @@ struct MxSegs {
     }
     __device__ int total_units() const { return (u_end - u) + (dp < tiles ? ((tiles - 1 - dp) / dp_step + 1) * chunks : 0); }
 };
+
+__device__ __forceinline__ void tma_load_1d(uint32_t dst, const CUtensorMap *map, int c0, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.1d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2}], [%3];" ::"r"(dst), "l"(map), "r"(c0), "r"(bar) : "memory");
+}
 
 // One lane's words to COUNT columns of this warp's lanes.
 __device__ __forceinline__ void tc_st_words(uint32_t taddr, const uint32_t (&v)[2])
@@ -270,7 +281,7 @@ __device__ __forceinline__ void mx_quantize_resident(const MxParams &p, int w, i
 template <int CG, int NW, bool RESIDENT, typename OT>
 __global__ void __launch_bounds__(32 * kMxWarps, NW == 2 ? 2 : 1)
 mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_w2,
-               const __grid_constant__ CUtensorMap tmap_ws, const __grid_constant__ CUtensorMap tmap_x)
+               const __grid_constant__ CUtensorMap tmap_ws, const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_xs)
 {
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[3 * kMxMaxStages + 4];
@@ -288,7 +299,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     const int x_stages = RESIDENT ? p.units : S;
     const uint32_t base = smem_u32(smem), w_bytes = (uint32_t)p.w_bytes, x_bytes = (uint32_t)(p.x_rows << p.fold_log) * kMxChunkBytes;
     const uint32_t x_ring = base + (uint32_t)S * w_bytes, ws_ring = x_ring + (uint32_t)x_stages * x_bytes, xs_ring = ws_ring + (uint32_t)S * kMxScaleBytes;
-    const uint32_t staging = xs_ring + (uint32_t)x_stages * (256u * NW);
+    const uint32_t staging = xs_ring + (uint32_t)(x_stages * p.xs_bytes);
     constexpr int kStageTokens = mx_stage_tokens(NW);
     constexpr uint32_t kTokPitch = kBlockRows * (uint32_t)sizeof(OT) + (sizeof(OT) == 2 ? 16 : 0);  // 16-bit results: 16 bytes more, so that a column of 8 tokens meets all banks
     constexpr uint32_t kStagingBytes = kStageTokens * kTokPitch;
@@ -301,7 +312,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 1) {
         auto count = [&](int i) {
-            if (i < kMxMaxStages) return RESIDENT ? 1 : 34;     // landed: weights, tokens, the lanes that copy their scales
+            if (i < kMxMaxStages) return RESIDENT ? 1 : NW == 2 ? 34 : 2;  // landed: weights, tokens, the lanes that copy their scales
             if (i < 2 * kMxMaxStages) return 4 * CG;            // full: the scale warps of each CTA
             return i < 3 * kMxMaxStages + 2 ? 1 : 4 * CG;       // empty, d_full: a commit; d_empty: the epilogue warps of each CTA
         };
@@ -312,6 +323,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
             prefetch_map(&tmap_w);
             prefetch_map(&tmap_ws);
             if (!RESIDENT) prefetch_map(&tmap_x);
+            if (NW > 2) prefetch_map(&tmap_xs);
         }
     }
     if (warp == 3) {
@@ -454,6 +466,8 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
         // ------------------------------------------------------------------ tokens' codes
         Ring ru;
         bool ok = true;
+        constexpr int kPieces = NW == 8 ? 2 : 1;  // 128 words each
+        const uint32_t xs_copy = (uint32_t)(min(N, 128) + 4) * 4u;
         depend();
         while (ok && segs.next()) {
             const int tok = segs.tok0 + rank * (tile_cols() / CG);
@@ -461,14 +475,23 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                 ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 211);
                 if (!ok) break;
                 if (elect_one_sync()) {
-                    mbar_expect_tx(landed + 8 * ru.idx, x_bytes);
-                    tma_load_3d(x_ring + (uint32_t)ru.idx * x_bytes, &tmap_x, 0, tok, c << p.fold_log, landed + 8 * ru.idx);
+                    const uint32_t bar = landed + 8 * ru.idx;
+                    mbar_expect_tx(bar, x_bytes + (NW > 2 ? 2 * kPieces * xs_copy : 0u));
+                    tma_load_3d(x_ring + (uint32_t)ru.idx * x_bytes, &tmap_x, 0, tok, c << p.fold_log, bar);
+                    if constexpr (NW > 2) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)  // a word behind the last one reads as zeros
+#pragma unroll
+                            for (int j = 0; j < kPieces; ++j)
+                                tma_load_1d(xs_ring + (uint32_t)(ru.idx * p.xs_bytes + (kPieces * h + j) * p.xs_pitch), &tmap_xs,
+                                            (int)((((unsigned)(2 * c + h) * (unsigned)p.n + (unsigned)segs.tok0) & ~3u) + 128u * j), bar);
+                    }
                 }
                 __syncwarp();
             }
         }
-    } else if (warp == 3 && !RESIDENT) {
-        // ------------------------------------------------------------------ tokens' scales
+    } else if (warp == 3 && !RESIDENT && NW == 2) {
+        // ------------------------------------------------------------------ tokens' scales in narrow tiles
         Ring ru;
         bool ok = true;
         depend();
@@ -476,25 +499,15 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
             for (int c = segs.c0; c < segs.c1; ++c, ru.advance(S)) {
                 ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 201);
                 if (!ok) break;
-                const uint32_t to = xs_ring + (uint32_t)ru.idx * (256u * NW) + 4u * lane;
-                if (NW > 2 || !p.fold_log) {
-                    const uint32_t *src = p.xs + (size_t)(2 * c) * p.n + segs.tok0 + lane;
+                const uint32_t to = xs_ring + (uint32_t)(ru.idx * p.xs_bytes) + 4u * lane;
 #pragma unroll
-                    for (int j = 0; j < NW; ++j) {
-                        if (32 * j + lane >= segs.valid) continue;  // whatever lies there scales columns that nobody reads
-                        cp_async_word(to + 128u * j, src + 32 * j, true);
-                        if (2 * c + 1 < p.words) cp_async_word(to + 128u * (NW + j), src + p.n + 32 * j, true);
-                    }
-                } else {  // token t of the stage's chunk f: zeros behind the last word, where the codes are zeros too
+                for (int j = 0; j < NW; ++j) {  // token t of the stage's chunk f: zeros behind the last word, where the codes are zeros too
+                    const int f = p.fold_log ? (32 * j + lane) / p.x_rows : 0, t = 32 * j + lane - f * p.x_rows;
+                    if (f >= fold || t >= segs.valid) continue;  // whatever lies there scales columns that nobody reads
 #pragma unroll
-                    for (int j = 0; j < NW; ++j) {
-                        const int f = (32 * j + lane) / p.x_rows, t = 32 * j + lane - f * p.x_rows;
-                        if (f >= fold || t >= segs.valid) continue;
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const int word = 2 * ((c << p.fold_log) + f) + h;
-                            cp_async_word(to + 128u * (NW * h + j), p.xs + (size_t)min(word, p.words - 1) * p.n + segs.tok0 + t, word < p.words);
-                        }
+                    for (int h = 0; h < 2; ++h) {
+                        const int word = 2 * ((c << p.fold_log) + f) + h;
+                        cp_async_word(to + 128u * (NW * h + j), p.xs + (size_t)min(word, p.words - 1) * p.n + segs.tok0 + t, word < p.words);
                     }
                 }
                 cp_async_arrive(landed + 8 * ru.idx);
@@ -509,34 +522,37 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
         Ring ru;
         bool ok = true;
         if (!RESIDENT) depend();
-        auto words = [&](auto &v, uint32_t at) {
-#pragma unroll
-            for (int i = 0; i < (int)(sizeof(v) / 4); ++i) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[i]) : "r"(at + 128u * i + 4u * lane));
-        };
         while (ok && segs.next()) {
             for (int c = segs.c0; c < segs.c1; ++c, ru.advance(S)) {
                 // a stage's copies have landed, so its MMAs of the round before are done, and its scales may be overwritten
                 ok = mbar_wait_warp(landed + 8 * ru.idx, ru.phase, abort_flag, p.status, 212);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t to = lanes + (uint32_t)ru.idx * kScaleCols, x_at = xs_ring + (uint32_t)(RESIDENT ? c : ru.idx) * (256u * NW);
+                const uint32_t to = lanes + (uint32_t)ru.idx * kScaleCols, x_at = xs_ring + (uint32_t)((RESIDENT ? c : ru.idx) * p.xs_bytes);
                 uint32_t w[8];  // of half i / 4: MMA row 32 (i % 4) + lane is row `of` of part f
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int row = 32 * (i & 3) + lane, f = row >> (7 - p.fold_log), of = row & (part - 1);
                     asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(ws_ring + (uint32_t)ru.idx * kMxScaleBytes + (uint32_t)((2 * f + (i >> 2)) * part + of) * 4u));
                 }
+                uint32_t x[2 * NW];  // column 32 (i % NW) + lane, half i / NW
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t skip = NW == 2 ? 0u : (((unsigned)(2 * c + h) * (unsigned)p.n + (unsigned)segs.tok0) & 3u) * 4u;
+#pragma unroll
+                    for (int j = 0; j < NW; ++j) {
+                        const uint32_t at = NW == 2 ? (uint32_t)(NW * h + j) * 128u : (uint32_t)((NW == 8 ? 2 * h + (j >> 2) : h) * p.xs_pitch) + (uint32_t)(j & 3) * 128u + skip;
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x[NW * h + j]) : "r"(x_at + at + 4u * lane));
+                    }
+                }
                 if constexpr (NW == 2) {
-                    uint32_t x0[2], x1[2];
-                    words(x0, x_at);
-                    words(x1, x_at + 256);
+                    const uint32_t x0[2] = {x[0], x[1]}, x1[2] = {x[2], x[3]};
                     tc_st_words(to + 8, x0);
                     tc_st_words(to + 8 + kTokenCols, x1);
+                } else if constexpr (NW == 4) {
+                    tc_st_words(to + 8, x);
                 } else {
-                    uint32_t x[2 * NW];
-                    words(x, x_at);
-                    if constexpr (NW == 4) tc_st_words(to + 8, x);
-                    else tc_st_x16(to + 8, x);
+                    tc_st_x16(to + 8, x);
                 }
                 tc_st_words(to, w);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -740,7 +756,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
 struct MxPlan {
     int cg, tile_tok, words, stages, nd, d_cols, d_step, sf_col;
     bool resident;
-    int flex, fold_log, row_tiles, cut, w_bytes, x_rows;
+    int flex, fold_log, row_tiles, cut, w_bytes, x_rows, xs_copy, xs_pitch, xs_bytes;
     int workers;
     size_t smem;
 };
@@ -778,9 +794,13 @@ static MxPlan mx_plan(int m, int n, int k, int experts, int x_type, int o_type, 
     const int words = l.words = std::max(mx_token_words(l.d_cols), 2 * l.cg);
     const size_t room = words == 2 ? 111 * 1024 : kMxSmemMax - 2048;
     const size_t pitch = kBlockRows * (o_type == TUNA_FP32 ? 4 : 2) + (o_type == TUNA_FP32 ? 0 : 16);
-    const size_t tail = (l.fold_log ? kMxFoldBytes : l.tile_tok > kMxDirectTokens ? 2 * mx_stage_tokens(words) * pitch : 0) + (3 * (size_t)experts + 1) * 4;
+    const size_t tail = (l.fold_log ? kMxFoldBytes : l.tile_tok > kMxDirectTokens ? 2 * mx_stage_tokens(words) * pitch : 0) + (3 * (size_t)experts + 1) * 4 +
+                        kMxSlackBytes;
     const size_t w_stage = (size_t)l.w_bytes + kMxScaleBytes;
-    size_t x_stage = (size_t)l.x_rows * fold * kMxChunkBytes + 256 * words;
+    l.xs_copy = std::min(l.tile_tok, 128) + 4;  // words
+    l.xs_pitch = div_up(l.xs_copy * 4, 128) * 128;
+    l.xs_bytes = words == 2 ? 512 : 2 * (words == 8 ? 2 : 1) * l.xs_pitch;
+    size_t x_stage = (size_t)l.x_rows * fold * kMxChunkBytes + l.xs_bytes;
     // tokens' codes that stay in shared memory: what is left has to hold stages enough
     const size_t resident = (size_t)div_up(chunks, fold) * (div_up(n, 8) * 8 * fold * kMxChunkBytes + 512);
     l.resident = x_type != TUNA_MXFP4 && !grouped && n * div_up(chunks, fold) * fold <= 4 * (kMxWarps - 1) && l.flex && resident + 4 * w_stage + tail <= room && resident + 60 * 1024 <= room;
@@ -820,7 +840,7 @@ size_t mx_gemm_workspace_bytes(int m, int n, int k, int experts, int sm_count)
 }
 
 struct MxMaps {
-    CUtensorMap w, w2, ws, x;
+    CUtensorMap w, w2, ws, x, xs;
 };
 
 template <int CG, int NW, bool RESIDENT, typename OT>
@@ -850,7 +870,7 @@ static int launch_mx(const MxParams &p, const MxMaps &maps, int ctas, size_t sme
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     lc.attrs = attr;
     lc.numAttrs = CG == 1 ? 1 : 2;
-    return cudaLaunchKernelEx(&lc, mx_gemm_kernel<CG, NW, RESIDENT, OT>, p, maps.w, maps.w2, maps.ws, maps.x) == cudaSuccess ? TUNA_OK : TUNA_ERR_LAUNCH;
+    return cudaLaunchKernelEx(&lc, mx_gemm_kernel<CG, NW, RESIDENT, OT>, p, maps.w, maps.w2, maps.ws, maps.x, maps.xs) == cudaSuccess ? TUNA_OK : TUNA_ERR_LAUNCH;
 }
 
 template <typename OT>
@@ -877,7 +897,7 @@ int launch_mx_gemm(const MxGemmArgs &a)
     p.words = div_up(a.k, kMxScaleCols);
     p.last_steps = div_up(a.k - (p.chunks - 1) * kMxChunk, 64);
     p.units = div_up(p.chunks, 1 << l.fold_log); p.fold_log = l.fold_log;
-    p.row_tiles = l.row_tiles; p.w_bytes = l.w_bytes; p.x_rows = l.x_rows; p.flex = l.flex; p.groups = a.m / 8; p.cut = l.cut;
+    p.row_tiles = l.row_tiles; p.w_bytes = l.w_bytes; p.x_rows = l.x_rows; p.xs_pitch = l.xs_pitch; p.xs_bytes = l.xs_bytes; p.flex = l.flex; p.groups = a.m / 8; p.cut = l.cut;
     p.stages = l.stages; p.nd = l.nd; p.d_cols = l.d_cols; p.d_step = l.d_step; p.sf_col = l.sf_col;
     p.ahead = a.offsets == nullptr && a.n <= kMxAheadTokens;
     p.counters = (unsigned int *)a.workspace;
@@ -885,7 +905,7 @@ int launch_mx_gemm(const MxGemmArgs &a)
     p.status = device_status_word();
     if (!p.status) return TUNA_ERR_NO_DEVICE;
     const long long tiles = ((long long)div_up(a.n, l.tile_tok) + a.experts - 1) * p.row_tiles;  // at most
-    if (tiles >= 1ll << 30 || (tiles / l.workers + 2) * p.chunks >= 1ll << 30 || (long long)a.sm_count * p.chunks >= 1ll << 30 || (long long)a.experts * p.words >= 1ll << 30) return TUNA_ERR_TOO_LARGE;
+    if (tiles >= 1ll << 30 || (tiles / l.workers + 2) * p.chunks >= 1ll << 30 || (long long)a.sm_count * p.chunks >= 1ll << 30 || (long long)a.experts * p.words >= 1ll << 30 || (long long)(p.words + 8) * a.n >= 1ll << 31) return TUNA_ERR_TOO_LARGE;
 
     MxMaps maps;
     auto tiles_of = [](CUtensorMap *map, const void *at, uint64_t rows, uint64_t chunks, uint32_t box_rows, uint32_t box_chunks) {  // [chunks][rows][128 bytes]
@@ -893,11 +913,16 @@ int launch_mx_gemm(const MxGemmArgs &a)
                                   CU_TENSOR_MAP_SWIZZLE_128B);
     };
     if (!tiles_of(&maps.w, a.q, (uint64_t)a.m, (uint64_t)a.experts * p.chunks, l.flex ? 8u * (uint32_t)div_up(p.groups, l.row_tiles) : kBlockRows, 1)) return TUNA_ERR_NO_DEVICE;
-    maps.w2 = maps.x = maps.w;
+    maps.w2 = maps.x = maps.xs = maps.w;
     if (l.flex && p.groups % l.row_tiles && !tiles_of(&maps.w2, a.q, (uint64_t)a.m, (uint64_t)p.chunks, 8u * (uint32_t)(p.groups / l.row_tiles), 1)) return TUNA_ERR_NO_DEVICE;
     if (!l.resident && !tiles_of(&maps.x, a.x, (uint64_t)a.n, (uint64_t)p.chunks, (uint32_t)l.x_rows, 1u << l.fold_log)) return TUNA_ERR_NO_DEVICE;
     if (!make_tensor_map_2d(&maps.ws, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.s, (uint64_t)a.m, (uint64_t)a.experts * p.words, (uint64_t)a.m * 4, (uint32_t)kBlockRows >> l.fold_log, 2, CU_TENSOR_MAP_SWIZZLE_NONE))
         return TUNA_ERR_NO_DEVICE;
+    if (l.words > 2) {
+        const uint64_t dim = (uint64_t)p.words * a.n;
+        const uint32_t box = (uint32_t)l.xs_copy;
+        if (!make_tensor_map_nd(&maps.xs, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.xs, 1, &dim, nullptr, &box, CU_TENSOR_MAP_SWIZZLE_NONE)) return TUNA_ERR_NO_DEVICE;
+    }
     const int ctas = l.workers * l.cg;
     switch (a.o_type) {
         case TUNA_FP16: return launch_mx_as<__half>(l, p, maps, ctas, a.stream);
