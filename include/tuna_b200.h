@@ -292,10 +292,12 @@ int tuna_mx_dequant(const void *q, const void *s, void *o, int o_type, int rows,
  * o[n, m] (fp16, bf16 or fp32) = x[n, k] * w[m, k]^T, w given by q and s, fp32 accumulation, one rounding; results are
  * bit-identical from run to run.  x_type TUNA_MXFP4: x and xs are codes and scales of the tokens.  TUNA_FP16 or TUNA_BF16: x is
  * [n, k] of that type, xs is not read, and the call quantizes x as tuna_mx_quantize does.  m a multiple of 8, k of 32, any
- * n >= 1.  Alignment: 16 bytes.  Ordinary stream order for everything.
- * Workspace: tuna_mx_workspace_bytes (with experts = 1), its first tuna_mx_workspace_zero_bytes() bytes ZERO before
- * the first call; every call leaves them so, and one allocation of the largest size serves consecutive calls of any shapes on a
- * stream.  Calls that overlap on the device need separate ones, and so do graphs that are replayed side by side.
+ * n >= 1.  Alignment: 16 bytes.
+ * Workspace: tuna_mx_workspace_bytes (with experts = 1) bytes for the codes and scales of tokens in 16 bits, none for
+ * TUNA_MXFP4; it is written before it is read.  Calls that overlap on the device need separate ones.
+ * Order: ordinary stream order for everything but q and s of a tuna_mx_matmul of up to 64 tokens, which count as constants as in
+ * tuna_matmul: a kernel that writes them right before such a call must not let dependent launches start early (this library's
+ * quantizers do not).
  */
 int tuna_mx_matmul(const void *x, int x_type, const void *xs, const void *q, const void *s, void *o, int o_type, int m, int n, int k, void *workspace,
                    size_t workspace_bytes, void *stream);
@@ -310,10 +312,6 @@ int tuna_mx_matmul(const void *x, int x_type, const void *xs, const void *q, con
 int tuna_mx_matmul_grouped(const void *x, int x_type, const void *xs, const void *q, const void *s, const void *offsets, void *o, int o_type, int m, int n,
                            int k, int experts, void *workspace, size_t workspace_bytes, void *stream);
 size_t tuna_mx_workspace_bytes(int m, int n, int k, int experts, int x_type);
-size_t tuna_mx_workspace_zero_bytes(void);
-
-/* A number for the CUDA graph capture that `stream` is part of, different for each; 0 outside of one. */
-unsigned long long tuna_stream_capture_id(void *stream);
 
 const char *tuna_status_string(int status);
 

@@ -106,21 +106,19 @@ def test_tokens_in_16_bits_are_quantized_by_the_call(m, n, k, dtype):
     assert torch.equal(o, o2)
 
 
-def test_runs_agree_bit_for_bit_and_leave_the_workspace_clean():
-    m, n, k = 2000, 24, 8192
-    (xq, xs), _ = random_packed(n, k, 1)
+@pytest.mark.parametrize("n", [3, 24])
+def test_runs_agree_bit_for_bit_in_any_workspace(n):
+    m, k = 2000, 8192
     (wq, ws), _ = random_packed(m, k, 2)
-    args = dev(xq, xs, wq, ws)
-    need = _lib.load().tuna_mx_workspace_bytes(m, n, k, 1, 3)
-    zero = _lib.load().tuna_mx_workspace_zero_bytes()
-    work = torch.zeros(need, dtype=torch.uint8, device="cuda")
+    q, s = dev(wq, ws)
+    x = torch.randn(n, k, device="cuda", dtype=torch.float16)
     outs = []
-    for _ in range(5):
+    for fill in (None, 0, 255):
+        work = None if fill is None else torch.full((1 << 20,), fill, dtype=torch.uint8, device="cuda")
         o = torch.full((n, m), float("nan"), device="cuda")
-        tuna_b200.mx_matmul(*args, o, m, n, k, workspace=work)
+        tuna_b200.mx_matmul(x, None, q, s, o, m, n, k, workspace=work)
         outs.append(o)
     finish()
-    assert not work[:zero].any()
     assert all(torch.equal(outs[0], o) for o in outs[1:])
 
 
@@ -333,7 +331,8 @@ def test_refusals():
     with pytest.raises(TypeError):
         tuna_b200.mx_matmul(torch.empty(n, k, device="cuda"), None, wq, ws, o, m, n, k)
     with pytest.raises(tuna_b200.TunaError):
-        tuna_b200.mx_matmul(xq, xs, wq, ws, o, m, n, k, workspace=torch.zeros(64, dtype=torch.uint8, device="cuda"))
+        tuna_b200.mx_matmul(torch.empty(40, k, device="cuda", dtype=torch.bfloat16), None, wq, ws, torch.empty(40, m, device="cuda"), m, 40, k,
+                            workspace=torch.zeros(64, dtype=torch.uint8, device="cuda"))
     with pytest.raises(ValueError):
         tuna_b200.mx_matmul_grouped(xq, xs, wq, ws, off, o, m, n, k)  # no leading dimension
     with pytest.raises(TypeError):

@@ -95,21 +95,22 @@ def test_argument_validation_needs_no_gpu(tuna_lib):
     assert mm(m=60) == -2 and mm(n=0) == -2 and mm(k=48) == -2 and mm(k=0) == -2 and mm(m=-8) == -2
     assert mm(x_type=2) == -5 and mm(x_type=4) == -5 and mm(o_type=3) == -5
     assert mm(x=odd) == -3 and mm(xs=odd) == -3 and mm(q=odd) == -3 and mm(s=odd) == -3 and mm(o=odd) == -3 and mm(ws=odd) == -3
-    assert mm(ws=None) == -4 and mm(ws_bytes=16) == -4
-    assert mm(x_type=0, ws_bytes=tuna_lib.tuna_mx_workspace_bytes(64, 1, 64, 1, 3)) == -4  # no room for the tokens' codes
+    # tokens in 16 bits that a launch of their own quantizes: room for their codes and scales
+    need = tuna_lib.tuna_mx_workspace_bytes(64, 33, 64, 1, 0)
+    assert need >= 33 * (128 + 4) and tuna_lib.tuna_mx_workspace_bytes(64, 33, 64, 1, 3) == 0
+    assert mm(x_type=0, n=33, ws=None) == -4 and mm(x_type=0, n=33, ws_bytes=need - 1) == -4
 
-    def grouped(offsets=p, experts=2, n=4, **kw):
-        return tuna_lib.tuna_mx_matmul_grouped(p, 3, p, p, p, offsets, p, 0, 64, n, 64, experts, p, kw.get("ws_bytes", big), None)
+    def grouped(offsets=p, experts=2, n=4, x_type=3, ws_bytes=big):
+        return tuna_lib.tuna_mx_matmul_grouped(p, x_type, p, p, p, offsets, p, 0, 64, n, 64, experts, p, ws_bytes, None)
 
     assert grouped(offsets=None) == -1
     assert grouped(experts=0) == -2
     assert grouped(experts=1025) == -9
     assert grouped(offsets=ctypes.c_void_p(base + 2)) == -3
-    assert grouped(ws_bytes=0) == -4
+    assert grouped(x_type=1, ws_bytes=0) == -4
     assert grouped(n=0) == 0 and grouped(n=-1) == -2
     assert tuna_lib.tuna_mx_workspace_bytes(60, 1, 64, 1, 3) == 0
-    assert tuna_lib.tuna_mx_workspace_bytes(64, 1, 64, 1025, 3) == 0
-    assert tuna_lib.tuna_mx_workspace_zero_bytes() < tuna_lib.tuna_mx_workspace_bytes(64, 1, 64, 1, 3)
+    assert tuna_lib.tuna_mx_workspace_bytes(64, 1, 64, 1025, 0) == 0
 
 
 def test_types_match_the_header():

@@ -6,7 +6,7 @@ import ctypes
 import functools
 import sysconfig
 import warnings
-from ctypes import c_char_p, c_int, c_int32, c_longlong, c_size_t, c_ulonglong, c_void_p
+from ctypes import c_char_p, c_int, c_int32, c_longlong, c_size_t, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libtuna_b200.so"
@@ -82,8 +82,6 @@ SYMBOLS = {
     "tuna_mx_matmul": (c_int, [c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 4 + [c_void_p, c_size_t, c_void_p]),
     "tuna_mx_matmul_grouped": (c_int, [c_void_p, c_int] + [c_void_p] * 5 + [c_int] * 5 + [c_void_p, c_size_t, c_void_p]),
     "tuna_mx_workspace_bytes": (c_size_t, [c_int] * 5),
-    "tuna_mx_workspace_zero_bytes": (c_size_t, []),
-    "tuna_stream_capture_id": (c_ulonglong, [c_void_p]),
     "tuna_check_device_status": (c_int, [c_void_p]),
     "tuna_selftest_bounded_wait": (c_int, [c_void_p]),
     "tuna_status_string": (c_char_p, [c_int]),

@@ -25,10 +25,10 @@ PyObject *g_workspaces = nullptr;  // the dict (device, stream) -> tensor that o
 // place while this one is in use.  Null where there is none.
 struct Workspace {
     PyObject *tensor = nullptr;
-    Workspace(int device, void *stream) : Workspace(g_workspaces, Py_BuildValue("(iK)", device, (unsigned long long)stream)) {}
-    Workspace(PyObject *workspaces, PyObject *key)  // takes the reference to `key`
+    Workspace(int device, void *stream)
     {
-        PyObject *found = key ? PyDict_GetItemWithError(workspaces, key) : nullptr;
+        PyObject *key = Py_BuildValue("(iK)", device, (unsigned long long)stream);
+        PyObject *found = key ? PyDict_GetItemWithError(g_workspaces, key) : nullptr;
         Py_XDECREF(key);
         if (found && THPVariable_Check(found)) tensor = Py_NewRef(found);
         PyErr_Clear();
@@ -96,9 +96,8 @@ struct {
                   size_t workspace_bytes, void *stream);
     int (*matmul_grouped)(const void *x, int x_type, const void *xs, const void *q, const void *s, const void *offsets, void *o, int o_type, int m, int n, int k,
                           int experts, void *workspace, size_t workspace_bytes, void *stream);
-    unsigned long long (*capture_id)(void *stream);
+    size_t (*workspace_bytes)(int m, int n, int k, int experts, int x_type);
 } g_mx = {};
-PyObject *g_mx_workspaces = nullptr;  // (device, stream, capture) -> tensor
 
 int type_of(at::ScalarType t) { return t == at::kHalf ? TUNA_FP16 : t == at::kBFloat16 ? TUNA_BF16 : t == at::kFloat ? TUNA_FP32 : -1; }
 
@@ -151,17 +150,16 @@ int launch_mx_product(PyObject *const *args, bool grouped)
                      *o = numbers(tail[0], n * m, device, &o_type);
     if (!q || !s || !o) return kPythonWay;
     void *stream = c10::cuda::getCurrentCUDAStream(device).stream();
-    const Workspace ws(g_mx_workspaces, Py_BuildValue("(iKK)", device, (unsigned long long)stream, g_mx.capture_id(stream)));
-    if (!ws.tensor) return kPythonWay;
+    const size_t bytes = packed ? 0 : g_mx.workspace_bytes((int)m, (int)n, (int)k, (int)experts, x_type);
+    at::Tensor ws;  // this call's own, in stream order: what a graph captures comes from its pool
+    if (bytes > 0) ws = at::detail::empty_cuda({(int64_t)bytes}, at::kByte, x->device(), std::nullopt);
     const void *xp = x->const_data_ptr(), *xsp = xs ? xs->const_data_ptr() : nullptr, *qp = q->const_data_ptr(), *sp = s->const_data_ptr(),
                *fp = offsets ? offsets->const_data_ptr() : nullptr;
-    void *op = o->mutable_data_ptr(), *wp = ws.ptr();
-    const size_t bytes = ws.bytes();
+    void *op = o->mutable_data_ptr(), *wp = bytes > 0 ? ws.mutable_data_ptr() : nullptr;
     const auto f = g_mx;
     const Unlocked unlocked;
-    const int st = grouped ? f.matmul_grouped(xp, x_type, xsp, qp, sp, fp, op, o_type, (int)m, (int)n, (int)k, (int)experts, wp, bytes, stream)
-                           : f.matmul(xp, x_type, xsp, qp, sp, op, o_type, (int)m, (int)n, (int)k, wp, bytes, stream);
-    return st == TUNA_ERR_WORKSPACE ? kPythonWay : st;
+    return grouped ? f.matmul_grouped(xp, x_type, xsp, qp, sp, fp, op, o_type, (int)m, (int)n, (int)k, (int)experts, wp, bytes, stream)
+                   : f.matmul(xp, x_type, xsp, qp, sp, op, o_type, (int)m, (int)n, (int)k, wp, bytes, stream);
 }
 
 // q, s, o, m, k
@@ -232,14 +230,12 @@ PyObject *fast_mx_quantize(PyObject *, PyObject *const *args, Py_ssize_t nargs)
     return q && s ? Py_BuildValue("(NN)", q, s) : nullptr;
 }
 
-// bind_mx(addresses of the five functions, dict of the workspaces)
+// bind_mx(addresses of the five functions)
 PyObject *bind_mx(PyObject *, PyObject *args)
 {
     unsigned long long f[5];
-    PyObject *workspaces;
-    if (!PyArg_ParseTuple(args, "KKKKKO!", &f[0], &f[1], &f[2], &f[3], &f[4], &PyDict_Type, &workspaces)) return nullptr;
-    g_mx = {(decltype(g_mx.quantize))f[0], (decltype(g_mx.dequant))f[1], (decltype(g_mx.matmul))f[2], (decltype(g_mx.matmul_grouped))f[3], (decltype(g_mx.capture_id))f[4]};
-    Py_XSETREF(g_mx_workspaces, Py_NewRef(workspaces));
+    if (!PyArg_ParseTuple(args, "KKKKK", &f[0], &f[1], &f[2], &f[3], &f[4])) return nullptr;
+    g_mx = {(decltype(g_mx.quantize))f[0], (decltype(g_mx.dequant))f[1], (decltype(g_mx.matmul))f[2], (decltype(g_mx.matmul_grouped))f[3], (decltype(g_mx.workspace_bytes))f[4]};
     Py_RETURN_NONE;
 }
 

@@ -96,22 +96,20 @@ size_t exchange_region_bytes(const tuna_gemm_desc *d, int count, int world);
 int launch_exchange_reduce(const tuna_exchange &ex, const tuna_gemm_desc *d, const long long *slab0_off, int count, int tile_tok,
                            long long region_bytes, cudaStream_t stream);
 
-// Microscaled 4-bit matrices.  Types are tuna_type's; workspace: counters, zero before the first use and left zero, then partial sums.
+// Microscaled 4-bit matrices.  Types are tuna_type's.
 struct MxGemmArgs {
     const void *x, *xs, *q, *s;
     const void *offsets;  // device, experts + 1 of them; nullptr: one matrix
     void *o;
     int m, n, k, experts, x_type, o_type;
-    void *workspace;
     cudaStream_t stream;
     int sm_count;
 };
-constexpr size_t kMxCounterBytes = 4096;
 // chained: right before the product that reads q and s
 cudaError_t launch_mx_quantize(const void *x, int type, long long row_stride, void *q, void *s, int rows, int k, int batch, cudaStream_t stream, bool chained = false);
 cudaError_t launch_mx_dequant(const void *q, const void *s, void *o, int type, int rows, int k, int batch, cudaStream_t stream);
 int launch_mx_gemm(const MxGemmArgs &a);
+// Whether the product takes tokens of this type as they are; otherwise it wants their codes and scales.
 bool mx_gemm_takes(int m, int n, int k, int experts, int x_type, bool grouped, int sm_count);
-size_t mx_gemm_workspace_bytes(int m, int n, int k, int experts, int sm_count);
 
 }  // namespace tuna

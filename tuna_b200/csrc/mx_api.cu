@@ -1,4 +1,5 @@
 // C ABI of the microscaled 4-bit operators: argument checks, workspace layout, dispatch.
+#include <algorithm>
 #include "launchers.h"
 #include "mx_format.cuh"
 
@@ -16,18 +17,15 @@ static int check_matrix(int rows, int k, int batch)
     return TUNA_OK;
 }
 
-// The workspace: what the product needs, then the codes and scales of tokens that the call quantizes itself.
+// The workspace holds the codes and scales of tokens that a launch before the product quantizes.
 struct MxWorkspace {
-    size_t codes, scales, total;
+    size_t scales, total;
 };
-static MxWorkspace mx_workspace(int m, int n, int k, int experts, int x_type, int sm_count)
+static MxWorkspace mx_workspace(int m, int n, int k, int experts, int x_type, bool grouped, int sm_count)
 {
-    MxWorkspace w;
-    w.codes = mx_gemm_workspace_bytes(m, n, k, experts, sm_count);
-    w.scales = w.codes;
-    w.total = w.codes;
-    if (x_type != TUNA_MXFP4) {
-        w.scales += (size_t)div_up(k, kMxChunk) * n * kMxChunkBytes;
+    MxWorkspace w = {0, 0};
+    if (!mx_gemm_takes(m, n, k, experts, x_type, grouped, sm_count)) {
+        w.scales = (size_t)div_up(k, kMxChunk) * n * kMxChunkBytes;
         w.total = w.scales + (size_t)div_up(k, kMxScaleCols) * n * 4;
     }
     return w;
@@ -44,17 +42,16 @@ static int mx_product(const void *x, int x_type, const void *xs, const void *q, 
     if (!aligned_to(x, 16) || !aligned_to(q, 16) || !aligned_to(s, 16) || !aligned_to(o, 16) || !aligned_to(xs, 16) || !aligned_to(offsets, 4) || !aligned_to(workspace, 16))
         return TUNA_ERR_MISALIGNED;
     const int sms = device_sm_count();
-    const MxWorkspace w = mx_workspace(m, n, k, experts, x_type, sms);
-    if (!workspace || workspace_bytes < w.total) return TUNA_ERR_WORKSPACE;
+    const MxWorkspace w = mx_workspace(m, n, k, experts, x_type, offsets != nullptr, sms);
+    if (w.total > 0 && (!workspace || workspace_bytes < w.total)) return TUNA_ERR_WORKSPACE;
     MxGemmArgs a;
     a.x = x; a.xs = xs; a.q = q; a.s = s; a.offsets = offsets; a.o = o;
     a.m = m; a.n = n; a.k = k; a.experts = experts; a.x_type = x_type; a.o_type = o_type;
-    a.workspace = workspace; a.stream = (cudaStream_t)stream; a.sm_count = sms;
-    if (!mx_gemm_takes(m, n, k, experts, x_type, offsets != nullptr, sms)) {
-        a.x_type = TUNA_MXFP4;
-        a.x = (uint8_t *)workspace + w.codes;
-        a.xs = (uint8_t *)workspace + w.scales;
-        if (launch_mx_quantize(x, x_type, k, (uint8_t *)workspace + w.codes, (uint8_t *)workspace + w.scales, n, k, 1, a.stream, true) != cudaSuccess) return TUNA_ERR_LAUNCH;
+    a.stream = (cudaStream_t)stream; a.sm_count = sms;
+    if (w.total > 0) {
+        uint8_t *codes = (uint8_t *)workspace, *scales = codes + w.scales;
+        if (launch_mx_quantize(x, x_type, k, codes, scales, n, k, 1, a.stream, true) != cudaSuccess) return TUNA_ERR_LAUNCH;
+        a.x = codes; a.xs = scales; a.x_type = TUNA_MXFP4;
     }
     return launch_mx_gemm(a);
 }
@@ -101,18 +98,6 @@ extern "C" int tuna_mx_matmul_grouped(const void *x, int x_type, const void *xs,
 extern "C" size_t tuna_mx_workspace_bytes(int m, int n, int k, int experts, int x_type)
 {
     if (m < 1 || m % 8 || n < 1 || k < 1 || k % kMxBlock || experts < 1 || experts > TUNA_MX_MAX_EXPERTS) return 0;
-    return mx_workspace(m, n, k, experts, x_type, device_sm_count()).total;
-}
-
-extern "C" size_t tuna_mx_workspace_zero_bytes(void) { return kMxCounterBytes; }
-
-extern "C" unsigned long long tuna_stream_capture_id(void *stream)
-{
-    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-    unsigned long long id = 0;
-    if (cudaStreamGetCaptureInfo((cudaStream_t)stream, &status, &id) != cudaSuccess) {
-        cudaGetLastError();  // the legacy stream beside a capture elsewhere: an answer, not a failure
-        return 0;
-    }
-    return status == cudaStreamCaptureStatusActive ? id : 0;
+    const int sms = device_sm_count();
+    return std::max(experts == 1 ? mx_workspace(m, n, k, 1, x_type, false, sms).total : 0, mx_workspace(m, n, k, experts, x_type, true, sms).total);
 }

@@ -24,18 +24,18 @@
 // RESIDENT: up to 16 tokens in 16 bits are quantized by the CTA itself before its first MMA, all of K, and stay in shared memory:
 // no launch before this one.
 //
-// Work split.  Tiles are numbered expert by expert.  With few tokens one matrix may be cut into row tiles of equal height, a multiple
-// of 8 up to 128, a whole number of them for every CTA: the MMAs compute 128 rows whatever the height, which costs nothing where
-// the weights' bytes are the bound, and no sum is cut.  Otherwise tiles have 128 rows (256 for a pair); whole waves of them
-// go out one tile per worker, and what is left over (everything, if there are fewer tiles than workers) may be cut evenly along
-// K.  A cut tile is finished by the CTA that arrives last, which adds the fp32 partial sums in K order: the result does not
-// depend on the order of arrival.
+// Work split.  Tiles are numbered expert by expert and handed out in turn; no sum is cut, so nothing is added up outside of a
+// tile.  Up to 16 tokens one matrix is cut into row tiles of equal height, a multiple of 8 up to 128, a whole number of them for
+// every CTA: the MMAs compute 128 rows whatever the height, which costs nothing where the weights' bytes are the bound.  Where
+// a tile has at most 64 (32) of the 128 rows, two (four) chunks of K lie side by side in it ("folded"): the MMA's rows are
+// those of the tile for each chunk in turn, its columns the tokens for each chunk, and the epilogue adds up the blocks where the
+// two belong together (4096x4096 at 1 token 6.6 us unfolded, 4.5 folded).  More tokens, and experts, go in tiles of 256 rows
+// on pairs, of as many tokens as an estimate (mx_pair_tokens) says.
 //
 // Every wait is bounded, as in the other pipeline kernels.
 #include <algorithm>
+#include <cmath>
 #include <cstring>
-#include <cstdio>
-#include <cstdlib>
 #include <mutex>
 #include "launchers.h"
 #include "mx_format.cuh"
@@ -48,21 +48,19 @@ constexpr int kMxWarps = 12;
 constexpr int kMxEpilogueWarp0 = 4;
 constexpr int kMxScaleWarp0 = 8;
 constexpr int kMxMaxStages = 12;
-__host__ __device__ constexpr int mx_stage_tokens(int token_words) { return token_words == 2 ? 32 : 64; }  // of an output staging buffer
+constexpr int kMxStageTokens = 64;      // tokens of an output staging buffer
 constexpr int kMxDirectTokens = 16;     // tiles of up to so many tokens are stored from registers
 constexpr int kMxSlackBytes = 1024;     // of shared memory at the end: scales of columns that a tile does not have are read from behind its own
-constexpr int kMxFoldTokens = 32;
-constexpr uint32_t kMxFoldBytes = kMxFoldTokens * kBlockRows * 4;  // where the parts of a folded tile are added up
+constexpr uint32_t kMxFoldBytes = kMxDirectTokens * kBlockRows * 4;  // where the parts of a folded tile are added up
 constexpr int kMxAheadTokens = 64;      // one matrix: up to here weights are read ahead of the dependency wait
 constexpr uint32_t kMxScaleBytes = 2 * kBlockRows * 4;  // of the weights' scales in a stage
-constexpr int kMxSmemMax = 227 * 1024;  // of a CTA alone on its SM, static part included
+constexpr int kMxSmemMax = 225 * 1024;   // dynamic shared memory of a CTA alone on its SM (1 KB is the kernel's static part, 1 KB the system's)
+constexpr int kMxSmemHalf = 111 * 1024;  // of one that leaves room for another
 
 struct MxParams {
     const uint32_t *xs;   // words of the tokens' scales [words][n]
     const int *offsets;   // first token of each expert, and the end; nullptr: one matrix, all tokens
     void *o;
-    float *partials;
-    unsigned int *counters;
     DeviceStatus *status;
     int m, n, k;
     int experts;
@@ -80,7 +78,6 @@ struct MxParams {
     int groups;     // m / 8
     int x_bf16;     // RESIDENT: type of the tokens
     const void *x;  // RESIDENT: the tokens [n][k]
-    int cut;        // tiles may be cut along K
     int last_steps; // MMAs of the last chunk: 64 columns each
     int stages;
     int nd;         // accumulators that are free of one another
@@ -90,74 +87,37 @@ struct MxParams {
     int ahead;      // weights are taken from before the dependency wait
 };
 
-// How the launch's tiles are handed out: tiles 0 .. sk_tiles - 1 cut along K over workers 0 .. sk_workers - 1 in ranges of
-// sk_q units (the first sk_r one more), the others whole.
-struct MxSplit {
-    int tiles, sk_tiles, sk_workers, sk_q, sk_r;
-};
-
-__device__ __forceinline__ MxSplit mx_split(int tiles, int chunks, int workers, int cut)
-{
-    MxSplit s = {tiles, 0, 0, 1, 0};
-    const int rest = tiles % workers;
-    if (rest == 0 || !cut) return s;
-    const int ctas = min(workers, rest * chunks / 2);  // two chunks at least
-    if (ctas <= rest) return s;
-    s.sk_tiles = rest;
-    s.sk_workers = ctas;
-    s.sk_q = rest * chunks / ctas;
-    s.sk_r = rest * chunks % ctas;
-    return s;
-}
-
-// The segments of a worker in order, and where each lies.
-struct MxSegs {
-    int u, u_end, dp, dp_step, tiles, chunks, row_tiles, tile_tok;  // chunks: a tile's stages
+// The tiles of a worker in order, and where each lies.
+struct MxTiles {
+    int next_tile, step, tiles, units, row_tiles, tile_tok;
     const int *first_tile, *begin, *count;  // per expert (shared memory)
-    int e;
-    int tile, c0, c1;     // the segment
-    int rt, tok0, valid;  // its rows' tile, its first token and how many there are
-    __device__ void init(const MxParams &p, const MxSplit &s, int worker, int workers, const int *tables)
+    int e, rt, tok0, valid;  // the tile: its expert, its rows' number, its first token and how many there are
+    __device__ void init(const MxParams &p, int worker, int workers, const int *tables)
     {
-        u = worker * s.sk_q + min(worker, s.sk_r);
-        u_end = u + (worker < s.sk_workers ? s.sk_q + (worker < s.sk_r ? 1 : 0) : 0);
-        if (s.sk_tiles == 0) u = u_end = 0;
-        dp = s.sk_tiles + worker;
-        dp_step = workers;
-        tiles = s.tiles;
-        chunks = p.units;
+        next_tile = worker;
+        step = workers;
+        units = p.units;
         row_tiles = p.row_tiles;
         tile_tok = p.tile_tok;
         begin = tables;
         count = tables + p.experts;
         first_tile = tables + 2 * p.experts;
+        tiles = first_tile[p.experts];
         e = 0;
     }
-    __device__ bool more() const { return u < u_end || dp < tiles; }
     __device__ bool next()
     {
-        if (u < u_end) {
-            tile = u / chunks;
-            c0 = u - tile * chunks;
-            c1 = min(chunks, c0 + (u_end - u));
-            u += c1 - c0;
-        } else if (dp < tiles) {
-            tile = dp;
-            c0 = 0;
-            c1 = chunks;
-            dp += dp_step;
-        } else {
-            return false;
-        }
-        while (tile >= first_tile[e + 1]) ++e;  // tiles come in increasing order, and the last expert's end is their number
-        const int local = tile - first_tile[e], tok_tiles = div_up(count[e], tile_tok);
+        if (next_tile >= tiles) return false;
+        while (next_tile >= first_tile[e + 1]) ++e;  // tiles come in increasing order, and the last expert's end is their number
+        const int local = next_tile - first_tile[e], tok_tiles = div_up(count[e], tile_tok);
         rt = local / tok_tiles;
         const int tt = local - rt * tok_tiles;
         tok0 = begin[e] + tt * tile_tok;
         valid = min(tile_tok, count[e] - tt * tile_tok);
+        next_tile += step;
         return true;
     }
-    __device__ int total_units() const { return (u_end - u) + (dp < tiles ? ((tiles - 1 - dp) / dp_step + 1) * chunks : 0); }
+    __device__ int total_units() const { return next_tile < tiles ? ((tiles - 1 - next_tile) / step + 1) * units : 0; }
 };
 
 __device__ __forceinline__ void tma_load_1d(uint32_t dst, const CUtensorMap *map, int c0, uint32_t bar)
@@ -217,10 +177,6 @@ template <> __device__ __forceinline__ uint32_t mx_pack2<__nv_bfloat16>(float lo
     const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&h);
 }
-
-__device__ __forceinline__ void mx_store_shared(uint32_t a, __half v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(__half_as_ushort(v)) : "memory"); }
-__device__ __forceinline__ void mx_store_shared(uint32_t a, __nv_bfloat16 v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(a), "h"(__bfloat16_as_ushort(v)) : "memory"); }
-__device__ __forceinline__ void mx_store_shared(uint32_t a, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(a), "f"(v) : "memory"); }
 
 // Words of a half (128 columns) of the tokens' scales that a lane holds, for so many columns of an accumulator.
 __host__ __device__ constexpr int mx_token_words(int cols) { return cols <= 64 ? 2 : cols <= 128 ? 4 : 8; }
@@ -286,8 +242,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     extern __shared__ __align__(1024) uint8_t smem[];
     __shared__ __align__(8) uint64_t bars[3 * kMxMaxStages + 4];
     __shared__ uint32_t s_tmem_base;
-    __shared__ int s_abort, s_last;
-    __shared__ MxSplit s_split;
+    __shared__ int s_abort;
 
     constexpr uint32_t kTmemCols = NW == 2 ? 256 : 512;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -300,9 +255,8 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     const uint32_t base = smem_u32(smem), w_bytes = (uint32_t)p.w_bytes, x_bytes = (uint32_t)(p.x_rows << p.fold_log) * kMxChunkBytes;
     const uint32_t x_ring = base + (uint32_t)S * w_bytes, ws_ring = x_ring + (uint32_t)x_stages * x_bytes, xs_ring = ws_ring + (uint32_t)S * kMxScaleBytes;
     const uint32_t staging = xs_ring + (uint32_t)(x_stages * p.xs_bytes);
-    constexpr int kStageTokens = mx_stage_tokens(NW);
     constexpr uint32_t kTokPitch = kBlockRows * (uint32_t)sizeof(OT) + (sizeof(OT) == 2 ? 16 : 0);  // 16-bit results: 16 bytes more, so that a column of 8 tokens meets all banks
-    constexpr uint32_t kStagingBytes = kStageTokens * kTokPitch;
+    constexpr uint32_t kStagingBytes = kMxStageTokens * kTokPitch;
     int *tables = reinterpret_cast<int *>(smem + (staging - base) + (p.fold_log ? kMxFoldBytes : N > kMxDirectTokens ? 2 * kStagingBytes : 0));
 
     // landed: a stage's copies; full: its scales are written as well; empty: its MMAs are done
@@ -364,10 +318,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
             }
             before += __shfl_sync(0xffffffffu, sum, 31);
         }
-        if (lane == 0) {
-            tables[3 * p.experts] = before;
-            s_split = mx_split(before, p.units, workers, p.cut);
-        }
+        if (lane == 0) tables[3 * p.experts] = before;
     }
     tc_fence_before();
     __syncthreads();
@@ -377,10 +328,10 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     const uint32_t sf_col = (uint32_t)p.sf_col;
     const int fold = 1 << p.fold_log, part = kBlockRows >> p.fold_log;  // rows of a part
     constexpr uint32_t kScaleCols = mx_scale_cols(NW), kTokenCols = NW < 4 ? 4 : NW;  // of a stage, and of a half of its tokens
-    MxSegs segs;
-    segs.init(p, s_split, worker, workers, tables);
-    const int total = segs.total_units();
-    auto tile_cols = [&] { return (segs.valid + 8 * CG - 1) & -(8 * CG); };  // tokens that the tile's MMAs cover
+    MxTiles tile;
+    tile.init(p, worker, workers, tables);
+    const int total = tile.total_units();
+    auto tile_cols = [&] { return (tile.valid + 8 * CG - 1) & -(8 * CG); };  // tokens that the tile's MMAs cover
 
     if (RESIDENT && warp != 1) {  // the weights are on their way meanwhile
         depend();
@@ -399,13 +350,13 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
             int second = 0;  // which accumulator
             // -------------------------------------------------------------- MMA issue
             constexpr uint64_t sw128 = ((uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29))) << 32;  // 8-row groups 1024 bytes apart, version 1, 128-byte swizzle
-            while (ok && segs.next()) {
+            while (ok && tile.next()) {
                 const uint32_t idesc = mx_idesc<CG>(p.fold_log ? p.d_cols : tile_cols(), 0);
                 constexpr uint32_t kHalf = mx_idesc<CG>(0, 1) ^ mx_idesc<CG>(0, 0);
                 ok = mbar_wait_warp(d_empty + 8 * rd.idx, rd.phase ^ 1, abort_flag, p.status, 203);
                 const uint32_t d = tmem + (uint32_t)(second * p.d_step);
                 second ^= 1;
-                for (int c = segs.c0; ok && c < segs.c1; ++c) {
+                for (int c = 0; ok && c < p.units; ++c) {
                     ok = mbar_wait_warp(full + 8 * ru.idx, ru.phase, abort_flag, p.status, 204);
                     if (!ok) break;
                     tc_fence_after();
@@ -418,13 +369,13 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                         for (int kk = 0; kk < 4; ++kk)
                             if (kk < steps)
                                 tc_mma_mx<CG>(d, a + 2 * kk, b + 2 * kk, (kk & 1) ? idesc ^ kHalf : idesc, sfa + 4 * (kk >> 1), sfb + kTokenCols * (kk >> 1),
-                                              c == segs.c0 && kk == 0 ? 0u : 1u);
+                                              c == 0 && kk == 0 ? 0u : 1u);
                         if (CG == 1) {
                             tc_commit(empty + 8 * ru.idx);
-                            if (c + 1 == segs.c1) tc_commit(d_full + 8 * rd.idx);
+                            if (c + 1 == p.units) tc_commit(d_full + 8 * rd.idx);
                         } else {
                             tc_commit_pair(empty + 8 * ru.idx);
-                            if (c + 1 == segs.c1) tc_commit_pair(d_full + 8 * rd.idx);
+                            if (c + 1 == p.units) tc_commit_pair(d_full + 8 * rd.idx);
                         }
                     }
                     __syncwarp();
@@ -439,10 +390,10 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
         bool ok = true;
         int issued = 0;
         if (!p.ahead) depend();
-        while (ok && segs.next()) {
-            const int block = CG * segs.rt + rank, row = mx_row(p, block), rows = mx_row(p, block + 1) - row;
+        while (ok && tile.next()) {
+            const int block = CG * tile.rt + rank, row = mx_row(p, block), rows = mx_row(p, block + 1) - row;
             const CUtensorMap *map = !p.flex || rows == 8 * div_up(p.groups, p.row_tiles) ? &tmap_w : &tmap_w2;  // boxes of the taller and of the lower tiles
-            for (int c = segs.c0; c < segs.c1; ++c, ru.advance(S)) {
+            for (int c = 0; c < p.units; ++c, ru.advance(S)) {
                 if (issued++ == S) depend();
                 ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 200);
                 if (!ok) break;
@@ -451,8 +402,8 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                     mbar_expect_tx(bar, (uint32_t)(rows << p.fold_log) * kMxChunkBytes + kMxScaleBytes);
                     for (int f = 0; f < fold; ++f) {  // chunks behind the last one read as zeros
                         const int chunk = (c << p.fold_log) + f;
-                        tma_load_3d(base + (uint32_t)ru.idx * w_bytes + (uint32_t)(f * part) * kMxChunkBytes, map, 0, row, segs.e * p.chunks + chunk, bar);
-                        tma_load_2d(ws_ring + (uint32_t)ru.idx * kMxScaleBytes + (uint32_t)(f * part) * 8u, &tmap_ws, row, segs.e * p.words + 2 * chunk, bar);
+                        tma_load_3d(base + (uint32_t)ru.idx * w_bytes + (uint32_t)(f * part) * kMxChunkBytes, map, 0, row, tile.e * p.chunks + chunk, bar);
+                        tma_load_2d(ws_ring + (uint32_t)ru.idx * kMxScaleBytes + (uint32_t)(f * part) * 8u, &tmap_ws, row, tile.e * p.words + 2 * chunk, bar);
                     }
                 }
                 __syncwarp();
@@ -469,9 +420,9 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
         constexpr int kPieces = NW == 8 ? 2 : 1;  // 128 words each
         const uint32_t xs_copy = (uint32_t)(min(N, 128) + 4) * 4u;
         depend();
-        while (ok && segs.next()) {
-            const int tok = segs.tok0 + rank * (tile_cols() / CG);
-            for (int c = segs.c0; c < segs.c1; ++c, ru.advance(S)) {
+        while (ok && tile.next()) {
+            const int tok = tile.tok0 + rank * (tile_cols() / CG);
+            for (int c = 0; c < p.units; ++c, ru.advance(S)) {
                 ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 211);
                 if (!ok) break;
                 if (elect_one_sync()) {
@@ -484,7 +435,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
 #pragma unroll
                             for (int j = 0; j < kPieces; ++j)
                                 tma_load_1d(xs_ring + (uint32_t)(ru.idx * p.xs_bytes + (kPieces * h + j) * p.xs_pitch), &tmap_xs,
-                                            (int)((((unsigned)(2 * c + h) * (unsigned)p.n + (unsigned)segs.tok0) & ~3u) + 128u * j), bar);
+                                            (int)((((unsigned)(2 * c + h) * (unsigned)p.n + (unsigned)tile.tok0) & ~3u) + 128u * j), bar);
                     }
                 }
                 __syncwarp();
@@ -495,19 +446,19 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
         Ring ru;
         bool ok = true;
         depend();
-        while (ok && segs.next()) {
-            for (int c = segs.c0; c < segs.c1; ++c, ru.advance(S)) {
+        while (ok && tile.next()) {
+            for (int c = 0; c < p.units; ++c, ru.advance(S)) {
                 ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 201);
                 if (!ok) break;
                 const uint32_t to = xs_ring + (uint32_t)(ru.idx * p.xs_bytes) + 4u * lane;
 #pragma unroll
                 for (int j = 0; j < NW; ++j) {  // token t of the stage's chunk f: zeros behind the last word, where the codes are zeros too
                     const int f = p.fold_log ? (32 * j + lane) / p.x_rows : 0, t = 32 * j + lane - f * p.x_rows;
-                    if (f >= fold || t >= segs.valid) continue;  // whatever lies there scales columns that nobody reads
+                    if (f >= fold || t >= tile.valid) continue;  // whatever lies there scales columns that nobody reads
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int word = 2 * ((c << p.fold_log) + f) + h;
-                        cp_async_word(to + 128u * (NW * h + j), p.xs + (size_t)min(word, p.words - 1) * p.n + segs.tok0 + t, word < p.words);
+                        cp_async_word(to + 128u * (NW * h + j), p.xs + (size_t)min(word, p.words - 1) * p.n + tile.tok0 + t, word < p.words);
                     }
                 }
                 cp_async_arrive(landed + 8 * ru.idx);
@@ -522,8 +473,8 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
         Ring ru;
         bool ok = true;
         if (!RESIDENT) depend();
-        while (ok && segs.next()) {
-            for (int c = segs.c0; c < segs.c1; ++c, ru.advance(S)) {
+        while (ok && tile.next()) {
+            for (int c = 0; c < p.units; ++c, ru.advance(S)) {
                 // a stage's copies have landed, so its MMAs of the round before are done, and its scales may be overwritten
                 ok = mbar_wait_warp(landed + 8 * ru.idx, ru.phase, abort_flag, p.status, 212);
                 if (!ok) break;
@@ -538,7 +489,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                 uint32_t x[2 * NW];  // column 32 (i % NW) + lane, half i / NW
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t skip = NW == 2 ? 0u : (((unsigned)(2 * c + h) * (unsigned)p.n + (unsigned)segs.tok0) & 3u) * 4u;
+                    const uint32_t skip = NW == 2 ? 0u : (((unsigned)(2 * c + h) * (unsigned)p.n + (unsigned)tile.tok0) & 3u) * 4u;
 #pragma unroll
                     for (int j = 0; j < NW; ++j) {
                         const uint32_t at = NW == 2 ? (uint32_t)(NW * h + j) * 128u : (uint32_t)((NW == 8 ? 2 * h + (j >> 2) : h) * p.xs_pitch) + (uint32_t)(j & 3) * 128u + skip;
@@ -568,36 +519,26 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
         // ------------------------------------------------------------------ epilogue
         const int quarter = warp & 3, thread = threadIdx.x - 32 * kMxEpilogueWarp0;
         const uint32_t tmem_q = tmem + ((uint32_t)(32 * quarter) << 16);
-        const size_t slot_floats = (size_t)kBlockRows * N;
         OT *o = static_cast<OT *>(p.o);
         Ring rd;
         uint32_t buf = 0;
         depend();
         int row0 = 0, rows = 0;
-        // Up to 16 tokens of this thread's row, from registers.
-        auto store_direct = [&](const float (&v)[16]) {
-            OT *to = o + (size_t)segs.tok0 * p.m + row0 + thread;
-            if (thread < rows) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    if (i < segs.valid) to[(size_t)i * p.m] = mx_convert<OT>(v[i]);
-            }
-        };
-        // Tokens t0 .. t0 + 63 through a staging buffer: fill(t, at) puts 32 tokens from t on to `at`; one bulk copy per token.
+        // A staging buffer's tokens from t0 on to memory: fill(t, at) puts 32 tokens from t on to `at`; one bulk copy per token.
         auto store_block = [&](int t0, auto fill) {
             const uint32_t to = staging + buf * kStagingBytes;
             buf ^= 1;
-            if (lane < kStageTokens / 4) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the buffer's previous tokens have left it
+            if (lane < kMxStageTokens / 4) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the buffer's previous tokens have left it
             asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll
-            for (int h = 0; h < kStageTokens; h += 32)
-                if (t0 + h < segs.valid) fill(t0 + h, to + h * kTokPitch);
+            for (int h = 0; h < kMxStageTokens; h += 32)
+                if (t0 + h < tile.valid) fill(t0 + h, to + h * kTokPitch);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (lane < kStageTokens / 4) {
-                const int t = kStageTokens / 4 * quarter + lane;
-                if (t0 + t < segs.valid && rows > 0)
-                    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(o + (size_t)(segs.tok0 + t0 + t) * p.m + row0),
+            if (lane < kMxStageTokens / 4) {
+                const int t = kMxStageTokens / 4 * quarter + lane;
+                if (t0 + t < tile.valid && rows > 0)
+                    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(o + (size_t)(tile.tok0 + t0 + t) * p.m + row0),
                                  "r"(to + (uint32_t)t * kTokPitch), "r"((uint32_t)rows * (uint32_t)sizeof(OT))
                                  : "memory");
                 asm volatile("cp.async.bulk.commit_group;" ::: "memory");
@@ -636,108 +577,55 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
             }
         };
         int second = 0;
-        for (; segs.next(); second ^= 1) {
+        for (; tile.next(); second ^= 1) {
             const bool ok = mbar_wait_warp(d_full + 8 * rd.idx, rd.phase, abort_flag, p.status, 206);
             if (bar_any(1, 128, !ok)) break;  // the four warps go on together or not at all
             tc_fence_after();
             const uint32_t d = tmem_q + (uint32_t)(second * p.d_step);
-            row0 = mx_row(p, CG * segs.rt + rank);
-            rows = min(mx_row(p, CG * segs.rt + rank + 1), p.m) - row0;
+            row0 = mx_row(p, CG * tile.rt + rank);
+            rows = min(mx_row(p, CG * tile.rt + rank + 1), p.m) - row0;
             if (p.fold_log) {
                 // Part f's sums of row i are lane part * f + i, columns x_rows * f ..: added up in the order of the parts.
                 const int f = thread >> (7 - p.fold_log);
                 float *sums = reinterpret_cast<float *>(smem + (staging - base));
-                for (int t0 = 0; t0 < segs.valid; t0 += 16) {
-                    float v[16];
-                    tc_ld_x16(d + f * p.x_rows + t0, v);
+                float v[16];
+                tc_ld_x16(d + f * p.x_rows, v);
 #pragma unroll
-                    for (int t = 0; t < 16; ++t)
-                        if (t0 + t < segs.valid) sums[(t0 + t) * kBlockRows + thread] = v[t];
-                }
+                for (int t = 0; t < 16; ++t)
+                    if (t < tile.valid) sums[t * kBlockRows + thread] = v[t];
                 drained();
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 const int i = thread & (part - 1);
-                for (int t = f; t < segs.valid && i < rows; t += fold) {
+                for (int t = f; t < tile.valid && i < rows; t += fold) {
                     float sum = sums[t * kBlockRows + i];
                     for (int g = 1; g < fold; ++g) sum += sums[t * kBlockRows + g * part + i];
-                    o[(size_t)(segs.tok0 + t) * p.m + row0 + i] = mx_convert<OT>(sum);
+                    o[(size_t)(tile.tok0 + t) * p.m + row0 + i] = mx_convert<OT>(sum);
                 }
                 asm volatile("bar.sync 1, 128;" ::: "memory");  // they have been read
-            } else if (segs.c0 == 0 && segs.c1 == p.units) {
-                if (N <= kMxDirectTokens) {
-                    float v[16];
-                    tc_ld_x16(d, v);
-                    drained();
-                    store_direct(v);
-                } else {
-                    // Of two accumulators that overlap, the columns they share first: then the other one may be written.
-                    const bool shared = p.nd == 1 && p.d_step;
-                    const int turn = shared && second == 0 ? p.d_step : 0;
-                    for (int b = 0; b < N; b += kStageTokens) {
-                        const int t0 = b + turn < N ? b + turn : b + turn - N;
-                        if (t0 < segs.valid) store_block(t0, [&](int t, uint32_t at) { fill_from(d, t, at); });
-                        if (shared && b + kStageTokens == N - p.d_step) drained();
-                    }
-                    if (!shared) drained();
+            } else if (N <= kMxDirectTokens) {
+                float v[16];
+                tc_ld_x16(d, v);
+                drained();
+                OT *to = o + (size_t)tile.tok0 * p.m + row0 + thread;
+                if (thread < rows) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (i < tile.valid) to[(size_t)i * p.m] = mx_convert<OT>(v[i]);
                 }
             } else {
-                // [4-token group][128 lanes] float4: a warp store is 512 contiguous bytes
-                float4 *dst = reinterpret_cast<float4 *>(p.partials + (size_t)(2 * blockIdx.x + (segs.c0 == 0 ? 1 : 0)) * slot_floats) + thread;
-                for (int t0 = 0; t0 < segs.valid; t0 += 16) {
-                    float v[16];
-                    tc_ld_x16(d + t0, v);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) dst[(size_t)(t0 / 4 + i) * kBlockRows] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+                // Of two accumulators that overlap, the columns they share first: then the other one may be written.
+                const bool shared = p.nd == 1 && p.d_step;
+                const int turn = shared && second == 0 ? p.d_step : 0;
+                for (int b = 0; b < N; b += kMxStageTokens) {
+                    const int t0 = b + turn < N ? b + turn : b + turn - N;
+                    if (t0 < tile.valid) store_block(t0, [&](int t, uint32_t at) { fill_from(d, t, at); });
+                    if (shared && b + kMxStageTokens == N - p.d_step) drained();
                 }
-                drained();
-                auto worker_of = [&](int unit) {
-                    const int big = s_split.sk_r * (s_split.sk_q + 1);
-                    return unit < big ? unit / (s_split.sk_q + 1) : s_split.sk_r + (unit - big) / s_split.sk_q;
-                };
-                const int first = worker_of(segs.tile * p.units), nseg = worker_of((segs.tile + 1) * p.units - 1) - first + 1;
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                if (thread == 0) {
-                    unsigned int old;
-                    // releases the four warps' partials (ordered before it by the barrier) and acquires the others'
-                    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(old) : "l"(p.counters + CG * segs.tile + rank) : "memory");
-                    s_last = old == (unsigned)nseg - 1;
-                    if (s_last) p.counters[CG * segs.tile + rank] = 0;  // left clean for the next call
-                }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                if (s_last) {
-                    auto sum16 = [&](int t, float (&v)[16]) {
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] = 0.f;
-                        for (int s = 0; s < nseg; ++s) {
-                            const float4 *src = reinterpret_cast<const float4 *>(p.partials + (size_t)(2 * (CG * (first + s) + rank) + (s == 0 ? 1 : 0)) * slot_floats) + (size_t)(t / 4) * kBlockRows + thread;
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const float4 w = __ldcg(src + i * kBlockRows);
-                                v[4 * i] += w.x; v[4 * i + 1] += w.y; v[4 * i + 2] += w.z; v[4 * i + 3] += w.w;
-                            }
-                        }
-                    };
-                    if (N <= kMxDirectTokens) {
-                        float v[16];
-                        sum16(0, v);
-                        store_direct(v);
-                    } else {
-                        for (int t0 = 0; t0 < segs.valid; t0 += kStageTokens)
-                            store_block(t0, [&](int t, uint32_t at) {
-                                for (int h = 0; h < 32 && t + h < segs.valid; h += 16) {
-                                    float v[16];
-                                    sum16(t + h, v);
-#pragma unroll
-                                    for (int i = 0; i < 16; ++i) mx_store_shared(at + (uint32_t)(h + i) * kTokPitch + (uint32_t)thread * (uint32_t)sizeof(OT), mx_convert<OT>(v[i]));
-                                }
-                            });
-                    }
-                }
-                asm volatile("bar.sync 1, 128;" ::: "memory");  // s_last has been read
+                if (!shared) drained();
             }
             rd.advance(p.nd);
         }
-        if (lane < kStageTokens / 4) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        if (lane < kMxStageTokens / 4) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 
     __syncwarp();
@@ -756,69 +644,91 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
 struct MxPlan {
     int cg, tile_tok, words, stages, nd, d_cols, d_step, sf_col;
     bool resident;
-    int flex, fold_log, row_tiles, cut, w_bytes, x_rows, xs_copy, xs_pitch, xs_bytes;
+    int flex, fold_log, row_tiles, w_bytes, x_rows, xs_copy, xs_pitch, xs_bytes;
     int workers;
     size_t smem;
 };
 
+// Microseconds that tiles of 256 rows and `cols` tokens take on `pairs` pairs: rounds of tiles, each with its steps of 256 columns
+// (the tensor pipe's and what comes with a step; wide tiles at the rate of the copies to shared memory as well) and, of wide
+// tiles, what of the epilogue nothing hides; what all tiles copy, from L2; the weights, from HBM.  Fitted to 550 launches
+// (graph replay; 7 matrices from 1024x1024 to 57344x8192, 17 to 2048 tokens, every width): what it chooses takes 2 % longer than
+// the fastest width in the mean, 15 % at worst.
+static double mx_pair_us(int m, int n, int k, int cols, int pairs)
+{
+    const int row_tiles = div_up(m, 2 * kBlockRows), chunks = div_up(k, kMxChunk);
+    const double tiles = (double)row_tiles * div_up(n, cols);
+    const double rounds = std::ceil(tiles / pairs);
+    const double step = cols <= 128 ? 0.186 : 0.043 + 0.00104 * cols;
+    const double work = rounds * (std::max(0.0, 0.0144 * cols - 0.5) + chunks * step);
+    const double copies = tiles * (2 * kBlockRows + cols) * chunks * 136.0 / 22.4e6, weights = (double)m * k * (17.0 / 32) / 8.3e6;
+    return std::sqrt(work * work + copies * copies + weights * weights);
+}
+
+static int mx_pair_tokens(int m, int n, int k, int pairs)
+{
+    int best = 0;
+    double best_us = 0;
+    for (int cols = 256; cols >= 16; cols -= cols > 128 ? 32 : 16) {
+        if (cols - 16 >= n) continue;  // wider than the tokens
+        const double us = mx_pair_us(m, n, k, cols, pairs);
+        if (!best || us < best_us) best = cols, best_us = us;
+    }
+    return best;
+}
+
+// Tokens of a tile of experts: their numbers are on the device, so it goes by the mean.  Narrow enough that an expert of the mean
+// size fills a good part of a tile, wide enough that popular ones do not read their weights often (us, 64 / 128 / 192 / 256: eight experts
+// 28672x4096 of 4 in the mean 70 / - / - / -, eight 4096x14336 of 37 52 / 44 / 47 / 48 and of 187 103 / 75 / 73 / 74, sixteen 4096x4096 of
+// 250 75 / 56 / 60 / 56, 64 2048x1024 of 2 14.5 / - / - / -).
+static int mx_expert_tokens(int mean) { return mean <= 24 ? 64 : mean <= 128 ? 128 : 256; }
+
 static MxPlan mx_plan(int m, int n, int k, int experts, int x_type, int o_type, bool grouped, int sm_count)
 {
     MxPlan l = {};
-    const int each = div_up(n, experts), chunks = div_up(k, kMxChunk);
-    l.cg = each > 128 ? 2 : 1;
-    l.tile_tok = std::min(l.cg == 2 ? 256 : 128, div_up(each, 16) * 16);
-    if (grouped) l.tile_tok = each <= 16 ? 16 : each <= 32 ? 32 : each <= 64 ? 64 : each <= 128 ? 128 : 256;
-    if (!grouped && l.cg == 1) l.flex = 1;
-    int rt = 0, fl = -1;
-    if (const char *env = getenv("MXPLAN")) {  // cg,N,flex[,row tiles,fold]
-        sscanf(env, "%d,%d,%d,%d,%d", &l.cg, &l.tile_tok, &l.flex, &rt, &fl);
-        if (l.cg == 2) l.flex = 0;
-    }
-    l.cut = l.cg == 1;
-    l.row_tiles = div_up(m, kBlockRows * l.cg);
-    l.w_bytes = kBlockRows * kMxChunkBytes;
-    if (l.flex) {
-        const int waves = div_up(m, kBlockRows * sm_count);
-        l.row_tiles = std::min(m / 8, waves * sm_count);
-        if (rt >= div_up(m, kBlockRows) && rt <= m / 8) l.row_tiles = rt;
-        l.cut = 0;
-        const int height = 8 * div_up(m / 8, l.row_tiles);
-        l.fold_log = height <= 32 && n <= 16 ? 2 : height <= 64 && n <= kMxFoldTokens ? 1 : 0;
-        if (fl >= 0) l.fold_log = std::min(l.fold_log, fl);
-        if (!l.fold_log) l.w_bytes = height * kMxChunkBytes;
-    }
+    const int chunks = div_up(k, kMxChunk);
+    l.cg = grouped || n > kMxDirectTokens ? 2 : 1;
     l.workers = sm_count / l.cg;
+    if (l.cg == 1) {
+        l.flex = 1;
+        l.tile_tok = kMxDirectTokens;
+        l.row_tiles = std::min(m / 8, div_up(m, kBlockRows * sm_count) * sm_count);
+        const int height = 8 * div_up(m / 8, l.row_tiles);
+        l.fold_log = height <= 32 ? 2 : height <= 64 ? 1 : 0;
+        l.w_bytes = (l.fold_log ? kBlockRows : height) * kMxChunkBytes;
+    } else {
+        l.tile_tok = grouped ? mx_expert_tokens(div_up(n, experts)) : mx_pair_tokens(m, n, k, l.workers);
+        l.row_tiles = div_up(m, 2 * kBlockRows);
+        l.w_bytes = kBlockRows * kMxChunkBytes;
+    }
     const int fold = 1 << l.fold_log;
     l.x_rows = l.fold_log ? div_up(n, 8) * 8 : l.tile_tok / l.cg;
     l.d_cols = l.fold_log ? l.x_rows * fold : l.tile_tok;
-    const int words = l.words = std::max(mx_token_words(l.d_cols), 2 * l.cg);
-    const size_t room = words == 2 ? 111 * 1024 : kMxSmemMax - 2048;
+    const int words = l.words = l.cg == 1 ? 2 : std::max(4, mx_token_words(l.d_cols));  // the kernels that there are: launch_mx_as
+    const size_t room = words == 2 ? kMxSmemHalf : kMxSmemMax;
     const size_t pitch = kBlockRows * (o_type == TUNA_FP32 ? 4 : 2) + (o_type == TUNA_FP32 ? 0 : 16);
-    const size_t tail = (l.fold_log ? kMxFoldBytes : l.tile_tok > kMxDirectTokens ? 2 * mx_stage_tokens(words) * pitch : 0) + (3 * (size_t)experts + 1) * 4 +
-                        kMxSlackBytes;
+    size_t fixed = (l.fold_log ? kMxFoldBytes : l.tile_tok > kMxDirectTokens ? 2 * kMxStageTokens * pitch : 0) + (3 * (size_t)experts + 1) * 4 + kMxSlackBytes;
     const size_t w_stage = (size_t)l.w_bytes + kMxScaleBytes;
     l.xs_copy = std::min(l.tile_tok, 128) + 4;  // words
     l.xs_pitch = div_up(l.xs_copy * 4, 128) * 128;
     l.xs_bytes = words == 2 ? 512 : 2 * (words == 8 ? 2 : 1) * l.xs_pitch;
     size_t x_stage = (size_t)l.x_rows * fold * kMxChunkBytes + l.xs_bytes;
-    // tokens' codes that stay in shared memory: what is left has to hold stages enough
-    const size_t resident = (size_t)div_up(chunks, fold) * (div_up(n, 8) * 8 * fold * kMxChunkBytes + 512);
-    l.resident = x_type != TUNA_MXFP4 && !grouped && n * div_up(chunks, fold) * fold <= 4 * (kMxWarps - 1) && l.flex && resident + 4 * w_stage + tail <= room && resident + 60 * 1024 <= room;
-    size_t fixed = tail;
+    // Tokens that the CTAs quantize themselves: one round of the quantizing warps, and shared memory left for stages enough.  (4096x4096 in
+    // bf16, us, so / a quantizing launch before it: 1 token 4.7 / 6.8, 4 tokens 7.2 / 6.6.)
+    const int rows8 = div_up(n, 8) * 8, units = div_up(chunks, fold);
+    const size_t resident = (size_t)units * (rows8 * fold * kMxChunkBytes + l.xs_bytes);
+    l.resident = l.cg == 1 && x_type != TUNA_MXFP4 && n * units * fold <= 4 * (kMxWarps - 1) && resident + 4 * w_stage + fixed <= room;
     if (l.resident) {
-        l.x_rows = div_up(n, 8) * 8;
+        l.x_rows = rows8;
         fixed += resident;
         x_stage = 0;
     }
     l.stages = (int)std::min<size_t>(kMxMaxStages, (room - fixed) / (w_stage + x_stage));
     const int tmem_cols = words == 2 ? 256 : 512, scale_cols = (int)mx_scale_cols(words);
     l.nd = 2 * l.d_cols + l.stages * scale_cols <= tmem_cols ? 2 : 1;
-    l.d_step = l.nd == 2 ? l.d_cols : 0;
-    // two accumulators of which the columns in the middle are shared, where two whole ones do not fit
-    if (l.nd == 1 && l.cg == 2 && l.d_cols % (2 * mx_stage_tokens(words)) == 0) {
-        l.d_step = l.d_cols / 2;
-        l.stages = std::min(l.stages, (tmem_cols - l.d_cols - l.d_step) / scale_cols);
-    }
+    // two accumulators that share the columns in the middle, where two whole ones do not fit
+    if (l.nd == 2) l.d_step = l.d_cols;
+    else if (l.cg == 2 && l.d_cols % (2 * kMxStageTokens) == 0) l.d_step = l.d_cols / 2;
     l.sf_col = l.d_cols + l.d_step;
     l.stages = std::min(l.stages, (tmem_cols - l.sf_col) / scale_cols);
     // the last stage's MMAs read 128 rows
@@ -826,17 +736,10 @@ static MxPlan mx_plan(int m, int n, int k, int experts, int x_type, int o_type, 
     return l;
 }
 
-// Whether the product quantizes tokens of this type itself; otherwise it wants their codes and scales.
 bool mx_gemm_takes(int m, int n, int k, int experts, int x_type, bool grouped, int sm_count)
 {
-    return x_type == TUNA_MXFP4 || mx_plan(m, n, k, experts, x_type, TUNA_FP16, grouped, sm_count).resident;
-}
-
-size_t mx_gemm_workspace_bytes(int m, int n, int k, int experts, int sm_count)
-{
-    size_t floats = 0;  // of the plan for one matrix and the one for experts
-    for (int grouped = 0; grouped < 2; ++grouped) floats = std::max(floats, (size_t)kBlockRows * mx_plan(m, n, k, experts, TUNA_MXFP4, TUNA_FP16, grouped, sm_count).tile_tok);
-    return kMxCounterBytes + 2 * (size_t)sm_count * floats * 4;
+    if (x_type == TUNA_MXFP4) return true;
+    return !grouped && n <= kMxDirectTokens && mx_plan(m, n, k, experts, x_type, TUNA_FP16, grouped, sm_count).resident;
 }
 
 struct MxMaps {
@@ -853,7 +756,7 @@ static int launch_mx(const MxParams &p, const MxMaps &maps, int ctas, size_t sme
     {
         std::lock_guard<std::mutex> lock(mu);
         if (!attr_set[dev]) {
-            if (cudaFuncSetAttribute(mx_gemm_kernel<CG, NW, RESIDENT, OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMxSmemMax - 2048) != cudaSuccess) return TUNA_ERR_NO_DEVICE;
+            if (cudaFuncSetAttribute(mx_gemm_kernel<CG, NW, RESIDENT, OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kMxSmemMax) != cudaSuccess) return TUNA_ERR_NO_DEVICE;
             attr_set[dev] = true;
         }
     }
@@ -876,12 +779,8 @@ static int launch_mx(const MxParams &p, const MxMaps &maps, int ctas, size_t sme
 template <typename OT>
 static int launch_mx_as(const MxPlan &l, const MxParams &p, const MxMaps &maps, int ctas, cudaStream_t stream)
 {
-    switch (10 * l.cg + l.words) {
-        case 12: return l.resident ? launch_mx<1, 2, true, OT>(p, maps, ctas, l.smem, stream) : launch_mx<1, 2, false, OT>(p, maps, ctas, l.smem, stream);
-        case 14: return launch_mx<1, 4, false, OT>(p, maps, ctas, l.smem, stream);
-        case 28: return launch_mx<2, 8, false, OT>(p, maps, ctas, l.smem, stream);
-        default: return launch_mx<2, 4, false, OT>(p, maps, ctas, l.smem, stream);
-    }
+    if (l.cg == 1) return l.resident ? launch_mx<1, 2, true, OT>(p, maps, ctas, l.smem, stream) : launch_mx<1, 2, false, OT>(p, maps, ctas, l.smem, stream);
+    return l.words == 4 ? launch_mx<2, 4, false, OT>(p, maps, ctas, l.smem, stream) : launch_mx<2, 8, false, OT>(p, maps, ctas, l.smem, stream);
 }
 
 int launch_mx_gemm(const MxGemmArgs &a)
@@ -897,15 +796,17 @@ int launch_mx_gemm(const MxGemmArgs &a)
     p.words = div_up(a.k, kMxScaleCols);
     p.last_steps = div_up(a.k - (p.chunks - 1) * kMxChunk, 64);
     p.units = div_up(p.chunks, 1 << l.fold_log); p.fold_log = l.fold_log;
-    p.row_tiles = l.row_tiles; p.w_bytes = l.w_bytes; p.x_rows = l.x_rows; p.xs_pitch = l.xs_pitch; p.xs_bytes = l.xs_bytes; p.flex = l.flex; p.groups = a.m / 8; p.cut = l.cut;
+    p.row_tiles = l.row_tiles; p.w_bytes = l.w_bytes; p.flex = l.flex; p.groups = a.m / 8;
+    p.x_rows = l.x_rows; p.xs_pitch = l.xs_pitch; p.xs_bytes = l.xs_bytes;
     p.stages = l.stages; p.nd = l.nd; p.d_cols = l.d_cols; p.d_step = l.d_step; p.sf_col = l.sf_col;
     p.ahead = a.offsets == nullptr && a.n <= kMxAheadTokens;
-    p.counters = (unsigned int *)a.workspace;
-    p.partials = (float *)((uint8_t *)a.workspace + kMxCounterBytes);
     p.status = device_status_word();
     if (!p.status) return TUNA_ERR_NO_DEVICE;
+    // the kernel numbers tiles, a worker's stages, and words of scales in 32 bits
     const long long tiles = ((long long)div_up(a.n, l.tile_tok) + a.experts - 1) * p.row_tiles;  // at most
-    if (tiles >= 1ll << 30 || (tiles / l.workers + 2) * p.chunks >= 1ll << 30 || (long long)a.sm_count * p.chunks >= 1ll << 30 || (long long)a.experts * p.words >= 1ll << 30 || (long long)(p.words + 8) * a.n >= 1ll << 31) return TUNA_ERR_TOO_LARGE;
+    if (tiles >= 1ll << 30 || (tiles / l.workers + 2) * p.chunks >= 1ll << 30 || (long long)a.experts * p.words >= 1ll << 30 ||
+        (long long)(p.words + 8) * a.n >= 1ll << 31)
+        return TUNA_ERR_TOO_LARGE;
 
     MxMaps maps;
     auto tiles_of = [](CUtensorMap *map, const void *at, uint64_t rows, uint64_t chunks, uint32_t box_rows, uint32_t box_chunks) {  // [chunks][rows][128 bytes]
@@ -915,9 +816,9 @@ int launch_mx_gemm(const MxGemmArgs &a)
     if (!tiles_of(&maps.w, a.q, (uint64_t)a.m, (uint64_t)a.experts * p.chunks, l.flex ? 8u * (uint32_t)div_up(p.groups, l.row_tiles) : kBlockRows, 1)) return TUNA_ERR_NO_DEVICE;
     maps.w2 = maps.x = maps.xs = maps.w;
     if (l.flex && p.groups % l.row_tiles && !tiles_of(&maps.w2, a.q, (uint64_t)a.m, (uint64_t)p.chunks, 8u * (uint32_t)(p.groups / l.row_tiles), 1)) return TUNA_ERR_NO_DEVICE;
-    if (!l.resident && !tiles_of(&maps.x, a.x, (uint64_t)a.n, (uint64_t)p.chunks, (uint32_t)l.x_rows, 1u << l.fold_log)) return TUNA_ERR_NO_DEVICE;
     if (!make_tensor_map_2d(&maps.ws, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.s, (uint64_t)a.m, (uint64_t)a.experts * p.words, (uint64_t)a.m * 4, (uint32_t)kBlockRows >> l.fold_log, 2, CU_TENSOR_MAP_SWIZZLE_NONE))
         return TUNA_ERR_NO_DEVICE;
+    if (!l.resident && !tiles_of(&maps.x, a.x, (uint64_t)a.n, (uint64_t)p.chunks, (uint32_t)l.x_rows, 1u << l.fold_log)) return TUNA_ERR_NO_DEVICE;
     if (l.words > 2) {
         const uint64_t dim = (uint64_t)p.words * a.n;
         const uint32_t box = (uint32_t)l.xs_copy;

@@ -21,7 +21,6 @@ from .ops import _expect, _on_device, _stream_ptr
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _MXFP4 = 3
-_workspaces: dict = {}
 
 
 class _NoFront:
@@ -42,7 +41,7 @@ def _front():
         return _NoFront
     lib = _lib.load()
     front.bind_mx(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in
-                    ("tuna_mx_quantize", "tuna_mx_dequant", "tuna_mx_matmul", "tuna_mx_matmul_grouped", "tuna_stream_capture_id")), _workspaces)
+                    ("tuna_mx_quantize", "tuna_mx_dequant", "tuna_mx_matmul", "tuna_mx_matmul_grouped", "tuna_mx_workspace_bytes")))
     return front
 
 
@@ -78,22 +77,13 @@ def _expect_output(o, numel, device):
     _expect(o, "o", o.dtype, numel, device)
 
 
-def _workspace(need: int, device) -> torch.Tensor:
-    """The workspace of `device`'s current stream.  A graph that is being captured gets one of its own, from its own pool, whose
-    counters it zeroes at every replay: graphs may be replayed side by side, and beside calls on the stream that captured them."""
-    stream = _stream_ptr(device)
-    lib = _lib.load()
-    capture = int(lib.tuna_stream_capture_id(stream))
-    key = (device.index, stream, capture)
-    ws = _workspaces.get(key)
-    if ws is None or ws.numel() < need:
-        if capture:  # those of finished captures stay reserved in their graphs' pools without a reference from here
-            for old in [k for k in _workspaces if k[0] == device.index and k[2] not in (0, capture)]:
-                _workspaces.pop(old, None)
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
-        ws[:int(lib.tuna_mx_workspace_zero_bytes())].zero_()
-        _workspaces[key] = ws
-    return ws
+def _workspace(given, *shape_and_type):
+    """Address and size of the workspace: `given`, or one of this call's own (in stream order, from the pool of the graph that is being captured,
+    if one is)."""
+    if given is None:
+        need = int(_lib.load().tuna_mx_workspace_bytes(*shape_and_type))
+        given = torch.empty(need, dtype=torch.uint8, device="cuda") if need else None
+    return given, (0, 0) if given is None else (given.data_ptr(), given.numel() * given.element_size())
 
 
 def mx_quantize(x):
@@ -167,9 +157,9 @@ def mx_matmul(x, xs, q, s, o, m: int, n: int, k: int, *, workspace=None) -> None
     _expect_output(o, n * m, dev)
     lib = _lib.load()
     with _on_device(dev):
-        ws = workspace if workspace is not None else _workspace(int(lib.tuna_mx_workspace_bytes(m, n, k, 1, kind)), dev)
+        _keep, ws = _workspace(workspace, m, n, k, 1, kind)
         check(lib.tuna_mx_matmul(x.data_ptr(), kind, 0 if xs is None else xs.data_ptr(), q.data_ptr(), s.data_ptr(), o.data_ptr(), _TYPES[o.dtype], m, n, k,
-                                 ws.data_ptr(), ws.numel() * ws.element_size(), _stream_ptr(dev)))
+                                 *ws, _stream_ptr(dev)))
 
 
 def mx_matmul_grouped(x, xs, q, s, offsets, o, m: int, n: int, k: int, *, workspace=None) -> None:
@@ -191,9 +181,9 @@ def mx_matmul_grouped(x, xs, q, s, offsets, o, m: int, n: int, k: int, *, worksp
         return
     lib = _lib.load()
     with _on_device(dev):
-        ws = workspace if workspace is not None else _workspace(int(lib.tuna_mx_workspace_bytes(m, n, k, experts, kind)), dev)
+        _keep, ws = _workspace(workspace, m, n, k, experts, kind)
         check(lib.tuna_mx_matmul_grouped(x.data_ptr(), kind, 0 if xs is None else xs.data_ptr(), q.data_ptr(), s.data_ptr(), offsets.data_ptr(), o.data_ptr(),
-                                         _TYPES[o.dtype], m, n, k, experts, ws.data_ptr(), ws.numel() * ws.element_size(), _stream_ptr(dev)))
+                                         _TYPES[o.dtype], m, n, k, experts, *ws, _stream_ptr(dev)))
 
 
 def mx_pack(codes, scales):
