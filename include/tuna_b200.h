@@ -293,7 +293,7 @@ int tuna_mx_dequant(const void *q, const void *s, void *o, int o_type, int rows,
  * bit-identical from run to run.  x_type TUNA_MXFP4: x and xs are codes and scales of the tokens.  TUNA_FP16 or TUNA_BF16: x is
  * [n, k] of that type, xs is not read, and the call quantizes x as tuna_mx_quantize does.  m a multiple of 8, k of 32, any
  * n >= 1.  Alignment: 16 bytes.
- * Workspace: tuna_mx_workspace_bytes (with experts = 1) bytes for the codes and scales of tokens in 16 bits, none for
+ * Workspace: tuna_mx_workspace_bytes (experts = 0 for this call) bytes for the codes and scales of tokens in 16 bits, none for
  * TUNA_MXFP4; it is written before it is read.  Calls that overlap on the device need separate ones.
  * Order: ordinary stream order for everything but q and s of a tuna_mx_matmul of up to 64 tokens, which count as constants as in
  * tuna_matmul: a kernel that writes them right before such a call must not let dependent launches start early (this library's

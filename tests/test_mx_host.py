@@ -96,8 +96,8 @@ def test_argument_validation_needs_no_gpu(tuna_lib):
     assert mm(x_type=2) == -5 and mm(x_type=4) == -5 and mm(o_type=3) == -5
     assert mm(x=odd) == -3 and mm(xs=odd) == -3 and mm(q=odd) == -3 and mm(s=odd) == -3 and mm(o=odd) == -3 and mm(ws=odd) == -3
     # tokens in 16 bits that a launch of their own quantizes: room for their codes and scales
-    need = tuna_lib.tuna_mx_workspace_bytes(64, 33, 64, 1, 0)
-    assert need >= 33 * (128 + 4) and tuna_lib.tuna_mx_workspace_bytes(64, 33, 64, 1, 3) == 0
+    need = tuna_lib.tuna_mx_workspace_bytes(64, 33, 64, 0, 0)
+    assert need >= 33 * (128 + 4) and tuna_lib.tuna_mx_workspace_bytes(64, 33, 64, 0, 3) == 0
     assert mm(x_type=0, n=33, ws=None) == -4 and mm(x_type=0, n=33, ws_bytes=need - 1) == -4
 
     def grouped(offsets=p, experts=2, n=4, x_type=3, ws_bytes=big):
@@ -109,7 +109,7 @@ def test_argument_validation_needs_no_gpu(tuna_lib):
     assert grouped(offsets=ctypes.c_void_p(base + 2)) == -3
     assert grouped(x_type=1, ws_bytes=0) == -4
     assert grouped(n=0) == 0 and grouped(n=-1) == -2
-    assert tuna_lib.tuna_mx_workspace_bytes(60, 1, 64, 1, 3) == 0
+    assert tuna_lib.tuna_mx_workspace_bytes(60, 33, 64, 0, 0) == 0
     assert tuna_lib.tuna_mx_workspace_bytes(64, 1, 64, 1025, 0) == 0
 
 

@@ -150,7 +150,7 @@ int launch_mx_product(PyObject *const *args, bool grouped)
                      *o = numbers(tail[0], n * m, device, &o_type);
     if (!q || !s || !o) return kPythonWay;
     void *stream = c10::cuda::getCurrentCUDAStream(device).stream();
-    const size_t bytes = packed ? 0 : g_mx.workspace_bytes((int)m, (int)n, (int)k, (int)experts, x_type);
+    const size_t bytes = packed ? 0 : g_mx.workspace_bytes((int)m, (int)n, (int)k, grouped ? (int)experts : 0, x_type);
     at::Tensor ws;  // this call's own, in stream order: what a graph captures comes from its pool
     if (bytes > 0) ws = at::detail::empty_cuda({(int64_t)bytes}, at::kByte, x->device(), std::nullopt);
     const void *xp = x->const_data_ptr(), *xsp = xs ? xs->const_data_ptr() : nullptr, *qp = q->const_data_ptr(), *sp = s->const_data_ptr(),

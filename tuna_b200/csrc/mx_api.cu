@@ -97,7 +97,6 @@ extern "C" int tuna_mx_matmul_grouped(const void *x, int x_type, const void *xs,
 
 extern "C" size_t tuna_mx_workspace_bytes(int m, int n, int k, int experts, int x_type)
 {
-    if (m < 1 || m % 8 || n < 1 || k < 1 || k % kMxBlock || experts < 1 || experts > TUNA_MX_MAX_EXPERTS) return 0;
-    const int sms = device_sm_count();
-    return std::max(experts == 1 ? mx_workspace(m, n, k, 1, x_type, false, sms).total : 0, mx_workspace(m, n, k, experts, x_type, true, sms).total);
+    if (m < 1 || m % 8 || n < 1 || k < 1 || k % kMxBlock || experts < 0 || experts > TUNA_MX_MAX_EXPERTS) return 0;
+    return mx_workspace(m, n, k, std::max(1, experts), x_type, experts > 0, device_sm_count()).total;
 }

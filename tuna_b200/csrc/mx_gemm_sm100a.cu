@@ -52,6 +52,7 @@ constexpr int kMxStageTokens = 64;      // tokens of an output staging buffer
 constexpr int kMxDirectTokens = 16;     // tiles of up to so many tokens are stored from registers
 constexpr int kMxSlackBytes = 1024;     // of shared memory at the end: scales of columns that a tile does not have are read from behind its own
 constexpr uint32_t kMxFoldBytes = kMxDirectTokens * kBlockRows * 4;  // where the parts of a folded tile are added up
+constexpr int kMxResidentRows = 8;      // loads in flight of a quantizing warp
 constexpr int kMxAheadTokens = 64;      // one matrix: up to here weights are read ahead of the dependency wait
 constexpr uint32_t kMxScaleBytes = 2 * kBlockRows * 4;  // of the weights' scales in a stage
 constexpr int kMxSmemMax = 225 * 1024;   // dynamic shared memory of a CTA alone on its SM (1 KB is the kernel's static part, 1 KB the system's)
@@ -195,10 +196,9 @@ __device__ __forceinline__ void cp_async_arrive(uint32_t bar) { asm volatile("cp
 
 // Quantizes the tokens' numbers, all of K: warp `w` of `warps` takes every warps-th (chunk, token).  Codes as TMA would have put
 // them (128-byte swizzle), scale words [stage][half][token of a chunk of the stage].
-template <typename T>
+template <typename T, int R>  // R: loads in flight
 __device__ __forceinline__ void mx_quantize_resident(const MxParams &p, int w, int warps, int lane, uint32_t codes_at, uint32_t words_at)
 {
-    constexpr int R = 4;  // loads in flight
     const int items = (p.units << p.fold_log) * p.n;  // chunks behind the last one are zeros
     for (int i0 = w; i0 < items; i0 += R * warps) {
         Mx8<T> v[R];
@@ -336,8 +336,13 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     if (RESIDENT && warp != 1) {  // the weights are on their way meanwhile
         depend();
         const int w = warp == 0 ? 0 : warp - 1;
-        if (p.x_bf16) mx_quantize_resident<__nv_bfloat16>(p, w, kMxWarps - 1, lane, x_ring, xs_ring);
-        else mx_quantize_resident<__half>(p, w, kMxWarps - 1, lane, x_ring, xs_ring);
+        auto quantize = [&](auto type) {
+            using T = decltype(type);
+            if ((p.units << p.fold_log) * p.n <= 2 * (kMxWarps - 1)) mx_quantize_resident<T, 2>(p, w, kMxWarps - 1, lane, x_ring, xs_ring);
+            else mx_quantize_resident<T, kMxResidentRows>(p, w, kMxWarps - 1, lane, x_ring, xs_ring);
+        };
+        if (p.x_bf16) quantize(__nv_bfloat16());
+        else quantize(__half());
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the MMAs read the codes
         asm volatile("bar.sync 2, %0;" ::"n"(32 * (kMxWarps - 1)) : "memory");
     }
@@ -714,10 +719,10 @@ static MxPlan mx_plan(int m, int n, int k, int experts, int x_type, int o_type, 
     l.xs_bytes = words == 2 ? 512 : 2 * (words == 8 ? 2 : 1) * l.xs_pitch;
     size_t x_stage = (size_t)l.x_rows * fold * kMxChunkBytes + l.xs_bytes;
     // Tokens that the CTAs quantize themselves: one round of the quantizing warps, and shared memory left for stages enough.  (4096x4096 in
-    // bf16, us, so / a quantizing launch before it: 1 token 4.7 / 6.8, 4 tokens 7.2 / 6.6.)
+    // bf16, us, so / a quantizing launch before it: 1 token 4.4 / 6.0, 4 tokens 5.5 / 6.4, 5 tokens 6.0 / 6.5, two rounds at 6 tokens 7.2 / 6.6.)
     const int rows8 = div_up(n, 8) * 8, units = div_up(chunks, fold);
     const size_t resident = (size_t)units * (rows8 * fold * kMxChunkBytes + l.xs_bytes);
-    l.resident = l.cg == 1 && x_type != TUNA_MXFP4 && n * units * fold <= 4 * (kMxWarps - 1) && resident + 4 * w_stage + fixed <= room;
+    l.resident = l.cg == 1 && x_type != TUNA_MXFP4 && n * units * fold <= kMxResidentRows * (kMxWarps - 1) && resident + 4 * w_stage + fixed <= room;
     if (l.resident) {
         l.x_rows = rows8;
         fixed += resident;

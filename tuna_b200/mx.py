@@ -157,7 +157,7 @@ def mx_matmul(x, xs, q, s, o, m: int, n: int, k: int, *, workspace=None) -> None
     _expect_output(o, n * m, dev)
     lib = _lib.load()
     with _on_device(dev):
-        _keep, ws = _workspace(workspace, m, n, k, 1, kind)
+        _keep, ws = _workspace(workspace, m, n, k, 0, kind)
         check(lib.tuna_mx_matmul(x.data_ptr(), kind, 0 if xs is None else xs.data_ptr(), q.data_ptr(), s.data_ptr(), o.data_ptr(), _TYPES[o.dtype], m, n, k,
                                  *ws, _stream_ptr(dev)))
 
