@@ -15,8 +15,8 @@
 //   warp 3     tensor-memory allocation; scales of the tokens in tiles of up to 64 columns, as 4-byte copies (cp.async).  In wide
 //              tiles this warp would set the pace (0.30 us per 256 columns of a 256-token tile before any other work), in narrow
 //              ones the small TMA copies would (4096x4096 at 1 token 7.3 us, so 4.5)
-//   warps 4-7  epilogue: tensor memory -> registers -> output type -> memory, of more than 16 tokens by way of shared memory
-//              and one bulk copy per token
+//   warps 4-7  epilogue: tensor memory -> registers -> output type -> memory, of more than 16 tokens by way of shared memory,
+//              where rows become contiguous.  Up to 128 tokens leave tensor memory before the first goes to memory
 //   warps 8-11 scales, one warp per lane quarter: a word of scales is four blocks (128 columns) of one row or token, and the MMAs want that of
 //              row r at lane r % 32, column r / 32, in every quarter.  So each warp reads all words of a stage from shared memory and
 //              writes them to its quarter (tcgen05.st).  Copies by the tensor pipe (tcgen05.cp) take its time: 57344x8192 at 4096
@@ -48,7 +48,7 @@ constexpr int kMxWarps = 12;
 constexpr int kMxEpilogueWarp0 = 4;
 constexpr int kMxScaleWarp0 = 8;
 constexpr int kMxMaxStages = 12;
-constexpr int kMxStageTokens = 64;      // tokens of an output staging buffer
+constexpr int kMxStageTokens = 128;     // tokens of the output staging buffer
 constexpr int kMxDirectTokens = 16;     // tiles of up to so many tokens are stored from registers
 constexpr int kMxSlackBytes = 1024;     // of shared memory at the end: scales of columns that a tile does not have are read from behind its own
 constexpr uint32_t kMxFoldBytes = kMxDirectTokens * kBlockRows * 4;  // where the parts of a folded tile are added up
@@ -126,12 +126,8 @@ __device__ __forceinline__ void tma_load_1d(uint32_t dst, const CUtensorMap *map
     asm volatile("cp.async.bulk.tensor.1d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2}], [%3];" ::"r"(dst), "l"(map), "r"(c0), "r"(bar) : "memory");
 }
 
-// One lane's words to COUNT columns of this warp's lanes.
-__device__ __forceinline__ void tc_st_words(uint32_t taddr, const uint32_t (&v)[2])
-{
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x2.b32 [%0], {%1, %2};" ::"r"(taddr), "r"(v[0]), "r"(v[1]) : "memory");
-}
-__device__ __forceinline__ void tc_st_words(uint32_t taddr, const uint32_t (&v)[8])
+// One lane's words to eight columns of this warp's lanes.
+__device__ __forceinline__ void tc_st_x8(uint32_t taddr, const uint32_t (&v)[8])
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
                  "r"(v[5]), "r"(v[6]), "r"(v[7])
@@ -182,7 +178,7 @@ template <> __device__ __forceinline__ uint32_t mx_pack2<__nv_bfloat16>(float lo
 // Words of a half (128 columns) of the tokens' scales that a lane holds, for so many columns of an accumulator.
 __host__ __device__ constexpr int mx_token_words(int cols) { return cols <= 64 ? 2 : cols <= 128 ? 4 : 8; }
 // Tensor-memory columns of a stage's scales: four per half for the weights, four per half and 128 tokens.
-__host__ __device__ constexpr uint32_t mx_scale_cols(int token_words) { return 8 + 2 * (token_words < 4 ? 4 : token_words); }
+__host__ __device__ constexpr uint32_t mx_scale_cols(int token_words) { return token_words == 8 ? 24 : 16; }
 
 // First row of row block b (a CTA's share of a tile).
 __device__ __forceinline__ int mx_row(const MxParams &p, int b) { return p.flex ? 8 * (int)((long long)b * p.groups / p.row_tiles) : b * kBlockRows; }
@@ -257,7 +253,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     const uint32_t staging = xs_ring + (uint32_t)(x_stages * p.xs_bytes);
     constexpr uint32_t kTokPitch = kBlockRows * (uint32_t)sizeof(OT) + (sizeof(OT) == 2 ? 16 : 0);  // 16-bit results: 16 bytes more, so that a column of 8 tokens meets all banks
     constexpr uint32_t kStagingBytes = kMxStageTokens * kTokPitch;
-    int *tables = reinterpret_cast<int *>(smem + (staging - base) + (p.fold_log ? kMxFoldBytes : N > kMxDirectTokens ? 2 * kStagingBytes : 0));
+    int *tables = reinterpret_cast<int *>(smem + (staging - base) + (p.fold_log ? kMxFoldBytes : N > kMxDirectTokens ? kStagingBytes : 0));
 
     // landed: a stage's copies; full: its scales are written as well; empty: its MMAs are done
     const uint32_t landed = smem_u32(&bars[0]), full = landed + 8 * kMxMaxStages, empty = full + 8 * kMxMaxStages, d_full = empty + 8 * kMxMaxStages, d_empty = d_full + 16;
@@ -327,7 +323,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     const uint32_t tmem = s_tmem_base;
     const uint32_t sf_col = (uint32_t)p.sf_col;
     const int fold = 1 << p.fold_log, part = kBlockRows >> p.fold_log;  // rows of a part
-    constexpr uint32_t kScaleCols = mx_scale_cols(NW), kTokenCols = NW < 4 ? 4 : NW;  // of a stage, and of a half of its tokens
+    constexpr int kScaleCols = (int)mx_scale_cols(NW), kTokenCols = NW < 4 ? 4 : NW;  // of a stage, and of a half of its tokens
     MxTiles tile;
     tile.init(p, worker, workers, tables);
     const int total = tile.total_units();
@@ -368,7 +364,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                     if (elect_one_sync()) {
                         const uint64_t a = sw128 | (uint64_t)(((base + (uint32_t)ru.idx * w_bytes) & 0x3FFFFu) >> 4);
                         const uint64_t b = sw128 | (uint64_t)(((x_ring + (uint32_t)(RESIDENT ? c : ru.idx) * x_bytes) & 0x3FFFFu) >> 4);
-                        const uint32_t sfa = tmem + sf_col + (uint32_t)ru.idx * kScaleCols, sfb = sfa + 8;
+                        const uint32_t sfa = tmem + sf_col + (uint32_t)(ru.idx * kScaleCols), sfb = sfa + 8;
                         const int steps = c + 1 == p.units && !p.fold_log ? p.last_steps : 4;
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
@@ -484,33 +480,38 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                 ok = mbar_wait_warp(landed + 8 * ru.idx, ru.phase, abort_flag, p.status, 212);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t to = lanes + (uint32_t)ru.idx * kScaleCols, x_at = xs_ring + (uint32_t)((RESIDENT ? c : ru.idx) * p.xs_bytes);
-                uint32_t w[8];  // of half i / 4: MMA row 32 (i % 4) + lane is row `of` of part f
+                const uint32_t to = lanes + (uint32_t)(ru.idx * kScaleCols), x_at = xs_ring + (uint32_t)((RESIDENT ? c : ru.idx) * p.xs_bytes);
+                // One store if it fits: what a store takes from the MMAs is hardly a matter of its size (57344x8192 at 4096 tokens, 721 us without any:
+                // with 8 columns 75 more, with 16 83, with 32 102, with 8 and 16 apart 138; but 32 columns a stage leave room for four
+                // stages of 256 tokens instead of five, 770 us against 735).
+                uint32_t v[kScaleCols];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < 8; ++i) {  // weights, half i / 4: MMA row 32 (i % 4) + lane is row `of` of part f
                     const int row = 32 * (i & 3) + lane, f = row >> (7 - p.fold_log), of = row & (part - 1);
-                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[i]) : "r"(ws_ring + (uint32_t)ru.idx * kMxScaleBytes + (uint32_t)((2 * f + (i >> 2)) * part + of) * 4u));
+                    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[i]) : "r"(ws_ring + (uint32_t)ru.idx * kMxScaleBytes + (uint32_t)((2 * f + (i >> 2)) * part + of) * 4u));
                 }
-                uint32_t x[2 * NW];  // column 32 (i % NW) + lane, half i / NW
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (int i = 8; i < (int)kScaleCols; ++i) v[i] = 0;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {  // tokens: column 32 j + lane, half h
                     const uint32_t skip = NW == 2 ? 0u : (((unsigned)(2 * c + h) * (unsigned)p.n + (unsigned)tile.tok0) & 3u) * 4u;
 #pragma unroll
                     for (int j = 0; j < NW; ++j) {
                         const uint32_t at = NW == 2 ? (uint32_t)(NW * h + j) * 128u : (uint32_t)((NW == 8 ? 2 * h + (j >> 2) : h) * p.xs_pitch) + (uint32_t)(j & 3) * 128u + skip;
-                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x[NW * h + j]) : "r"(x_at + at + 4u * lane));
+                        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[8 + kTokenCols * h + j]) : "r"(x_at + at + 4u * lane));
                     }
                 }
-                if constexpr (NW == 2) {
-                    const uint32_t x0[2] = {x[0], x[1]}, x1[2] = {x[2], x[3]};
-                    tc_st_words(to + 8, x0);
-                    tc_st_words(to + 8 + kTokenCols, x1);
-                } else if constexpr (NW == 4) {
-                    tc_st_words(to + 8, x);
-                } else {
+                if constexpr (NW == 8) {
+                    uint32_t w[8], x[16];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) w[i] = v[i];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i] = v[8 + i];
+                    tc_st_x8(to, w);
                     tc_st_x16(to + 8, x);
+                } else {
+                    tc_st_x16(to, v);
                 }
-                tc_st_words(to, w);
                 asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 tc_fence_before();
                 __syncwarp();
@@ -526,27 +527,19 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
         const uint32_t tmem_q = tmem + ((uint32_t)(32 * quarter) << 16);
         OT *o = static_cast<OT *>(p.o);
         Ring rd;
-        uint32_t buf = 0;
         depend();
         int row0 = 0, rows = 0;
-        // A staging buffer's tokens from t0 on to memory: fill(t, at) puts 32 tokens from t on to `at`; one bulk copy per token.
-        auto store_block = [&](int t0, auto fill) {
-            const uint32_t to = staging + buf * kStagingBytes;
-            buf ^= 1;
-            if (lane < kMxStageTokens / 4) asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory");  // the buffer's previous tokens have left it
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-#pragma unroll
-            for (int h = 0; h < kMxStageTokens; h += 32)
-                if (t0 + h < tile.valid) fill(t0 + h, to + h * kTokPitch);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (lane < kMxStageTokens / 4) {
-                const int t = kMxStageTokens / 4 * quarter + lane;
-                if (t0 + t < tile.valid && rows > 0)
-                    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(o + (size_t)(tile.tok0 + t0 + t) * p.m + row0),
-                                 "r"(to + (uint32_t)t * kTokPitch), "r"((uint32_t)rows * (uint32_t)sizeof(OT))
-                                 : "memory");
-                asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        // The staging buffer's tokens, which are the tile's from t0 on, to memory: 16 bytes a thread and step.
+        auto copy_out = [&](int t0) {
+            constexpr int kPieces = kBlockRows * (int)sizeof(OT) / 16, kStep = 128 / kPieces;
+            const int piece = thread % kPieces, end = min(kMxStageTokens, tile.valid - t0);
+            if (piece * (16 / (int)sizeof(OT)) >= rows) return;
+            uint8_t *to = reinterpret_cast<uint8_t *>(o + (size_t)(tile.tok0 + t0) * p.m + row0) + 16 * piece;
+#pragma unroll 8
+            for (int t = thread / kPieces; t < end; t += kStep) {
+                uint4 v;
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(staging + (uint32_t)t * kTokPitch + 16u * piece));
+                *reinterpret_cast<uint4 *>(to + (size_t)t * p.m * sizeof(OT)) = v;
             }
         };
         // 32 tokens of the accumulator at `d`, columns from t on.
@@ -623,14 +616,17 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                 const int turn = shared && second == 0 ? p.d_step : 0;
                 for (int b = 0; b < N; b += kMxStageTokens) {
                     const int t0 = b + turn < N ? b + turn : b + turn - N;
-                    if (t0 < tile.valid) store_block(t0, [&](int t, uint32_t at) { fill_from(d, t, at); });
-                    if (shared && b + kMxStageTokens == N - p.d_step) drained();
+                    asm volatile("bar.sync 1, 128;" ::: "memory");  // what was staged before has been copied
+#pragma unroll
+                    for (int h = 0; h < kMxStageTokens; h += 32)
+                        if (t0 + h < tile.valid) fill_from(d, t0 + h, staging + (uint32_t)h * kTokPitch);
+                    if (shared ? b == 0 : b + kMxStageTokens >= N) drained();
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    copy_out(t0);
                 }
-                if (!shared) drained();
             }
             rd.advance(p.nd);
         }
-        if (lane < kMxStageTokens / 4) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
 
     __syncwarp();
@@ -712,7 +708,7 @@ static MxPlan mx_plan(int m, int n, int k, int experts, int x_type, int o_type, 
     const int words = l.words = l.cg == 1 ? 2 : std::max(4, mx_token_words(l.d_cols));  // the kernels that there are: launch_mx_as
     const size_t room = words == 2 ? kMxSmemHalf : kMxSmemMax;
     const size_t pitch = kBlockRows * (o_type == TUNA_FP32 ? 4 : 2) + (o_type == TUNA_FP32 ? 0 : 16);
-    size_t fixed = (l.fold_log ? kMxFoldBytes : l.tile_tok > kMxDirectTokens ? 2 * kMxStageTokens * pitch : 0) + (3 * (size_t)experts + 1) * 4 + kMxSlackBytes;
+    size_t fixed = (l.fold_log ? kMxFoldBytes : l.tile_tok > kMxDirectTokens ? kMxStageTokens * pitch : 0) + (3 * (size_t)experts + 1) * 4 + kMxSlackBytes;
     const size_t w_stage = (size_t)l.w_bytes + kMxScaleBytes;
     l.xs_copy = std::min(l.tile_tok, 128) + 4;  // words
     l.xs_pitch = div_up(l.xs_copy * 4, 128) * 128;
@@ -730,10 +726,10 @@ static MxPlan mx_plan(int m, int n, int k, int experts, int x_type, int o_type, 
     }
     l.stages = (int)std::min<size_t>(kMxMaxStages, (room - fixed) / (w_stage + x_stage));
     const int tmem_cols = words == 2 ? 256 : 512, scale_cols = (int)mx_scale_cols(words);
-    l.nd = 2 * l.d_cols + l.stages * scale_cols <= tmem_cols ? 2 : 1;
+    l.nd = 2 * l.d_cols + std::min(l.stages, 4) * scale_cols <= tmem_cols ? 2 : 1;
     // two accumulators that share the columns in the middle, where two whole ones do not fit
     if (l.nd == 2) l.d_step = l.d_cols;
-    else if (l.cg == 2 && l.d_cols % (2 * kMxStageTokens) == 0) l.d_step = l.d_cols / 2;
+    else if (l.d_cols == 2 * kMxStageTokens) l.d_step = kMxStageTokens;
     l.sf_col = l.d_cols + l.d_step;
     l.stages = std::min(l.stages, (tmem_cols - l.sf_col) / scale_cols);
     // the last stage's MMAs read 128 rows
