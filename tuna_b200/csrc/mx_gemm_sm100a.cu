@@ -650,19 +650,19 @@ struct MxPlan {
     size_t smem;
 };
 
-// Microseconds that tiles of 256 rows and `cols` tokens take on `pairs` pairs: rounds of tiles, each with its steps of 256 columns
-// (the tensor pipe's and what comes with a step; wide tiles at the rate of the copies to shared memory as well) and, of wide
-// tiles, what of the epilogue nothing hides; what all tiles copy, from L2; the weights, from HBM.  Fitted to 550 launches
-// (graph replay; 7 matrices from 1024x1024 to 57344x8192, 17 to 2048 tokens, every width): what it chooses takes 2 % longer than
-// the fastest width in the mean, 15 % at worst.
+// Microseconds that tiles of 256 rows and `cols` tokens take on `pairs` pairs, beside what a launch costs: rounds of tiles, each with its
+// steps of 256 columns (the tensor pipe's four MMAs, which take hardly less for few tokens; wide tiles at the rate of the copies
+// to shared memory as well) and what of a wide tile's epilogue nothing hides; what all tiles copy, from L2; the weights,
+// from HBM.  Fitted to 1100 launches (graph replay; 11 matrices from 512x16384 to 57344x8192, 17 to 4096 tokens, every width): what it
+// chooses takes 1.5 % longer than the fastest width in the mean, 14 % at worst but for one (512x16384 at 17 tokens).
 static double mx_pair_us(int m, int n, int k, int cols, int pairs)
 {
     const int row_tiles = div_up(m, 2 * kBlockRows), chunks = div_up(k, kMxChunk);
     const double tiles = (double)row_tiles * div_up(n, cols);
     const double rounds = std::ceil(tiles / pairs);
-    const double step = cols <= 128 ? 0.186 : 0.043 + 0.00104 * cols;
-    const double work = rounds * (std::max(0.0, 0.0144 * cols - 0.5) + chunks * step);
-    const double copies = tiles * (2 * kBlockRows + cols) * chunks * 136.0 / 22.4e6, weights = (double)m * k * (17.0 / 32) / 8.3e6;
+    const double step = cols <= 128 ? 0.174 + 0.0002 * cols : 0.05 + 0.00104 * cols;
+    const double work = rounds * (std::max(0.0, 0.0087 * cols - 0.456) + chunks * step);
+    const double copies = tiles * (2 * kBlockRows + cols) * chunks * 136.0 / 18.8e6, weights = (double)m * k * (17.0 / 32) / 8.3e6;
     return std::sqrt(work * work + copies * copies + weights * weights);
 }
 
