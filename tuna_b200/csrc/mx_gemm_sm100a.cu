@@ -112,9 +112,9 @@ struct MxTiles {
         while (next_tile >= first_tile[e + 1]) ++e;  // tiles come in increasing order, and the last expert's end is their number
         const int local = next_tile - first_tile[e], tok_tiles = div_up(count[e], tile_tok);
         rt = local / tok_tiles;
-        const int tt = local - rt * tok_tiles;
-        tok0 = begin[e] + tt * tile_tok;
-        valid = min(tile_tok, count[e] - tt * tile_tok);
+        const int tt = local - rt * tok_tiles, width = (div_up(count[e], tok_tiles) + 15) & ~15;  // tiles of equal width, as many as the widest need
+        tok0 = begin[e] + tt * width;
+        valid = min(width, count[e] - tt * width);
         next_tile += step;
         return true;
     }
@@ -660,6 +660,7 @@ static double mx_pair_us(int m, int n, int k, int cols, int pairs)
     const int row_tiles = div_up(m, 2 * kBlockRows), chunks = div_up(k, kMxChunk);
     const double tiles = (double)row_tiles * div_up(n, cols);
     const double rounds = std::ceil(tiles / pairs);
+    cols = div_up(div_up(n, div_up(n, cols)), 16) * 16;  // tiles are of equal width
     const double step = cols <= 128 ? 0.174 + 0.0002 * cols : 0.05 + 0.00104 * cols;
     const double work = rounds * (std::max(0.0, 0.0087 * cols - 0.456) + chunks * step);
     const double copies = tiles * (2 * kBlockRows + cols) * chunks * 136.0 / 18.8e6, weights = (double)m * k * (17.0 / 32) / 8.3e6;
@@ -668,10 +669,12 @@ static double mx_pair_us(int m, int n, int k, int cols, int pairs)
 
 static int mx_pair_tokens(int m, int n, int k, int pairs)
 {
+    static const int widths[] = {256, 192, 176, 160, 128, 112, 96, 80, 64, 48, 32, 16, 0};
     int best = 0;
     double best_us = 0;
-    for (int cols = 256; cols >= 16; cols -= cols > 128 ? 32 : 16) {
-        if (cols - 16 >= n) continue;  // wider than the tokens
+    for (int i = 0; widths[i]; ++i) {
+        const int cols = widths[i];
+        if (div_up(n, div_up(n, cols)) <= widths[i + 1]) continue;  // the next narrower one holds the same tiles
         const double us = mx_pair_us(m, n, k, cols, pairs);
         if (!best || us < best_us) best = cols, best_us = us;
     }
@@ -698,6 +701,8 @@ static MxPlan mx_plan(int m, int n, int k, int experts, int x_type, int o_type, 
         l.fold_log = height <= 32 ? 2 : height <= 64 ? 1 : 0;
         l.w_bytes = (l.fold_log ? kBlockRows : height) * kMxChunkBytes;
     } else {
+        // Rows in tiles of 256, also where that leaves the last round of tiles short: lower ones that fill it copy more tokens per row
+        // (us, 256 / lower: 28672x4096 at 43 tokens 14.0 / 15.0, 4096x14336 at 256 17.0 / 20.1, 57344x8192 at 43 43.1 / 42.7).
         l.tile_tok = grouped ? mx_expert_tokens(div_up(n, experts)) : mx_pair_tokens(m, n, k, l.workers);
         l.row_tiles = div_up(m, 2 * kBlockRows);
         l.w_bytes = kBlockRows * kMxChunkBytes;
@@ -814,9 +819,9 @@ int launch_mx_gemm(const MxGemmArgs &a)
         return make_tensor_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, at, kMxChunkBytes, rows, chunks, kMxChunkBytes, rows * kMxChunkBytes, kMxChunkBytes, box_rows, box_chunks,
                                   CU_TENSOR_MAP_SWIZZLE_128B);
     };
-    if (!tiles_of(&maps.w, a.q, (uint64_t)a.m, (uint64_t)a.experts * p.chunks, l.flex ? 8u * (uint32_t)div_up(p.groups, l.row_tiles) : kBlockRows, 1)) return TUNA_ERR_NO_DEVICE;
+    if (!tiles_of(&maps.w, a.q, (uint64_t)a.m, (uint64_t)a.experts * p.chunks, l.flex ? 8u * (uint32_t)div_up(p.groups, p.row_tiles) : kBlockRows, 1)) return TUNA_ERR_NO_DEVICE;
     maps.w2 = maps.x = maps.xs = maps.w;
-    if (l.flex && p.groups % l.row_tiles && !tiles_of(&maps.w2, a.q, (uint64_t)a.m, (uint64_t)p.chunks, 8u * (uint32_t)(p.groups / l.row_tiles), 1)) return TUNA_ERR_NO_DEVICE;
+    if (l.flex && p.groups % p.row_tiles && !tiles_of(&maps.w2, a.q, (uint64_t)a.m, (uint64_t)p.chunks, 8u * (uint32_t)(p.groups / p.row_tiles), 1)) return TUNA_ERR_NO_DEVICE;
     if (!make_tensor_map_2d(&maps.ws, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.s, (uint64_t)a.m, (uint64_t)a.experts * p.words, (uint64_t)a.m * 4, (uint32_t)kBlockRows >> l.fold_log, 2, CU_TENSOR_MAP_SWIZZLE_NONE))
         return TUNA_ERR_NO_DEVICE;
     if (!l.resident && !tiles_of(&maps.x, a.x, (uint64_t)a.n, (uint64_t)p.chunks, (uint32_t)l.x_rows, 1u << l.fold_log)) return TUNA_ERR_NO_DEVICE;
