@@ -653,17 +653,17 @@ struct MxPlan {
 // Microseconds that tiles of 256 rows and `cols` tokens take on `pairs` pairs, beside what a launch costs: rounds of tiles, each with its
 // steps of 256 columns (the tensor pipe's four MMAs, which take hardly less for few tokens; wide tiles at the rate of the copies
 // to shared memory as well) and what of a wide tile's epilogue nothing hides; what all tiles copy, from L2; the weights,
-// from HBM.  Fitted to 1100 launches (graph replay; 11 matrices from 512x16384 to 57344x8192, 17 to 4096 tokens, every width): what it
-// chooses takes 1.5 % longer than the fastest width in the mean, 14 % at worst but for one (512x16384 at 17 tokens).
+// from HBM.  Fitted to 1250 launches (graph replay; 11 matrices from 512x16384 to 57344x8192, 17 to 4096 tokens, every width): what it
+// chooses takes 1.6 % longer than the fastest width in the mean, 20 % at worst (2048x2048 at 17 tokens).
 static double mx_pair_us(int m, int n, int k, int cols, int pairs)
 {
     const int row_tiles = div_up(m, 2 * kBlockRows), chunks = div_up(k, kMxChunk);
     const double tiles = (double)row_tiles * div_up(n, cols);
     const double rounds = std::ceil(tiles / pairs);
-    cols = div_up(div_up(n, div_up(n, cols)), 16) * 16;  // tiles are of equal width
-    const double step = cols <= 128 ? 0.174 + 0.0002 * cols : 0.05 + 0.00104 * cols;
-    const double work = rounds * (std::max(0.0, 0.0087 * cols - 0.456) + chunks * step);
-    const double copies = tiles * (2 * kBlockRows + cols) * chunks * 136.0 / 18.8e6, weights = (double)m * k * (17.0 / 32) / 8.3e6;
+    const int width = div_up(div_up(n, div_up(n, cols)), 16) * 16;  // tiles are of equal width
+    const double step = cols <= 128 ? 0.183 + 0.00013 * width : 0.036 + 0.00118 * width;
+    const double work = rounds * (std::max(0.0, 0.0086 * width - 0.5) + chunks * step);
+    const double copies = tiles * (2 * kBlockRows + cols) * chunks * 136.0 / 21.7e6, weights = (double)m * k * (17.0 / 32) / 8.1e6;
     return std::sqrt(work * work + copies * copies + weights * weights);
 }
 
