@@ -53,7 +53,6 @@ constexpr int kMxDirectTokens = 16;     // tiles of up to so many tokens are sto
 constexpr int kMxSlackBytes = 1024;     // of shared memory at the end: scales of columns that a tile does not have are read from behind its own
 constexpr uint32_t kMxFoldBytes = kMxDirectTokens * kBlockRows * 4;  // where the parts of a folded tile are added up
 constexpr int kMxResidentRows = 8;      // loads in flight of a quantizing warp
-constexpr int kMxAheadTokens = 64;      // one matrix: up to here weights are read ahead of the dependency wait
 constexpr uint32_t kMxScaleBytes = 2 * kBlockRows * 4;  // of the weights' scales in a stage
 constexpr int kMxSmemMax = 225 * 1024;   // dynamic shared memory of a CTA alone on its SM (1 KB is the kernel's static part, 1 KB the system's)
 constexpr int kMxSmemHalf = 111 * 1024;  // of one that leaves room for another
@@ -85,7 +84,7 @@ struct MxParams {
     int d_cols;     // tensor-memory columns of an accumulator: tokens of a tile times fold
     int d_step;     // where the second one starts; nd = 1: 0, or where it overlaps the first
     int sf_col;     // where the scales start
-    int ahead;      // weights are taken from before the dependency wait
+    int ahead;      // one matrix: weights are read from before the dependency wait (which those of an expert there is work for are not known)
 };
 
 // The tiles of a worker in order, and where each lies.
@@ -682,10 +681,10 @@ static int mx_pair_tokens(int m, int n, int k, int pairs)
 }
 
 // Tokens of a tile of experts: their numbers are on the device, so it goes by the mean.  Narrow enough that an expert of the mean
-// size fills a good part of a tile, wide enough that popular ones do not read their weights often (us, 64 / 128 / 192 / 256: eight experts
-// 28672x4096 of 4 in the mean 70 / - / - / -, eight 4096x14336 of 37 52 / 44 / 47 / 48 and of 187 103 / 75 / 73 / 74, sixteen 4096x4096 of
-// 250 75 / 56 / 60 / 56, 64 2048x1024 of 2 14.5 / - / - / -).
-static int mx_expert_tokens(int mean) { return mean <= 24 ? 64 : mean <= 128 ? 128 : 256; }
+// size fills a good part of a tile, wide enough that popular ones do not read their weights often (us, 64 / 128 / 176 / 256: eight experts
+// 28672x4096 of 4 in the mean 70 / - / - / -, eight 4096x14336 of 37 51 / 43 / 45 / 47 and of 187 101 / 72 / 68 / 72, sixteen 4096x4096 of
+// 250 73 / 55 / 51 / 52, eight 14336x4096 of 100 68 / 57 / 60 / 57, 64 2048x1024 of 2 13.5 / - / - / -).
+static int mx_expert_tokens(int mean) { return mean <= 24 ? 64 : mean <= 110 ? 128 : 176; }
 
 static MxPlan mx_plan(int m, int n, int k, int experts, int x_type, int o_type, bool grouped, int sm_count)
 {
@@ -805,7 +804,7 @@ int launch_mx_gemm(const MxGemmArgs &a)
     p.row_tiles = l.row_tiles; p.w_bytes = l.w_bytes; p.flex = l.flex; p.groups = a.m / 8;
     p.x_rows = l.x_rows; p.xs_pitch = l.xs_pitch; p.xs_bytes = l.xs_bytes;
     p.stages = l.stages; p.nd = l.nd; p.d_cols = l.d_cols; p.d_step = l.d_step; p.sf_col = l.sf_col;
-    p.ahead = a.offsets == nullptr && a.n <= kMxAheadTokens;
+    p.ahead = a.offsets == nullptr;  // 28672x4096 at 43 tokens 13.6 us, 14.9 with the weights after the wait
     p.status = device_status_word();
     if (!p.status) return TUNA_ERR_NO_DEVICE;
     // the kernel numbers tiles, a worker's stages, and words of scales in 32 bits
