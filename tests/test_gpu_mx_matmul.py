@@ -122,6 +122,50 @@ def test_runs_agree_bit_for_bit_in_any_workspace(n):
     assert all(torch.equal(outs[0], o) for o in outs[1:])
 
 
+@pytest.mark.parametrize("n", [1, 2, 5, 7, 16, 40])
+def test_tokens_with_infinities_and_nan_spoil_only_their_own_outputs(n):
+    m, k = 200, 1184
+    (wq, ws), w = random_packed(m, k, 8)
+    x = torch.randn(n, k, device="cuda", dtype=torch.bfloat16)
+    x[0, 5] = float("inf")
+    if n > 1:
+        x[n - 1, k - 1] = float("nan")
+    o = torch.empty(n, m, device="cuda")
+    tuna_b200.mx_matmul(x, None, *dev(wq, ws), o, m, n, k)
+    finish()
+    assert torch.isnan(o[0]).all() and torch.isnan(o[n - 1]).all()
+    check_product(o, mxo.decode(*mxo.quantize(x.double().cpu().numpy())), w)
+
+
+@pytest.mark.parametrize("m", [8, 24, 264, 1184, 2368, 4736, 9472, 18944, 19000])
+def test_row_tiles_of_every_height(m):
+    """Up to 16 tokens: one to 128 rows a tile, folded four ways, two ways and not, with and without a remainder."""
+    for n, k in ((1, 416), (9, 1312)):
+        product(m, n, k, seed=m)
+    x = torch.randn(3, 672, device="cuda", dtype=torch.float16)
+    (wq, ws), w = random_packed(m, 672, 5)
+    o = torch.empty(3, m, device="cuda")
+    tuna_b200.mx_matmul(x, None, *dev(wq, ws), o, m, 3, 672)
+    finish()
+    check_product(o, mxo.decode(*mxo.quantize(x.double().cpu().numpy())), w)
+
+
+@pytest.mark.parametrize("n", [17, 33, 49, 65, 97, 129, 145, 161, 177, 193, 225, 257, 353, 400, 530])
+def test_token_tiles_of_every_width(n):
+    product(2600, n, 320, seed=n)
+
+
+def test_an_output_of_more_than_2_31_elements():
+    m, n, k = 65536, 33000, 32
+    (xq, xs), x = random_packed(n, k, 1)
+    (wq, ws), w = random_packed(m, k, 2)
+    o = torch.empty(n, m, device="cuda", dtype=torch.bfloat16)
+    tuna_b200.mx_matmul(*dev(xq, xs, wq, ws), o, m, n, k)
+    finish()
+    for rows in (slice(0, 3), slice(16000, 16003), slice(n - 300, n)):
+        check_product(o[rows], x[rows], w)
+
+
 # ------------------------------------------------------------------ experts
 
 def grouped(counts, m, k, *, before=0, behind=0, dtype=torch.float32, seed=0, quantized=True, offsets=None):
@@ -255,6 +299,36 @@ def test_two_graphs_of_one_stream_replayed_side_by_side():
     finish()
     for _, o, x, w in cases:
         check_product(o, x, w)
+
+
+@pytest.mark.parametrize("n", [2, 24])
+def test_graphs_with_tokens_in_16_bits(n):
+    """Captured calls that quantize their tokens, replayed with new ones side by side with eager calls on another stream."""
+    m, k = 1024, 4096
+    (wq, ws), w = random_packed(m, k, 2)
+    q, s = dev(wq, ws)
+    xs = [torch.zeros(n, k, device="cuda", dtype=torch.float16) for _ in range(2)]
+    outs = [torch.zeros(n, m, device="cuda") for _ in range(3)]
+    graphs = []
+    for x, o in zip(xs, outs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            tuna_b200.mx_matmul(x, None, q, s, o, m, n, k)
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    eager = torch.randn(n, k, device="cuda", dtype=torch.float16)
+    for round_ in range(5):
+        for x in xs:
+            x.normal_()
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        with torch.cuda.stream(streams[2]):
+            tuna_b200.mx_matmul(eager, None, q, s, outs[2], m, n, k)
+        finish()
+        for x, o in zip(xs + [eager], outs):
+            check_product(o, mxo.decode(*mxo.quantize(x.double().cpu().numpy())), w)
 
 
 def test_calls_on_two_streams_at_once():

@@ -111,6 +111,23 @@ def test_every_scale_byte_reads_back():
         assert torch.equal(torch.nan_to_num(o.cpu().float(), nan=12345.0), torch.nan_to_num(numbers.to(t).float(), nan=12345.0))
 
 
+def test_more_than_2_31_elements():
+    rows, k = 68000, 32768
+    x = torch.zeros(rows, k, device="cuda", dtype=torch.bfloat16)
+    at = torch.tensor([0, 33333, 65535, 65536, 67997, 67998, 67999], device="cuda")
+    x[at] = torch.randn(len(at), k, device="cuda", dtype=torch.bfloat16)
+    q, s = tuna_b200.mx_quantize(x)
+    small = tuna_b200.mx_quantize(x[at])
+    assert torch.equal(q[:, at], small[0]) and torch.equal(s[:, at], small[1])
+    o = torch.full((rows, k), 7.0, device="cuda", dtype=torch.bfloat16)
+    tuna_b200.mx_dequant(q, s, o, rows, k)
+    want = torch.empty(len(at), k, device="cuda", dtype=torch.bfloat16)
+    tuna_b200.mx_dequant(*small, want, len(at), k)
+    assert torch.equal(o[at], want)
+    o[at] = 0
+    assert not o.any()
+
+
 def test_nothing_is_written_behind_the_last_row():
     lib = _lib.load()
     x = torch.randn(5, 160, device="cuda", dtype=torch.float16)

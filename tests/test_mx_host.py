@@ -100,6 +100,9 @@ def test_argument_validation_needs_no_gpu(tuna_lib):
     assert need >= 33 * (128 + 4) and tuna_lib.tuna_mx_workspace_bytes(64, 33, 64, 0, 3) == 0
     assert mm(x_type=0, n=33, ws=None) == -4 and mm(x_type=0, n=33, ws_bytes=need - 1) == -4
 
+    # nothing is launched - not the tokens' quantizer either - for what the product refuses
+    assert mm(x_type=0, m=8, n=(1 << 31) - 1, k=1024, ws_bytes=1 << 60) in (-7, -9)
+
     def grouped(offsets=p, experts=2, n=4, x_type=3, ws_bytes=big):
         return tuna_lib.tuna_mx_matmul_grouped(p, x_type, p, p, p, offsets, p, 0, 64, n, 64, experts, p, ws_bytes, None)
 

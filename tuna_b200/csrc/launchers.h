@@ -102,6 +102,8 @@ struct MxGemmArgs {
     const void *offsets;  // device, experts + 1 of them; nullptr: one matrix
     void *o;
     int m, n, k, experts, x_type, o_type;
+    // Tokens of x_type that the product does not take as they are: quantized into x and xs by a launch before it, once nothing can be refused.
+    const void *numbers;
     cudaStream_t stream;
     int sm_count;
 };

@@ -48,10 +48,11 @@ static int mx_product(const void *x, int x_type, const void *xs, const void *q, 
     a.x = x; a.xs = xs; a.q = q; a.s = s; a.offsets = offsets; a.o = o;
     a.m = m; a.n = n; a.k = k; a.experts = experts; a.x_type = x_type; a.o_type = o_type;
     a.stream = (cudaStream_t)stream; a.sm_count = sms;
+    a.numbers = nullptr;
     if (w.total > 0) {
-        uint8_t *codes = (uint8_t *)workspace, *scales = codes + w.scales;
-        if (launch_mx_quantize(x, x_type, k, codes, scales, n, k, 1, a.stream, true) != cudaSuccess) return TUNA_ERR_LAUNCH;
-        a.x = codes; a.xs = scales; a.x_type = TUNA_MXFP4;
+        a.numbers = x;
+        a.x = workspace;
+        a.xs = (uint8_t *)workspace + w.scales;
     }
     return launch_mx_gemm(a);
 }

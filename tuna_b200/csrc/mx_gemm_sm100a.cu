@@ -790,7 +790,7 @@ static int launch_mx_as(const MxPlan &l, const MxParams &p, const MxMaps &maps, 
 
 int launch_mx_gemm(const MxGemmArgs &a)
 {
-    const MxPlan l = mx_plan(a.m, a.n, a.k, a.experts, a.x_type, a.o_type, a.offsets != nullptr, a.sm_count);
+    const MxPlan l = mx_plan(a.m, a.n, a.k, a.experts, a.numbers ? TUNA_MXFP4 : a.x_type, a.o_type, a.offsets != nullptr, a.sm_count);
     MxParams p;
     std::memset(&p, 0, sizeof(p));
     p.xs = (const uint32_t *)a.xs; p.x = a.x; p.offsets = (const int *)a.offsets; p.o = a.o;
@@ -829,6 +829,8 @@ int launch_mx_gemm(const MxGemmArgs &a)
         const uint32_t box = (uint32_t)l.xs_copy;
         if (!make_tensor_map_nd(&maps.xs, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.xs, 1, &dim, nullptr, &box, CU_TENSOR_MAP_SWIZZLE_NONE)) return TUNA_ERR_NO_DEVICE;
     }
+    if (a.numbers && launch_mx_quantize(a.numbers, a.x_type, a.k, const_cast<void *>(a.x), const_cast<void *>(a.xs), a.n, a.k, 1, a.stream, true) != cudaSuccess)
+        return TUNA_ERR_LAUNCH;
     const int ctas = l.workers * l.cg;
     switch (a.o_type) {
         case TUNA_FP16: return launch_mx_as<__half>(l, p, maps, ctas, a.stream);
