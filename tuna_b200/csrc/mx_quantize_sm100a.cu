@@ -1,8 +1,12 @@
 // Microscaled 4-bit quantizer and its inverse (format and layout: mx_format.cuh).
 //
-// A warp takes eight rows of one 256-column chunk: a lane eight columns of each, so a block of 32 is four lanes and its largest
-// magnitude takes two shuffles.  A row's 128 bytes of codes are one warp store, eight rows' 1 KB of one run of memory; the rows'
-// scale words are gathered into one lane each and leave as two runs of 32 bytes.
+// A warp takes a few rows of one 256-column chunk: a lane eight columns of each, so a block of 32 is four lanes and its largest
+// magnitude takes two shuffles.  A row's 128 bytes of codes are one warp store and neighbouring rows' one run of memory; the rows'
+// scale words are gathered into one lane each.  Numbers stay as they were loaded until they are needed and maxima of 16-bit
+// types are taken in pairs: with fp32 copies of eight rows 57344x8192 took 369 us, waiting for loads with 40 % of the warps that fit, so 191.
+//
+// HBM bounds both: 57344x8192 in fp16 191 us and 195 back, 6.2 and 6.1 TB/s, where a copy reaches 6.55; 5000x8224 in fp32 28 us (6.6 TB/s)
+// and 34 back (5.4 TB/s, seven eighths of it stores).
 #include <algorithm>
 #include "launchers.h"
 #include "mx_format.cuh"
@@ -10,7 +14,6 @@
 namespace tuna {
 
 constexpr int kMxqWarps = 4;
-constexpr int kMxqRows = 4;
 
 // The warps of a CTA take neighbouring chunks, 1 << log_c of them, of as many row groups as that leaves; grid (row groups, chunks).
 struct MxqPlace {
@@ -158,6 +161,11 @@ static cudaError_t mxq_launch(int rows, int k, int batch, int rows_per_warp, Ker
     return kernel(dim3((unsigned)div_up_ll(groups, 4 >> log_c), (unsigned)div_up(chunks, 1 << log_c)), chunks, log_c);
 }
 
+// Rows of a warp: many where bandwidth counts (57344x8192 in fp16: quantizing 2 rows 227 us, 4 191, 8 188, but of 1999x14336 in bf16 15.3, 13.1,
+// 15.1; back 2 rows 202, 4 193, 8 195 and 15.0, 14.0, 13.6), two where the launch is short (4096 columns in bf16, us, quantizing 2 / 4 and
+// back 2 / 8: 1 row 1.28 / 1.54 and 1.28 / 1.79, 64 1.79 / 2.05 and 1.54 / 2.18, 512 2.56 / 2.97 and 2.69 / 3.08, 1024 3.72 / 3.84 and 4.10 / 3.86).
+static bool mxq_short(int rows, int k, int batch) { return (long long)rows * batch * div_up(k, kMxChunk) <= 8192; }
+
 template <typename T, int ROWS>
 static cudaError_t quantize_as(const void *x, long long row_stride, void *q, void *s, int rows, int k, int batch, bool chained, cudaStream_t stream)
 {
@@ -175,12 +183,19 @@ static cudaError_t quantize_as(const void *x, long long row_stride, void *q, voi
     });
 }
 
+template <typename T>
+static cudaError_t quantize_any(const void *x, long long row_stride, void *q, void *s, int rows, int k, int batch, bool chained, cudaStream_t stream)
+{
+    return mxq_short(rows, k, batch) ? quantize_as<T, 2>(x, row_stride, q, s, rows, k, batch, chained, stream)
+                                     : quantize_as<T, 4>(x, row_stride, q, s, rows, k, batch, chained, stream);
+}
+
 cudaError_t launch_mx_quantize(const void *x, int type, long long row_stride, void *q, void *s, int rows, int k, int batch, cudaStream_t stream, bool chained)
 {
     switch (type) {
-        case TUNA_FP16: return quantize_as<__half, kMxqRows>(x, row_stride, q, s, rows, k, batch, chained, stream);
-        case TUNA_BF16: return quantize_as<__nv_bfloat16, kMxqRows>(x, row_stride, q, s, rows, k, batch, chained, stream);
-        default: return quantize_as<float, kMxqRows>(x, row_stride, q, s, rows, k, batch, chained, stream);
+        case TUNA_FP16: return quantize_any<__half>(x, row_stride, q, s, rows, k, batch, chained, stream);
+        case TUNA_BF16: return quantize_any<__nv_bfloat16>(x, row_stride, q, s, rows, k, batch, chained, stream);
+        default: return quantize_any<float>(x, row_stride, q, s, rows, k, batch, chained, stream);
     }
 }
 
@@ -193,12 +208,18 @@ static cudaError_t dequant_as(const void *q, const void *s, void *o, int rows, i
     });
 }
 
+template <typename T>
+static cudaError_t dequant_any(const void *q, const void *s, void *o, int rows, int k, int batch, cudaStream_t stream)
+{
+    return mxq_short(rows, k, batch) ? dequant_as<T, 2>(q, s, o, rows, k, batch, stream) : dequant_as<T, 8>(q, s, o, rows, k, batch, stream);
+}
+
 cudaError_t launch_mx_dequant(const void *q, const void *s, void *o, int type, int rows, int k, int batch, cudaStream_t stream)
 {
     switch (type) {
-        case TUNA_FP16: return dequant_as<__half, 8>(q, s, o, rows, k, batch, stream);
-        case TUNA_BF16: return dequant_as<__nv_bfloat16, 8>(q, s, o, rows, k, batch, stream);
-        default: return dequant_as<float, 8>(q, s, o, rows, k, batch, stream);
+        case TUNA_FP16: return dequant_any<__half>(q, s, o, rows, k, batch, stream);
+        case TUNA_BF16: return dequant_any<__nv_bfloat16>(q, s, o, rows, k, batch, stream);
+        default: return dequant_any<float>(q, s, o, rows, k, batch, stream);
     }
 }
 
