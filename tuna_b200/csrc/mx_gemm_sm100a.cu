@@ -21,8 +21,8 @@
 //              row r at lane r % 32, column r / 32, in every quarter.  So each warp reads all words of a stage from shared memory and
 //              writes them to its quarter (tcgen05.st).  Copies by the tensor pipe (tcgen05.cp) take its time: 57344x8192 at 4096
 //              tokens 923 us with them, 756 without.
-// RESIDENT: up to 16 tokens in 16 bits are quantized by the CTA itself before its first MMA, all of K, and stay in shared memory:
-// no launch before this one.
+// RESIDENT: a few tokens in 16 bits are quantized by the CTA itself before its first MMA, all of K, and stay in shared memory: no
+// launch before this one.
 //
 // Work split.  Tiles are numbered expert by expert and handed out in turn; no sum is cut, so nothing is added up outside of a
 // tile.  Up to 16 tokens one matrix is cut into row tiles of equal height, a multiple of 8 up to 128, a whole number of them for
@@ -52,7 +52,7 @@ constexpr int kMxStageTokens = 128;     // tokens of the output staging buffer
 constexpr int kMxDirectTokens = 16;     // tiles of up to so many tokens are stored from registers
 constexpr int kMxSlackBytes = 1024;     // of shared memory at the end: scales of columns that a tile does not have are read from behind its own
 constexpr uint32_t kMxFoldBytes = kMxDirectTokens * kBlockRows * 4;  // where the parts of a folded tile are added up
-constexpr int kMxResidentRows = 8;      // loads in flight of a quantizing warp
+constexpr int kMxResidentRows = 4;      // loads in flight of a quantizing warp
 constexpr uint32_t kMxScaleBytes = 2 * kBlockRows * 4;  // of the weights' scales in a stage
 constexpr int kMxSmemMax = 225 * 1024;   // dynamic shared memory of a CTA alone on its SM (1 KB is the kernel's static part, 1 KB the system's)
 constexpr int kMxSmemHalf = 111 * 1024;  // of one that leaves room for another
@@ -718,8 +718,9 @@ static MxPlan mx_plan(int m, int n, int k, int experts, int x_type, int o_type, 
     l.xs_pitch = div_up(l.xs_copy * 4, 128) * 128;
     l.xs_bytes = words == 2 ? 512 : 2 * (words == 8 ? 2 : 1) * l.xs_pitch;
     size_t x_stage = (size_t)l.x_rows * fold * kMxChunkBytes + l.xs_bytes;
-    // Tokens that the CTAs quantize themselves: one round of the quantizing warps, and shared memory left for stages enough.  (4096x4096 in
-    // bf16, us, so / a quantizing launch before it: 1 token 4.4 / 6.0, 4 tokens 5.5 / 6.4, 5 tokens 6.0 / 6.5, two rounds at 6 tokens 7.2 / 6.6.)
+    // Tokens that the CTAs quantize themselves: one round of the quantizing warps, and shared memory left for stages enough.  (bf16, us, so / a
+    // quantizing launch before it: 4096x4096 at 1 token 4.4 / 5.5, at 2 4.6 / 5.5, with eight loads in flight at 4 5.7 / 5.7; 28672x4096 at 1 13.1 /
+    // 13.5.)
     const int rows8 = div_up(n, 8) * 8, units = div_up(chunks, fold);
     const size_t resident = (size_t)units * (rows8 * fold * kMxChunkBytes + l.xs_bytes);
     l.resident = l.cg == 1 && x_type != TUNA_MXFP4 && n * units * fold <= kMxResidentRows * (kMxWarps - 1) && resident + 4 * w_stage + fixed <= room;
