@@ -389,6 +389,41 @@ def test_a_device_that_is_not_the_current_one():
     check_product(o, x, w)
 
 
+def test_calls_checked_in_python_are_the_same_calls(monkeypatch):
+    """Without the native front every call goes through the checks and the binding of mx.py."""
+    m, n, k = 264, 21, 544
+    w = torch.randn(3, m, k, device="cuda")
+    x = torch.randn(n, k, device="cuda", dtype=torch.float16)
+    off = torch.tensor([0, 4, 4, 19], dtype=torch.int32, device="cuda")
+
+    def calls():
+        q, s = tuna_b200.mx_quantize(w)
+        xq, xs = tuna_b200.mx_quantize(x)
+        outs = [q, s, xq, xs] + [torch.zeros(n, m, device="cuda") for _ in range(4)] + [torch.empty(m, k, device="cuda", dtype=torch.bfloat16)]
+        tuna_b200.mx_matmul(x, None, q[0], s[0], outs[4], m, n, k)
+        tuna_b200.mx_matmul(xq, xs, q[0], s[0], outs[5], m, n, k)
+        tuna_b200.mx_matmul_grouped(x, None, q, s, off, outs[6], m, n, k)
+        tuna_b200.mx_matmul_grouped(xq, xs, q, s, off, outs[7], m, n, k)
+        tuna_b200.mx_dequant(q[1], s[1], outs[8], m, k)
+        finish()
+        return outs
+
+    native = calls()
+    monkeypatch.setattr(tuna_b200.mx, "_front", lambda: tuna_b200.mx._NoFront)
+    for a, b in zip(native, calls()):
+        assert torch.equal(a, b)
+
+
+def test_errors_of_a_launch_are_raised_by_the_native_front():
+    x = torch.randn(5 * 256 + 8, device="cuda", dtype=torch.float16)[4:4 + 4 * 256].view(4, 256)  # 8 bytes off
+    (wq, ws), _ = random_packed(128, 256, 1)
+    with pytest.raises(tuna_b200.TunaError) as e:
+        tuna_b200.mx_matmul(x, None, *dev(wq, ws), torch.empty(4, 128, device="cuda"), 128, 4, 256)
+    assert e.value.status == -3
+    with pytest.raises(tuna_b200.TunaError):
+        tuna_b200.mx_quantize(x)
+
+
 def test_refusals():
     m, n, k = 128, 4, 256
     (xq, xs), _ = random_packed(n, k, 1)
