@@ -306,8 +306,8 @@ int tuna_mx_matmul(const void *x, int x_type, const void *xs, const void *q, con
  * The same for the experts of a mixture (1 to TUNA_MX_MAX_EXPERTS), the tokens lying expert by expert: row t of x with
  * offsets[e] <= t < offsets[e + 1] is multiplied with matrix e of q [experts, ..] and s [experts, ..].  `offsets` (int32,
  * experts + 1, not decreasing) is in DEVICE memory, as a router leaves it: nothing is read back.  n counts the rows of x and o,
- * which may be more than offsets[experts] (0: nothing to do): rows before offsets[0] or behind offsets[experts] of o are left as they were.  Offsets outside
- * 0 .. n are taken as the nearest of these; of experts whose ranges overlap any one may have written the rows in common.
+ * which may be more than offsets[experts] (0: nothing to do): rows before offsets[0] or behind offsets[experts] of o are left as they were.  An offset
+ * outside of 0 .. n is taken as the nearest of these, one that is less than one before it as that one.
  */
 int tuna_mx_matmul_grouped(const void *x, int x_type, const void *xs, const void *q, const void *s, const void *offsets, void *o, int o_type, int m, int n,
                            int k, int experts, void *workspace, size_t workspace_bytes, void *stream);

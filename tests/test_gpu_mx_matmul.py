@@ -202,6 +202,25 @@ def test_experts_in_a_larger_buffer(dtype, quantized):
     grouped([3, 0, 21, 7], 136, 416, before=5, behind=9, dtype=dtype, quantized=quantized)
 
 
+def test_decreasing_offsets_of_many_experts():
+    """Every offset counts as the largest up to it: 70 experts, of which most get nothing."""
+    m, n, k, experts = 64, 90, 96, 70
+    rng = np.random.default_rng(7)
+    offsets = rng.integers(-20, n + 20, experts + 1).astype(np.int32)
+    offsets[:40] = rng.integers(-5, 30, 40)
+    mats = [random_packed(m, k, i) for i in range(experts)]
+    q, s = dev(np.stack([p[0][0] for p in mats]), np.stack([p[0][1] for p in mats]))
+    (xq, xs), x = random_packed(n, k, 999)
+    o = torch.full((n, m), 7.0, device="cuda")
+    tuna_b200.mx_matmul_grouped(*dev(xq, xs), q, s, torch.from_numpy(offsets).cuda(), o, m, n, k)
+    finish()
+    ends = np.maximum.accumulate(np.clip(offsets, 0, n))
+    for e in range(experts):
+        if ends[e] < ends[e + 1]:
+            check_product(o[ends[e]:ends[e + 1]], x[ends[e]:ends[e + 1]], mats[e][1])
+    assert (o[:ends[0]] == 7).all() and (o[ends[-1]:] == 7).all()
+
+
 def test_many_experts():
     rng = np.random.default_rng(0)
     grouped(list(rng.integers(0, 4, 1024)), 16, 96, seed=3)
@@ -219,7 +238,7 @@ def test_experts_without_tokens_at_all():
     finish()
 
 
-@pytest.mark.parametrize("offsets", [[0, 99, 20], [-5, 3, 8], [4, 2, 6], [-2147483648, 0, 2147483647]], ids=str)
+@pytest.mark.parametrize("offsets", [[0, 99, 20], [-5, 3, 8], [4, 2, 6], [7, 3, 1], [-2147483648, 0, 2147483647]], ids=str)
 def test_offsets_outside_the_tokens_stay_inside_the_output(offsets):
     m, n, k = 128, 8, 256
     mats = [random_packed(m, k, i) for i in range(2)]
@@ -230,13 +249,12 @@ def test_offsets_outside_the_tokens_stay_inside_the_output(offsets):
     tuna_b200.mx_matmul_grouped(*dev(xq, xs), q, s, torch.tensor(offsets, dtype=torch.int32, device="cuda"), hold.view, m, n, k)
     finish()
     assert hold.guards_intact()
-    clamped = np.clip(offsets, 0, n)
+    clamped = np.maximum.accumulate(np.clip(offsets, 0, n))
     covered = np.zeros(n, dtype=bool)
     for e in range(2):
         covered[clamped[e]:max(clamped[e], clamped[e + 1])] = True
     assert (hold.view[torch.from_numpy(~covered).cuda()] == 7).all()
-    only = [r for r in range(n) if sum(clamped[e] <= r < clamped[e + 1] for e in range(2)) == 1]
-    for r in only:
+    for r in np.flatnonzero(covered):
         e = next(e for e in range(2) if clamped[e] <= r < clamped[e + 1])
         check_product(hold.view[r:r + 1], x[r:r + 1], mats[e][1])
 

@@ -287,19 +287,23 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     auto depend = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
     if (warp == 0) {  // the experts' tiles: first token, tokens, tiles before
         if (p.offsets) depend();
-        int before = 0;
+        int before = 0, reached = 0;
         for (int e0 = 0; e0 < p.experts; e0 += 32) {
             const int e = e0 + lane;
-            int begin = 0, cnt = 0;
-            if (e < p.experts) {
-                if (p.offsets) {  // whatever they are, inside the tokens
-                    begin = min(max(__ldcg(p.offsets + e), 0), p.n);
-                    cnt = max(min(max(__ldcg(p.offsets + e + 1), 0), p.n) - begin, 0);
-                } else {
-                    cnt = p.n;
-                }
+            int begin = 0, cnt = p.n;
+            if (p.offsets) {  // whatever they are: inside the tokens, and none below one before it
+                auto largest = [&](int v) {
+#pragma unroll
+                    for (int d = 1; d < 32; d <<= 1) v = max(v, __shfl_up_sync(0xffffffffu, v, d));
+                    return max(v, reached);
+                };
+                begin = largest(min(max(__ldcg(p.offsets + min(e, p.experts)), 0), p.n));
+                const int end = max(begin, min(max(__ldcg(p.offsets + min(e + 1, p.experts)), 0), p.n));
+                cnt = end - begin;
+                reached = __shfl_sync(0xffffffffu, end, 31);
             }
             const int mine = div_up(cnt, N) * p.row_tiles;
+            if (e >= p.experts) cnt = 0;
             int sum = mine;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {

@@ -164,7 +164,8 @@ def mx_matmul(x, xs, q, s, o, m: int, n: int, k: int, *, workspace=None) -> None
 
 def mx_matmul_grouped(x, xs, q, s, offsets, o, m: int, n: int, k: int, *, workspace=None) -> None:
     """`mx_matmul` for the experts of a mixture, whose tokens lie expert by expert: rows offsets[e] up to offsets[e + 1] of x are
-    multiplied with matrix e of `q` `[experts, ceil(k/256), m, 128]` and `s`.  `offsets` int32 `[experts + 1]`, not decreasing, stays on
+    multiplied with matrix e of `q` `[experts, ceil(k/256), m, 128]` and `s`.  `offsets` int32 `[experts + 1]`, not decreasing (one that is less
+    than one before it counts as that one), stays on
     the device (a router's cumulative counts): nothing waits for it on the host.  x and o have n rows, which may be more than
     offsets[experts]: rows of o that no expert has are left as they were.  n = 0 is nothing to do."""
     if workspace is None and _launched(_front().mx_matmul_grouped(x, xs, q, s, offsets, o, m, n, k)):
