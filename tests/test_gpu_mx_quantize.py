@@ -139,6 +139,18 @@ def test_nothing_is_written_behind_the_last_row():
     assert torch.equal(q.view, q2) and torch.equal(s.view, s2)
 
 
+@pytest.mark.parametrize("rows", [1, 3])
+def test_as_many_columns_as_there_may_be(rows):
+    k = 67107840
+    levels = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6, 0, -0.5, -1, -1.5, -2, -3, -4, -6], device="cuda", dtype=torch.float16)
+    x = levels[torch.randint(0, 16, (rows, k), device="cuda", dtype=torch.uint8).int()]
+    x[:, ::32] = 6  # every block's scale is 1: nothing is rounded
+    q, s = tuna_b200.mx_quantize(x)
+    back = torch.empty_like(x)
+    tuna_b200.mx_dequant(q, s, back, rows, k)
+    assert torch.equal(back, x) and (s == 127).all()
+
+
 def test_refusals():
     x = torch.randn(8, 256, device="cuda")
     for bad in (x[:, :40], x.t(), x[:, ::2], x[None].expand(2, 8, 256), x.view(-1), x[:0]):

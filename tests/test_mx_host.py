@@ -112,6 +112,17 @@ def test_argument_validation_needs_no_gpu(tuna_lib):
     assert grouped(offsets=ctypes.c_void_p(base + 2)) == -3
     assert grouped(x_type=1, ws_bytes=0) == -4
     assert grouped(n=0) == 0 and grouped(n=-1) == -2
+    # sizes that rounded up to a whole tile would no longer have 32 bits, more columns than a grid has chunks for
+    long = (1 << 31) - 32
+    for type_ in (0, 3):
+        assert mm(x_type=type_, m=8, n=(1 << 31) - 1, k=32, ws_bytes=1 << 60) == -9 and mm(x_type=type_, m=long, k=32) == -9
+        for k in (67107840 + 32, long):
+            assert mm(x_type=type_, m=8, k=k, ws_bytes=1 << 60) == -9
+    assert qz(p, 0, 32, p, p, (1 << 31) - 1, 32, 1, None) == -9 and dq(p, p, p, 0, (1 << 31) - 1, 32, 1, None) == -9
+    for k in (67107840 + 32, long):
+        assert qz(p, 0, k, p, p, 1, k, 1, None) == -9 and dq(p, p, p, 0, 1, k, 1, None) == -9
+        assert tuna_lib.tuna_mx_workspace_bytes(8, 1, k, 0, 0) == 0
+
     assert tuna_lib.tuna_mx_workspace_bytes(60, 33, 64, 0, 0) == 0
     assert tuna_lib.tuna_mx_workspace_bytes(64, 1, 64, 1025, 0) == 0
 

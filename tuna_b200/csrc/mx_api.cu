@@ -9,11 +9,14 @@ static bool aligned_to(const void *p, size_t a) { return (reinterpret_cast<uintp
 static bool is_number_type(int t) { return t == TUNA_FP16 || t == TUNA_BF16 || t == TUNA_FP32; }
 static int type_bytes(int t) { return t == TUNA_FP32 ? 4 : 2; }
 
+// Sizes in 32 bits leave room for being rounded up to whole tiles; the quantizers' grids have the chunks, by fours, in y.
+static bool too_long(int rows, int k) { return rows > 0x7fffffff - 1023 || k > 65535 * 4 * kMxChunk; }
+
 // rows x k elements, `batch` of them: what the kernels number in 64 bits, but grids in 32
 static int check_matrix(int rows, int k, int batch)
 {
     if (rows < 1 || k < 1 || batch < 1 || k % kMxBlock) return TUNA_ERR_BAD_SHAPE;
-    if ((double)rows * k * batch > (double)(1ll << 41) || (double)rows * batch > (double)(1ll << 31)) return TUNA_ERR_TOO_LARGE;
+    if (too_long(rows, k) || (double)rows * k * batch > (double)(1ll << 41) || (double)rows * batch > (double)(1ll << 31)) return TUNA_ERR_TOO_LARGE;
     return TUNA_OK;
 }
 
@@ -38,7 +41,7 @@ static int mx_product(const void *x, int x_type, const void *xs, const void *q, 
     if (!x || !q || !s || !o || (packed && !xs)) return TUNA_ERR_NULL_POINTER;
     if (m < 1 || m % 8 || n < 1 || k < 1 || k % kMxBlock || experts < 1) return TUNA_ERR_BAD_SHAPE;
     if ((!packed && x_type != TUNA_FP16 && x_type != TUNA_BF16) || !is_number_type(o_type)) return TUNA_ERR_BAD_CONFIG;
-    if (experts > TUNA_MX_MAX_EXPERTS || (double)experts * m * k > (double)(1ll << 41) || (double)n * k > (double)(1ll << 41)) return TUNA_ERR_TOO_LARGE;
+    if (too_long(m, k) || too_long(n, k) || experts > TUNA_MX_MAX_EXPERTS || (double)experts * m * k > (double)(1ll << 41) || (double)n * k > (double)(1ll << 41)) return TUNA_ERR_TOO_LARGE;
     if (!aligned_to(x, 16) || !aligned_to(q, 16) || !aligned_to(s, 16) || !aligned_to(o, 16) || !aligned_to(xs, 16) || !aligned_to(offsets, 4) || !aligned_to(workspace, 16))
         return TUNA_ERR_MISALIGNED;
     const int sms = device_sm_count();
@@ -98,6 +101,6 @@ extern "C" int tuna_mx_matmul_grouped(const void *x, int x_type, const void *xs,
 
 extern "C" size_t tuna_mx_workspace_bytes(int m, int n, int k, int experts, int x_type)
 {
-    if (m < 1 || m % 8 || n < 1 || k < 1 || k % kMxBlock || experts < 0 || experts > TUNA_MX_MAX_EXPERTS) return 0;
+    if (m < 1 || m % 8 || n < 1 || k < 1 || k % kMxBlock || experts < 0 || experts > TUNA_MX_MAX_EXPERTS || too_long(m, k) || too_long(n, k)) return 0;
     return mx_workspace(m, n, k, std::max(1, experts), x_type, experts > 0, device_sm_count()).total;
 }
