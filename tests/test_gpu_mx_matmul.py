@@ -460,6 +460,15 @@ def test_refusals():
     with pytest.raises(tuna_b200.TunaError):
         tuna_b200.mx_matmul(torch.empty(40, k, device="cuda", dtype=torch.bfloat16), None, wq, ws, torch.empty(40, m, device="cuda"), m, 40, k,
                             workspace=torch.zeros(64, dtype=torch.uint8, device="cuda"))
+    x16, o16, need = torch.zeros(40, k, device="cuda", dtype=torch.bfloat16), torch.empty(40, m, device="cuda"), 40 * 264
+    for bad in (torch.zeros(need, dtype=torch.uint8), torch.zeros(1, dtype=torch.uint8, device="cuda").expand(need),
+                torch.zeros(2 * need, dtype=torch.uint8, device="cuda")[::2]):  # off the GPU, not as long as it says, with gaps
+        with pytest.raises(ValueError, match="workspace"):
+            tuna_b200.mx_matmul(x16, None, wq, ws, o16, m, 40, k, workspace=bad)
+        with pytest.raises(ValueError, match="workspace"):
+            tuna_b200.mx_matmul_grouped(x16, None, wq[None], ws[None], off, o16, m, 40, k, workspace=bad)
+    with pytest.raises(TypeError, match="workspace"):
+        tuna_b200.mx_matmul(x16, None, wq, ws, o16, m, 40, k, workspace=4096)
     with pytest.raises(ValueError):
         tuna_b200.mx_matmul_grouped(xq, xs, wq, ws, off, o, m, n, k)  # no leading dimension
     with pytest.raises(TypeError):

@@ -160,6 +160,8 @@ def test_refusals():
         tuna_b200.mx_quantize(x.to(torch.int32))
     with pytest.raises(tuna_b200.TunaError):  # rows not on 16 bytes
         tuna_b200.mx_quantize(torch.randn(8, 130, device="cuda")[:, :128])
+    with pytest.raises(ValueError, match="2147483647"):  # ctypes would make 32 of it
+        tuna_b200.mx_quantize(torch.empty(1, 2 ** 32 + 32, dtype=torch.float16, device="cuda"))
     q, s = tuna_b200.mx_quantize(x)
     with pytest.raises(TypeError):
         tuna_b200.mx_dequant(q, s, torch.empty(8, 256, device="cuda", dtype=torch.float64), 8, 256)

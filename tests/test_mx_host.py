@@ -66,6 +66,15 @@ def test_tensors_off_the_gpu_are_refused():
         tuna_b200.mx_matmul(torch.zeros(1, 256), None, q, s, o, 8, 1, 256)
 
 
+def test_sizes_of_more_than_32_bits_are_refused():
+    t, big = torch.zeros(1, dtype=torch.uint8), 2 ** 32
+    for call in (lambda: tuna_b200.mx_matmul(t, t, t, t, t, 8, 1, big + 32), lambda: tuna_b200.mx_matmul(t, t, t, t, t, big + 8, 1, 32),
+                 lambda: tuna_b200.mx_matmul(t, t, t, t, t, 8, big + 1, 32), lambda: tuna_b200.mx_dequant(t, t, t, 1, big + 32),
+                 lambda: tuna_b200.mx_matmul_grouped(t, t, t, t, t, t, 8, big, 32)):
+        with pytest.raises(ValueError, match="2147483647"):
+            call()
+
+
 def test_argument_validation_needs_no_gpu(tuna_lib):
     buf = ctypes.create_string_buffer(4096 + 64)
     base = (ctypes.addressof(buf) + 63) & ~63
@@ -103,15 +112,6 @@ def test_argument_validation_needs_no_gpu(tuna_lib):
     # nothing is launched - not the tokens' quantizer either - for what the product refuses
     assert mm(x_type=0, m=8, n=(1 << 31) - 1, k=1024, ws_bytes=1 << 60) in (-7, -9)
 
-    def grouped(offsets=p, experts=2, n=4, x_type=3, ws_bytes=big):
-        return tuna_lib.tuna_mx_matmul_grouped(p, x_type, p, p, p, offsets, p, 0, 64, n, 64, experts, p, ws_bytes, None)
-
-    assert grouped(offsets=None) == -1
-    assert grouped(experts=0) == -2
-    assert grouped(experts=1025) == -9
-    assert grouped(offsets=ctypes.c_void_p(base + 2)) == -3
-    assert grouped(x_type=1, ws_bytes=0) == -4
-    assert grouped(n=0) == 0 and grouped(n=-1) == -2
     # sizes that rounded up to a whole tile would no longer have 32 bits, more columns than a grid has chunks for
     long = (1 << 31) - 32
     for type_ in (0, 3):
@@ -123,6 +123,15 @@ def test_argument_validation_needs_no_gpu(tuna_lib):
         assert qz(p, 0, k, p, p, 1, k, 1, None) == -9 and dq(p, p, p, 0, 1, k, 1, None) == -9
         assert tuna_lib.tuna_mx_workspace_bytes(8, 1, k, 0, 0) == 0
 
+    def grouped(offsets=p, experts=2, n=4, x_type=3, ws_bytes=big):
+        return tuna_lib.tuna_mx_matmul_grouped(p, x_type, p, p, p, offsets, p, 0, 64, n, 64, experts, p, ws_bytes, None)
+
+    assert grouped(offsets=None) == -1
+    assert grouped(experts=0) == -2
+    assert grouped(experts=1025) == -9
+    assert grouped(offsets=ctypes.c_void_p(base + 2)) == -3
+    assert grouped(x_type=1, ws_bytes=0) == -4
+    assert grouped(n=0) == 0 and grouped(n=-1) == -2
     assert tuna_lib.tuna_mx_workspace_bytes(60, 33, 64, 0, 0) == 0
     assert tuna_lib.tuna_mx_workspace_bytes(64, 1, 64, 1025, 0) == 0
 

@@ -12,7 +12,7 @@
 //   warp 1     TMA producer of the weights' codes and scales
 //   warp 2     TMA producer of the tokens' codes and, in wide tiles, their scales.  A tile starts at any token, a copy at a multiple
 //              of four words: the scales' copies start up to three words early, and the readers skip those
-//   warp 3     tensor-memory allocation; scales of the tokens in tiles of up to 64 columns, as 4-byte copies (cp.async).  In wide
+//   warp 3     tensor-memory allocation; scales of the tokens in tiles of up to 16 tokens, as 4-byte copies (cp.async).  In wide
 //              tiles this warp would set the pace (0.30 us per 256 columns of a 256-token tile before any other work), in narrow
 //              ones the small TMA copies would (4096x4096 at 1 token 7.3 us, so 4.5)
 //   warps 4-7  epilogue: tensor memory -> registers -> output type -> memory, of more than 16 tokens by way of shared memory,
@@ -228,7 +228,8 @@ __device__ __forceinline__ void mx_quantize_resident(const MxParams &p, int w, i
 }
 
 // CG: CTAs of a worker (1 or 2).  NW: mx_token_words.  RESIDENT: the tokens are numbers in 16 bits and quantized here.
-// Tiles of up to 64 tokens leave room for a second CTA on the SM: that of the next launch, which copies its first weights meanwhile.
+// Tiles of up to 16 tokens of one matrix (NW 2) leave room for a second CTA on the SM: that of the next launch, which copies its first
+// weights meanwhile.
 template <int CG, int NW, bool RESIDENT, typename OT>
 __global__ void __launch_bounds__(32 * kMxWarps, NW == 2 ? 2 : 1)
 mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_w2,
@@ -244,7 +245,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     const int rank = CG == 1 ? 0 : (int)cluster_ctarank();
     const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
     const int N = p.tile_tok, S = p.stages;
-    // [stages of weights][of tokens][of the weights' scales][of the tokens' scales][staging buffers][tables]; the MMAs read 128
+    // [stages of weights][of tokens][of the weights' scales][of the tokens' scales][staging buffer][tables]; the MMAs read 128
     // rows, in low tiles past their stage's end.  RESIDENT: of tokens, all of a tile's stages.
     const int x_stages = RESIDENT ? p.units : S;
     const uint32_t base = smem_u32(smem), w_bytes = (uint32_t)p.w_bytes, x_bytes = (uint32_t)(p.x_rows << p.fold_log) * kMxChunkBytes;
@@ -302,8 +303,8 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                 cnt = end - begin;
                 reached = __shfl_sync(0xffffffffu, end, 31);
             }
-            const int mine = div_up(cnt, N) * p.row_tiles;
             if (e >= p.experts) cnt = 0;
+            const int mine = div_up(cnt, N) * p.row_tiles;
             int sum = mine;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {

@@ -60,6 +60,12 @@ def _scale_shape(rows: int, k: int):
     return (-(-k // 128), rows, 4)
 
 
+def _expect_sizes(*sizes):
+    """The library's sizes have 32 bits, and ctypes would cut longer ones down to them."""
+    if max(sizes) > 0x7fffffff:
+        raise ValueError(f"sizes must not be above 2147483647, got {max(sizes)}")
+
+
 def _numel(shape) -> int:
     return shape[0] * shape[1] * shape[2]
 
@@ -77,10 +83,12 @@ def _expect_output(o, numel, device):
     _expect(o, "o", o.dtype, numel, device)
 
 
-def _workspace(given, *shape_and_type):
+def _workspace(given, device, *shape_and_type):
     """Address and size of the workspace: `given`, or one of this call's own (in stream order, from the pool of the graph that is being captured,
     if one is)."""
-    if given is None:
+    if given is not None:
+        _expect(given, "workspace", getattr(given, "dtype", None), given.numel() if isinstance(given, torch.Tensor) else 0, device)
+    else:
         need = int(_lib.load().tuna_mx_workspace_bytes(*shape_and_type))
         given = torch.empty(need, dtype=torch.uint8, device="cuda") if need else None
     return given, (0, 0) if given is None else (given.data_ptr(), given.numel() * given.element_size())
@@ -101,6 +109,7 @@ def mx_quantize(x):
     if x.dim() not in (2, 3) or x.numel() == 0:
         raise ValueError("x must be a [rows, k] or [matrices, rows, k] tensor with at least one row")
     rows, k = x.shape[-2:]
+    _expect_sizes(rows, k)
     if k % 32:
         raise ValueError(f"k must be a multiple of 32, got {k}")
     stride = k
@@ -124,6 +133,7 @@ def mx_dequant(q, s, o, m: int, k: int) -> None:
     and o, all its matrices."""
     if _launched(_front().mx_dequant(q, s, o, m, k)):
         return
+    _expect_sizes(m, k)
     dev = q.device if isinstance(q, torch.Tensor) else None
     matrices = q.shape[0] if isinstance(q, torch.Tensor) and q.dim() == 4 else 1
     _expect_codes(q, s, ("q", "s"), m, k, dev, matrices)
@@ -151,13 +161,14 @@ def mx_matmul(x, xs, q, s, o, m: int, n: int, k: int, *, workspace=None) -> None
     `mx_quantize` does.  m a multiple of 8, k of 32.  Enqueued on the current stream of x's device."""
     if workspace is None and _launched(_front().mx_matmul(x, xs, q, s, o, m, n, k)):
         return
+    _expect_sizes(m, n, k)
     kind = _tokens(x, xs, n, k)
     dev = x.device
     _expect_codes(q, s, ("q", "s"), m, k, dev)
     _expect_output(o, n * m, dev)
     lib = _lib.load()
     with _on_device(dev):
-        _keep, ws = _workspace(workspace, m, n, k, 0, kind)
+        _keep, ws = _workspace(workspace, dev, m, n, k, 0, kind)
         check(lib.tuna_mx_matmul(x.data_ptr(), kind, 0 if xs is None else xs.data_ptr(), q.data_ptr(), s.data_ptr(), o.data_ptr(), _TYPES[o.dtype], m, n, k,
                                  *ws, _stream_ptr(dev)))
 
@@ -170,6 +181,7 @@ def mx_matmul_grouped(x, xs, q, s, offsets, o, m: int, n: int, k: int, *, worksp
     offsets[experts]: rows of o that no expert has are left as they were.  n = 0 is nothing to do."""
     if workspace is None and _launched(_front().mx_matmul_grouped(x, xs, q, s, offsets, o, m, n, k)):
         return
+    _expect_sizes(m, n, k)
     if not isinstance(q, torch.Tensor) or q.dim() != 4:
         raise ValueError("q must be a [experts, ceil(k/256), m, 128] tensor")
     experts = q.shape[0]
@@ -182,7 +194,7 @@ def mx_matmul_grouped(x, xs, q, s, offsets, o, m: int, n: int, k: int, *, worksp
         return
     lib = _lib.load()
     with _on_device(dev):
-        _keep, ws = _workspace(workspace, m, n, k, experts, kind)
+        _keep, ws = _workspace(workspace, dev, m, n, k, experts, kind)
         check(lib.tuna_mx_matmul_grouped(x.data_ptr(), kind, 0 if xs is None else xs.data_ptr(), q.data_ptr(), s.data_ptr(), offsets.data_ptr(), o.data_ptr(),
                                          _TYPES[o.dtype], m, n, k, experts, *ws, _stream_ptr(dev)))
 
