@@ -292,7 +292,7 @@ int tuna_mx_dequant(const void *q, const void *s, void *o, int o_type, int rows,
  * o[n, m] (fp16, bf16 or fp32) = x[n, k] * w[m, k]^T, w given by q and s, fp32 accumulation, one rounding; results are
  * bit-identical from run to run.  x_type TUNA_MXFP4: x and xs are codes and scales of the tokens.  TUNA_FP16 or TUNA_BF16: x is
  * [n, k] of that type, xs is not read, and the call quantizes x as tuna_mx_quantize does.  m a multiple of 8, k of 32, any
- * n >= 1.  Alignment: 16 bytes.
+ * n >= 1.  Alignment: 16 bytes, of xs 4 (those of a column range of an odd number of tokens).
  * Workspace: tuna_mx_workspace_bytes (experts = 0 for this call) bytes for the codes and scales of tokens in 16 bits, none for
  * TUNA_MXFP4; it is written before it is read.  Calls that overlap on the device need separate ones.
  * Order: ordinary stream order for everything but q and s, which count as constants as in tuna_matmul: they are read while the

@@ -259,6 +259,29 @@ def test_offsets_outside_the_tokens_stay_inside_the_output(offsets):
         check_product(hold.view[r:r + 1], x[r:r + 1], mats[e][1])
 
 
+@pytest.mark.parametrize("n", [1, 2, 16, 17, 19, 43, 130, 515])
+@pytest.mark.parametrize("first,last", [(1, 4), (2, 3), (3, 5), (0, 2)])
+def test_column_ranges_are_views(n, first, last):
+    """Columns 256 first .. 256 last of both operands, which start on 4 bytes where the tokens' scales do."""
+    m, k = 264, 1216
+    (wq, ws), w = random_packed(m, k, 5)
+    (xq, xs), x = random_packed(n, k, 6)
+    a, b = 256 * first, min(k, 256 * last)
+    wq, ws, xq, xs = dev(wq, ws, xq, xs)
+    words = slice(2 * first, 2 * first + -(-(b - a) // 128))
+    o = torch.empty(n, m, device="cuda")
+    tuna_b200.mx_matmul(xq[first:last], xs[words], wq[first:last], ws[words], o, m, n, b - a)
+    finish()
+    check_product(o, x[:, a:b], w[:, a:b])
+    if first:
+        off = torch.tensor([0, n // 2, n], dtype=torch.int32, device="cuda")
+        two = torch.empty_like(o)
+        tuna_b200.mx_matmul_grouped(xq[first:last], xs[words], wq[first:last].expand(2, -1, -1, -1).contiguous(), ws[words].expand(2, -1, -1, -1).contiguous(), off, two,
+                                    m, n, b - a)
+        finish()
+        check_product(two, x[:, a:b], w[:, a:b])
+
+
 # ------------------------------------------------------------------ streams, graphs, devices, a layer
 
 def test_a_mixture_layer_from_activations_to_outputs():

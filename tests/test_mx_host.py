@@ -103,7 +103,7 @@ def test_argument_validation_needs_no_gpu(tuna_lib):
     assert mm(x=None) == -1 and mm(xs=None) == -1 and mm(q=None) == -1 and mm(s=None) == -1 and mm(o=None) == -1
     assert mm(m=60) == -2 and mm(n=0) == -2 and mm(k=48) == -2 and mm(k=0) == -2 and mm(m=-8) == -2
     assert mm(x_type=2) == -5 and mm(x_type=4) == -5 and mm(o_type=3) == -5
-    assert mm(x=odd) == -3 and mm(xs=odd) == -3 and mm(q=odd) == -3 and mm(s=odd) == -3 and mm(o=odd) == -3 and mm(ws=odd) == -3
+    assert mm(x=odd) == -3 and mm(xs=ctypes.c_void_p(base + 2)) == -3 and mm(q=odd) == -3 and mm(s=odd) == -3 and mm(o=odd) == -3 and mm(ws=odd) == -3
     # tokens in 16 bits that a launch of their own quantizes: room for their codes and scales
     need = tuna_lib.tuna_mx_workspace_bytes(64, 33, 64, 0, 0)
     assert need >= 33 * (128 + 4) and tuna_lib.tuna_mx_workspace_bytes(64, 33, 64, 0, 3) == 0

@@ -42,7 +42,7 @@ static int mx_product(const void *x, int x_type, const void *xs, const void *q, 
     if (m < 1 || m % 8 || n < 1 || k < 1 || k % kMxBlock || experts < 1) return TUNA_ERR_BAD_SHAPE;
     if ((!packed && x_type != TUNA_FP16 && x_type != TUNA_BF16) || !is_number_type(o_type)) return TUNA_ERR_BAD_CONFIG;
     if (too_long(m, k) || too_long(n, k) || experts > TUNA_MX_MAX_EXPERTS || (double)experts * m * k > (double)(1ll << 41) || (double)n * k > (double)(1ll << 41)) return TUNA_ERR_TOO_LARGE;
-    if (!aligned_to(x, 16) || !aligned_to(q, 16) || !aligned_to(s, 16) || !aligned_to(o, 16) || !aligned_to(xs, 16) || !aligned_to(offsets, 4) || !aligned_to(workspace, 16))
+    if (!aligned_to(x, 16) || !aligned_to(q, 16) || !aligned_to(s, 16) || !aligned_to(o, 16) || !aligned_to(xs, 4) || !aligned_to(offsets, 4) || !aligned_to(workspace, 16))
         return TUNA_ERR_MISALIGNED;
     const int sms = device_sm_count();
     const MxWorkspace w = mx_workspace(m, n, k, experts, x_type, offsets != nullptr, sms);

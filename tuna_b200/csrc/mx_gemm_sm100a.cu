@@ -74,6 +74,7 @@ struct MxParams {
     int x_rows;     // tokens in a stage of a CTA
     int xs_pitch;   // bytes between the copies of a stage's token scales
     int xs_bytes;   // of all of them
+    int xs_skew;    // words from where tmap_xs starts, which is a multiple of 16 bytes, to p.xs
     int flex;       // row tiles of equal height: tile t has the groups of 8 rows t * groups / row_tiles up to the next tile's
     int groups;     // m / 8
     int x_bf16;     // RESIDENT: type of the tokens
@@ -440,7 +441,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
 #pragma unroll
                             for (int j = 0; j < kPieces; ++j)
                                 tma_load_1d(xs_ring + (uint32_t)(ru.idx * p.xs_bytes + (kPieces * h + j) * p.xs_pitch), &tmap_xs,
-                                            (int)((((unsigned)(2 * c + h) * (unsigned)p.n + (unsigned)tile.tok0) & ~3u) + 128u * j), bar);
+                                            (int)((((unsigned)(2 * c + h) * (unsigned)p.n + (unsigned)(tile.tok0 + p.xs_skew)) & ~3u) + 128u * j), bar);
                     }
                 }
                 __syncwarp();
@@ -498,7 +499,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                 for (int i = 8; i < (int)kScaleCols; ++i) v[i] = 0;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {  // tokens: column 32 j + lane, half h
-                    const uint32_t skip = NW == 2 ? 0u : (((unsigned)(2 * c + h) * (unsigned)p.n + (unsigned)tile.tok0) & 3u) * 4u;
+                    const uint32_t skip = NW == 2 ? 0u : (((unsigned)(2 * c + h) * (unsigned)p.n + (unsigned)(tile.tok0 + p.xs_skew)) & 3u) * 4u;
 #pragma unroll
                     for (int j = 0; j < NW; ++j) {
                         const uint32_t at = NW == 2 ? (uint32_t)(NW * h + j) * 128u : (uint32_t)((NW == 8 ? 2 * h + (j >> 2) : h) * p.xs_pitch) + (uint32_t)(j & 3) * 128u + skip;
@@ -831,9 +832,10 @@ int launch_mx_gemm(const MxGemmArgs &a)
         return TUNA_ERR_NO_DEVICE;
     if (!l.resident && !tiles_of(&maps.x, a.x, (uint64_t)a.n, (uint64_t)p.chunks, (uint32_t)l.x_rows, 1u << l.fold_log)) return TUNA_ERR_NO_DEVICE;
     if (l.words > 2) {
-        const uint64_t dim = (uint64_t)p.words * a.n;
+        p.xs_skew = (int)((reinterpret_cast<uintptr_t>(a.xs) & 15) / 4);
+        const uint64_t dim = (uint64_t)p.words * a.n + p.xs_skew;
         const uint32_t box = (uint32_t)l.xs_copy;
-        if (!make_tensor_map_nd(&maps.xs, CU_TENSOR_MAP_DATA_TYPE_UINT32, a.xs, 1, &dim, nullptr, &box, CU_TENSOR_MAP_SWIZZLE_NONE)) return TUNA_ERR_NO_DEVICE;
+        if (!make_tensor_map_nd(&maps.xs, CU_TENSOR_MAP_DATA_TYPE_UINT32, (const uint32_t *)a.xs - p.xs_skew, 1, &dim, nullptr, &box, CU_TENSOR_MAP_SWIZZLE_NONE)) return TUNA_ERR_NO_DEVICE;
     }
     if (a.numbers && launch_mx_quantize(a.numbers, a.x_type, a.k, const_cast<void *>(a.x), const_cast<void *>(a.xs), a.n, a.k, 1, a.stream, true) != cudaSuccess)
         return TUNA_ERR_LAUNCH;
