@@ -126,6 +126,14 @@ __device__ __forceinline__ void tma_load_1d(uint32_t dst, const CUtensorMap *map
     asm volatile("cp.async.bulk.tensor.1d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2}], [%3];" ::"r"(dst), "l"(map), "r"(c0), "r"(bar) : "memory");
 }
 
+// The same as tma_load_3d, the lines it brings to L2 being kept there by `policy`.
+__device__ __forceinline__ void tma_load_3d_policy(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, uint32_t bar, uint64_t policy)
+{
+    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(dst), "l"(map),
+                 "r"(c0), "r"(c1), "r"(c2), "r"(bar), "l"(policy)
+                 : "memory");
+}
+
 // One lane's words to eight columns of this warp's lanes.
 __device__ __forceinline__ void tc_st_x8(uint32_t taddr, const uint32_t (&v)[8])
 {
@@ -395,6 +403,13 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
         Ring ru;
         bool ok = true;
         int issued = 0;
+        // The weights of tiles of up to 128 tokens, which few tiles want, leave L2 first.  A program that goes through a few times what L2 holds, again
+        // and again, then finds a part of it there the next time, where the oldest lines leaving first would have replaced all (us: going
+        // round 0.3 GB of matrices 28672x4096 at 16 tokens 13.4 -> 12.5, 57344x8192 at 43 43.6 -> 40.9; 0.6 GB 13.4 -> 12.5, 43.9 -> 42.5;
+        // 3 GB the same).  Wider tiles, which others like them want again, are the slower for it (57344x8192 at 4096 tokens 753 -> 761), and a choice
+        // made here as the kernel runs costs more than it gives (4096x14336 at 256 16.1 -> 17.5).
+        uint64_t first_out;
+        if constexpr (NW < 8) asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(first_out));
         if (!p.ahead) depend();
         while (ok && tile.next()) {
             const int block = CG * tile.rt + rank, row = mx_row(p, block), rows = mx_row(p, block + 1) - row;
@@ -408,7 +423,9 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
                     mbar_expect_tx(bar, (uint32_t)(rows << p.fold_log) * kMxChunkBytes + kMxScaleBytes);
                     for (int f = 0; f < fold; ++f) {  // chunks behind the last one read as zeros
                         const int chunk = (c << p.fold_log) + f;
-                        tma_load_3d(base + (uint32_t)ru.idx * w_bytes + (uint32_t)(f * part) * kMxChunkBytes, map, 0, row, tile.e * p.chunks + chunk, bar);
+                        const uint32_t to = base + (uint32_t)ru.idx * w_bytes + (uint32_t)(f * part) * kMxChunkBytes;
+                        if constexpr (NW < 8) tma_load_3d_policy(to, map, 0, row, tile.e * p.chunks + chunk, bar, first_out);
+                        else tma_load_3d(to, map, 0, row, tile.e * p.chunks + chunk, bar);
                         tma_load_2d(ws_ring + (uint32_t)ru.idx * kMxScaleBytes + (uint32_t)(f * part) * 8u, &tmap_ws, row, tile.e * p.words + 2 * chunk, bar);
                     }
                 }
