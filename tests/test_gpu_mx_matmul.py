@@ -372,6 +372,49 @@ def test_graphs_with_tokens_in_16_bits(n):
             check_product(o, mxo.decode(*mxo.quantize(x.double().cpu().numpy())), w)
 
 
+@pytest.mark.parametrize("experts,captured", [(3, False), (3, True), (70, True)])
+def test_offsets_written_right_before_the_call(experts, captured):
+    """A kernel writes the offsets, the call quantizes its tokens, and the next kernel writes other offsets, without a wait in between."""
+    m, n, k, rounds = 512, 80, 1024, 6
+    rng = np.random.default_rng(experts)
+    q, s = tuna_b200.mx_quantize(torch.randn(experts, m, k, device="cuda"))
+    x = torch.randn(n, k, device="cuda", dtype=torch.bfloat16)
+    xq, xs = tuna_b200.mx_quantize(x)
+    counts = [torch.from_numpy(np.diff(np.sort(rng.integers(0, n + 1, experts - 1)), prepend=0, append=n).astype(np.int32)).cuda() for _ in range(rounds)]
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    off = torch.zeros(experts + 1, dtype=torch.int32, device="cuda")
+    outs = [torch.full((n, m), 7.0, device="cuda") for _ in range(rounds)]
+
+    def run():
+        for c, o in zip(counts, outs):
+            torch.cumsum(torch.cat([zero, c]), 0, dtype=torch.int32, out=off)
+            tuna_b200.mx_matmul_grouped(x, None, q, s, off, o, m, n, k)
+
+    if captured:
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            run()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            run()
+        for _ in range(5):
+            for o in outs:
+                o.fill_(7.0)
+            graph.replay()
+    else:
+        for _ in range(5):
+            run()
+    finish()
+    for c, o in zip(counts, outs):
+        torch.cumsum(torch.cat([zero, c]), 0, dtype=torch.int32, out=off)
+        want = torch.empty_like(o)
+        torch.cuda.synchronize()
+        tuna_b200.mx_matmul_grouped(xq, xs, q, s, off, want, m, n, k)
+        finish()
+        assert torch.equal(o, want)
+
+
 def test_calls_on_two_streams_at_once():
     m, n, k = 1024, 16, 4096
     (xq, xs), x = random_packed(n, k, 1)

@@ -107,8 +107,9 @@ struct MxGemmArgs {
     cudaStream_t stream;
     int sm_count;
 };
-// chained: right before the product that reads q and s
-cudaError_t launch_mx_quantize(const void *x, int type, long long row_stride, void *q, void *s, int rows, int k, int batch, cudaStream_t stream, bool chained = false);
+// Right before the product that reads q and s: the product may start with this launch, or once the kernels before this one are done
+enum MxChained { kMxAlone = 0, kMxChained = 1, kMxChainedAfter = 2 };
+cudaError_t launch_mx_quantize(const void *x, int type, long long row_stride, void *q, void *s, int rows, int k, int batch, cudaStream_t stream, MxChained chained = kMxAlone);
 cudaError_t launch_mx_dequant(const void *q, const void *s, void *o, int type, int rows, int k, int batch, cudaStream_t stream);
 int launch_mx_gemm(const MxGemmArgs &a);
 // Whether the product takes tokens of this type as they are; otherwise it wants their codes and scales.

@@ -85,7 +85,7 @@ struct MxParams {
     int d_cols;     // tensor-memory columns of an accumulator: tokens of a tile times fold
     int d_step;     // where the second one starts; nd = 1: 0, or where it overlaps the first
     int sf_col;     // where the scales start
-    int ahead;      // one matrix: weights are read from before the dependency wait (which those of an expert there is work for are not known)
+    int ahead;      // what says which weights are wanted is there before the dependency wait, and they are read from then on
 };
 
 // The tiles of a worker in order, and where each lies.
@@ -296,7 +296,7 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
     }
     auto depend = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
     if (warp == 0) {  // the experts' tiles: first token, tokens, tiles before
-        if (p.offsets) depend();
+        if (p.offsets && !p.ahead) depend();
         int before = 0, reached = 0;
         for (int e0 = 0; e0 < p.experts; e0 += 32) {
             const int e = e0 + lane;
@@ -828,7 +828,9 @@ int launch_mx_gemm(const MxGemmArgs &a)
     p.row_tiles = l.row_tiles; p.w_bytes = l.w_bytes; p.flex = l.flex; p.groups = a.m / 8;
     p.x_rows = l.x_rows; p.xs_pitch = l.xs_pitch; p.xs_bytes = l.xs_bytes;
     p.stages = l.stages; p.nd = l.nd; p.d_cols = l.d_cols; p.d_step = l.d_step; p.sf_col = l.sf_col;
-    p.ahead = a.offsets == nullptr;  // 28672x4096 at 43 tokens 13.6 us, 14.9 with the weights after the wait
+    // One matrix: 28672x4096 at 43 tokens 13.6 us, 14.9 with the weights after the wait.  Experts: after a quantizing launch, which lets this one start
+    // when the kernels that may have written the offsets are done.
+    p.ahead = !a.offsets || a.numbers;
     p.status = device_status_word();
     if (!p.status) return TUNA_ERR_NO_DEVICE;
     // the kernel numbers tiles, a worker's stages, and words of scales in 32 bits
@@ -854,7 +856,7 @@ int launch_mx_gemm(const MxGemmArgs &a)
         const uint32_t box = (uint32_t)l.xs_copy;
         if (!make_tensor_map_nd(&maps.xs, CU_TENSOR_MAP_DATA_TYPE_UINT32, (const uint32_t *)a.xs - p.xs_skew, 1, &dim, nullptr, &box, CU_TENSOR_MAP_SWIZZLE_NONE)) return TUNA_ERR_NO_DEVICE;
     }
-    if (a.numbers && launch_mx_quantize(a.numbers, a.x_type, a.k, const_cast<void *>(a.x), const_cast<void *>(a.xs), a.n, a.k, 1, a.stream, true) != cudaSuccess)
+    if (a.numbers && launch_mx_quantize(a.numbers, a.x_type, a.k, const_cast<void *>(a.x), const_cast<void *>(a.xs), a.n, a.k, 1, a.stream, a.offsets ? kMxChainedAfter : kMxChained) != cudaSuccess)
         return TUNA_ERR_LAUNCH;
     const int ctas = l.workers * l.cg;
     switch (a.o_type) {

@@ -37,13 +37,12 @@ __device__ __forceinline__ MxqPlace mxq_place(int rows, int chunks, int batch, i
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(kMxqWarps * 32)
 mx_quantize_kernel(const T *__restrict__ x, long long row_stride, uint8_t *__restrict__ q, uint32_t *__restrict__ s, int rows, int k, int chunks, int batch,
-                   int log_c, int chained)
+                   int log_c, MxChained chained)
 {
-    // Chained: part of a product, which may start (and read its weights, not this kernel's) while this one runs.
-    if (chained) {
-        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-        asm volatile("griddepcontrol.wait;" ::: "memory");
-    }
+    // Part of a product, which may start (and read its weights, not this kernel's) while this one runs.
+    if (chained == kMxChained) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (chained) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (chained == kMxChainedAfter) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int lane = threadIdx.x & 31;
     const MxqPlace l = mxq_place<ROWS>(rows, chunks, batch, log_c);
     if (!l.any) return;
@@ -167,7 +166,7 @@ static cudaError_t mxq_launch(int rows, int k, int batch, int rows_per_warp, Ker
 static bool mxq_short(int rows, int k, int batch) { return (long long)rows * batch * div_up(k, kMxChunk) <= 8192; }
 
 template <typename T, int ROWS>
-static cudaError_t quantize_as(const void *x, long long row_stride, void *q, void *s, int rows, int k, int batch, bool chained, cudaStream_t stream)
+static cudaError_t quantize_as(const void *x, long long row_stride, void *q, void *s, int rows, int k, int batch, MxChained chained, cudaStream_t stream)
 {
     return mxq_launch(rows, k, batch, ROWS, [&](dim3 grid, int chunks, int log_c) {
         cudaLaunchConfig_t lc = {};
@@ -179,18 +178,18 @@ static cudaError_t quantize_as(const void *x, long long row_stride, void *q, voi
         attr[0].val.programmaticStreamSerializationAllowed = 1;
         lc.attrs = attr;
         lc.numAttrs = chained ? 1 : 0;
-        return cudaLaunchKernelEx(&lc, mx_quantize_kernel<T, ROWS>, (const T *)x, row_stride, (uint8_t *)q, (uint32_t *)s, rows, k, chunks, batch, log_c, (int)chained);
+        return cudaLaunchKernelEx(&lc, mx_quantize_kernel<T, ROWS>, (const T *)x, row_stride, (uint8_t *)q, (uint32_t *)s, rows, k, chunks, batch, log_c, chained);
     });
 }
 
 template <typename T>
-static cudaError_t quantize_any(const void *x, long long row_stride, void *q, void *s, int rows, int k, int batch, bool chained, cudaStream_t stream)
+static cudaError_t quantize_any(const void *x, long long row_stride, void *q, void *s, int rows, int k, int batch, MxChained chained, cudaStream_t stream)
 {
     return mxq_short(rows, k, batch) ? quantize_as<T, 2>(x, row_stride, q, s, rows, k, batch, chained, stream)
                                      : quantize_as<T, 4>(x, row_stride, q, s, rows, k, batch, chained, stream);
 }
 
-cudaError_t launch_mx_quantize(const void *x, int type, long long row_stride, void *q, void *s, int rows, int k, int batch, cudaStream_t stream, bool chained)
+cudaError_t launch_mx_quantize(const void *x, int type, long long row_stride, void *q, void *s, int rows, int k, int batch, cudaStream_t stream, MxChained chained)
 {
     switch (type) {
         case TUNA_FP16: return quantize_any<__half>(x, row_stride, q, s, rows, k, batch, chained, stream);
