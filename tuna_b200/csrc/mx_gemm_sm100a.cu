@@ -404,8 +404,8 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
         bool ok = true;
         int issued = 0;
         // The weights of tiles of up to 128 tokens, which few tiles want, leave L2 first.  A program that goes through a few times what L2 holds, again
-        // and again, then finds a part of it there the next time, where the oldest lines leaving first would have replaced all (us: going
-        // round 0.3 GB of matrices 28672x4096 at 16 tokens 13.4 -> 12.5, 57344x8192 at 43 43.6 -> 40.9; 0.6 GB 13.4 -> 12.5, 43.9 -> 42.5;
+        // and again, then finds a part of it there the next time, where the oldest lines leaving first would have replaced all (us, of 0.3 GB
+        // of matrices in turn 28672x4096 at 16 tokens 13.4 -> 12.5, 57344x8192 at 43 43.6 -> 40.9; 0.6 GB 13.4 -> 12.5, 43.9 -> 42.5;
         // 3 GB the same).  Wider tiles, which others like them want again, are the slower for it (57344x8192 at 4096 tokens 753 -> 761), and a choice
         // made here as the kernel runs costs more than it gives (4096x14336 at 256 16.1 -> 17.5).
         uint64_t first_out;
