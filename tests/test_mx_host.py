@@ -143,3 +143,17 @@ def test_types_match_the_header():
     header = (Path(__file__).resolve().parents[1] / "include" / "tuna_b200.h").read_text()
     values = {n: int(v) for n, v in re.findall(r"(TUNA_(?:FP16|BF16|FP32|MXFP4)) = (\d)", header)}
     assert values == {"TUNA_FP16": mx._TYPES[torch.float16], "TUNA_BF16": mx._TYPES[torch.bfloat16], "TUNA_FP32": mx._TYPES[torch.float32], "TUNA_MXFP4": mx._MXFP4}
+
+
+def test_tokens_are_not_loaded_through_the_read_only_path():
+    """Kernels that quantize a product's tokens start before the kernel that writes these has ended, and PTX allows ld.global.nc (and
+    __ldg) only for what nobody writes while the kernel lives."""
+    import re
+    from pathlib import Path
+
+    source = re.sub(r"//[^\n]*", "", (Path(mx.__file__).parent / "csrc" / "mx_format.cuh").read_text())
+    loads = re.findall(r"void load\(const \w+ \*p\) \{([^}]*)\}", source)
+    assert len(loads) == 3
+    for load in loads:
+        assert set(re.findall(r"(\w+)\(p", load)) == {"mx_load_u4"}
+    assert ".nc" not in source and "ldg" not in source

@@ -13,6 +13,15 @@ constexpr int kMxChunk = 256;      // columns of a chunk of codes: 128 bytes, on
 constexpr int kMxScaleCols = 128;  // columns of a word of scales
 constexpr int kMxChunkBytes = kMxChunk / 2;
 
+// Numbers are read once and kept out of L1, by a coherent load: the kernels that quantize a product's tokens are resident while the kernel
+// that writes these may still run, and the read-only path (ld.global.nc) is for memory that nobody writes as long as the reading kernel lives.
+__device__ __forceinline__ uint4 mx_load_u4(const void *p)
+{
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.L2::128B.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p) : "memory");
+    return v;
+}
+
 // Eight numbers of type T as they lie in memory, their largest magnitude and their values.
 template <typename T>
 struct Mx8;
@@ -20,7 +29,7 @@ template <>
 struct Mx8<__half> {
     uint4 r;
     __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
-    __device__ __forceinline__ void load(const __half *p) { r = ldg_stream_u4(p); }
+    __device__ __forceinline__ void load(const __half *p) { r = mx_load_u4(p); }
     __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w; }
     __device__ __forceinline__ __half2 pair(int i) const { const uint32_t w = word(i); return *reinterpret_cast<const __half2 *>(&w); }
     // Bits (fp32) of the largest magnitude of the four lanes' 32 numbers; NaN's if there is one.
@@ -45,7 +54,7 @@ template <>
 struct Mx8<__nv_bfloat16> {
     uint4 r;
     __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
-    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { r = ldg_stream_u4(p); }
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { r = mx_load_u4(p); }
     __device__ __forceinline__ uint32_t word(int i) const { return i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w; }
     __device__ __forceinline__ __nv_bfloat162 pair(int i) const { const uint32_t w = word(i); return *reinterpret_cast<const __nv_bfloat162 *>(&w); }
     __device__ __forceinline__ uint32_t largest() const
@@ -68,7 +77,7 @@ template <>
 struct Mx8<float> {
     uint4 r, t;
     __device__ __forceinline__ void zero() { r = t = make_uint4(0, 0, 0, 0); }
-    __device__ __forceinline__ void load(const float *p) { r = ldg_stream_u4(p); t = ldg_stream_u4(p + 4); }
+    __device__ __forceinline__ void load(const float *p) { r = mx_load_u4(p); t = mx_load_u4(p + 4); }
     __device__ __forceinline__ uint32_t largest() const
     {
         const uint32_t w[8] = {r.x, r.y, r.z, r.w, t.x, t.y, t.z, t.w};
