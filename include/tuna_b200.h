@@ -295,9 +295,11 @@ int tuna_mx_dequant(const void *q, const void *s, void *o, int o_type, int rows,
  * n >= 1.  Alignment: 16 bytes, of xs 4 (those of a column range of an odd number of tokens).
  * Workspace: tuna_mx_workspace_bytes (experts = 0 for this call) bytes for the codes and scales of tokens in 16 bits, none for
  * TUNA_MXFP4; it is written before it is read.  Calls that overlap on the device need separate ones.
- * Order: ordinary stream order for everything but q and s, which count as constants as in tuna_matmul: they are read while the
- * kernel before the call in its stream still drains, and a kernel that writes them right before must not let dependent launches
- * start early (this library's quantizers do not).
+ * Order: x, xs, offsets, o and the workspace follow ordinary stream order.  So do q and s above 64 tokens, and of experts.  Up to 64
+ * tokens of one matrix q and s count as constants, as in tuna_matmul, and are read while the kernel before the call in its stream
+ * still drains: a kernel that writes them right before such a call must not let dependent launches start early
+ * (griddepcontrol.launch_dependents; this library's quantizers do not); behind one that does, enqueue something that is not a kernel
+ * (a copy, a memset) in between, or synchronise.
  */
 int tuna_mx_matmul(const void *x, int x_type, const void *xs, const void *q, const void *s, void *o, int o_type, int m, int n, int k, void *workspace,
                    size_t workspace_bytes, void *stream);

@@ -91,3 +91,106 @@ def test_an_output_that_is_the_next_ones_tokens(name, dtype, grouped):
                 torch.cuda.synchronize()
                 assert torch.equal(got, w)
     finish()
+
+
+# ------------------------------------------------------------------ a kernel that lets its dependents start before it writes
+
+# Lets its dependents start at once, writes only some 50 us later.
+LATE_WRITER = """
+extern "C" __global__ void late_writer(unsigned char *a, const unsigned char *a_src, int a_n, unsigned char *b, const unsigned char *b_src, int b_n)
+{
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const long long t0 = clock64();
+    while (clock64() - t0 < 100000) { }
+    for (int i = threadIdx.x; i < a_n; i += blockDim.x) a[i] = a_src[i];
+    for (int i = threadIdx.x; i < b_n; i += blockDim.x) b[i] = b_src[i];
+}
+"""
+
+M, K = 264, 800
+
+
+def _operands(n, experts, packed):
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    lead = (experts,) if experts else ()
+    q, s = tuna_b200.mx_quantize(torch.randn(*lead, M, K, generator=gen, device="cuda"))
+    x = torch.randn(n, K, generator=gen, device="cuda", dtype=torch.bfloat16)
+    tokens = dict(zip(("x", "xs"), tuna_b200.mx_quantize(x))) if packed else {"x": x}
+    args = {**tokens, "q": q, "s": s}
+    if experts:
+        args["offsets"] = torch.tensor([n * e // experts for e in range(experts + 1)], dtype=torch.int32, device="cuda")
+    return args
+
+
+def _call(args, o, n):
+    if "offsets" in args:
+        tuna_b200.mx_matmul_grouped(args["x"], args.get("xs"), args["q"], args["s"], args["offsets"], o, M, n, K)
+    else:
+        tuna_b200.mx_matmul(args["x"], args.get("xs"), args["q"], args["s"], o, M, n, K)
+
+
+def _late(names, n, experts, packed, graph):
+    """What `names` say is written by the kernel right before the call."""
+    args = _operands(n, experts, packed)
+    out, want = (torch.zeros(n, M, device="cuda") for _ in range(2))
+    _call(args, want, n)
+    finish()
+    assert torch.isfinite(want).all() and float(want.std()) > 1
+    late = {name: torch.zeros_like(args[name]) for name in names}
+    writer = torch.cuda._compile_kernel(LATE_WRITER, "late_writer")
+    pairs = []
+    for name in (names * 2)[:2]:
+        to, src = late[name], args[name]
+        pairs += [to.view(torch.uint8), src.view(torch.uint8), src.numel() * src.element_size()]
+
+    def calls():
+        writer(grid=(1, 1, 1), block=(256, 1, 1), args=pairs)
+        _call({**args, **late}, out, n)
+
+    run = calls
+    if graph:
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=side):
+                calls()
+        run = g.replay
+    for _ in range(3):
+        torch.cuda.synchronize()
+        for t in late.values():
+            t.zero_()
+        out.fill_(float("nan"))
+        torch.cuda.synchronize()
+        run()
+        finish()
+        assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("graph", [False, True], ids=["eager", "graph"])
+@pytest.mark.parametrize("packed", [True, False], ids=["codes", "numbers"])
+@pytest.mark.parametrize("n", [65, 100, 256, 300])
+def test_weights_of_the_kernel_before(n, packed, graph):
+    """Above 64 tokens weights and their scales follow ordinary stream order, whatever the kernel before does about its dependents."""
+    _late(["q", "s"], n, 0, packed, graph)
+
+
+@pytest.mark.parametrize("graph", [False, True], ids=["eager", "graph"])
+@pytest.mark.parametrize("packed", [True, False], ids=["codes", "numbers"])
+@pytest.mark.parametrize("n", [1, 16, 70, 300])
+def test_experts_weights_of_the_kernel_before(n, packed, graph):
+    _late(["q", "s"], n, 3, packed, graph)
+
+
+@pytest.mark.parametrize("graph", [False, True], ids=["eager", "graph"])
+@pytest.mark.parametrize("experts", [0, 3])
+@pytest.mark.parametrize("packed", [True, False], ids=["codes", "numbers"])
+@pytest.mark.parametrize("n", [1, 2, 16, 40, 64, 65, 300])
+def test_tokens_of_the_kernel_before(n, packed, experts, graph):
+    _late(["x", "xs"] if packed else ["x"], n, experts, packed, graph)
+
+
+@pytest.mark.parametrize("graph", [False, True], ids=["eager", "graph"])
+@pytest.mark.parametrize("packed", [True, False], ids=["codes", "numbers"])
+@pytest.mark.parametrize("n", [1, 16, 40, 300])
+def test_offsets_of_the_kernel_before(n, packed, graph):
+    _late(["offsets"], n, 3, packed, graph)

@@ -52,6 +52,12 @@ constexpr int kMxStageTokens = 128;     // tokens of the output staging buffer
 constexpr int kMxDirectTokens = 16;     // tiles of up to so many tokens are stored from registers
 constexpr int kMxSlackBytes = 1024;     // of shared memory at the end: scales of columns that a tile does not have are read from behind its own
 constexpr uint32_t kMxFoldBytes = kMxDirectTokens * kBlockRows * 4;  // where the parts of a folded tile are added up
+// Up to here the weights of one matrix count as constants and are copied ahead of the dependency wait; above, they follow ordinary stream order as in
+// tuna_matmul: a kernel before this one that has let its dependents start may still be writing them.  Graph replay, us, ahead / after: codes, 512x512
+// at 100 tokens 3.2 / 3.5, 4096x4096 at 65 6.4 / 7.6, 6144x4096 at 256 8.6 / 9.0, 10240x8192 at 777 and 8192x8192 at 4096 the same;
+// below the line 28672x4096 at 43 13.6 / 14.9.  Copies into L2 ahead of the wait, which would be in order, do not help (4096x4096 at 65
+// 7.6, 11000x4128 at 70 8.9 -> 10.0).
+constexpr int kMxAheadTokens = 64;
 constexpr int kMxResidentRows = 4;      // loads in flight of a quantizing warp
 constexpr uint32_t kMxScaleBytes = 2 * kBlockRows * 4;  // of the weights' scales in a stage
 constexpr int kMxSmemMax = 225 * 1024;   // dynamic shared memory of a CTA alone on its SM (1 KB is the kernel's static part, 1 KB the system's)
@@ -828,9 +834,8 @@ int launch_mx_gemm(const MxGemmArgs &a)
     p.row_tiles = l.row_tiles; p.w_bytes = l.w_bytes; p.flex = l.flex; p.groups = a.m / 8;
     p.x_rows = l.x_rows; p.xs_pitch = l.xs_pitch; p.xs_bytes = l.xs_bytes;
     p.stages = l.stages; p.nd = l.nd; p.d_cols = l.d_cols; p.d_step = l.d_step; p.sf_col = l.sf_col;
-    // One matrix: 28672x4096 at 43 tokens 13.6 us, 14.9 with the weights after the wait.  Experts: after a quantizing launch, which lets this one start
-    // when the kernels that may have written the offsets are done.
-    p.ahead = !a.offsets || a.numbers;
+    // Experts: after a quantizing launch, which lets this one start when the kernels that may have written the offsets and weights are done.
+    p.ahead = a.offsets ? a.numbers != nullptr : a.n <= kMxAheadTokens;
     p.status = device_status_word();
     if (!p.status) return TUNA_ERR_NO_DEVICE;
     // the kernel numbers tiles, a worker's stages, and words of scales in 32 bits

@@ -158,7 +158,10 @@ def _tokens(x, xs, n, k):
 def mx_matmul(x, xs, q, s, o, m: int, n: int, k: int, *, workspace=None) -> None:
     """o `[n, m]` (fp16, bf16 or fp32, overwritten) = x `[n, k]` times the transposed matrix of `(q, s)` `[m, k]`, fp32 accumulation,
     one rounding.  x is codes with their scales `xs`, or fp16 or bf16 with `xs=None`: the call quantizes it as
-    `mx_quantize` does.  m a multiple of 8, k of 32.  Enqueued on the current stream of x's device."""
+    `mx_quantize` does.  m a multiple of 8, k of 32.  Enqueued on the current stream of x's device, in whose order it reads and writes; only
+    q and s, up to 64 tokens, count as constants and are read while the kernel before still drains.  A kernel that writes them right
+    before such a call must not let its dependents start early (`mx_quantize` does not); behind one that does, put a copy that is not a
+    kernel in between, or synchronise."""
     if workspace is None and _launched(_front().mx_matmul(x, xs, q, s, o, m, n, k)):
         return
     _expect_sizes(m, n, k)
@@ -178,7 +181,8 @@ def mx_matmul_grouped(x, xs, q, s, offsets, o, m: int, n: int, k: int, *, worksp
     multiplied with matrix e of `q` `[experts, ceil(k/256), m, 128]` and `s`.  `offsets` int32 `[experts + 1]`, not decreasing (one that is less
     than one before it counts as that one), stays on
     the device (a router's cumulative counts): nothing waits for it on the host.  x and o have n rows, which may be more than
-    offsets[experts]: rows of o that no expert has are left as they were.  n = 0 is nothing to do."""
+    offsets[experts]: rows of o that no expert has are left as they were.  n = 0 is nothing to do.  All that it reads, q and s too, follows the
+    order of the stream."""
     if workspace is None and _launched(_front().mx_matmul_grouped(x, xs, q, s, offsets, o, m, n, k)):
         return
     _expect_sizes(m, n, k)
