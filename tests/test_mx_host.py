@@ -157,3 +157,17 @@ def test_tokens_are_not_loaded_through_the_read_only_path():
     for load in loads:
         assert set(re.findall(r"(\w+)\(p", load)) == {"mx_load_u4"}
     assert ".nc" not in source and "ldg" not in source
+
+
+def test_as_many_output_features_as_are_accepted(tuna_lib):
+    """A plan that rounds m up to whole tiles on every SM must not pass 32 bits for any m that is not refused: the tokens of a call this small are
+    quantized by the product itself, whatever m is."""
+    most = (1 << 31) - 1024
+    for m in (8 * 1000, 1 << 30, most - 128 * 148, most - 18936, most - 8, most):
+        for n in (1, 2, 16):
+            assert tuna_lib.tuna_mx_workspace_bytes(m, n, 32, 0, 0) == 0, (m, n)
+    assert tuna_lib.tuna_mx_workspace_bytes(most, 17, 32, 0, 0) == 17 * (128 + 4)
+    assert tuna_lib.tuna_mx_workspace_bytes(most + 8, 1, 32, 0, 0) == 0
+    buf = ctypes.create_string_buffer(4096 + 64)
+    p = ctypes.c_void_p((ctypes.addressof(buf) + 63) & ~63)
+    assert tuna_lib.tuna_mx_matmul(p, 3, p, p, p, p, 0, most + 8, 1, 32, p, 1 << 40, None) == -9

@@ -724,7 +724,7 @@ static MxPlan mx_plan(int m, int n, int k, int experts, int x_type, int o_type, 
     if (l.cg == 1) {
         l.flex = 1;
         l.tile_tok = kMxDirectTokens;
-        l.row_tiles = std::min(m / 8, div_up(m, kBlockRows * sm_count) * sm_count);
+        l.row_tiles = (int)std::min<long long>(m / 8, div_up_ll(m, (long long)kBlockRows * sm_count) * sm_count);
         const int height = 8 * div_up(m / 8, l.row_tiles);
         l.fold_log = height <= 32 ? 2 : height <= 64 ? 1 : 0;
         l.w_bytes = (l.fold_log ? kBlockRows : height) * kMxChunkBytes;
