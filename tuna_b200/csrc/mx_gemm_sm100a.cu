@@ -409,11 +409,13 @@ mx_gemm_kernel(const __grid_constant__ MxParams p, const __grid_constant__ CUten
         Ring ru;
         bool ok = true;
         int issued = 0;
-        // The weights of tiles of up to 128 tokens, which few tiles want, leave L2 first.  A program that goes through a few times what L2 holds, again
-        // and again, then finds a part of it there the next time, where the oldest lines leaving first would have replaced all (us, of 0.3 GB
-        // of matrices in turn 28672x4096 at 16 tokens 13.4 -> 12.5, 57344x8192 at 43 43.6 -> 40.9; 0.6 GB 13.4 -> 12.5, 43.9 -> 42.5;
-        // 3 GB the same).  Wider tiles, which others like them want again, are the slower for it (57344x8192 at 4096 tokens 753 -> 761), and a choice
-        // made here as the kernel runs costs more than it gives (4096x14336 at 256 16.1 -> 17.5).
+        // The weights of tiles of up to 128 tokens leave L2 first.  A program that goes through a few times what L2 holds, again and again, then
+        // finds a part of it there the next time, where the oldest lines leaving first would have replaced all (us, first / as other lines, of 0.3 GB of
+        // matrices in turn: 28672x4096 at 16 tokens 12.5 / 13.4, 57344x8192 at 43 42.0 / 45.3, eight 28672x4096 of 32 67.3 / 71.0; of 0.6 GB
+        // 28672x4096 at 16 12.5 / 13.4, 57344x8192 at 43 42.5 / 43.9; 3 GB the same).  Where several tiles of tokens want the same weights, they mostly want them at
+        // once: 512x4096 at 4096 tokens (32 tiles) 9.2 / 9.1, 512x16384 at 1000 17.5 / 17.3, 4096x14336 at 500 20.6 / 20.6, eight 14336x4096 of
+        // 800, 600 of them one expert's, 63.4 / 64.2, eight 4096x14336 of 710, 500 one's, 56.3 / 58.4; asking, tile by tile, for the number of
+        // token tiles gives 9.4, 17.5, 21.0, 63.5, 59.0.  In wider tiles it costs (57344x8192 at 4096 tokens 753 -> 761).
         uint64_t first_out;
         if constexpr (NW < 8) asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(first_out));
         if (!p.ahead) depend();
