@@ -171,3 +171,13 @@ def test_as_many_output_features_as_are_accepted(tuna_lib):
     buf = ctypes.create_string_buffer(4096 + 64)
     p = ctypes.c_void_p((ctypes.addressof(buf) + 63) & ~63)
     assert tuna_lib.tuna_mx_matmul(p, 3, p, p, p, p, 0, most + 8, 1, 32, p, 1 << 40, None) == -9
+
+
+def test_row_scales_are_not_loaded_through_the_read_only_path():
+    """The codebook kernels start early as well, and absmax follows ordinary stream order."""
+    import re
+    from pathlib import Path
+
+    for path in (Path(mx.__file__).parent / "csrc").glob("gemm_*.cu"):
+        source = re.sub(r"//[^\n]*", "", path.read_text())
+        assert "absmax" in source and "__ldg(" not in source, path.name

@@ -338,7 +338,8 @@ __global__ void __launch_bounds__(kStreamThreads, 1) gemm_stream_kernel(const St
                 // four scalar loads: absmax only has to be 4-byte aligned (a slice of a larger scale buffer)
                 const float *scp = reinterpret_cast<const float *>(
                     reinterpret_cast<const uint8_t *>(p.absmax) + (size_t)tile_b * (size_t)p.absmax_stride + (size_t)row * 4);
-                const float4 sc = make_float4(__ldg(scp), __ldg(scp + 1), __ldg(scp + 2), __ldg(scp + 3));
+                // coherent: the kernel before this one may have written them while this one was resident
+                const float4 sc = make_float4(__ldcg(scp), __ldcg(scp + 1), __ldcg(scp + 2), __ldcg(scp + 3));
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
