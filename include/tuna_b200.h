@@ -271,8 +271,9 @@ int tuna_quantize_nf4(const void *w, void *q, void *absmax, void *code_out, int 
  *   q        u8 [ceil(k/256), rows, 128]  codes in chunks of 256 columns: byte j of a chunk's row holds column 2j in its
  *                                         LOW and 2j+1 in its HIGH nibble
  *   s        u8 [ceil(k/128), rows, 4]    scale bytes in words of 128 columns
- * k is a multiple of 32, up to 67107840; what lies behind column k in the last chunk or word is zero, and has to be.  A set of `batch` or
- * `experts` matrices has them one after another.
+ * k is a multiple of 32, up to 67107840; what lies behind column k in the last chunk or word is zero, and has to be: products take some
+ * of it in.  So a column range of a wider matrix starts at a multiple of 256 and ends at one, or at the matrix's end.  A set of
+ * `batch` or `experts` matrices has them one after another.
  */
 typedef enum tuna_type { TUNA_FP16 = 0, TUNA_BF16 = 1, TUNA_FP32 = 2, TUNA_MXFP4 = 3 } tuna_type;
 #define TUNA_MX_MAX_EXPERTS 1024

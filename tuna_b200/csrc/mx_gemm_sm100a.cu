@@ -684,7 +684,8 @@ struct MxPlan {
 // steps of 256 columns (the tensor pipe's four MMAs, which take hardly less for few tokens; wide tiles at the rate of the copies
 // to shared memory as well) and what of a wide tile's epilogue nothing hides; what all tiles copy, from L2; the weights,
 // from HBM.  Fitted to 1250 launches (graph replay; 11 matrices from 512x16384 to 57344x8192, 17 to 4096 tokens, every width): what it
-// chooses takes 1.6 % longer than the fastest width in the mean, 20 % at worst (2048x2048 at 17 tokens).
+// chooses takes 1.6 % longer than the fastest width in the mean, 20 % at worst (2048x2048 at 17 tokens). All of them read weights ahead of
+// the dependency wait, as those above 64 tokens no longer do; that adds up to 1.2 us to a launch in a chain and was not fitted again.
 static double mx_pair_us(int m, int n, int k, int cols, int pairs)
 {
     const int row_tiles = div_up(m, 2 * kBlockRows), chunks = div_up(k, kMxChunk);

@@ -3,7 +3,9 @@
 A matrix `[rows, k]` (k a multiple of 32) is a pair of uint8 tensors: codes `q` `[ceil(k/256), rows, 128]`, column 2j of a
 256-column chunk in the low nibble of byte j and 2j+1 in the high one, and scales `s` `[ceil(k/128), rows, 4]`, a byte
 (exponent plus 127; 255 is NaN) for every 32 columns.  What lies behind column k in the last chunk is zero.  A set of
-experts' matrices has a leading dimension.  Column ranges that start at a multiple of 256 are views of the leading dimension.
+experts' matrices has a leading dimension.  Column ranges are views of the leading dimension of chunks and words where they start at a
+multiple of 256 and end at one, or at the matrix's end.  A range that ends inside a chunk has the columns behind it there instead of
+zeros, and has to be copied and cleared: products take them in, as many as the number of tokens makes them.
 
 The reference has no counterpart: its one 4-bit format is the codebook of `matmul`.
 """
