@@ -275,7 +275,7 @@ int tuna_quantize_nf4(const void *w, void *q, void *absmax, void *code_out, int 
  * of it in.  So a column range of a wider matrix starts at a multiple of 256 and ends at one, or at the matrix's end.  A set of
  * `batch` or `experts` matrices has them one after another.
  */
-typedef enum tuna_type { TUNA_FP16 = 0, TUNA_BF16 = 1, TUNA_FP32 = 2, TUNA_MXFP4 = 3 } tuna_type;
+typedef enum tuna_type { TUNA_FP16 = 0, TUNA_BF16 = 1, TUNA_FP32 = 2, TUNA_MXFP4 = 3, TUNA_FP8 = 4 } tuna_type;
 #define TUNA_MX_MAX_EXPERTS 1024
 
 /*
@@ -315,6 +315,70 @@ int tuna_mx_matmul(const void *x, int x_type, const void *xs, const void *q, con
 int tuna_mx_matmul_grouped(const void *x, int x_type, const void *xs, const void *q, const void *s, const void *offsets, void *o, int o_type, int m, int n,
                            int k, int experts, void *workspace, size_t workspace_bytes, void *stream);
 size_t tuna_mx_workspace_bytes(int m, int n, int k, int experts, int x_type);
+
+/*
+ * 8-bit block-scaled matrices.  No counterpart in the reference.
+ *   numbers  code e4m3 (one byte: sign, four bits of exponent, three of mantissa; largest 448, 0x7f and 0xff are NaN) x scale 2^(byte - 127);
+ *            128 columns of a row, 128 rows of a column or 128 x 128 share a scale byte, and byte 255 makes them NaN
+ *   q        u8 [rows, k], row by row
+ *   s        TUNA_FP8_ROW     u8 [ceil(k/512), rows, 4]       what a product sums over the columns of (activations, their gradients)
+ *            TUNA_FP8_COLUMN  u8 [ceil(rows/512), k, 4]       what it sums over the rows of (both, for a weight's gradient)
+ *            TUNA_FP8_SQUARE  u8 [ceil(rows/128), ceil(k/128)] weights
+ * k, and m and f below, are multiples of 16 of up to 8388608 (m = 2f); n and rows are any number from 1 on.  Alignment: 16 bytes, of xs 4, of
+ * square scales 1.
+ */
+typedef enum tuna_fp8_blocks { TUNA_FP8_ROW = 0, TUNA_FP8_COLUMN = 1, TUNA_FP8_BOTH = 2, TUNA_FP8_SQUARE = 3 } tuna_fp8_blocks;
+/* g * sigma(g), or GELU in its tanh form: g * (1 + tanh(sqrt(2/pi) (g + 0.044715 g^3))) / 2 */
+typedef enum tuna_activation { TUNA_SILU = 0, TUNA_GELU = 1 } tuna_activation;
+
+/*
+ * Quantizer: x [rows, k] of x_type (fp16, bf16 or fp32), rows row_stride elements apart -> q and s; TUNA_FP8_BOTH: by row into q and s, by column into
+ * q2 and s2, which the others do not use.  The scale of a block is the smallest power of two over which its largest magnitude is not above 448,
+ * not below 2^-127; codes are its numbers over the scale, rounded to nearest with ties to even.  A block that holds an infinity or
+ * NaN gets scale byte 255.  Scale bytes of blocks that the last word does not have are zero.
+ */
+int tuna_fp8_quantize(const void *x, int x_type, long long row_stride, int blocks, void *q, void *s, void *q2, void *s2, int rows, int k, void *stream);
+
+/* o [rows, k] of o_type (fp16, bf16 or fp32) = the numbers of q and s (row, column or square), rounded once. */
+int tuna_fp8_dequant(const void *q, const void *s, int blocks, void *o, int o_type, int rows, int k, void *stream);
+
+/*
+ * o[n, m] (fp16, bf16 or fp32) = x[n, k] * w[m, k]^T, w given by q and s (square), fp32 accumulation, one rounding; results are bit-identical from
+ * run to run.  x_type TUNA_FP8: x and xs are codes and scales of the tokens, by row.  TUNA_FP16 or TUNA_BF16: x is [n, k] of that
+ * type, xs is not read, and the call quantizes x as tuna_fp8_quantize does.
+ * Workspace, here and below: tuna_fp8_workspace_bytes bytes, written before they are read; null where that is 0.  Calls that overlap on the device
+ * need separate ones.
+ * Order: as tuna_mx_matmul, q and s up to 64 tokens counting as constants; everything else, and all that the gradients' calls read, follows
+ * ordinary stream order.
+ */
+int tuna_fp8_matmul(const void *x, int x_type, const void *xs, const void *q, const void *s, void *o, int o_type, int m, int n, int k, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
+/*
+ * The gradients of tuna_fp8_matmul, given dy[n, m] of dy_type (fp16 or bf16), the output's:
+ *   dx[n, k] = dy * w    dy quantized by row
+ *   dw[m, k] = dy^T * x  dy and x quantized by column; the gradient of the numbers that q and s stand for
+ * Either of dx and dw (fp16, bf16 or fp32) may be null, and what only it reads (q and s; x and xs) too.  x_type TUNA_FP8: x and xs are codes and
+ * scales by COLUMN.  What is quantized has the quantizer's rounding: dx and dw are the exact sums of these, in fp32, rounded once.
+ */
+int tuna_fp8_matmul_backward(const void *dy, int dy_type, const void *x, int x_type, const void *xs, const void *q, const void *s, void *dx, int dx_type, void *dw,
+                             int dw_type, int m, int n, int k, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * The first half of a gated feed-forward block in one launch: h[n, f] (fp16, bf16 or fp32) = activation(g) * u, where g[n, f] and u[n, f] are x
+ * times the transposed first and last f rows of w[2f, k].  x as in tuna_fp8_matmul.  z (null, or [n, 2f] of h_type, which is fp16 or bf16 then)
+ * keeps g and u side by side for the gradients; h is made of g and u before they are rounded.
+ */
+int tuna_fp8_gated(const void *x, int x_type, const void *xs, const void *q, const void *s, void *h, int h_type, void *z, int f, int n, int k, int activation,
+                   void *workspace, size_t workspace_bytes, void *stream);
+
+/* Its gradients, given dh[n, f] and z[n, 2f] of one type (fp16 or bf16): those of tuna_fp8_matmul for dy = [dh u activation'(g) | dh activation(g)]. */
+int tuna_fp8_gated_backward(const void *dh, const void *z, int type, const void *x, int x_type, const void *xs, const void *q, const void *s, void *dx, int dx_type,
+                            void *dw, int dw_type, int f, int n, int k, int activation, void *workspace, size_t workspace_bytes, void *stream);
+
+/* call: which of the four a workspace is for; m = 2f for a gated block.  x_type as there (without dw: TUNA_FP8). */
+typedef enum tuna_fp8_call { TUNA_FP8_MATMUL = 0, TUNA_FP8_GATED = 1, TUNA_FP8_BACKWARD = 2 } tuna_fp8_call;
+size_t tuna_fp8_workspace_bytes(int call, int m, int n, int k, int x_type);
 
 const char *tuna_status_string(int status);
 

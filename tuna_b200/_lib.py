@@ -82,6 +82,13 @@ SYMBOLS = {
     "tuna_mx_matmul": (c_int, [c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 4 + [c_void_p, c_size_t, c_void_p]),
     "tuna_mx_matmul_grouped": (c_int, [c_void_p, c_int] + [c_void_p] * 5 + [c_int] * 5 + [c_void_p, c_size_t, c_void_p]),
     "tuna_mx_workspace_bytes": (c_size_t, [c_int] * 5),
+    "tuna_fp8_quantize": (c_int, [c_void_p, c_int, c_longlong, c_int] + [c_void_p] * 4 + [c_int] * 2 + [c_void_p]),
+    "tuna_fp8_dequant": (c_int, [c_void_p] * 2 + [c_int, c_void_p] + [c_int] * 3 + [c_void_p]),
+    "tuna_fp8_matmul": (c_int, [c_void_p, c_int] + [c_void_p] * 4 + [c_int] * 4 + [c_void_p, c_size_t, c_void_p]),
+    "tuna_fp8_matmul_backward": (c_int, [c_void_p, c_int, c_void_p, c_int] + [c_void_p] * 4 + [c_int, c_void_p] + [c_int] * 4 + [c_void_p, c_size_t, c_void_p]),
+    "tuna_fp8_gated": (c_int, [c_void_p, c_int] + [c_void_p] * 4 + [c_int, c_void_p] + [c_int] * 4 + [c_void_p, c_size_t, c_void_p]),
+    "tuna_fp8_gated_backward": (c_int, [c_void_p] * 2 + [c_int, c_void_p, c_int] + [c_void_p] * 4 + [c_int, c_void_p] + [c_int] * 5 + [c_void_p, c_size_t, c_void_p]),
+    "tuna_fp8_workspace_bytes": (c_size_t, [c_int] * 5),
     "tuna_check_device_status": (c_int, [c_void_p]),
     "tuna_selftest_bounded_wait": (c_int, [c_void_p]),
     "tuna_status_string": (c_char_p, [c_int]),

@@ -21,7 +21,8 @@ CSRC = HERE / "csrc"
 LIB = HERE / "libtuna_b200.so"
 FAST_CALL = HERE / ("_fast_call" + sysconfig.get_config_var("EXT_SUFFIX"))
 SOURCES = ["tuna_api.cu", "host_util.cu", "dequant_sm100a.cu", "quantize_sm100a.cu", "gemm_stream_sm100a.cu", "gemm_tstream_sm100a.cu", "gemm_pair_sm100a.cu", "exchange_sm100a.cu", "ref_symbols.cu",
-           "mx_quantize_sm100a.cu", "mx_gemm_sm100a.cu", "mx_api.cu"]
+           "mx_quantize_sm100a.cu", "mx_gemm_sm100a.cu", "mx_api.cu",
+           "fp8_quantize_sm100a.cu", "fp8_gemm_sm100a.cu", "fp8_api.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-lineinfo", "-O3", "-std=c++17", "--expt-relaxed-constexpr",

@@ -1,0 +1,870 @@
+// Products of 8-bit block-scaled matrices (format: fp8_format.cuh) on the 5th-generation tensor cores of sm_100a, one kernel in four forms:
+//
+//   product  o[t][r]  = sum over c of x[t][c] w[r][c]                     x by row, w square
+//   gated    h[t][i]  = act(g) u, g and u the same sums for rows i and f + i of w; z = [g | u] on wish
+//   dx       dx[t][c] = sum over r of dy[t][r] w[r][c]                    dy by row, w square: the same codes and scales, read across
+//   dw       dw[r][c] = sum over t of dy[t][r] x[t][c]                    both by column: the blocks lie along the tokens
+//
+// (x, w and so on are the blocks' codes times their scales.)  The tensor cores apply the scales themselves (tcgen05.mma kind::mxf8f6f4, scale_vec::1X), so per
+// 128 of what is summed over a tile's codes are copied to shared memory as they lie in memory and four MMAs of 32 add to fp32
+// accumulators; the scales of four such blocks are one 32-bit word a row, written to tensor memory once for sixteen MMAs.
+//
+// What a lane of tensor memory has is what lies side by side in the output: operand A are its columns (weights' rows, or their columns in dx, x's in
+// dw), B its rows.  Where an operand's summed dimension is not the one that lies side by side in memory (w in dx, both in dw) it is
+// taken "MN-major": 128 bytes of a staged row are 128 rows of the operand, and nothing is ever transposed in memory.
+//
+// gated: a tile's rows are, by a four-dimensional tensor map, eight of the gate and the eight of the other projection that belong to them in turn.  So
+// the fragments that a thread takes out of tensor memory (lanes i and i + 8) hold both factors, and the product is made in its registers.
+//
+// Persistent CTAs (up to 16 tokens), or pairs of CTAs (cta_group::2: 256 rows of A, every CTA stages its own 128 and half of B), of 12 warps:
+//   warp 0     MMA issue (one elected lane; in a pair the first CTA's)
+//   warp 1, 2  TMA producers of A and of B
+//   warp 3     tensor-memory allocation; in a pair, tells the first CTA that a stage has landed
+//   warps 4-7  epilogue: tensor memory -> registers -> output type -> shared memory, where rows become contiguous -> memory
+//   warps 8-11 scales, one warp per lane quarter: global memory -> registers, a group of four stages ahead -> tensor memory, the word of row r at lane r % 32,
+//              column r / 32, in every quarter
+// RESIDENT: a few tokens in 16 bits are quantized by the CTA itself before its first MMA, all of K, and stay in shared memory.
+//
+// Work split.  No sum is cut.  Up to 16 tokens the weights are cut into row tiles of equal height, a whole number of them for every CTA: the MMAs compute 128
+// rows whatever the height, which costs nothing where the weights' bytes are the bound.  Where a tile has at most 64 (32) of the
+// 128 rows, two (four) blocks of K lie side by side in it ("folded"): the MMA's rows are those of the tile for each block in turn, its columns the tokens
+// for each block, and the epilogue adds up what belongs together.  Everything else goes in tiles of 256 rows on pairs, of as many columns as an estimate says.
+//
+// Every wait is bounded, as in the other pipeline kernels.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <mutex>
+#include "launchers.h"
+#include "fp8_format.cuh"
+#include "sm100_ptx.cuh"
+#include "tcgen05.cuh"
+
+namespace tuna {
+
+enum Fp8Form { kFp8Product, kFp8GatedProduct, kFp8Dx, kFp8Dw };
+
+constexpr int kFp8Warps = 12;
+constexpr int kFp8EpilogueWarp0 = 4;
+constexpr int kFp8ScaleWarp0 = 8;
+constexpr int kFp8MaxStages = 12;
+constexpr int kFp8DirectCols = 16;        // tokens up to which single CTAs take the tiles
+constexpr int kFp8StageCols = 64;         // columns of the output staging buffer
+constexpr int kFp8AheadTokens = 64;       // up to here weights count as constants and are copied ahead of the dependency wait, as in mx_gemm_sm100a.cu
+constexpr int kFp8ResidentLoads = 4;      // loads in flight of a quantizing warp
+constexpr int kFp8SfCols = 16;            // tensor-memory columns of a group's scales: A's words at 0 to 3, B's at 8 to 15
+constexpr uint32_t kFp8FoldBytes = kFp8DirectCols * kBlockRows * 4;
+constexpr int kFp8SmemMax = 225 * 1024;   // dynamic shared memory of a CTA alone on its SM (1 KB is the kernel's static part, 1 KB the system's)
+constexpr int kFp8SmemHalf = 111 * 1024;  // of one that leaves room for another
+
+struct Fp8Params {
+    const uint8_t *as;  // scales of A
+    const uint8_t *bs;  // of B
+    void *o, *z;
+    DeviceStatus *status;
+    int rows;        // of A; gated: 2f
+    int cols;        // of B
+    int red;         // what is summed over
+    int blocks;      // ceil(red / 128)
+    int units;       // stages of a tile: ceil(blocks / fold)
+    int fold_log;    // log2(fold): blocks side by side in a stage
+    int tile_cols;   // N
+    int width;       // columns of a tile, all but the last
+    int row_tiles, col_tiles;
+    int rows_inner;  // tiles follow one another along the rows
+    int group_rows;  // rows of a tile come in groups of 8, gated 16: eight features
+    int groups;
+    int flex;        // row tiles of equal height: tile t has the groups t * groups / row_tiles up to the next tile's
+    int a_bytes;     // of a stage of A
+    int b_rows;      // rows of B in a stage of a CTA (MN-major: 128)
+    int stages;
+    int last_steps;  // MMAs of the last block: 32 each
+    int nd;          // accumulators that are free of one another
+    int d_cols;      // tensor-memory columns of an accumulator: columns of a tile times fold
+    int d_step;      // where the second one starts
+    int sf_col;      // where the two buffers of scales start
+    int ahead;       // A is there before the dependency wait
+    int x_bf16;      // RESIDENT: type of the tokens
+    const void *x;   // RESIDENT: the tokens [cols][red]
+    int gelu;
+    int z_offset;    // gated: where z is staged
+};
+
+struct Fp8Tiles {
+    int next_tile, step, rt, col0, valid;
+    __device__ void init(int worker, int workers) { next_tile = worker; step = workers; }
+    __device__ bool next(const Fp8Params &p)
+    {
+        if (next_tile >= p.row_tiles * p.col_tiles) return false;
+        const int inner = p.rows_inner ? p.row_tiles : p.col_tiles, outer_at = next_tile / inner, inner_at = next_tile - outer_at * inner;
+        rt = p.rows_inner ? inner_at : outer_at;
+        col0 = (p.rows_inner ? outer_at : inner_at) * p.width;
+        valid = min(p.width, p.cols - col0);
+        next_tile += step;
+        return true;
+    }
+    __device__ int total(const Fp8Params &p) const { const int n = p.row_tiles * p.col_tiles; return next_tile < n ? (n - 1 - next_tile) / step + 1 : 0; }
+};
+
+// D[tmem] (+)= (A * scale A) (B * scale B), 32 columns of e4m3 with one scale
+template <int CG>
+__device__ __forceinline__ void tc_mma_fp8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate)
+{
+    if (CG == 1)
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+            " tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}"
+            ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p;\n setp.ne.b32 p, %6, 0;\n"
+            " tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n}"
+            ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
+            : "memory");
+}
+
+// Instruction descriptor, kind::mxf8f6f4: A and B e4m3 (0 at bits 7-9 and 10-12), A and B MN-major at bits 15 and 16, N >> 3 at bits 17-22, e8m0 scales
+// (bit 23), M >> 7 at bits 27-28, which byte of a scale word A and B use at bits 29-30 and 4-5.
+template <int CG>
+__host__ __device__ constexpr uint32_t fp8_idesc(int cols, bool a_mn, bool b_mn)
+{
+    return ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(cols >> 3) << 17) | (1u << 23) | ((uint32_t)CG << 27);
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int c0, int c1, int c2, int c3, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst), "l"(map), "r"(c0), "r"(c1),
+                 "r"(c2), "r"(c3), "r"(bar)
+                 : "memory");
+}
+
+// First row of row block b (a CTA's share of a tile).
+__device__ __forceinline__ int fp8_row(const Fp8Params &p, int b) { return p.flex ? p.group_rows * (int)((long long)b * p.groups / p.row_tiles) : b * kBlockRows; }
+
+// Quantizes the tokens' numbers, all of K: warp `w` of `warps` takes every warps-th (two blocks, token).  Codes as TMA would have put them (128-byte
+// swizzle); scale bytes in words [group of four stages][64 columns: token of a block of the stage].
+template <typename T>
+__device__ __forceinline__ void fp8_quantize_resident(const Fp8Params &p, int w, int warps, int lane, uint32_t codes_at, uint32_t words_at)
+{
+    const int items = ((p.units << p.fold_log) + 1) / 2 * p.cols, limit = p.units << p.fold_log;  // blocks behind the last one are zeros
+    for (int i0 = w; i0 < items; i0 += kFp8ResidentLoads * warps) {
+        Mx8<T> v[kFp8ResidentLoads];
+#pragma unroll
+        for (int r = 0; r < kFp8ResidentLoads; ++r) {
+            const int i = i0 + r * warps, c = i / p.cols, t = i - c * p.cols, col = c * 256 + lane * 8;
+            if (i < items && col < p.red) v[r].load(static_cast<const T *>(p.x) + (size_t)t * p.red + col);
+            else v[r].zero();
+        }
+#pragma unroll
+        for (int r = 0; r < kFp8ResidentLoads; ++r) {
+            const int i = i0 + r * warps, c = i / p.cols, t = i - c * p.cols, b = 2 * c + (lane >> 4);
+            if (i >= items) break;
+            uint32_t m = v[r].largest();
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            m = max(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            const uint32_t e = fp8_scale(m);
+            const float inverse = fp8_inverse(e);
+            float f[8];
+            v[r].values(f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) f[k] *= inverse;
+            uint32_t lo = fp8_encode4(f[0], f[1], f[2], f[3]), hi = fp8_encode4(f[4], f[5], f[6], f[7]);
+            if (e == 255u) lo = hi = 0;
+            if (b >= limit) continue;
+            // 16-byte piece (lane % 16) / 2 of the token's 128 bytes, XORed with the token's number mod 8
+            const uint32_t piece = (((uint32_t)lane >> 1) & 7u) ^ ((uint32_t)t & 7u);
+            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(codes_at + ((uint32_t)b * (uint32_t)p.b_rows + (uint32_t)t) * 128u + (piece << 4) + ((uint32_t)lane & 1u) * 8u),
+                         "r"(lo), "r"(hi)
+                         : "memory");
+            const int unit = b >> p.fold_log, at = (b - (unit << p.fold_log)) * p.b_rows + t;
+            if ((lane & 15) == 0) asm volatile("st.shared.u8 [%0], %1;" ::"r"(words_at + (uint32_t)(unit >> 2) * 256u + (uint32_t)at * 4u + ((uint32_t)unit & 3u)), "r"(e) : "memory");
+        }
+    }
+}
+
+__device__ __forceinline__ float fp8_activation(float g, float u, int gelu) { return gelu ? g * fp8_gate<true>(g) * u : g * fp8_gate<false>(g) * u; }
+
+// CG: CTAs of a worker (1 or 2).  Single CTAs leave room for a second one on the SM: that of the next launch, which copies its first weights meanwhile.
+template <int CG, int FORM, bool RESIDENT, typename OT>
+__global__ void __launch_bounds__(32 * kFp8Warps, CG == 1 ? 2 : 1)
+fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a2, const __grid_constant__ CUtensorMap tmap_b)
+{
+    extern __shared__ __align__(1024) uint8_t smem[];
+    // landed, full, empty: of the stages; d_full, d_empty, sf_full, sf_empty: two each
+    __shared__ __align__(8) uint64_t bars[3 * kFp8MaxStages + 8];
+    __shared__ uint32_t s_tmem_base;
+    __shared__ int s_abort;
+
+    constexpr bool kGated = FORM == kFp8GatedProduct, kAcrossA = FORM >= kFp8Dx, kAcrossB = FORM == kFp8Dw;
+    constexpr uint32_t kTmemCols = CG == 1 ? 256 : 512;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int rank = CG == 1 ? 0 : (int)cluster_ctarank();
+    const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
+    const int N = p.tile_cols, S = p.stages;
+    // [stages of A][of B][words of the resident tokens' scales][staging buffer]; the MMAs read 128 rows of A, in low tiles past their stage's end.
+    // RESIDENT: of B, all of a tile's stages.
+    const int b_stages = RESIDENT ? p.units : S, groups = (p.units + 3) >> 2;
+    const uint32_t base = smem_u32(smem), a_bytes = (uint32_t)p.a_bytes, b_bytes = (uint32_t)(p.b_rows << p.fold_log) * 128u;
+    const uint32_t b_ring = base + (uint32_t)S * a_bytes, words_at = b_ring + (uint32_t)b_stages * b_bytes, staging = words_at + (RESIDENT ? 256u * (uint32_t)groups : 0u);
+
+    const uint32_t landed = smem_u32(&bars[0]), full = CG == 1 ? landed : landed + 8 * kFp8MaxStages, empty = landed + 16 * kFp8MaxStages;
+    const uint32_t d_full = empty + 8 * kFp8MaxStages, d_empty = d_full + 16, sf_full = d_empty + 16, sf_empty = sf_full + 16;
+    volatile int *abort_flag = &s_abort;
+
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (warp == 1) {
+        auto count = [&](int i) {
+            if (i < kFp8MaxStages) return RESIDENT ? 1 : 2;       // landed: the producers
+            if (i < 2 * kFp8MaxStages) return 2;                  // full: both CTAs of the pair
+            if (i < 3 * kFp8MaxStages + 2) return 1;              // empty, d_full: a commit
+            if (i < 3 * kFp8MaxStages + 6) return 4 * CG;         // d_empty: the epilogue warps of each CTA; sf_full: the scale warps
+            return 1;                                             // sf_empty: a commit
+        };
+        for (int i = lane; i < 3 * kFp8MaxStages + 8; i += 32) mbar_init(landed + 8 * i, count(i));
+        if (lane == 0) s_abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (elect_one_sync()) {
+            prefetch_map(&tmap_a);
+            if (!RESIDENT) prefetch_map(&tmap_b);
+        }
+    }
+    if (warp == 3) {
+        if (CG == 1) {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)), "r"(kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)), "r"(kTmemCols) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        }
+    }
+    auto depend = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
+    tc_fence_before();
+    __syncthreads();
+    if (CG == 2) cluster_sync_all();  // the other CTA's barriers are there
+    tc_fence_after();
+    const uint32_t tmem = s_tmem_base;
+    const int fold = 1 << p.fold_log, part = kBlockRows >> p.fold_log;  // rows of a part
+    Fp8Tiles tile;
+    tile.init(worker, workers);
+    const int tiles = tile.total(p), total = tiles * p.units;
+    auto mma_cols = [&] {  // that the tile's MMAs cover; a half's first column is a multiple of 16 where it is a coordinate of bytes
+        constexpr int kUnit = kAcrossB ? 32 : 8 * CG;
+        return (tile.valid + kUnit - 1) & -kUnit;
+    };
+
+    if (RESIDENT && warp != 1) {  // the weights are on their way meanwhile
+        depend();
+        const int w = warp == 0 ? 0 : warp - 1;
+        if (p.x_bf16) fp8_quantize_resident<__nv_bfloat16>(p, w, kFp8Warps - 1, lane, b_ring, words_at);
+        else fp8_quantize_resident<__half>(p, w, kFp8Warps - 1, lane, b_ring, words_at);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the MMAs read the codes
+        asm volatile("bar.sync 2, %0;" ::"n"(32 * (kFp8Warps - 1)) : "memory");
+    }
+    // Whoever makes a bounded wait that ends only after the kernels before this one waits for those first.
+    if (warp == 0) {
+        if (CG == 1 || rank == 0) {
+            depend();
+            Ring ru, rd, rs;
+            bool ok = true;
+            int second = 0;  // which accumulator
+            // -------------------------------------------------------------- MMA issue
+            // Rows, or along the sum for what is read across, by eights 1024 bytes apart, version 1, 128-byte swizzle.  Read across, an MMA's 32 are 32
+            // staged rows of 128 bytes, otherwise 32 of a row's 128 bytes.
+            constexpr uint64_t sw128 = ((uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29))) << 32;
+            constexpr uint64_t kStepA = (kAcrossA ? 32 * 128 : 32) >> 4, kStepB = (kAcrossB ? 32 * 128 : 32) >> 4;
+            while (ok && tile.next(p)) {
+                const uint32_t idesc = fp8_idesc<CG>(p.fold_log ? p.d_cols : mma_cols(), kAcrossA, kAcrossB);
+                ok = mbar_wait_warp(d_empty + 8 * rd.idx, rd.phase ^ 1, abort_flag, p.status, 303);
+                const uint32_t d = tmem + (uint32_t)(second * p.d_step);
+                second ^= 1;
+                for (int c = 0; ok && c < p.units; ++c) {
+                    if ((c & 3) == 0) ok = mbar_wait_warp(sf_full + 8 * rs.idx, rs.phase, abort_flag, p.status, 304);
+                    ok = ok && mbar_wait_warp(full + 8 * ru.idx, ru.phase, abort_flag, p.status, 305);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const bool last = c + 1 == p.units, group_ends = last || (c & 3) == 3;
+                    if (elect_one_sync()) {
+                        const uint64_t a = sw128 | (uint64_t)(((base + (uint32_t)ru.idx * a_bytes) & 0x3FFFFu) >> 4);
+                        const uint64_t b = sw128 | (uint64_t)(((b_ring + (uint32_t)(RESIDENT ? c : ru.idx) * b_bytes) & 0x3FFFFu) >> 4);
+                        const uint32_t sfa = tmem + (uint32_t)(p.sf_col + rs.idx * kFp8SfCols), sfb = sfa + 8;
+                        const int steps = last && !p.fold_log ? p.last_steps : 4;
+                        const uint32_t id = idesc | ((uint32_t)(c & 3) << 29) | ((uint32_t)(c & 3) << 4);
+#pragma unroll
+                        for (int kk = 0; kk < 4; ++kk)
+                            if (kk < steps) tc_mma_fp8<CG>(d, a + kStepA * kk, b + kStepB * kk, id, sfa, sfb, c == 0 && kk == 0 ? 0u : 1u);
+                        if (CG == 1) {
+                            tc_commit(empty + 8 * ru.idx);
+                            if (group_ends) tc_commit(sf_empty + 8 * rs.idx);
+                            if (last) tc_commit(d_full + 8 * rd.idx);
+                        } else {
+                            tc_commit_pair(empty + 8 * ru.idx);
+                            if (group_ends) tc_commit_pair(sf_empty + 8 * rs.idx);
+                            if (last) tc_commit_pair(d_full + 8 * rd.idx);
+                        }
+                    }
+                    __syncwarp();
+                    ru.advance(S);
+                    if (group_ends) rs.advance(2);
+                }
+                rd.advance(p.nd);
+            }
+        }
+    } else if (warp == 1) {
+        // ------------------------------------------------------------------ A
+        Ring ru;
+        bool ok = true;
+        int issued = 0;
+        if (!p.ahead) depend();
+        while (ok && tile.next(p)) {
+            const int block = CG * tile.rt + rank, row = fp8_row(p, block), rows = p.flex ? fp8_row(p, block + 1) - row : kBlockRows;
+            const CUtensorMap *map = !p.flex || rows == p.group_rows * div_up(p.groups, p.row_tiles) ? &tmap_a : &tmap_a2;  // boxes of the taller and of the lower tiles
+            for (int c = 0; c < p.units; ++c, ru.advance(S)) {
+                if (issued++ == S) depend();
+                ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 300);
+                if (!ok) break;
+                if (elect_one_sync()) {
+                    const uint32_t bar = landed + 8 * ru.idx;
+                    mbar_expect_tx(bar, (uint32_t)(rows << p.fold_log) * 128u);
+                    for (int f = 0; f < fold; ++f) {  // what lies behind the last block reads as zeros
+                        const int at = ((c << p.fold_log) + f) * kFp8Block;
+                        const uint32_t to = base + (uint32_t)ru.idx * a_bytes + (uint32_t)(f * part) * 128u;
+                        if constexpr (kGated) tma_load_4d(to, map, at, 0, 0, row >> 4, bar);
+                        else if constexpr (kAcrossA) tma_load_2d(to, map, row, at, bar);
+                        else tma_load_2d(to, map, at, row, bar);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+        // The MMAs' commits have arrived at every stage in use before the CTA leaves.
+        depend();
+        if (total < S) ru = Ring();
+        for (int i = min(S, total); ok && i > 0; --i, ru.advance(S)) ok = mbar_wait_warp(empty + 8 * ru.idx, total < S ? 0u : ru.phase ^ 1, abort_flag, p.status, 310);
+    } else if (warp == 2 && !RESIDENT) {
+        // ------------------------------------------------------------------ B
+        Ring ru;
+        bool ok = true;
+        depend();
+        while (ok && tile.next(p)) {
+            const int col = tile.col0 + rank * (mma_cols() / CG);
+            for (int c = 0; c < p.units; ++c, ru.advance(S)) {
+                ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 301);
+                if (!ok) break;
+                if (elect_one_sync()) {
+                    const uint32_t bar = landed + 8 * ru.idx;
+                    mbar_expect_tx(bar, b_bytes);
+                    for (int f = 0; f < fold; ++f) {
+                        const int at = ((c << p.fold_log) + f) * kFp8Block;
+                        const uint32_t to = b_ring + (uint32_t)ru.idx * b_bytes + (uint32_t)(f * p.b_rows) * 128u;
+                        if constexpr (kAcrossB) tma_load_2d(to, &tmap_b, col, at, bar);
+                        else tma_load_2d(to, &tmap_b, at, col, bar);
+                    }
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == 3 && CG == 2) {
+        // ------------------------------------------------------------------ a stage has landed
+        const uint32_t leader_full = map_to_rank(full, 0);
+        Ring ru;
+        depend();
+        for (int i = 0; i < total; ++i, ru.advance(S)) {
+            if (!mbar_wait_warp(landed + 8 * ru.idx, ru.phase, abort_flag, p.status, 302)) break;
+            if (lane == 0) mbar_arrive_cluster(leader_full + 8 * ru.idx);
+        }
+    } else if (warp >= kFp8ScaleWarp0) {
+        // ------------------------------------------------------------------ scales to tensor memory
+        const int quarter = warp - kFp8ScaleWarp0;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)p.sf_col;
+        const uint32_t leader_full = CG == 1 ? sf_full : map_to_rank(sf_full, 0);
+        const int a_blocks = div_up(p.rows, kFp8Block);
+        uint32_t next[kFp8SfCols];
+#pragma unroll
+        for (int i = 0; i < kFp8SfCols; ++i) next[i] = 0;
+        // The words of group g of the tile: bytes are those of stages 4g .. 4g + 3.
+        auto fetch = [&](int g) {
+            const int row0 = fp8_row(p, CG * tile.rt + rank);
+            int had = -1;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {  // A: MMA row 32 i + lane is row `of` of part f
+                const int r = 32 * i + lane, f = r >> (7 - p.fold_log), of = r & (part - 1);
+                if constexpr (FORM == kFp8Dw) {
+                    next[i] = __ldcg(reinterpret_cast<const uint32_t *>(p.as) + (size_t)g * p.rows + min(row0 + r, p.rows - 1));
+                } else {
+                    int row = row0 + of;
+                    if constexpr (kGated) {
+                        const int feature = min((row0 >> 1) + ((of >> 4) << 3) + (of & 7), p.rows / 2 - 1);
+                        row = (of & 8) ? p.rows / 2 + feature : feature;
+                    }
+                    const int block = min(row, p.rows - 1) / kFp8Block, key = (block << 2) + f;
+                    if (key == had) {
+                        next[i] = next[i > 0 ? i - 1 : 0];
+                        continue;
+                    }
+                    had = key;
+                    uint32_t w = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int kb = ((4 * g + j) << p.fold_log) + f;
+                        if (kb < p.blocks) w |= (uint32_t)__ldcg(p.as + (FORM == kFp8Dx ? (size_t)kb * a_blocks + block : (size_t)block * p.blocks + kb)) << (8 * j);
+                    }
+                    next[i] = w;
+                }
+            }
+            if constexpr (RESIDENT) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(next[8 + j]) : "r"(words_at + 256u * (uint32_t)g + 128u * j + 4u * lane));
+            } else if (CG == 1 && p.fold_log) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {  // column t of block f of a stage
+                    const int at = 32 * j + lane, f = at / p.b_rows, t = at - f * p.b_rows;
+                    uint32_t w = 0;
+                    if (f < fold && t < tile.valid)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int kb = ((4 * g + i) << p.fold_log) + f;
+                            if (kb < p.blocks) w |= (uint32_t)__ldcg(p.bs + ((size_t)(kb >> 2) * p.cols + tile.col0 + t) * 4 + (kb & 3)) << (8 * i);
+                        }
+                    next[8 + j] = w;
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < (CG == 1 ? 1 : 8); ++j) {
+                    const int t = 32 * j + lane;
+                    if (32 * j < tile.valid) next[8 + j] = __ldcg(reinterpret_cast<const uint32_t *>(p.bs) + (size_t)g * p.cols + tile.col0 + min(t, tile.valid - 1));
+                }
+            }
+        };
+        Ring rs;
+        bool ok = true;
+        depend();
+        bool more = tile.next(p);
+        int g = 0;
+        if (more) fetch(0);
+        const int total_groups = tiles * groups;
+        while (more) {
+            uint32_t v[kFp8SfCols];
+#pragma unroll
+            for (int i = 0; i < kFp8SfCols; ++i) v[i] = next[i];
+            if (++g == groups) {
+                g = 0;
+                more = tile.next(p);
+            }
+            if (more) fetch(g);  // on its way while the group before is waited for
+            ok = mbar_wait_warp(sf_empty + 8 * rs.idx, rs.phase ^ 1, abort_flag, p.status, 306);
+            if (!ok) break;
+            tc_fence_after();
+            tc_st_x16(lanes + (uint32_t)(rs.idx * kFp8SfCols), v);
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (CG == 1) mbar_arrive(sf_full + 8 * rs.idx);
+                else mbar_arrive_cluster(leader_full + 8 * rs.idx);
+            }
+            rs.advance(2);
+        }
+        // the commits for the last two groups have arrived before the CTA leaves
+        if (total_groups == 1) rs = Ring();
+        for (int i = min(2, total_groups); ok && i > 0; --i, rs.advance(2)) ok = mbar_wait_warp(sf_empty + 8 * rs.idx, total_groups == 1 ? 0u : rs.phase ^ 1, abort_flag, p.status, 311);
+    } else if (warp >= kFp8EpilogueWarp0) {
+        // ------------------------------------------------------------------ epilogue
+        const int quarter = warp & 3, thread = threadIdx.x - 32 * kFp8EpilogueWarp0;
+        const uint32_t tmem_q = tmem + ((uint32_t)(32 * quarter) << 16);
+        OT *o = static_cast<OT *>(p.o), *z = static_cast<OT *>(p.z);
+        const int out = kGated ? p.rows / 2 : p.rows;  // numbers of a row of the output
+        constexpr int kTileOut = kGated ? kBlockRows / 2 : kBlockRows;
+        constexpr uint32_t kPitch = kTileOut * (uint32_t)sizeof(OT) + (sizeof(OT) == 2 || kGated ? 16 : 0);  // 16 bytes more, so that a column of 8 rows meets all banks
+        constexpr uint32_t kPitchZ = kBlockRows * 2 + 16;
+        const uint32_t z_staging = staging + (uint32_t)p.z_offset;
+        Ring rd;
+        depend();
+        int row0 = 0, rows = 0;
+        const uint32_t leader_d_empty = CG == 1 ? d_empty : map_to_rank(d_empty, 0);
+        auto drained = [&] {  // the accumulator may be overwritten
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (CG == 1) mbar_arrive(d_empty + 8 * rd.idx);
+                else mbar_arrive_cluster(leader_d_empty + 8 * rd.idx);
+            }
+        };
+        // The staging buffer, which has `have` of the tile's columns from t0 on (behind its last the first), to memory: 16 bytes a thread and step.
+        auto copy_out = [&](int t0, int have) {
+            constexpr int kPieces = kTileOut * (int)sizeof(OT) / 16, kStep = 128 / kPieces;
+            const int piece = thread % kPieces;
+            if (piece * (16 / (int)sizeof(OT)) < (kGated ? rows / 2 : rows)) {
+#pragma unroll 4
+                for (int t = thread / kPieces; t < have; t += kStep) {
+                    const int col = t0 + t < N ? t0 + t : t0 + t - N;
+                    uint4 v;
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(staging + (uint32_t)t * kPitch + 16u * piece));
+                    if (col < tile.valid) *reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(o + (size_t)(tile.col0 + col) * out + (kGated ? row0 / 2 : row0)) + 16 * piece) = v;
+                }
+            }
+            if constexpr (kGated && sizeof(OT) == 2) {
+                if (z) {
+                    const int which = (thread >> 3) & 1, group = thread & 7;  // of the projections, and eight features of it
+                    if (group < rows / 16) {
+                        OT *to = z + (size_t)tile.col0 * p.rows + (size_t)which * out + row0 / 2 + 8 * group;
+#pragma unroll 4
+                        for (int t = thread >> 4; t < have; t += 8) {
+                            const int col = t0 + t < N ? t0 + t : t0 + t - N;
+                            uint4 v;
+                            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                         : "r"(z_staging + (uint32_t)t * kPitchZ + 16u * (2 * group + which)));
+                            if (col < tile.valid) *reinterpret_cast<uint4 *>(to + (size_t)col * p.rows) = v;
+                        }
+                    }
+                }
+            }
+        };
+        // 32 columns of the accumulator at `d`, from t on, to column `at` of the staging buffer.
+        auto fill_from = [&](uint32_t d, int t, int at) {
+            const uint32_t to = staging + (uint32_t)at * kPitch;
+            auto f32 = [](uint32_t v) { return __uint_as_float(v); };
+            if constexpr (kGated || sizeof(OT) == 2) {
+                uint32_t lo[16], hi[16];
+                tc_ld_16x256b_x4(d + t, lo);
+                tc_ld_16x256b_x4(d + (16u << 16) + t, hi);
+                asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                // Fragments of 8 rows x 8 columns, packed, are written transposed (stmatrix): 16 bytes = 8 rows of one column.
+                auto rows_of_8 = [&](uint32_t at_, uint32_t pitch) {
+                    if constexpr (sizeof(OT) == 2) {
+                        const uint32_t dst = at_ + (uint32_t)(lane & 7) * pitch + (uint32_t)(4 * quarter + (lane >> 3)) * 16u;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            stmatrix_x4_trans(dst + 8u * i * pitch, mx_pack2<OT>(f32(lo[4 * i]), f32(lo[4 * i + 1])), mx_pack2<OT>(f32(lo[4 * i + 2]), f32(lo[4 * i + 3])),
+                                              mx_pack2<OT>(f32(hi[4 * i]), f32(hi[4 * i + 1])), mx_pack2<OT>(f32(hi[4 * i + 2]), f32(hi[4 * i + 3])));
+                    }
+                };
+                if constexpr (!kGated) {
+                    rows_of_8(to, kPitch);
+                } else {
+                    if (z) rows_of_8(z_staging + (uint32_t)at * kPitchZ, kPitchZ);
+                    auto act = [&](uint32_t g, uint32_t u) { return fp8_activation(f32(g), f32(u), p.gelu); };
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {  // lanes i and i + 8 of a half: gate and other projection of one feature, two columns
+                        const float l0 = act(lo[4 * i], lo[4 * i + 2]), l1 = act(lo[4 * i + 1], lo[4 * i + 3]);
+                        const float h0 = act(hi[4 * i], hi[4 * i + 2]), h1 = act(hi[4 * i + 1], hi[4 * i + 3]);
+                        if constexpr (sizeof(OT) == 2) {
+                            stmatrix_x2_trans(to + (uint32_t)(8 * i + (lane & 7)) * kPitch + (uint32_t)(2 * quarter + ((lane >> 3) & 1)) * 16u, mx_pack2<OT>(l0, l1), mx_pack2<OT>(h0, h1));
+                        } else {
+                            const uint32_t dst = to + (uint32_t)(8 * i + 2 * (lane & 3)) * kPitch + (uint32_t)(16 * quarter + (lane >> 2)) * 4u;
+                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst), "f"(l0) : "memory");
+                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + kPitch), "f"(l1) : "memory");
+                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + 32u), "f"(h0) : "memory");
+                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + kPitch + 32u), "f"(h1) : "memory");
+                        }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int h = 0; h < 32; h += 16) {
+                    float v[16];
+                    tc_ld_x16(d + t + h, v);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + (uint32_t)(h + i) * kPitch + (uint32_t)thread * 4u), "f"(v[i]) : "memory");
+                }
+            }
+        };
+        int second = 0;
+        for (; tile.next(p); second ^= 1) {
+            const bool ok = mbar_wait_warp(d_full + 8 * rd.idx, rd.phase, abort_flag, p.status, 307);
+            if (bar_any(1, 128, !ok)) break;  // the four warps go on together or not at all
+            tc_fence_after();
+            const uint32_t d = tmem_q + (uint32_t)(second * p.d_step);
+            row0 = fp8_row(p, CG * tile.rt + rank);
+            rows = max(0, min(p.flex ? fp8_row(p, CG * tile.rt + rank + 1) : row0 + kBlockRows, p.rows) - row0);
+            if constexpr (CG == 1) {
+                float v[16];
+                const int f = thread >> (7 - p.fold_log);
+                tc_ld_x16(d + f * p.b_rows, v);
+                drained();
+                if (!kGated && p.fold_log == 0) {
+                    OT *to = o + (size_t)tile.col0 * out + row0 + thread;
+                    if (thread < rows) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i)
+                            if (i < tile.valid) to[(size_t)i * out] = mx_convert<OT>(v[i]);
+                    }
+                } else {
+                    // Part f's sums of row i are lane part * f + i, columns b_rows * f ..: added up in the order of the parts.
+                    float *sums = reinterpret_cast<float *>(smem + (staging - base));
+#pragma unroll
+                    for (int t = 0; t < 16; ++t)
+                        if (t < tile.valid) sums[t * kBlockRows + thread] = v[t];
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    auto sum = [&](int t, int i) {
+                        float s = sums[t * kBlockRows + i];
+                        for (int g = 1; g < fold; ++g) s += sums[t * kBlockRows + g * part + i];
+                        return s;
+                    };
+                    if constexpr (kGated) {
+                        const int i = thread & 63, at = 2 * (i & ~7) + (i & 7);
+                        for (int t = thread >> 6; t < tile.valid && i < rows / 2; t += 2) {
+                            const float g = sum(t, at), u = sum(t, at + 8);
+                            o[(size_t)(tile.col0 + t) * out + row0 / 2 + i] = mx_convert<OT>(fp8_activation(g, u, p.gelu));
+                            if (z) {
+                                OT *to = z + (size_t)(tile.col0 + t) * p.rows + row0 / 2 + i;
+                                to[0] = mx_convert<OT>(g);
+                                to[out] = mx_convert<OT>(u);
+                            }
+                        }
+                    } else {
+                        const int i = thread & (part - 1);
+                        for (int t = f; t < tile.valid && i < rows; t += fold) o[(size_t)(tile.col0 + t) * out + row0 + i] = mx_convert<OT>(sum(t, i));
+                    }
+                    asm volatile("bar.sync 1, 128;" ::: "memory");  // they have been read
+                }
+            } else {
+                // Of two accumulators that overlap, the columns they share first: then the other one may be written.
+                const bool shared = p.nd == 1;
+                const int turn = shared && second == 0 ? p.d_step : 0;
+                for (int b = 0; b < N; b += kFp8StageCols) {
+                    const int t0 = b + turn < N ? b + turn : b + turn - N;
+                    asm volatile("bar.sync 1, 128;" ::: "memory");  // what was staged before has been copied
+#pragma unroll
+                    for (int h = 0; h < kFp8StageCols; h += 32) {
+                        const int t = t0 + h < N ? t0 + h : t0 + h - N;
+                        if (b + h < N && t < tile.valid) fill_from(d, t, h);
+                        if (shared && b == 0 && h == 0) drained();
+                    }
+                    if (!shared && b + kFp8StageCols >= N) drained();
+                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    copy_out(t0, min(kFp8StageCols, N - b));
+                }
+            }
+            rd.advance(p.nd);
+        }
+    }
+
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (CG == 2) cluster_sync_all();
+    if (warp == 3) {
+        tc_fence_after();
+        if (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+    }
+}
+
+// ------------------------------------------------------------------ host side
+
+struct Fp8Plan {
+    int cg, tile_cols, width, col_tiles, stages, nd, d_cols, d_step, sf_col;
+    bool resident;
+    int flex, fold_log, group_rows, row_tiles, a_bytes, b_rows, z_offset;
+    int workers;
+    size_t smem;
+};
+
+// Microseconds that tiles of 256 rows and `cols` columns take on `pairs` pairs, beside what a launch costs: rounds of tiles, each with its steps of 128 (the
+// tensor pipe's four MMAs, which take hardly less for few columns) and what of a wide tile's epilogue nothing hides; what all tiles copy, from L2; A, from HBM.
+static double fp8_pair_us(int rows, int n, int red, int cols, int pairs)
+{
+    const int row_tiles = div_up(rows, 2 * kBlockRows), blocks = div_up(red, kFp8Block);
+    const double tiles = (double)row_tiles * div_up(n, cols);
+    const double rounds = std::ceil(tiles / pairs);
+    const int width = div_up(div_up(n, div_up(n, cols)), 16) * 16;  // tiles are of equal width
+    const double step = cols <= 128 ? 0.183 + 0.00013 * width : 0.036 + 0.00118 * width;
+    const double work = rounds * (std::max(0.0, 0.0086 * width - 0.5) + blocks * step);
+    const double copies = tiles * (2 * kBlockRows + cols) * blocks * 128.0 / 21.7e6, weights = (double)rows * red / 6.5e6;
+    return std::sqrt(work * work + copies * copies + weights * weights);
+}
+
+static int fp8_pair_cols(int rows, int n, int red, int form, int pairs)
+{
+    static const int widths[] = {256, 224, 192, 160, 128, 96, 64, 32, 16, 0};  // of dw all but the last: what a CTA stages starts at a multiple of 16 columns
+    int best = 0;
+    double best_us = 0;
+    for (int i = 0; widths[i]; ++i) {
+        const int cols = widths[i];
+        if (form == kFp8Dw && cols < 32) break;
+        if (best && div_up(n, div_up(n, cols)) <= widths[i + 1]) continue;  // the next narrower one holds the same tiles
+        const double us = fp8_pair_us(rows, n, red, cols, pairs);
+        if (!best || us < best_us) best = cols, best_us = us;
+    }
+    return best;
+}
+
+// rows x red of A, n columns.  x_type: TUNA_FP8, or what B is before it is quantized.
+static Fp8Plan fp8_plan(int form, int rows, int n, int red, int x_type, int o_type, bool with_z, int sm_count)
+{
+    Fp8Plan l = {};
+    const bool gated = form == kFp8GatedProduct;
+    const int blocks = div_up(red, kFp8Block), o_bytes = o_type == TUNA_FP32 ? 4 : 2;
+    l.cg = form <= kFp8GatedProduct && n <= kFp8DirectCols ? 1 : 2;
+    l.workers = sm_count / l.cg;
+    l.group_rows = gated ? 16 : 8;
+    const int groups = rows / l.group_rows;
+    size_t fixed;
+    if (l.cg == 1) {
+        l.flex = 1;
+        l.tile_cols = l.width = kFp8DirectCols;
+        l.row_tiles = (int)std::min<long long>(groups, div_up_ll(rows, (long long)kBlockRows * sm_count) * sm_count);
+        const int height = l.group_rows * div_up(groups, l.row_tiles);
+        l.fold_log = height <= 32 ? 2 : height <= 64 ? 1 : 0;
+        l.a_bytes = (l.fold_log ? kBlockRows : height) * 128;
+        l.b_rows = l.fold_log ? div_up(n, 8) * 8 : kFp8DirectCols;
+        fixed = l.fold_log || gated ? kFp8FoldBytes : 0;
+    } else {
+        l.tile_cols = fp8_pair_cols(rows, n, red, form, l.workers);
+        const int unit = form == kFp8Dw ? 32 : 16;
+        l.width = div_up(div_up(n, div_up(n, l.tile_cols)), unit) * unit;
+        l.row_tiles = div_up(rows, 2 * kBlockRows);
+        l.a_bytes = kBlockRows * 128;
+        l.b_rows = form == kFp8Dw ? kBlockRows : l.tile_cols / 2;
+        const size_t pitch = gated ? 64 * o_bytes + 16 : kBlockRows * o_bytes + (o_bytes == 2 ? 16 : 0);
+        fixed = kFp8StageCols * pitch;
+        l.z_offset = (int)fixed;
+        if (with_z) fixed += kFp8StageCols * (kBlockRows * 2 + 16);
+    }
+    l.col_tiles = div_up(n, l.width);
+    const int fold = 1 << l.fold_log, units = div_up(blocks, fold);
+    l.d_cols = l.fold_log ? l.b_rows * fold : l.tile_cols;
+    const size_t room = l.cg == 1 ? kFp8SmemHalf : kFp8SmemMax;
+    size_t b_stage = (size_t)l.b_rows * fold * 128;
+    // Tokens that the CTAs quantize themselves: one round of the quantizing warps, and shared memory left for stages enough.
+    const int rows8 = div_up(n, 8) * 8;
+    const size_t resident = (size_t)units * rows8 * fold * 128 + 256 * (size_t)div_up(units, 4);
+    l.resident = l.cg == 1 && x_type != TUNA_FP8 && (long long)div_up(units * fold, 2) * n <= kFp8ResidentLoads * (kFp8Warps - 1) && resident + 4 * (size_t)l.a_bytes + fixed <= room;
+    if (l.resident) {
+        l.b_rows = rows8;
+        if (l.fold_log) l.d_cols = rows8 * fold;
+        fixed += resident;
+        b_stage = 0;
+    }
+    l.stages = (int)std::min<size_t>(kFp8MaxStages, (room - fixed) / (l.a_bytes + b_stage));
+    const int tmem_cols = (l.cg == 1 ? 256 : 512) - 2 * kFp8SfCols;
+    // Two accumulators, which share the columns in the middle where two whole ones do not fit
+    l.nd = 2 * l.d_cols <= tmem_cols ? 2 : 1;
+    l.d_step = l.nd == 2 ? l.d_cols : tmem_cols - l.d_cols;
+    l.sf_col = tmem_cols;
+    // the last stage's MMAs read 128 rows
+    l.smem = std::max((size_t)l.stages * (l.a_bytes + b_stage) + fixed, (size_t)(l.stages - 1) * l.a_bytes + kBlockRows * 128);
+    return l;
+}
+
+bool fp8_gemm_takes(bool gated, int rows, int n, int red, int x_type, int sm_count)
+{
+    if (x_type == TUNA_FP8) return true;
+    return n <= kFp8DirectCols && fp8_plan(gated ? kFp8GatedProduct : kFp8Product, rows, n, red, x_type, TUNA_FP16, false, sm_count).resident;
+}
+
+struct Fp8Maps {
+    CUtensorMap a, a2, b;
+};
+
+template <int CG, int FORM, bool RESIDENT, typename OT>
+static int launch_fp8(const Fp8Params &p, const Fp8Maps &maps, int ctas, size_t smem, cudaStream_t stream)
+{
+    static bool attr_set[64] = {false};
+    static std::mutex mu;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TUNA_ERR_NO_DEVICE;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        if (!attr_set[dev]) {
+            if (cudaFuncSetAttribute(fp8_gemm_kernel<CG, FORM, RESIDENT, OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp8SmemMax) != cudaSuccess) return TUNA_ERR_NO_DEVICE;
+            attr_set[dev] = true;
+        }
+    }
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)ctas);
+    lc.blockDim = dim3(32 * kFp8Warps);
+    lc.dynamicSmemBytes = smem;
+    lc.stream = stream;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = CG;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    lc.attrs = attr;
+    lc.numAttrs = CG == 1 ? 1 : 2;
+    return cudaLaunchKernelEx(&lc, fp8_gemm_kernel<CG, FORM, RESIDENT, OT>, p, maps.a, maps.a2, maps.b) == cudaSuccess ? TUNA_OK : TUNA_ERR_LAUNCH;
+}
+
+template <typename OT>
+static int launch_fp8_as(int form, const Fp8Plan &l, const Fp8Params &p, const Fp8Maps &maps, cudaStream_t stream)
+{
+    const int ctas = l.workers * l.cg;
+    if (l.cg == 1) {
+        if (form == kFp8Product) return l.resident ? launch_fp8<1, kFp8Product, true, OT>(p, maps, ctas, l.smem, stream) : launch_fp8<1, kFp8Product, false, OT>(p, maps, ctas, l.smem, stream);
+        return l.resident ? launch_fp8<1, kFp8GatedProduct, true, OT>(p, maps, ctas, l.smem, stream) : launch_fp8<1, kFp8GatedProduct, false, OT>(p, maps, ctas, l.smem, stream);
+    }
+    switch (form) {
+        case kFp8Product: return launch_fp8<2, kFp8Product, false, OT>(p, maps, ctas, l.smem, stream);
+        case kFp8GatedProduct: return launch_fp8<2, kFp8GatedProduct, false, OT>(p, maps, ctas, l.smem, stream);
+        case kFp8Dx: return launch_fp8<2, kFp8Dx, false, OT>(p, maps, ctas, l.smem, stream);
+        default: return launch_fp8<2, kFp8Dw, false, OT>(p, maps, ctas, l.smem, stream);
+    }
+}
+
+static int launch_fp8_form(int form, const Fp8Codes &a, int rows, const Fp8Codes &b, int cols, int red, const void *numbers, int x_type, void *o, int o_type, void *z, int gelu,
+                           int sm_count, cudaStream_t stream)
+{
+    const Fp8Plan l = fp8_plan(form, rows, cols, red, numbers && !b.q ? x_type : TUNA_FP8, o_type, z != nullptr, sm_count);
+    Fp8Params p;
+    std::memset(&p, 0, sizeof(p));
+    p.as = (const uint8_t *)a.s; p.bs = (const uint8_t *)b.s; p.o = o; p.z = z; p.x = numbers;
+    p.rows = rows; p.cols = cols; p.red = red;
+    p.blocks = div_up(red, kFp8Block);
+    p.fold_log = l.fold_log; p.units = div_up(p.blocks, 1 << l.fold_log);
+    p.last_steps = div_up(red - (p.blocks - 1) * kFp8Block, 32);
+    p.tile_cols = l.tile_cols; p.width = l.width; p.row_tiles = l.row_tiles; p.col_tiles = l.col_tiles;
+    p.rows_inner = l.row_tiles < l.col_tiles;
+    p.group_rows = l.group_rows; p.groups = rows / l.group_rows; p.flex = l.flex;
+    p.a_bytes = l.a_bytes; p.b_rows = l.b_rows; p.stages = l.stages; p.nd = l.nd; p.d_cols = l.d_cols; p.d_step = l.d_step; p.sf_col = l.sf_col;
+    p.ahead = form <= kFp8GatedProduct && cols <= kFp8AheadTokens;
+    p.x_bf16 = x_type == TUNA_BF16; p.gelu = gelu; p.z_offset = l.z_offset;
+    p.status = device_status_word();
+    if (!p.status) return TUNA_ERR_NO_DEVICE;
+    // the kernel numbers tiles and a worker's stages in 32 bits
+    const long long tiles = (long long)p.row_tiles * p.col_tiles;
+    if (tiles >= 1ll << 30 || (tiles / l.workers + 2) * p.units >= 1ll << 30) return TUNA_ERR_TOO_LARGE;
+
+    Fp8Maps maps;
+    auto matrix = [](CUtensorMap *map, const void *at, int inner, int outer, int box_outer) {  // row by row; boxes of 128 columns
+        return make_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, at, (uint64_t)inner, (uint64_t)outer, (uint64_t)inner, kFp8Block, (uint32_t)box_outer, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    auto weights = [&](CUtensorMap *map, int height) {
+        if (form == kFp8Product) return matrix(map, a.q, red, rows, height);
+        if (form != kFp8GatedProduct) return matrix(map, a.q, rows, red, kFp8Block);
+        const uint64_t k = (uint64_t)red, f = (uint64_t)rows / 2;  // [features by eight][gate or other][eight][k]
+        const uint64_t dims[4] = {k, 8, 2, f / 8}, strides[3] = {k, f * k, 8 * k};
+        const uint32_t box[4] = {kFp8Block, 8, 2, (uint32_t)height / 16};
+        return make_tensor_map_nd(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.q, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    if (!weights(&maps.a, l.flex ? l.group_rows * div_up(p.groups, p.row_tiles) : kBlockRows)) return TUNA_ERR_NO_DEVICE;
+    maps.a2 = maps.b = maps.a;
+    if (l.flex && p.groups % p.row_tiles && !weights(&maps.a2, l.group_rows * (p.groups / p.row_tiles))) return TUNA_ERR_NO_DEVICE;
+    if (!l.resident && !(form == kFp8Dw ? matrix(&maps.b, b.q, cols, red, kFp8Block) : matrix(&maps.b, b.q, red, cols, l.b_rows))) return TUNA_ERR_NO_DEVICE;
+    if (numbers && b.q && launch_fp8_quantize_rows(numbers, x_type, red, b.q, b.s, cols, red, true, stream) != cudaSuccess) return TUNA_ERR_LAUNCH;
+    switch (o_type) {
+        case TUNA_FP16: return launch_fp8_as<__half>(form, l, p, maps, stream);
+        case TUNA_BF16: return launch_fp8_as<__nv_bfloat16>(form, l, p, maps, stream);
+        default: return launch_fp8_as<float>(form, l, p, maps, stream);
+    }
+}
+
+int launch_fp8_product(const Fp8ProductArgs &a)
+{
+    return launch_fp8_form(a.gated ? kFp8GatedProduct : kFp8Product, a.w, a.m, a.x, a.n, a.k, a.numbers, a.x_type, a.o, a.o_type, a.z, a.gelu, a.sm_count, a.stream);
+}
+
+int launch_fp8_dx(const Fp8Codes &w, const Fp8Codes &dy, void *dx, int type, int m, int n, int k, int sm_count, cudaStream_t stream)
+{
+    return launch_fp8_form(kFp8Dx, w, k, dy, n, m, nullptr, TUNA_FP8, dx, type, nullptr, 0, sm_count, stream);
+}
+
+int launch_fp8_dw(const Fp8Codes &x, const Fp8Codes &dy, void *dw, int type, int m, int n, int k, int sm_count, cudaStream_t stream)
+{
+    return launch_fp8_form(kFp8Dw, x, k, dy, m, n, nullptr, TUNA_FP8, dw, type, nullptr, 0, sm_count, stream);
+}
+
+}  // namespace tuna

@@ -1,0 +1,379 @@
+// Quantizers of the 8-bit block-scaled format (fp8_format.cuh), their inverse, and the quantizer of a gated block's gradients.
+#include <algorithm>
+#include "launchers.h"
+#include "fp8_format.cuh"
+
+namespace tuna {
+
+// ---- blocks of a row
+
+constexpr int kFp8qWarps = 4;
+constexpr int kFp8Chunk = 256;  // columns of a warp: eight of a lane, sixteen lanes a block
+
+// A warp takes ROWS rows of 256 columns; grid (row groups, chunks by fours).
+template <typename T, int ROWS>
+__global__ void __launch_bounds__(kFp8qWarps * 32)
+fp8_quantize_rows_kernel(const T *x, long long row_stride, uint8_t *q, uint8_t *s, int rows, int k, int log_c, bool chained)
+{
+    // Part of a product, which may start (and read its weights, not this kernel's) while this one runs.
+    if (chained) {
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, blocks = div_up(k, kFp8Block);
+    const int c = (int)(blockIdx.y << log_c) + (warp & ((1 << log_c) - 1));
+    const long long row0 = (((long long)blockIdx.x << (2 - log_c)) + (warp >> log_c)) * ROWS;
+    if (c * kFp8Chunk >= k || row0 >= rows) return;
+    const int col = c * kFp8Chunk + lane * 8;
+    Mx8<T> v[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        if (col < k && row0 + r < rows) v[r].load(x + (row0 + r) * row_stride + col);
+        else v[r].zero();
+    }
+    uint32_t mine = 0;  // the scale of row lane % 16
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+        uint32_t m = v[r].largest();  // of four lanes
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 4));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        const uint32_t e = fp8_scale(m);
+        const float inverse = fp8_inverse(e);
+        float f[8];
+        v[r].values(f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] *= inverse;
+        uint2 codes = make_uint2(fp8_encode4(f[0], f[1], f[2], f[3]), fp8_encode4(f[4], f[5], f[6], f[7]));
+        if (e == 255u) codes = make_uint2(0, 0);
+        if (col < k && row0 + r < rows) *reinterpret_cast<uint2 *>(q + (row0 + r) * k + col) = codes;
+        if ((lane & 15) == r) mine = e;
+    }
+    const long long row = row0 + (lane & 15);
+    const int b = 2 * c + (lane >> 4);
+    if ((lane & 15) >= ROWS || row >= rows || b >= blocks) return;
+    uint8_t *at = s + ((long long)(b >> 2) * rows + row) * 4 + (b & 3);
+    *at = (uint8_t)mine;
+    if (b + 1 == blocks)
+        for (int i = 1; i < 4 - (b & 3); ++i) at[i] = 0;  // blocks that the last word does not have
+}
+
+template <typename T, int ROWS>
+static cudaError_t quantize_rows_as(const void *x, long long row_stride, void *q, void *s, int rows, int k, bool chained, cudaStream_t stream)
+{
+    const int chunks = div_up(k, kFp8Chunk), log_c = chunks >= 4 ? 2 : chunks >= 2 ? 1 : 0;
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)div_up(div_up(rows, ROWS), 4 >> log_c), (unsigned)div_up(chunks, 1 << log_c));
+    lc.blockDim = dim3(kFp8qWarps * 32);
+    lc.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = attr;
+    lc.numAttrs = chained ? 1 : 0;
+    return cudaLaunchKernelEx(&lc, fp8_quantize_rows_kernel<T, ROWS>, (const T *)x, row_stride, (uint8_t *)q, (uint8_t *)s, rows, k, log_c, chained);
+}
+
+template <typename T>
+static cudaError_t quantize_rows(const void *x, long long row_stride, void *q, void *s, int rows, int k, bool chained, cudaStream_t stream)
+{
+    return (long long)rows * div_up(k, kFp8Chunk) <= 8192 ? quantize_rows_as<T, 2>(x, row_stride, q, s, rows, k, chained, stream)
+                                                          : quantize_rows_as<T, 4>(x, row_stride, q, s, rows, k, chained, stream);
+}
+
+cudaError_t launch_fp8_quantize_rows(const void *x, int type, long long row_stride, void *q, void *s, int rows, int k, bool chained, cudaStream_t stream)
+{
+    switch (type) {
+        case TUNA_FP16: return quantize_rows<__half>(x, row_stride, q, s, rows, k, chained, stream);
+        case TUNA_BF16: return quantize_rows<__nv_bfloat16>(x, row_stride, q, s, rows, k, chained, stream);
+        default: return quantize_rows<float>(x, row_stride, q, s, rows, k, chained, stream);
+    }
+}
+
+// ---- tiles of 128 x 128: blocks of a column, of a row and a column, square ones
+
+constexpr int kFp8TileWarps = 8;
+constexpr int kFp8TileRows = kFp8Block / kFp8TileWarps;  // rows of a warp, four columns of a lane
+
+// Four numbers side by side, as fp32; coherent loads that keep out of L1 (a gated block's gradients are read twice, by tiles far apart).
+__device__ __forceinline__ float4 fp8_load4(const __half *p)
+{
+    uint2 v;
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&v.y));
+    return make_float4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ float4 fp8_load4(const __nv_bfloat16 *p)
+{
+    uint2 v;
+    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
+    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
+}
+__device__ __forceinline__ float4 fp8_load4(const float *p)
+{
+    float4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
+}
+
+// Where a tile's numbers come from.
+template <typename T>
+struct Fp8Plain {
+    const T *x;
+    long long row_stride;
+    __device__ __forceinline__ float4 load(long long row, int col) const { return fp8_load4(x + row * row_stride + col); }
+};
+// Columns 0 .. f - 1: the gradient of a gated block's gate, dh u act'(g); f .. 2f - 1: of the other projection, dh act(g).  z = [g | u].
+template <typename T, bool GELU>
+struct Fp8Gated {
+    const T *z, *dh;
+    int f;
+    __device__ __forceinline__ float4 load(long long row, int col) const
+    {
+        const bool gate = col < f;
+        const int at = gate ? col : col - f;  // f is a multiple of 16: four columns are of one kind
+        const T *zr = z + row * 2 * f + at;
+        const float4 g = fp8_load4(zr), d = fp8_load4(dh + row * f + at), u = gate ? fp8_load4(zr + f) : g;
+        auto one = [&](float g, float u, float d) {
+            const float sigma = fp8_gate<GELU>(g);
+            return gate ? d * u * fp8_gate_slope<GELU>(g, sigma) : d * (g * sigma);
+        };
+        return make_float4(one(g.x, u.x, d.x), one(g.y, u.y, d.y), one(g.z, u.z, d.z), one(g.w, u.w, d.w));
+    }
+};
+
+__device__ __forceinline__ uint32_t fp8_magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+// bits of magnitudes compare as the numbers do, NaN above infinity
+
+template <int WAYS, typename Source>  // WAYS: 1 << kFp8Row | 1 << kFp8Column, one of them, or 1 << kFp8Square
+__global__ void __launch_bounds__(32 * kFp8TileWarps)
+fp8_quantize_tile_kernel(const Source src, uint8_t *q, uint8_t *s, uint8_t *q2, uint8_t *s2, int rows, int cols, bool two_halves, bool chained)
+{
+    constexpr bool kRows = WAYS & (1 << kFp8Row), kCols = WAYS & (1 << kFp8Column), kSquare = WAYS & (1 << kFp8Square);
+    __shared__ uint4 s_max[kFp8TileWarps][32];
+    if (chained) {
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        asm volatile("griddepcontrol.wait;" ::: "memory");
+    }
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int col_tiles = gridDim.x, row_tiles = div_up(rows, kFp8Block);
+    // Halves of the columns that read the same: tile t of the one and of the other follow one another, so that L2 has it.
+    const int ct = !two_halves ? blockIdx.x : (blockIdx.x & 1) ? (col_tiles + 1) / 2 + (blockIdx.x >> 1) : blockIdx.x >> 1;
+    const int col = ct * kFp8Block + lane * 4;
+    const bool in = col < cols;
+    for (int rt = blockIdx.y; rt < row_tiles; rt += gridDim.y) {
+        const long long row0 = (long long)rt * kFp8Block + warp * kFp8TileRows;
+        float v[kFp8TileRows][4];
+#pragma unroll
+        for (int r = 0; r < kFp8TileRows; ++r) {
+            const float4 a = in && row0 + r < rows ? src.load(row0 + r, col) : make_float4(0, 0, 0, 0);
+            v[r][0] = a.x; v[r][1] = a.y; v[r][2] = a.z; v[r][3] = a.w;
+        }
+        auto write = [&](uint8_t *to, int r, const float (&inverse)[4], const bool (&none)[4]) {
+            uint32_t w = fp8_encode4(v[r][0] * inverse[0], v[r][1] * inverse[1], v[r][2] * inverse[2], v[r][3] * inverse[3]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (none[i]) w &= ~(0xffu << (8 * i));
+            if (in && row0 + r < rows) *reinterpret_cast<uint32_t *>(to + (row0 + r) * cols + col) = w;
+        };
+        if constexpr (kRows) {
+            uint32_t mine = 0;
+#pragma unroll
+            for (int r = 0; r < kFp8TileRows; ++r) {
+                uint32_t m = max(max(fp8_magnitude(v[r][0]), fp8_magnitude(v[r][1])), max(fp8_magnitude(v[r][2]), fp8_magnitude(v[r][3])));
+                m = __reduce_max_sync(0xffffffffu, m);
+                const uint32_t e = fp8_scale(m);
+                const float i = fp8_inverse(e);
+                const bool n = e == 255u;
+                write(q, r, {i, i, i, i}, {n, n, n, n});
+                if (lane == r) mine = e;
+            }
+            if (lane < kFp8TileRows && row0 + lane < rows) {
+                uint8_t *at = s + ((long long)(ct >> 2) * rows + row0 + lane) * 4 + (ct & 3);
+                *at = (uint8_t)mine;
+                if (ct + 1 == col_tiles)
+                    for (int i = 1; i < 4 - (ct & 3); ++i) at[i] = 0;
+            }
+        }
+        if constexpr (kCols || kSquare) {
+            uint4 m = make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < kFp8TileRows; ++r) {
+                m.x = max(m.x, fp8_magnitude(v[r][0]));
+                m.y = max(m.y, fp8_magnitude(v[r][1]));
+                m.z = max(m.z, fp8_magnitude(v[r][2]));
+                m.w = max(m.w, fp8_magnitude(v[r][3]));
+            }
+            if constexpr (kSquare) m.x = __reduce_max_sync(0xffffffffu, max(max(m.x, m.y), max(m.z, m.w)));
+            __syncthreads();  // what was there before has been read
+            s_max[warp][lane] = m;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kFp8TileWarps; ++w) {
+                const uint4 o = s_max[w][lane];
+                m = make_uint4(max(m.x, o.x), max(m.y, o.y), max(m.z, o.z), max(m.w, o.w));
+            }
+            uint8_t *to = kRows ? q2 : q, *words = kRows ? s2 : s;
+            const uint32_t e[4] = {fp8_scale(m.x), kSquare ? fp8_scale(m.x) : fp8_scale(m.y), kSquare ? fp8_scale(m.x) : fp8_scale(m.z), kSquare ? fp8_scale(m.x) : fp8_scale(m.w)};
+            const float inverse[4] = {fp8_inverse(e[0]), fp8_inverse(e[1]), fp8_inverse(e[2]), fp8_inverse(e[3])};
+            const bool none[4] = {e[0] == 255u, e[1] == 255u, e[2] == 255u, e[3] == 255u};
+#pragma unroll
+            for (int r = 0; r < kFp8TileRows; ++r) write(to, r, inverse, none);
+            if constexpr (kSquare) {
+                if (threadIdx.x == 0) words[(long long)rt * col_tiles + ct] = (uint8_t)e[0];
+            } else if (warp == 0 && in) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint8_t *at = words + ((long long)(rt >> 2) * cols + col + i) * 4 + (rt & 3);
+                    *at = (uint8_t)e[i];
+                    if (rt + 1 == row_tiles)
+                        for (int j = 1; j < 4 - (rt & 3); ++j) at[j] = 0;
+                }
+            }
+        }
+    }
+}
+
+template <int WAYS, typename Source>
+static cudaError_t tile_launch(const Source &src, const Fp8Codes &to, const Fp8Codes &to2, int rows, int cols, bool two_halves, bool chained, cudaStream_t stream)
+{
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3((unsigned)div_up(cols, kFp8Block), (unsigned)std::min(div_up(rows, kFp8Block), 65535));
+    lc.blockDim = dim3(32 * kFp8TileWarps);
+    lc.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = attr;
+    lc.numAttrs = chained ? 1 : 0;
+    return cudaLaunchKernelEx(&lc, fp8_quantize_tile_kernel<WAYS, Source>, src, (uint8_t *)to.q, (uint8_t *)to.s, (uint8_t *)to2.q, (uint8_t *)to2.s, rows, cols, two_halves, chained);
+}
+
+template <typename Source>
+static cudaError_t tile_ways(const Source &src, int blocks, const Fp8Codes &to, const Fp8Codes &to2, int rows, int cols, bool two_halves, bool chained, cudaStream_t stream)
+{
+    switch (blocks) {
+        case kFp8Column: return tile_launch<1 << kFp8Column>(src, to, to2, rows, cols, two_halves, chained, stream);
+        case kFp8Square: return tile_launch<1 << kFp8Square>(src, to, to2, rows, cols, two_halves, chained, stream);
+        default: return tile_launch<1 << kFp8Row | 1 << kFp8Column>(src, to, to2, rows, cols, two_halves, chained, stream);
+    }
+}
+
+cudaError_t launch_fp8_quantize_tiles(const void *x, int type, long long row_stride, int blocks, const Fp8Codes &to, const Fp8Codes &to2, int rows, int k, bool chained,
+                                      cudaStream_t stream)
+{
+    switch (type) {
+        case TUNA_FP16: return tile_ways(Fp8Plain<__half>{(const __half *)x, row_stride}, blocks, to, to2, rows, k, false, chained, stream);
+        case TUNA_BF16: return tile_ways(Fp8Plain<__nv_bfloat16>{(const __nv_bfloat16 *)x, row_stride}, blocks, to, to2, rows, k, false, chained, stream);
+        default: return tile_ways(Fp8Plain<float>{(const float *)x, row_stride}, blocks, to, to2, rows, k, false, chained, stream);
+    }
+}
+
+template <typename Source>
+static cudaError_t gated_ways(const Source &src, const Fp8Codes &by_row, const Fp8Codes &by_column, int rows, int f, cudaStream_t stream)
+{
+    if (by_row.q && by_column.q) return tile_launch<1 << kFp8Row | 1 << kFp8Column>(src, by_row, by_column, rows, 2 * f, true, true, stream);
+    if (by_row.q) return tile_launch<1 << kFp8Row>(src, by_row, by_row, rows, 2 * f, true, true, stream);
+    return tile_launch<1 << kFp8Column>(src, by_column, by_column, rows, 2 * f, true, true, stream);
+}
+
+cudaError_t launch_fp8_gated_gradient(const void *z, const void *dh, int type, int gelu, const Fp8Codes &by_row, const Fp8Codes &by_column, int rows, int f, cudaStream_t stream)
+{
+    if (type == TUNA_FP16) {
+        if (gelu) return gated_ways(Fp8Gated<__half, true>{(const __half *)z, (const __half *)dh, f}, by_row, by_column, rows, f, stream);
+        return gated_ways(Fp8Gated<__half, false>{(const __half *)z, (const __half *)dh, f}, by_row, by_column, rows, f, stream);
+    }
+    if (gelu) return gated_ways(Fp8Gated<__nv_bfloat16, true>{(const __nv_bfloat16 *)z, (const __nv_bfloat16 *)dh, f}, by_row, by_column, rows, f, stream);
+    return gated_ways(Fp8Gated<__nv_bfloat16, false>{(const __nv_bfloat16 *)z, (const __nv_bfloat16 *)dh, f}, by_row, by_column, rows, f, stream);
+}
+
+// ---- the inverse
+
+__device__ __forceinline__ void fp8_store8(float *p, const float (&v)[8])
+{
+    reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void fp8_store8(__half *p, const float (&v)[8])
+{
+    *reinterpret_cast<uint4 *>(p) = make_uint4(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]), pack_half2(v[4], v[5]), pack_half2(v[6], v[7]));
+}
+__device__ __forceinline__ void fp8_store8(__nv_bfloat16 *p, const float (&v)[8])
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// o = code * scale in fp32 (exact: four significant bits; below fp32's range it rounds), rounded once to T.  A thread has eight columns of ROWS rows, grid (columns, rows).
+template <typename T, int BLOCKS, int ROWS>
+__global__ void __launch_bounds__(128)
+fp8_dequant_kernel(const uint8_t *q, const uint8_t *s, T *o, int rows, int k)
+{
+    const int col = (blockIdx.x * 128 + threadIdx.x) * 8;
+    if (col >= k) return;
+    for (long long row0 = (long long)blockIdx.y * ROWS; row0 < rows; row0 += (long long)gridDim.y * ROWS) {
+        uint2 codes[ROWS];
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) codes[r] = row0 + r < rows ? __ldcg(reinterpret_cast<const uint2 *>(q + (row0 + r) * k + col)) : make_uint2(0, 0);
+        uint32_t byte[BLOCKS == kFp8Column ? 8 : ROWS];
+        if constexpr (BLOCKS == kFp8Column) {  // ROWS divides 128: the rows are of one block
+#pragma unroll
+            for (int i = 0; i < 8; ++i) byte[i] = __ldcg(s + ((row0 >> 9) * k + col + i) * 4 + ((row0 >> 7) & 3));
+        } else {
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) {
+                const long long row = min(row0 + r, (long long)rows - 1);
+                byte[r] = BLOCKS == kFp8Row ? __ldcg(s + ((long long)(col >> 9) * rows + row) * 4 + ((col >> 7) & 3)) : __ldcg(s + (row >> 7) * div_up(k, kFp8Block) + (col >> 7));
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r) {
+            if (row0 + r >= rows) continue;
+            uint32_t h[4];
+            fp8_decode4(codes[r].x, *reinterpret_cast<uint32_t(*)[2]>(h));
+            fp8_decode4(codes[r].y, *reinterpret_cast<uint32_t(*)[2]>(h + 2));
+            float v[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
+                v[2 * i] = f.x * mx_scale_value(byte[BLOCKS == kFp8Column ? 2 * i : r]);
+                v[2 * i + 1] = f.y * mx_scale_value(byte[BLOCKS == kFp8Column ? 2 * i + 1 : r]);
+            }
+            fp8_store8(o + (row0 + r) * k + col, v);
+        }
+    }
+}
+
+template <typename T, int BLOCKS>
+static cudaError_t dequant_as(const void *q, const void *s, void *o, int rows, int k, cudaStream_t stream)
+{
+    constexpr int kRows = 4;
+    const dim3 grid((unsigned)div_up(k, 8 * 128), (unsigned)std::min(div_up(rows, kRows), 65535));
+    fp8_dequant_kernel<T, BLOCKS, kRows><<<grid, 128, 0, stream>>>((const uint8_t *)q, (const uint8_t *)s, (T *)o, rows, k);
+    return cudaGetLastError();
+}
+
+template <typename T>
+static cudaError_t dequant_any(const void *q, const void *s, int blocks, void *o, int rows, int k, cudaStream_t stream)
+{
+    switch (blocks) {
+        case kFp8Row: return dequant_as<T, kFp8Row>(q, s, o, rows, k, stream);
+        case kFp8Column: return dequant_as<T, kFp8Column>(q, s, o, rows, k, stream);
+        default: return dequant_as<T, kFp8Square>(q, s, o, rows, k, stream);
+    }
+}
+
+cudaError_t launch_fp8_dequant(const void *q, const void *s, int blocks, void *o, int type, int rows, int k, cudaStream_t stream)
+{
+    switch (type) {
+        case TUNA_FP16: return dequant_any<__half>(q, s, blocks, o, rows, k, stream);
+        case TUNA_BF16: return dequant_any<__nv_bfloat16>(q, s, blocks, o, rows, k, stream);
+        default: return dequant_any<float>(q, s, blocks, o, rows, k, stream);
+    }
+}
+
+}  // namespace tuna

@@ -115,4 +115,32 @@ int launch_mx_gemm(const MxGemmArgs &a);
 // Whether the product takes tokens of this type as they are; otherwise it wants their codes and scales.
 bool mx_gemm_takes(int m, int n, int k, int experts, int x_type, bool grouped, int sm_count);
 
+// 8-bit block-scaled matrices (fp8_format.cuh).  Types are tuna_type's.
+enum Fp8Blocks { kFp8Row = TUNA_FP8_ROW, kFp8Column = TUNA_FP8_COLUMN, kFp8Both = TUNA_FP8_BOTH, kFp8Square = TUNA_FP8_SQUARE };
+struct Fp8Codes {
+    void *q, *s;
+};
+// `chained`: part of a call whose next launch may start with this one, and waits for it before it reads what this one writes
+cudaError_t launch_fp8_quantize_rows(const void *x, int type, long long row_stride, void *q, void *s, int rows, int k, bool chained, cudaStream_t stream);
+// Column, square, or both: `to` by row and `to2` by column
+cudaError_t launch_fp8_quantize_tiles(const void *x, int type, long long row_stride, int blocks, const Fp8Codes &to, const Fp8Codes &to2, int rows, int k, bool chained,
+                                      cudaStream_t stream);
+// The gradients of a gated block's two projections, [rows, 2f], by row and by column (one of which may have null pointers: it is not wanted)
+cudaError_t launch_fp8_gated_gradient(const void *z, const void *dh, int type, int gelu, const Fp8Codes &by_row, const Fp8Codes &by_column, int rows, int f, cudaStream_t stream);
+cudaError_t launch_fp8_dequant(const void *q, const void *s, int blocks, void *o, int type, int rows, int k, cudaStream_t stream);
+
+struct Fp8ProductArgs {
+    Fp8Codes w, x;        // x.q is null where the product takes the numbers as they are
+    const void *numbers;  // tokens of x_type; where x has room for their codes they are quantized by a launch before the product, once nothing can be refused
+    void *o, *z;
+    int m, n, k, x_type, o_type, gated, gelu;
+    cudaStream_t stream;
+    int sm_count;
+};
+int launch_fp8_product(const Fp8ProductArgs &a);
+int launch_fp8_dx(const Fp8Codes &w, const Fp8Codes &dy, void *dx, int type, int m, int n, int k, int sm_count, cudaStream_t stream);
+int launch_fp8_dw(const Fp8Codes &x, const Fp8Codes &dy, void *dw, int type, int m, int n, int k, int sm_count, cudaStream_t stream);
+// Whether the product takes tokens of this type as they are; otherwise it wants their codes and scales.
+bool fp8_gemm_takes(bool gated, int rows, int n, int red, int x_type, int sm_count);
+
 }  // namespace tuna

@@ -95,6 +95,22 @@ struct Mx8<float> {
     }
 };
 
+// A sum in fp32 as a number of the output's type, and two side by side of the 16-bit types.
+template <typename T>
+__device__ __forceinline__ T mx_convert(float v);
+template <> __device__ __forceinline__ __half mx_convert<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 mx_convert<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ float mx_convert<float>(float v) { return v; }
+
+template <typename T>
+__device__ __forceinline__ uint32_t mx_pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t mx_pack2<__half>(float lo, float hi) { return pack_half2(lo, hi); }
+template <> __device__ __forceinline__ uint32_t mx_pack2<__nv_bfloat16>(float lo, float hi)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
 // The scale of a block whose largest magnitude has the bits `largest` (fp32): floor(log2(largest)) - 2, so that the largest
 // lies between 4 and 8 times the scale (what is above 6 saturates), not below 2^-127.  Infinity or NaN: a NaN scale.
 __device__ __forceinline__ uint32_t mx_scale(uint32_t largest)

@@ -174,21 +174,6 @@ __host__ __device__ constexpr uint32_t mx_idesc(int cols, int half)
     return (1u << 7) | (1u << 10) | ((uint32_t)(cols >> 3) << 17) | (1u << 23) | ((uint32_t)CG << 27) | ((uint32_t)(2 * half) << 29) | ((uint32_t)(2 * half) << 4);
 }
 
-template <typename T>
-__device__ __forceinline__ T mx_convert(float v);
-template <> __device__ __forceinline__ __half mx_convert<__half>(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_bfloat16 mx_convert<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ float mx_convert<float>(float v) { return v; }
-
-template <typename T>
-__device__ __forceinline__ uint32_t mx_pack2(float lo, float hi);
-template <> __device__ __forceinline__ uint32_t mx_pack2<__half>(float lo, float hi) { return pack_half2(lo, hi); }
-template <> __device__ __forceinline__ uint32_t mx_pack2<__nv_bfloat16>(float lo, float hi)
-{
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-}
-
 // Words of a half (128 columns) of the tokens' scales that a lane holds, for so many columns of an accumulator.
 __host__ __device__ constexpr int mx_token_words(int cols) { return cols <= 64 ? 2 : cols <= 128 ? 4 : 8; }
 // Tensor-memory columns of a stage's scales: four per half for the weights, four per half and 128 tokens.
