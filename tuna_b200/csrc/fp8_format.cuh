@@ -43,7 +43,7 @@ template <bool GELU>
 __device__ __forceinline__ float fp8_gate(float g)
 {
     const float p = GELU ? kGeluA * fmaf(kGeluB * g * g, g, g) : g;
-    return __fdividef(1.0f, 1.0f + expf(-p));  // exp overflows to infinity, and the quotient is 0 then
+    return __fdividef(1.0f, 1.0f + __expf(-p));  // exp overflows to infinity, and the quotient is 0 then
 }
 // ... and its derivative, sigma + g sigma (1 - sigma) p', given sigma.  Where sigma has become 0 or 1 the second term is 0, whatever p' is.
 template <bool GELU>

@@ -20,7 +20,7 @@
 //   warp 0     MMA issue (one elected lane; in a pair the first CTA's)
 //   warp 1, 2  TMA producers of A and of B
 //   warp 3     tensor-memory allocation; in a pair, tells the first CTA that a stage has landed
-//   warps 4-7  epilogue: tensor memory -> registers -> output type -> shared memory, where rows become contiguous -> memory
+//   warps 4-7  epilogue: tensor memory -> registers -> output type -> shared memory, where rows become contiguous -> memory; in a pair 12-15 too
 //   warps 8-11 scales, one warp per lane quarter: global memory -> registers, a group of four stages ahead -> tensor memory, the word of row r at lane r % 32,
 //              column r / 32, in every quarter
 // RESIDENT: a few tokens in 16 bits are quantized by the CTA itself before its first MMA, all of K, and stay in shared memory.
@@ -44,12 +44,14 @@ namespace tuna {
 
 enum Fp8Form { kFp8Product, kFp8GatedProduct, kFp8Dx, kFp8Dw };
 
-constexpr int kFp8Warps = 12;
+// Warps of a CTA: pairs have eight for the epilogue, two groups of four that take turns on 32 columns.  With four, gated tiles of 256 columns waited for them (4096 features
+// of K: 14336x4096 at 2048 tokens 206 us, with z 233).
+__host__ __device__ constexpr int fp8_warps(int cg) { return cg == 1 ? 12 : 16; }
 constexpr int kFp8EpilogueWarp0 = 4;
 constexpr int kFp8ScaleWarp0 = 8;
 constexpr int kFp8MaxStages = 12;
 constexpr int kFp8DirectCols = 16;        // tokens up to which single CTAs take the tiles
-constexpr int kFp8StageCols = 64;         // columns of the output staging buffer
+constexpr int kFp8StageCols = 32;         // columns of a group's output staging buffer
 constexpr int kFp8AheadTokens = 64;       // up to here weights count as constants and are copied ahead of the dependency wait, as in mx_gemm_sm100a.cu
 constexpr int kFp8ResidentLoads = 4;      // loads in flight of a quantizing warp
 constexpr int kFp8SfCols = 16;            // tensor-memory columns of a group's scales: A's words at 0 to 3, B's at 8 to 15
@@ -86,6 +88,7 @@ struct Fp8Params {
     int ahead;       // A is there before the dependency wait
     int x_bf16;      // RESIDENT: type of the tokens
     const void *x;   // RESIDENT: the tokens [cols][red]
+    int stagger;     // row tiles start their sums at different groups
     int gelu;
     int z_offset;    // gated: where z is staged
 };
@@ -103,7 +106,19 @@ struct Fp8Tiles {
         next_tile += step;
         return true;
     }
+    // Stages come in groups of four (one word of scales); a tile starts with this one and goes round.
+    __device__ int first_group(const Fp8Params &p, int groups) const { return p.stagger ? rt % groups : 0; }
     __device__ int total(const Fp8Params &p) const { const int n = p.row_tiles * p.col_tiles; return next_tile < n ? (n - 1 - next_tile) / step + 1 : 0; }
+};
+
+// The stages of a tile in order.
+struct Fp8Stages {
+    int c, units;
+    __device__ Fp8Stages(const Fp8Params &p, int first_group) : c(4 * first_group), units(p.units) {}
+    __device__ void advance()
+    {
+        if (++c == units) c = 0;
+    }
 };
 
 // D[tmem] (+)= (A * scale A) (B * scale B), 32 columns of e4m3 with one scale
@@ -187,7 +202,7 @@ __device__ __forceinline__ float fp8_activation(float g, float u, int gelu) { re
 
 // CG: CTAs of a worker (1 or 2).  Single CTAs leave room for a second one on the SM: that of the next launch, which copies its first weights meanwhile.
 template <int CG, int FORM, bool RESIDENT, typename OT>
-__global__ void __launch_bounds__(32 * kFp8Warps, CG == 1 ? 2 : 1)
+__global__ void __launch_bounds__(32 * fp8_warps(CG), CG == 1 ? 2 : 1)
 fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a2, const __grid_constant__ CUtensorMap tmap_b)
 {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -218,7 +233,8 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
             if (i < kFp8MaxStages) return RESIDENT ? 1 : 2;       // landed: the producers
             if (i < 2 * kFp8MaxStages) return 2;                  // full: both CTAs of the pair
             if (i < 3 * kFp8MaxStages + 2) return 1;              // empty, d_full: a commit
-            if (i < 3 * kFp8MaxStages + 6) return 4 * CG;         // d_empty: the epilogue warps of each CTA; sf_full: the scale warps
+            if (i < 3 * kFp8MaxStages + 4) return CG == 1 ? 4 : 16;  // d_empty: the epilogue warps of each CTA
+            if (i < 3 * kFp8MaxStages + 6) return 4 * CG;         // sf_full: the scale warps of each CTA
             return 1;                                             // sf_empty: a commit
         };
         for (int i = lane; i < 3 * kFp8MaxStages + 8; i += 32) mbar_init(landed + 8 * i, count(i));
@@ -256,10 +272,10 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
     if (RESIDENT && warp != 1) {  // the weights are on their way meanwhile
         depend();
         const int w = warp == 0 ? 0 : warp - 1;
-        if (p.x_bf16) fp8_quantize_resident<__nv_bfloat16>(p, w, kFp8Warps - 1, lane, b_ring, words_at);
-        else fp8_quantize_resident<__half>(p, w, kFp8Warps - 1, lane, b_ring, words_at);
+        if (p.x_bf16) fp8_quantize_resident<__nv_bfloat16>(p, w, fp8_warps(CG) - 1, lane, b_ring, words_at);
+        else fp8_quantize_resident<__half>(p, w, fp8_warps(CG) - 1, lane, b_ring, words_at);
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the MMAs read the codes
-        asm volatile("bar.sync 2, %0;" ::"n"(32 * (kFp8Warps - 1)) : "memory");
+        asm volatile("bar.sync 2, %0;" ::"n"(32 * (fp8_warps(CG) - 1)) : "memory");
     }
     // Whoever makes a bounded wait that ends only after the kernels before this one waits for those first.
     if (warp == 0) {
@@ -278,21 +294,23 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
                 ok = mbar_wait_warp(d_empty + 8 * rd.idx, rd.phase ^ 1, abort_flag, p.status, 303);
                 const uint32_t d = tmem + (uint32_t)(second * p.d_step);
                 second ^= 1;
-                for (int c = 0; ok && c < p.units; ++c) {
-                    if ((c & 3) == 0) ok = mbar_wait_warp(sf_full + 8 * rs.idx, rs.phase, abort_flag, p.status, 304);
+                Fp8Stages st(p, tile.first_group(p, groups));
+                for (int i = 0; ok && i < p.units; ++i, st.advance()) {
+                    const int c = st.c;
+                    if (i == 0 || (c & 3) == 0) ok = mbar_wait_warp(sf_full + 8 * rs.idx, rs.phase, abort_flag, p.status, 304);
                     ok = ok && mbar_wait_warp(full + 8 * ru.idx, ru.phase, abort_flag, p.status, 305);
                     if (!ok) break;
                     tc_fence_after();
-                    const bool last = c + 1 == p.units, group_ends = last || (c & 3) == 3;
+                    const bool last = i + 1 == p.units, group_ends = c + 1 == p.units || (c & 3) == 3;
                     if (elect_one_sync()) {
                         const uint64_t a = sw128 | (uint64_t)(((base + (uint32_t)ru.idx * a_bytes) & 0x3FFFFu) >> 4);
                         const uint64_t b = sw128 | (uint64_t)(((b_ring + (uint32_t)(RESIDENT ? c : ru.idx) * b_bytes) & 0x3FFFFu) >> 4);
                         const uint32_t sfa = tmem + (uint32_t)(p.sf_col + rs.idx * kFp8SfCols), sfb = sfa + 8;
-                        const int steps = last && !p.fold_log ? p.last_steps : 4;
+                        const int steps = c + 1 == p.units && !p.fold_log ? p.last_steps : 4;
                         const uint32_t id = idesc | ((uint32_t)(c & 3) << 29) | ((uint32_t)(c & 3) << 4);
 #pragma unroll
                         for (int kk = 0; kk < 4; ++kk)
-                            if (kk < steps) tc_mma_fp8<CG>(d, a + kStepA * kk, b + kStepB * kk, id, sfa, sfb, c == 0 && kk == 0 ? 0u : 1u);
+                            if (kk < steps) tc_mma_fp8<CG>(d, a + kStepA * kk, b + kStepB * kk, id, sfa, sfb, i == 0 && kk == 0 ? 0u : 1u);
                         if (CG == 1) {
                             tc_commit(empty + 8 * ru.idx);
                             if (group_ends) tc_commit(sf_empty + 8 * rs.idx);
@@ -319,7 +337,9 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
         while (ok && tile.next(p)) {
             const int block = CG * tile.rt + rank, row = fp8_row(p, block), rows = p.flex ? fp8_row(p, block + 1) - row : kBlockRows;
             const CUtensorMap *map = !p.flex || rows == p.group_rows * div_up(p.groups, p.row_tiles) ? &tmap_a : &tmap_a2;  // boxes of the taller and of the lower tiles
-            for (int c = 0; c < p.units; ++c, ru.advance(S)) {
+            Fp8Stages st(p, tile.first_group(p, groups));
+            for (int i = 0; i < p.units; ++i, st.advance(), ru.advance(S)) {
+                const int c = st.c;
                 if (issued++ == S) depend();
                 ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 300);
                 if (!ok) break;
@@ -348,7 +368,9 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
         depend();
         while (ok && tile.next(p)) {
             const int col = tile.col0 + rank * (mma_cols() / CG);
-            for (int c = 0; c < p.units; ++c, ru.advance(S)) {
+            Fp8Stages st(p, tile.first_group(p, groups));
+            for (int i = 0; i < p.units; ++i, st.advance(), ru.advance(S)) {
+                const int c = st.c;
                 ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 301);
                 if (!ok) break;
                 if (elect_one_sync()) {
@@ -373,85 +395,120 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
             if (!mbar_wait_warp(landed + 8 * ru.idx, ru.phase, abort_flag, p.status, 302)) break;
             if (lane == 0) mbar_arrive_cluster(leader_full + 8 * ru.idx);
         }
-    } else if (warp >= kFp8ScaleWarp0) {
+    } else if (warp >= kFp8ScaleWarp0 && warp < kFp8ScaleWarp0 + 4) {
         // ------------------------------------------------------------------ scales to tensor memory
         const int quarter = warp - kFp8ScaleWarp0;
         const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)p.sf_col;
         const uint32_t leader_full = CG == 1 ? sf_full : map_to_rank(sf_full, 0);
         const int a_blocks = div_up(p.rows, kFp8Block);
-        uint32_t next[kFp8SfCols];
+        // Of a group, as loaded: A's words (dw) or, spread over the lanes, its bytes; B's words or (folded) bytes of two.  They are put together when the group
+        // before has been written, so that nothing waits for the loads before that.
+        constexpr bool kWordsA = FORM == kFp8Dw;
+        uint32_t raw_a[4] = {0, 0, 0, 0}, raw_b[8];
 #pragma unroll
-        for (int i = 0; i < kFp8SfCols; ++i) next[i] = 0;
-        // The words of group g of the tile: bytes are those of stages 4g .. 4g + 3.
-        auto fetch = [&](int g) {
+        for (int i = 0; i < 8; ++i) raw_b[i] = 0;
+        // Square scales: a tile's rows are of one block or two, gated of as many for each projection.  A group has 4 * fold bytes of each, which lie side by side: byte
+        // `pos` of slot `slot` is lane (slot * 4 * fold + pos) % 32's.  (A byte for every row, loaded by all lanes, made one line of L2 what all SMs waited for:
+        // 8192x8192 at 4096 tokens 205 -> 290 us.)
+        const int fold_log = CG == 1 ? p.fold_log : 0;
+        auto block_of = [&](int slot, int row0) {
+            if (FORM == kFp8Dx) return row0 / kFp8Block;
+            if (kGated) return min(((slot >> 1) * (p.rows / 2) + (row0 >> 1)) / kFp8Block + (slot & 1), a_blocks - 1);
+            return min(row0 / kFp8Block + (slot & 1), a_blocks - 1);
+        };
+        // Group g of the tile: stages 4g .. 4g + 3.  What lies behind the last block or column is any of them: nothing is multiplied with it.
+        auto fetch_a = [&](int g) {
             const int row0 = fp8_row(p, CG * tile.rt + rank);
-            int had = -1;
+            if constexpr (kWordsA) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {  // A: MMA row 32 i + lane is row `of` of part f
-                const int r = 32 * i + lane, f = r >> (7 - p.fold_log), of = r & (part - 1);
-                if constexpr (FORM == kFp8Dw) {
-                    next[i] = __ldcg(reinterpret_cast<const uint32_t *>(p.as) + (size_t)g * p.rows + min(row0 + r, p.rows - 1));
-                } else {
-                    int row = row0 + of;
-                    if constexpr (kGated) {
-                        const int feature = min((row0 >> 1) + ((of >> 4) << 3) + (of & 7), p.rows / 2 - 1);
-                        row = (of & 8) ? p.rows / 2 + feature : feature;
-                    }
-                    const int block = min(row, p.rows - 1) / kFp8Block, key = (block << 2) + f;
-                    if (key == had) {
-                        next[i] = next[i > 0 ? i - 1 : 0];
-                        continue;
-                    }
-                    had = key;
-                    uint32_t w = 0;
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int kb = ((4 * g + j) << p.fold_log) + f;
-                        if (kb < p.blocks) w |= (uint32_t)__ldcg(p.as + (FORM == kFp8Dx ? (size_t)kb * a_blocks + block : (size_t)block * p.blocks + kb)) << (8 * j);
-                    }
-                    next[i] = w;
-                }
-            }
-            if constexpr (RESIDENT) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(next[8 + j]) : "r"(words_at + 256u * (uint32_t)g + 128u * j + 4u * lane));
-            } else if (CG == 1 && p.fold_log) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {  // column t of block f of a stage
-                    const int at = 32 * j + lane, f = at / p.b_rows, t = at - f * p.b_rows;
-                    uint32_t w = 0;
-                    if (f < fold && t < tile.valid)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int kb = ((4 * g + i) << p.fold_log) + f;
-                            if (kb < p.blocks) w |= (uint32_t)__ldcg(p.bs + ((size_t)(kb >> 2) * p.cols + tile.col0 + t) * 4 + (kb & 3)) << (8 * i);
-                        }
-                    next[8 + j] = w;
-                }
+                for (int i = 0; i < 4; ++i) raw_a[i] = __ldcg(reinterpret_cast<const uint32_t *>(p.as) + (size_t)g * p.rows + min(row0 + 32 * i + lane, p.rows - 1));
             } else {
 #pragma unroll
-                for (int j = 0; j < (CG == 1 ? 1 : 8); ++j) {
-                    const int t = 32 * j + lane;
-                    if (32 * j < tile.valid) next[8 + j] = __ldcg(reinterpret_cast<const uint32_t *>(p.bs) + (size_t)g * p.cols + tile.col0 + min(t, tile.valid - 1));
+                for (int i = 0; i < 2; ++i) {
+                    const int idx = 32 * i + lane, slot = idx >> (2 + fold_log), kb = min((4 * g << fold_log) + (idx & ((4 << fold_log) - 1)), p.blocks - 1);
+                    if (slot < (FORM == kFp8Dx ? 1 : kGated ? 4 : 2)) {
+                        const int block = block_of(slot, row0);
+                        raw_a[i] = __ldcg(p.as + (FORM == kFp8Dx ? (size_t)kb * a_blocks + block : (size_t)block * p.blocks + kb));
+                    }
                 }
             }
         };
+        // MMA row 32 i + lane is row `of` of part f
+        auto word_a = [&](int i) {
+            if constexpr (kWordsA) {
+                return raw_a[i];
+            } else {
+                const int row0 = fp8_row(p, CG * tile.rt + rank), r = 32 * i + lane, f = r >> (7 - fold_log), of = r & ((kBlockRows >> fold_log) - 1);
+                int slot = 0;
+                if constexpr (kGated) {
+                    const int base = (of & 8) ? p.rows / 2 : 0, first = row0 >> 1, feature = min(first + ((of >> 4) << 3) + (of & 7), p.rows / 2 - 1);
+                    slot = ((of & 8) >> 2) + (base + feature) / kFp8Block - (base + first) / kFp8Block;
+                } else if (FORM == kFp8Product) {
+                    slot = min(row0 + of, p.rows - 1) / kFp8Block - row0 / kFp8Block;
+                }
+                uint32_t w = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int idx = (slot << (2 + fold_log)) + (j << fold_log) + f;
+                    uint32_t b = __shfl_sync(0xffffffffu, raw_a[0], idx & 31);
+                    if (CG == 1) {
+                        const uint32_t b2 = __shfl_sync(0xffffffffu, raw_a[1], idx & 31);
+                        if (idx >= 32) b = b2;
+                    }
+                    w |= b << (8 * j);
+                }
+                return w;
+            }
+        };
+        auto fetch_b = [&](int g) {
+            if constexpr (RESIDENT) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(raw_b[j]) : "r"(words_at + 256u * (uint32_t)g + 128u * j + 4u * lane));
+            } else if (CG == 1 && p.fold_log) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {  // column t of block f of a stage
+                    const int at = 32 * j + lane, f = at / p.b_rows, t = min(at - f * p.b_rows, tile.valid - 1);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int kb = min(((4 * g + i) << p.fold_log) + f, p.blocks - 1);
+                        raw_b[4 * j + i] = __ldcg(p.bs + ((size_t)(kb >> 2) * p.cols + tile.col0 + t) * 4 + (kb & 3));
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < (CG == 1 ? 1 : 8); ++j)
+                    if (32 * j < tile.valid) raw_b[j] = __ldcg(reinterpret_cast<const uint32_t *>(p.bs) + (size_t)g * p.cols + tile.col0 + min(32 * j + lane, tile.valid - 1));
+            }
+        };
+        auto word = [](const uint32_t *b) { return b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24); };
         Ring rs;
         bool ok = true;
-        depend();
+        if (!p.ahead) depend();
         bool more = tile.next(p);
-        int g = 0;
-        if (more) fetch(0);
+        int g = more ? tile.first_group(p, groups) : 0, left = groups;
+        if (more) fetch_a(g);
+        depend();
+        if (more) fetch_b(g);
         const int total_groups = tiles * groups;
         while (more) {
             uint32_t v[kFp8SfCols];
 #pragma unroll
-            for (int i = 0; i < kFp8SfCols; ++i) v[i] = next[i];
-            if (++g == groups) {
-                g = 0;
+            for (int i = 0; i < 4; ++i) v[i] = word_a(i);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[8 + i] = CG == 2 || i < 2 ? raw_b[i] : 0u;
+            if (CG == 1 && !RESIDENT && p.fold_log) v[8] = word(raw_b), v[9] = word(raw_b + 4);
+#pragma unroll
+            for (int i = 4; i < 8; ++i) v[i] = 0;
+            if (++g == groups) g = 0;
+            if (--left == 0) {
+                left = groups;
                 more = tile.next(p);
+                if (more) g = tile.first_group(p, groups);
             }
-            if (more) fetch(g);  // on its way while the group before is waited for
+            if (more) {  // on their way while the group before is waited for
+                fetch_a(g);
+                fetch_b(g);
+            }
             ok = mbar_wait_warp(sf_empty + 8 * rs.idx, rs.phase ^ 1, abort_flag, p.status, 306);
             if (!ok) break;
             tc_fence_after();
@@ -470,14 +527,15 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
         for (int i = min(2, total_groups); ok && i > 0; --i, rs.advance(2)) ok = mbar_wait_warp(sf_empty + 8 * rs.idx, total_groups == 1 ? 0u : rs.phase ^ 1, abort_flag, p.status, 311);
     } else if (warp >= kFp8EpilogueWarp0) {
         // ------------------------------------------------------------------ epilogue
-        const int quarter = warp & 3, thread = threadIdx.x - 32 * kFp8EpilogueWarp0;
+        const int quarter = warp & 3, thread = threadIdx.x & 127, half = warp / (kFp8ScaleWarp0 + 4);  // which group
         const uint32_t tmem_q = tmem + ((uint32_t)(32 * quarter) << 16);
         OT *o = static_cast<OT *>(p.o), *z = static_cast<OT *>(p.z);
         const int out = kGated ? p.rows / 2 : p.rows;  // numbers of a row of the output
         constexpr int kTileOut = kGated ? kBlockRows / 2 : kBlockRows;
         constexpr uint32_t kPitch = kTileOut * (uint32_t)sizeof(OT) + (sizeof(OT) == 2 || kGated ? 16 : 0);  // 16 bytes more, so that a column of 8 rows meets all banks
         constexpr uint32_t kPitchZ = kBlockRows * 2 + 16;
-        const uint32_t z_staging = staging + (uint32_t)p.z_offset;
+        const uint32_t out_staging = staging + (uint32_t)(half * kFp8StageCols) * kPitch, z_staging = staging + (uint32_t)p.z_offset + (uint32_t)(half * kFp8StageCols) * kPitchZ;
+        auto meet = [&] { asm volatile("bar.sync %0, 128;" ::"r"(1 + 2 * half) : "memory"); };  // the group's four warps
         Ring rd;
         depend();
         int row0 = 0, rows = 0;
@@ -490,40 +548,39 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
                 else mbar_arrive_cluster(leader_d_empty + 8 * rd.idx);
             }
         };
-        // The staging buffer, which has `have` of the tile's columns from t0 on (behind its last the first), to memory: 16 bytes a thread and step.
-        auto copy_out = [&](int t0, int have) {
+        // The group's staging buffer, which has 32 columns of the tile from t0 on, to memory: 16 bytes a thread and step.
+        auto copy_out = [&](int t0) {
             constexpr int kPieces = kTileOut * (int)sizeof(OT) / 16, kStep = 128 / kPieces;
-            const int piece = thread % kPieces;
+            const int piece = thread % kPieces, have = min(kFp8StageCols, tile.valid - t0);
             if (piece * (16 / (int)sizeof(OT)) < (kGated ? rows / 2 : rows)) {
-#pragma unroll 4
-                for (int t = thread / kPieces; t < have; t += kStep) {
-                    const int col = t0 + t < N ? t0 + t : t0 + t - N;
+                uint8_t *to = reinterpret_cast<uint8_t *>(o + (size_t)(tile.col0 + t0) * out + (kGated ? row0 / 2 : row0)) + 16 * piece;
+#pragma unroll
+                for (int t = thread / kPieces; t < kFp8StageCols; t += kStep) {
                     uint4 v;
-                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(staging + (uint32_t)t * kPitch + 16u * piece));
-                    if (col < tile.valid) *reinterpret_cast<uint4 *>(reinterpret_cast<uint8_t *>(o + (size_t)(tile.col0 + col) * out + (kGated ? row0 / 2 : row0)) + 16 * piece) = v;
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(out_staging + (uint32_t)t * kPitch + 16u * piece));
+                    if (t < have) *reinterpret_cast<uint4 *>(to + (size_t)t * out * sizeof(OT)) = v;
                 }
             }
             if constexpr (kGated && sizeof(OT) == 2) {
                 if (z) {
                     const int which = (thread >> 3) & 1, group = thread & 7;  // of the projections, and eight features of it
                     if (group < rows / 16) {
-                        OT *to = z + (size_t)tile.col0 * p.rows + (size_t)which * out + row0 / 2 + 8 * group;
-#pragma unroll 4
-                        for (int t = thread >> 4; t < have; t += 8) {
-                            const int col = t0 + t < N ? t0 + t : t0 + t - N;
+                        OT *to = z + (size_t)(tile.col0 + t0) * p.rows + (size_t)which * out + row0 / 2 + 8 * group;
+#pragma unroll
+                        for (int t = thread >> 4; t < kFp8StageCols; t += 8) {
                             uint4 v;
                             asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
                                          : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                                          : "r"(z_staging + (uint32_t)t * kPitchZ + 16u * (2 * group + which)));
-                            if (col < tile.valid) *reinterpret_cast<uint4 *>(to + (size_t)col * p.rows) = v;
+                            if (t < have) *reinterpret_cast<uint4 *>(to + (size_t)t * p.rows) = v;
                         }
                     }
                 }
             }
         };
-        // 32 columns of the accumulator at `d`, from t on, to column `at` of the staging buffer.
-        auto fill_from = [&](uint32_t d, int t, int at) {
-            const uint32_t to = staging + (uint32_t)at * kPitch;
+        // 32 columns of the accumulator at `d`, from t on, to the group's staging buffer.
+        auto fill_from = [&](uint32_t d, int t) {
+            const uint32_t to = out_staging;
             auto f32 = [](uint32_t v) { return __uint_as_float(v); };
             if constexpr (kGated || sizeof(OT) == 2) {
                 uint32_t lo[16], hi[16];
@@ -543,7 +600,7 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
                 if constexpr (!kGated) {
                     rows_of_8(to, kPitch);
                 } else {
-                    if (z) rows_of_8(z_staging + (uint32_t)at * kPitchZ, kPitchZ);
+                    if (z) rows_of_8(z_staging, kPitchZ);
                     auto act = [&](uint32_t g, uint32_t u) { return fp8_activation(f32(g), f32(u), p.gelu); };
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {  // lanes i and i + 8 of a half: gate and other projection of one feature, two columns
@@ -573,7 +630,7 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
         int second = 0;
         for (; tile.next(p); second ^= 1) {
             const bool ok = mbar_wait_warp(d_full + 8 * rd.idx, rd.phase, abort_flag, p.status, 307);
-            if (bar_any(1, 128, !ok)) break;  // the four warps go on together or not at all
+            if (bar_any(1 + 2 * half, 128, !ok)) break;  // the group's four warps go on together or not at all
             tc_fence_after();
             const uint32_t d = tmem_q + (uint32_t)(second * p.d_step);
             row0 = fp8_row(p, CG * tile.rt + rank);
@@ -596,7 +653,7 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
 #pragma unroll
                     for (int t = 0; t < 16; ++t)
                         if (t < tile.valid) sums[t * kBlockRows + thread] = v[t];
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
+                    meet();
                     auto sum = [&](int t, int i) {
                         float s = sums[t * kBlockRows + i];
                         for (int g = 1; g < fold; ++g) s += sums[t * kBlockRows + g * part + i];
@@ -617,25 +674,24 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
                         const int i = thread & (part - 1);
                         for (int t = f; t < tile.valid && i < rows; t += fold) o[(size_t)(tile.col0 + t) * out + row0 + i] = mx_convert<OT>(sum(t, i));
                     }
-                    asm volatile("bar.sync 1, 128;" ::: "memory");  // they have been read
+                    meet();  // they have been read
                 }
             } else {
-                // Of two accumulators that overlap, the columns they share first: then the other one may be written.
+                // Of two accumulators that overlap, the columns they share first (32 of them, the first group's): then the other one may be written, which both
+                // groups have read by now.
                 const bool shared = p.nd == 1;
                 const int turn = shared && second == 0 ? p.d_step : 0;
-                for (int b = 0; b < N; b += kFp8StageCols) {
+                if (shared && half == 1) drained();
+                for (int b = half * kFp8StageCols; b < N; b += 2 * kFp8StageCols) {
                     const int t0 = b + turn < N ? b + turn : b + turn - N;
-                    asm volatile("bar.sync 1, 128;" ::: "memory");  // what was staged before has been copied
-#pragma unroll
-                    for (int h = 0; h < kFp8StageCols; h += 32) {
-                        const int t = t0 + h < N ? t0 + h : t0 + h - N;
-                        if (b + h < N && t < tile.valid) fill_from(d, t, h);
-                        if (shared && b == 0 && h == 0) drained();
-                    }
-                    if (!shared && b + kFp8StageCols >= N) drained();
-                    asm volatile("bar.sync 1, 128;" ::: "memory");
-                    copy_out(t0, min(kFp8StageCols, N - b));
+                    meet();  // what was staged before has been copied
+                    if (t0 < tile.valid) fill_from(d, t0);
+                    if (shared && b == 0) drained();
+                    if (!shared && b + 2 * kFp8StageCols >= N) drained();
+                    meet();
+                    copy_out(t0);
                 }
+                if (!shared && half * kFp8StageCols >= N) drained();
             }
             rd.advance(p.nd);
         }
@@ -719,9 +775,9 @@ static Fp8Plan fp8_plan(int form, int rows, int n, int red, int x_type, int o_ty
         l.a_bytes = kBlockRows * 128;
         l.b_rows = form == kFp8Dw ? kBlockRows : l.tile_cols / 2;
         const size_t pitch = gated ? 64 * o_bytes + 16 : kBlockRows * o_bytes + (o_bytes == 2 ? 16 : 0);
-        fixed = kFp8StageCols * pitch;
+        fixed = 2 * kFp8StageCols * pitch;
         l.z_offset = (int)fixed;
-        if (with_z) fixed += kFp8StageCols * (kBlockRows * 2 + 16);
+        if (with_z) fixed += 2 * kFp8StageCols * (kBlockRows * 2 + 16);
     }
     l.col_tiles = div_up(n, l.width);
     const int fold = 1 << l.fold_log, units = div_up(blocks, fold);
@@ -731,7 +787,7 @@ static Fp8Plan fp8_plan(int form, int rows, int n, int red, int x_type, int o_ty
     // Tokens that the CTAs quantize themselves: one round of the quantizing warps, and shared memory left for stages enough.
     const int rows8 = div_up(n, 8) * 8;
     const size_t resident = (size_t)units * rows8 * fold * 128 + 256 * (size_t)div_up(units, 4);
-    l.resident = l.cg == 1 && x_type != TUNA_FP8 && (long long)div_up(units * fold, 2) * n <= kFp8ResidentLoads * (kFp8Warps - 1) && resident + 4 * (size_t)l.a_bytes + fixed <= room;
+    l.resident = l.cg == 1 && x_type != TUNA_FP8 && (long long)div_up(units * fold, 2) * n <= kFp8ResidentLoads * (fp8_warps(1) - 1) && resident + 4 * (size_t)l.a_bytes + fixed <= room;
     if (l.resident) {
         l.b_rows = rows8;
         if (l.fold_log) l.d_cols = rows8 * fold;
@@ -775,7 +831,7 @@ static int launch_fp8(const Fp8Params &p, const Fp8Maps &maps, int ctas, size_t 
     }
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((unsigned)ctas);
-    lc.blockDim = dim3(32 * kFp8Warps);
+    lc.blockDim = dim3(32 * fp8_warps(CG));
     lc.dynamicSmemBytes = smem;
     lc.stream = stream;
     cudaLaunchAttribute attr[2];
@@ -821,6 +877,7 @@ static int launch_fp8_form(int form, const Fp8Codes &a, int rows, const Fp8Codes
     p.group_rows = l.group_rows; p.groups = rows / l.group_rows; p.flex = l.flex;
     p.a_bytes = l.a_bytes; p.b_rows = l.b_rows; p.stages = l.stages; p.nd = l.nd; p.d_cols = l.d_cols; p.d_step = l.d_step; p.sf_col = l.sf_col;
     p.ahead = form <= kFp8GatedProduct && cols <= kFp8AheadTokens;
+    p.stagger = form <= kFp8GatedProduct && !l.fold_log;
     p.x_bf16 = x_type == TUNA_BF16; p.gelu = gelu; p.z_offset = l.z_offset;
     p.status = device_status_word();
     if (!p.status) return TUNA_ERR_NO_DEVICE;

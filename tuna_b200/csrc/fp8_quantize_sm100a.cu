@@ -91,65 +91,154 @@ cudaError_t launch_fp8_quantize_rows(const void *x, int type, long long row_stri
 
 // ---- tiles of 128 x 128: blocks of a column, of a row and a column, square ones
 
+// A warp has 16 rows of the tile, a lane eight of them (every second) and eight columns: 16 lanes are a row's block.  All of a lane's numbers are loaded before
+// the first is used.
 constexpr int kFp8TileWarps = 8;
-constexpr int kFp8TileRows = kFp8Block / kFp8TileWarps;  // rows of a warp, four columns of a lane
+constexpr int kFp8TileRows = kFp8Block / kFp8TileWarps;
+constexpr int kFp8LaneRows = kFp8TileRows / 2;
 
-// Four numbers side by side, as fp32; coherent loads that keep out of L1 (a gated block's gradients are read twice, by tiles far apart).
-__device__ __forceinline__ float4 fp8_load4(const __half *p)
-{
-    uint2 v;
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
-    const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&v.x)), b = __half22float2(*reinterpret_cast<const __half2 *>(&v.y));
-    return make_float4(a.x, a.y, b.x, b.y);
-}
-__device__ __forceinline__ float4 fp8_load4(const __nv_bfloat16 *p)
-{
-    uint2 v;
-    asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p) : "memory");
-    return make_float4(__uint_as_float(v.x << 16), __uint_as_float(v.x & 0xffff0000u), __uint_as_float(v.y << 16), __uint_as_float(v.y & 0xffff0000u));
-}
-__device__ __forceinline__ float4 fp8_load4(const float *p)
-{
-    float4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
-    return v;
-}
+__device__ __forceinline__ uint32_t fp8_magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }  // compare as the numbers do, NaN above infinity
 
-// Where a tile's numbers come from.
+// A lane's numbers as they were loaded, the bits (fp32) of their largest magnitudes, and their values.
+template <typename T>
+struct Fp8Raw {  // 16 bits: maxima in pairs
+    Mx8<T> v[kFp8LaneRows];
+    using Pair = decltype(v[0].pair(0));
+    __device__ __forceinline__ static Pair largest(Pair a, Pair b) { return __hmax2_nan(a, __habs2(b)); }
+    __device__ __forceinline__ static uint32_t bits(Pair p)
+    {
+        const float2 f = widen(p);
+        return max(fp8_magnitude(f.x), fp8_magnitude(f.y));
+    }
+    __device__ __forceinline__ static float2 widen(__half2 p) { return __half22float2(p); }
+    __device__ __forceinline__ static float2 widen(__nv_bfloat162 p) { return __bfloat1622float2(p); }
+    __device__ __forceinline__ uint32_t row_max(int r) const
+    {
+        Pair m = largest(largest(__habs2(v[r].pair(0)), v[r].pair(1)), __hmax2_nan(__habs2(v[r].pair(2)), __habs2(v[r].pair(3))));
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+        return bits(m);
+    }
+    __device__ __forceinline__ void col_max(uint32_t (&m)[8]) const  // of the warp's 16 rows
+    {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            Pair p = __habs2(v[0].pair(i));
+#pragma unroll
+            for (int r = 1; r < kFp8LaneRows; ++r) p = largest(p, v[r].pair(i));
+            p = __hmax2_nan(p, __shfl_xor_sync(0xffffffffu, p, 16));
+            const float2 f = widen(p);
+            m[2 * i] = fp8_magnitude(f.x);
+            m[2 * i + 1] = fp8_magnitude(f.y);
+        }
+    }
+    __device__ __forceinline__ void values(int r, float (&f)[8]) const { v[r].values(f); }
+};
+struct Fp8RawFloat {
+    float v[kFp8LaneRows][8];
+    __device__ __forceinline__ uint32_t row_max(int r) const
+    {
+        uint32_t m = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, fp8_magnitude(v[r][i]));
+#pragma unroll
+        for (int d = 1; d < 16; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+        return m;
+    }
+    __device__ __forceinline__ void col_max(uint32_t (&m)[8]) const
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            m[i] = 0;
+#pragma unroll
+            for (int r = 0; r < kFp8LaneRows; ++r) m[i] = max(m[i], fp8_magnitude(v[r][i]));
+            m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], 16));
+        }
+    }
+    __device__ __forceinline__ void values(int r, float (&f)[8]) const
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = v[r][i];
+    }
+};
+template <> struct Fp8Raw<float> : Fp8RawFloat {};
+
+// Where a tile's numbers come from: rows row0, row0 + 2 .. of columns col .. col + 7.
 template <typename T>
 struct Fp8Plain {
     const T *x;
     long long row_stride;
-    __device__ __forceinline__ float4 load(long long row, int col) const { return fp8_load4(x + row * row_stride + col); }
+    using Raw = Fp8Raw<T>;
+    __device__ __forceinline__ void load(Raw &to, long long row0, int col, int rows, int cols) const
+    {
+#pragma unroll
+        for (int r = 0; r < kFp8LaneRows; ++r) {
+            const bool in = col < cols && row0 + 2 * r < rows;
+            const T *at = x + (row0 + 2 * r) * row_stride + col;
+            if constexpr (sizeof(T) == 2) {
+                if (in) to.v[r].load(at);
+                else to.v[r].zero();
+            } else {
+                Mx8<float> v;
+                if (in) v.load(at);
+                else v.zero();
+                v.values(to.v[r]);
+            }
+        }
+    }
 };
 // Columns 0 .. f - 1: the gradient of a gated block's gate, dh u act'(g); f .. 2f - 1: of the other projection, dh act(g).  z = [g | u].
 template <typename T, bool GELU>
 struct Fp8Gated {
     const T *z, *dh;
     int f;
-    __device__ __forceinline__ float4 load(long long row, int col) const
+    using Raw = Fp8RawFloat;
+    __device__ __forceinline__ void load(Raw &to, long long row0, int col, int rows, int cols) const
     {
+        constexpr int kBatch = 4;  // rows in flight
         const bool gate = col < f;
-        const int at = gate ? col : col - f;  // f is a multiple of 16: four columns are of one kind
-        const T *zr = z + row * 2 * f + at;
-        const float4 g = fp8_load4(zr), d = fp8_load4(dh + row * f + at), u = gate ? fp8_load4(zr + f) : g;
-        auto one = [&](float g, float u, float d) {
-            const float sigma = fp8_gate<GELU>(g);
-            return gate ? d * u * fp8_gate_slope<GELU>(g, sigma) : d * (g * sigma);
-        };
-        return make_float4(one(g.x, u.x, d.x), one(g.y, u.y, d.y), one(g.z, u.z, d.z), one(g.w, u.w, d.w));
+        const int at = gate ? col : col - f;  // f is a multiple of 16: eight columns are of one kind
+#pragma unroll
+        for (int r0 = 0; r0 < kFp8LaneRows; r0 += kBatch) {
+            Mx8<T> g[kBatch], u[kBatch], d[kBatch];
+#pragma unroll
+            for (int r = 0; r < kBatch; ++r) {
+                const long long row = row0 + 2 * (r0 + r);
+                const bool in = col < cols && row < rows;
+                const T *zr = z + row * 2 * f + at;
+                if (in) {
+                    g[r].load(zr);
+                    d[r].load(dh + row * f + at);
+                } else {
+                    g[r].zero();
+                    d[r].zero();
+                }
+                if (in && gate) u[r].load(zr + f);
+                else u[r].zero();
+            }
+#pragma unroll
+            for (int r = 0; r < kBatch; ++r) {
+                float gv[8], uv[8], dv[8];
+                g[r].values(gv);
+                u[r].values(uv);
+                d[r].values(dv);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float sigma = fp8_gate<GELU>(gv[i]);
+                    to.v[r0 + r][i] = gate ? dv[i] * uv[i] * fp8_gate_slope<GELU>(gv[i], sigma) : dv[i] * (gv[i] * sigma);
+                }
+            }
+        }
     }
 };
 
-__device__ __forceinline__ uint32_t fp8_magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-// bits of magnitudes compare as the numbers do, NaN above infinity
-
 template <int WAYS, typename Source>  // WAYS: 1 << kFp8Row | 1 << kFp8Column, one of them, or 1 << kFp8Square
-__global__ void __launch_bounds__(32 * kFp8TileWarps)
+__global__ void __launch_bounds__(32 * kFp8TileWarps, sizeof(typename Source::Raw) <= 128 ? 3 : 2)
 fp8_quantize_tile_kernel(const Source src, uint8_t *q, uint8_t *s, uint8_t *q2, uint8_t *s2, int rows, int cols, bool two_halves, bool chained)
 {
     constexpr bool kRows = WAYS & (1 << kFp8Row), kCols = WAYS & (1 << kFp8Column), kSquare = WAYS & (1 << kFp8Square);
-    __shared__ uint4 s_max[kFp8TileWarps][32];
+    __shared__ uint4 s_max[kFp8TileWarps][32];   // of a warp's rows, column by column
+    __shared__ uint32_t s_scale[kFp8Block];
     if (chained) {
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -158,76 +247,90 @@ fp8_quantize_tile_kernel(const Source src, uint8_t *q, uint8_t *s, uint8_t *q2, 
     const int col_tiles = gridDim.x, row_tiles = div_up(rows, kFp8Block);
     // Halves of the columns that read the same: tile t of the one and of the other follow one another, so that L2 has it.
     const int ct = !two_halves ? blockIdx.x : (blockIdx.x & 1) ? (col_tiles + 1) / 2 + (blockIdx.x >> 1) : blockIdx.x >> 1;
-    const int col = ct * kFp8Block + lane * 4;
-    const bool in = col < cols;
+    const int col = ct * kFp8Block + (lane & 15) * 8;
     for (int rt = blockIdx.y; rt < row_tiles; rt += gridDim.y) {
-        const long long row0 = (long long)rt * kFp8Block + warp * kFp8TileRows;
-        float v[kFp8TileRows][4];
-#pragma unroll
-        for (int r = 0; r < kFp8TileRows; ++r) {
-            const float4 a = in && row0 + r < rows ? src.load(row0 + r, col) : make_float4(0, 0, 0, 0);
-            v[r][0] = a.x; v[r][1] = a.y; v[r][2] = a.z; v[r][3] = a.w;
-        }
-        auto write = [&](uint8_t *to, int r, const float (&inverse)[4], const bool (&none)[4]) {
-            uint32_t w = fp8_encode4(v[r][0] * inverse[0], v[r][1] * inverse[1], v[r][2] * inverse[2], v[r][3] * inverse[3]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (none[i]) w &= ~(0xffu << (8 * i));
-            if (in && row0 + r < rows) *reinterpret_cast<uint32_t *>(to + (row0 + r) * cols + col) = w;
+        const long long row0 = (long long)rt * kFp8Block + warp * kFp8TileRows + (lane >> 4);
+        typename Source::Raw raw;
+        src.load(raw, row0, col, rows, cols);
+        auto write = [&](uint8_t *to, int r, uint32_t lo, uint32_t hi) {
+            if (col < cols && row0 + 2 * r < rows) *reinterpret_cast<uint2 *>(to + (row0 + 2 * r) * cols + col) = make_uint2(lo, hi);
         };
         if constexpr (kRows) {
-            uint32_t mine = 0;
+            uint32_t mine = 0;  // of row lane % 16 of the lane's
 #pragma unroll
-            for (int r = 0; r < kFp8TileRows; ++r) {
-                uint32_t m = max(max(fp8_magnitude(v[r][0]), fp8_magnitude(v[r][1])), max(fp8_magnitude(v[r][2]), fp8_magnitude(v[r][3])));
-                m = __reduce_max_sync(0xffffffffu, m);
-                const uint32_t e = fp8_scale(m);
+            for (int r = 0; r < kFp8LaneRows; ++r) {
+                const uint32_t e = fp8_scale(raw.row_max(r));
                 const float i = fp8_inverse(e);
-                const bool n = e == 255u;
-                write(q, r, {i, i, i, i}, {n, n, n, n});
-                if (lane == r) mine = e;
+                float f[8];
+                raw.values(r, f);
+                const uint32_t lo = fp8_encode4(f[0] * i, f[1] * i, f[2] * i, f[3] * i), hi = fp8_encode4(f[4] * i, f[5] * i, f[6] * i, f[7] * i);
+                write(q, r, e == 255u ? 0u : lo, e == 255u ? 0u : hi);
+                if ((lane & 15) == r) mine = e;
             }
-            if (lane < kFp8TileRows && row0 + lane < rows) {
-                uint8_t *at = s + ((long long)(ct >> 2) * rows + row0 + lane) * 4 + (ct & 3);
+            const long long row = row0 + 2 * (lane & 15);
+            if ((lane & 15) < kFp8LaneRows && row < rows) {
+                uint8_t *at = s + ((long long)(ct >> 2) * rows + row) * 4 + (ct & 3);
                 *at = (uint8_t)mine;
                 if (ct + 1 == col_tiles)
                     for (int i = 1; i < 4 - (ct & 3); ++i) at[i] = 0;
             }
         }
         if constexpr (kCols || kSquare) {
-            uint4 m = make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int r = 0; r < kFp8TileRows; ++r) {
-                m.x = max(m.x, fp8_magnitude(v[r][0]));
-                m.y = max(m.y, fp8_magnitude(v[r][1]));
-                m.z = max(m.z, fp8_magnitude(v[r][2]));
-                m.w = max(m.w, fp8_magnitude(v[r][3]));
-            }
-            if constexpr (kSquare) m.x = __reduce_max_sync(0xffffffffu, max(max(m.x, m.y), max(m.z, m.w)));
-            __syncthreads();  // what was there before has been read
-            s_max[warp][lane] = m;
-            __syncthreads();
-#pragma unroll
-            for (int w = 0; w < kFp8TileWarps; ++w) {
-                const uint4 o = s_max[w][lane];
-                m = make_uint4(max(m.x, o.x), max(m.y, o.y), max(m.z, o.z), max(m.w, o.w));
-            }
-            uint8_t *to = kRows ? q2 : q, *words = kRows ? s2 : s;
-            const uint32_t e[4] = {fp8_scale(m.x), kSquare ? fp8_scale(m.x) : fp8_scale(m.y), kSquare ? fp8_scale(m.x) : fp8_scale(m.z), kSquare ? fp8_scale(m.x) : fp8_scale(m.w)};
-            const float inverse[4] = {fp8_inverse(e[0]), fp8_inverse(e[1]), fp8_inverse(e[2]), fp8_inverse(e[3])};
-            const bool none[4] = {e[0] == 255u, e[1] == 255u, e[2] == 255u, e[3] == 255u};
-#pragma unroll
-            for (int r = 0; r < kFp8TileRows; ++r) write(to, r, inverse, none);
+            uint32_t m[8];
+            raw.col_max(m);
             if constexpr (kSquare) {
-                if (threadIdx.x == 0) words[(long long)rt * col_tiles + ct] = (uint8_t)e[0];
-            } else if (warp == 0 && in) {
+                m[0] = max(max(max(m[0], m[1]), max(m[2], m[3])), max(max(m[4], m[5]), max(m[6], m[7])));
+                m[0] = __reduce_max_sync(0xffffffffu, m[0]);
+            }
+            if (rt != (int)blockIdx.y) __syncthreads();  // what was there before has been read
+            if constexpr (kSquare) {
+                if (lane == 0) s_scale[warp] = m[0];
+            } else if (lane < 16) {
+                s_max[warp][2 * lane] = make_uint4(m[0], m[1], m[2], m[3]);
+                s_max[warp][2 * lane + 1] = make_uint4(m[4], m[5], m[6], m[7]);
+            }
+            __syncthreads();
+            uint8_t *to = kRows ? q2 : q, *words = kRows ? s2 : s;
+            uint32_t e[8];
+            if constexpr (kSquare) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint8_t *at = words + ((long long)(rt >> 2) * cols + col + i) * 4 + (rt & 3);
-                    *at = (uint8_t)e[i];
-                    if (rt + 1 == row_tiles)
-                        for (int j = 1; j < 4 - (rt & 3); ++j) at[j] = 0;
+                for (int w = 0; w < kFp8TileWarps; ++w) m[0] = max(m[0], s_scale[w]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) e[i] = fp8_scale(m[0]);
+                if (threadIdx.x == 0) words[(long long)rt * col_tiles + ct] = (uint8_t)e[0];
+            } else {
+                if (threadIdx.x < kFp8Block) {  // one column each
+                    uint32_t c = 0;
+#pragma unroll
+                    for (int w = 0; w < kFp8TileWarps; ++w) c = max(c, reinterpret_cast<const uint32_t *>(s_max[w])[threadIdx.x]);
+                    c = fp8_scale(c);
+                    s_scale[threadIdx.x] = c;
+                    const int at_col = ct * kFp8Block + threadIdx.x;
+                    if (at_col < cols) {
+                        uint8_t *at = words + ((long long)(rt >> 2) * cols + at_col) * 4 + (rt & 3);
+                        *at = (uint8_t)c;
+                        if (rt + 1 == row_tiles)
+                            for (int j = 1; j < 4 - (rt & 3); ++j) at[j] = 0;
+                    }
                 }
+                __syncthreads();
+                const uint4 a = *reinterpret_cast<const uint4 *>(s_scale + 8 * (lane & 15)), b = *reinterpret_cast<const uint4 *>(s_scale + 8 * (lane & 15) + 4);
+                e[0] = a.x; e[1] = a.y; e[2] = a.z; e[3] = a.w;
+                e[4] = b.x; e[5] = b.y; e[6] = b.z; e[7] = b.w;
+            }
+            float inverse[8];
+            uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                inverse[i] = fp8_inverse(e[i]);
+                if (e[i] == 255u) keep[i >> 2] &= ~(0xffu << (8 * (i & 3)));
+            }
+#pragma unroll
+            for (int r = 0; r < kFp8LaneRows; ++r) {
+                float f[8];
+                raw.values(r, f);
+                write(to, r, fp8_encode4(f[0] * inverse[0], f[1] * inverse[1], f[2] * inverse[2], f[3] * inverse[3]) & keep[0],
+                      fp8_encode4(f[4] * inverse[4], f[5] * inverse[5], f[6] * inverse[6], f[7] * inverse[7]) & keep[1]);
             }
         }
     }

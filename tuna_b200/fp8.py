@@ -16,19 +16,45 @@ The gradients are explicit calls, as everything here: none of them takes part in
 
 from __future__ import annotations
 
+import ctypes
+import functools
+
 import torch
 
 from . import _lib
 from ._lib import check
-from .mx import _expect_output, _expect_sizes
+from .mx import _expect_output, _expect_sizes, _launched
 from .ops import _expect, _on_device, _stream_ptr
 
 _TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _FP8 = 4
 _CODES = torch.float8_e4m3fn
 _BLOCKS = {"row": 0, "column": 1, "both": 2, "square": 3}
+_ONE_WAY = {b: c for b, c in _BLOCKS.items() if b != "both"}
 _ACTIVATIONS = {"silu": 0, "gelu": 1}
 _MATMUL, _GATED, _BACKWARD = 0, 1, 2
+
+
+class _NoFront:
+    """Where the native front is missing every call is checked here."""
+
+    @staticmethod
+    def _python_way(*args):
+        return False
+
+    fp8_quantize = fp8_dequant = fp8_matmul = fp8_matmul_backward = fp8_gated = fp8_gated_backward = _python_way
+
+
+@functools.lru_cache(maxsize=None)
+def _front():
+    """The native front (csrc/fast_call.cpp), which checks and launches the common calls, bound to the library."""
+    front = _lib.load_fast_call()
+    if front is None:
+        return _NoFront
+    lib = _lib.load()
+    front.bind_fp8(*(ctypes.cast(getattr(lib, "tuna_fp8_" + name), ctypes.c_void_p).value for name in
+                     ("quantize", "dequant", "matmul", "matmul_backward", "gated", "gated_backward", "workspace_bytes")))
+    return front
 
 
 def _scale_shape(rows: int, k: int, blocks: str):
@@ -88,6 +114,10 @@ def fp8_quantize(x, blocks: str = "row"):
     """`x` (fp16, bf16 or fp32, `[rows, k]`, whose rows may lie apart) -> codes and scales `(q, s)` of that kind of blocks, or, for `"both"`,
     `(q, s, q_column, s_column)` by row and by column in one pass."""
     kind = _choice(blocks, "blocks", _BLOCKS)
+    done = _front().fp8_quantize(x, kind)
+    if isinstance(done, tuple):
+        return done
+    _launched(done)
     if not isinstance(x, torch.Tensor) or not x.is_cuda:
         raise ValueError("x must be a CUDA tensor (there is no CPU path)")
     if x.dtype not in _TYPES:
@@ -116,7 +146,9 @@ def fp8_quantize(x, blocks: str = "row"):
 
 def fp8_dequant(q, s, o, m: int, k: int, blocks: str = "square") -> None:
     """The numbers of codes and scales, rounded once to o's type: o fp16, bf16 or fp32 `[m, k]`."""
-    kind = _choice(blocks, "blocks", {b: _BLOCKS[b] for b in ("row", "column", "square")})
+    kind = _choice(blocks, "blocks", _ONE_WAY)
+    if _launched(_front().fp8_dequant(q, s, o, m, k, kind)):
+        return
     _expect_sizes(m, k)
     _expect_codes(q, s, ("q", "s"), m, k, blocks)
     dev = q.device
@@ -130,6 +162,8 @@ def fp8_matmul(x, xs, q, s, o, m: int, n: int, k: int, *, workspace=None) -> Non
     one rounding.  x is codes with their scales `xs` (row blocks), or fp16 or bf16 with `xs=None`: the call quantizes it as `fp8_quantize` does.
     m and k multiples of 16.  Enqueued on the current stream of x's device, in whose order it reads and writes; only q and s, up to 64 tokens, count
     as constants and are read while the kernel before still drains, as in `mx_matmul`."""
+    if workspace is None and _launched(_front().fp8_matmul(x, xs, q, s, o, m, n, k)):
+        return
     _expect_sizes(m, n, k)
     kind = _tokens(x, xs, n, k, "row")
     dev = x.device
@@ -164,6 +198,8 @@ def fp8_matmul_backward(dy, x, xs, q, s, dx, dw, m: int, n: int, k: int, *, work
     wanted, and what only it needs may be None then (q and s; x and xs).  dy is quantized by row for dx and by column for dw; x `[n, k]` is
     fp16 or bf16 with `xs=None`, quantized by column, or codes with their scales of column blocks, which a forward pass may have kept
     (`fp8_quantize(x, "both")`).  m and k multiples of 16.  In the order of the current stream."""
+    if workspace is None and _launched(_front().fp8_matmul_backward(dy, x, xs, q, s, dx, dw, m, n, k)):
+        return
     _expect_sizes(m, n, k)
     dy_type = _expect_16bit(dy, "dy", n * m)
     dev = dy.device
@@ -181,6 +217,8 @@ def fp8_gated(x, xs, q, s, h, f: int, n: int, k: int, activation: str = "silu", 
     form.  z `[n, 2f]` of h's type (fp16 or bf16) keeps g and u, side by side, for `fp8_gated_backward`; h is made of g and u before they are
     rounded.  f and k multiples of 16."""
     act = _choice(activation, "activation", _ACTIVATIONS)
+    if workspace is None and _launched(_front().fp8_gated(x, xs, q, s, h, f, n, k, act, z)):
+        return
     _expect_sizes(2 * f, n, k)
     kind = _tokens(x, xs, n, k, "row")
     dev = x.device
@@ -197,6 +235,8 @@ def fp8_gated_backward(dh, z, x, xs, q, s, dx, dw, f: int, n: int, k: int, activ
     """The gradients of `fp8_gated` given dh `[n, f]` and z `[n, 2f]` (fp16 or bf16, one type): those of `fp8_matmul_backward`, dw `[2f, k]`, for
     dy = [dh u activation'(g) | dh activation(g)], which is made and quantized in one pass and never stored in 16 bits."""
     act = _choice(activation, "activation", _ACTIVATIONS)
+    if workspace is None and _launched(_front().fp8_gated_backward(dh, z, x, xs, q, s, dx, dw, f, n, k, act)):
+        return
     _expect_sizes(2 * f, n, k)
     kind16 = _expect_16bit(dh, "dh", n * f)
     dev = dh.device
