@@ -81,10 +81,7 @@ struct Fp8Params {
     int b_rows;      // rows of B in a stage of a CTA (MN-major: 128)
     int stages;
     int last_steps;  // MMAs of the last block: 32 each
-    int nd;          // accumulators that are free of one another
-    int d_cols;      // tensor-memory columns of an accumulator: columns of a tile times fold
-    int d_step;      // where the second one starts
-    int sf_col;      // where the two buffers of scales start
+    int d_cols;      // tensor-memory columns of each of the two accumulators: columns of a tile times fold
     int ahead;       // A is there before the dependency wait
     int x_bf16;      // RESIDENT: type of the tokens
     const void *x;   // RESIDENT: the tokens [cols][red]
@@ -212,7 +209,7 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
     __shared__ int s_abort;
 
     constexpr bool kGated = FORM == kFp8GatedProduct, kAcrossA = FORM >= kFp8Dx, kAcrossB = FORM == kFp8Dw;
-    constexpr uint32_t kTmemCols = CG == 1 ? 256 : 512;
+    constexpr uint32_t kTmemCols = CG == 1 ? 256 : 512, kSfCol = kTmemCols - 2 * kFp8SfCols;  // two accumulators below
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = CG == 1 ? 0 : (int)cluster_ctarank();
     const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
@@ -283,7 +280,6 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
             depend();
             Ring ru, rd, rs;
             bool ok = true;
-            int second = 0;  // which accumulator
             // -------------------------------------------------------------- MMA issue
             // Rows, or along the sum for what is read across, by eights 1024 bytes apart, version 1, 128-byte swizzle.  Read across, an MMA's 32 are 32
             // staged rows of 128 bytes, otherwise 32 of a row's 128 bytes.
@@ -292,8 +288,7 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
             while (ok && tile.next(p)) {
                 const uint32_t idesc = fp8_idesc<CG>(p.fold_log ? p.d_cols : mma_cols(), kAcrossA, kAcrossB);
                 ok = mbar_wait_warp(d_empty + 8 * rd.idx, rd.phase ^ 1, abort_flag, p.status, 303);
-                const uint32_t d = tmem + (uint32_t)(second * p.d_step);
-                second ^= 1;
+                const uint32_t d = tmem + (uint32_t)(rd.idx * p.d_cols);
                 Fp8Stages st(p, tile.first_group(p, groups));
                 for (int i = 0; ok && i < p.units; ++i, st.advance()) {
                     const int c = st.c;
@@ -305,7 +300,7 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
                     if (elect_one_sync()) {
                         const uint64_t a = sw128 | (uint64_t)(((base + (uint32_t)ru.idx * a_bytes) & 0x3FFFFu) >> 4);
                         const uint64_t b = sw128 | (uint64_t)(((b_ring + (uint32_t)(RESIDENT ? c : ru.idx) * b_bytes) & 0x3FFFFu) >> 4);
-                        const uint32_t sfa = tmem + (uint32_t)(p.sf_col + rs.idx * kFp8SfCols), sfb = sfa + 8;
+                        const uint32_t sfa = tmem + kSfCol + (uint32_t)(rs.idx * kFp8SfCols), sfb = sfa + 8;
                         const int steps = c + 1 == p.units && !p.fold_log ? p.last_steps : 4;
                         const uint32_t id = idesc | ((uint32_t)(c & 3) << 29) | ((uint32_t)(c & 3) << 4);
 #pragma unroll
@@ -325,7 +320,7 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
                     ru.advance(S);
                     if (group_ends) rs.advance(2);
                 }
-                rd.advance(p.nd);
+                rd.advance(2);
             }
         }
     } else if (warp == 1) {
@@ -398,7 +393,7 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
     } else if (warp >= kFp8ScaleWarp0 && warp < kFp8ScaleWarp0 + 4) {
         // ------------------------------------------------------------------ scales to tensor memory
         const int quarter = warp - kFp8ScaleWarp0;
-        const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + (uint32_t)p.sf_col;
+        const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + kSfCol;
         const uint32_t leader_full = CG == 1 ? sf_full : map_to_rank(sf_full, 0);
         const int a_blocks = div_up(p.rows, kFp8Block);
         // Of a group, as loaded: A's words (dw) or, spread over the lanes, its bytes; B's words or (folded) bytes of two.  They are put together when the group
@@ -627,12 +622,11 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
                 }
             }
         };
-        int second = 0;
-        for (; tile.next(p); second ^= 1) {
+        while (tile.next(p)) {
             const bool ok = mbar_wait_warp(d_full + 8 * rd.idx, rd.phase, abort_flag, p.status, 307);
             if (bar_any(1 + 2 * half, 128, !ok)) break;  // the group's four warps go on together or not at all
             tc_fence_after();
-            const uint32_t d = tmem_q + (uint32_t)(second * p.d_step);
+            const uint32_t d = tmem_q + (uint32_t)(rd.idx * p.d_cols);
             row0 = fp8_row(p, CG * tile.rt + rank);
             rows = max(0, min(p.flex ? fp8_row(p, CG * tile.rt + rank + 1) : row0 + kBlockRows, p.rows) - row0);
             if constexpr (CG == 1) {
@@ -677,23 +671,16 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
                     meet();  // they have been read
                 }
             } else {
-                // Of two accumulators that overlap, the columns they share first (32 of them, the first group's): then the other one may be written, which both
-                // groups have read by now.
-                const bool shared = p.nd == 1;
-                const int turn = shared && second == 0 ? p.d_step : 0;
-                if (shared && half == 1) drained();
-                for (int b = half * kFp8StageCols; b < N; b += 2 * kFp8StageCols) {
-                    const int t0 = b + turn < N ? b + turn : b + turn - N;
+                for (int t0 = half * kFp8StageCols; t0 < N; t0 += 2 * kFp8StageCols) {
                     meet();  // what was staged before has been copied
                     if (t0 < tile.valid) fill_from(d, t0);
-                    if (shared && b == 0) drained();
-                    if (!shared && b + 2 * kFp8StageCols >= N) drained();
+                    if (t0 + 2 * kFp8StageCols >= N) drained();
                     meet();
                     copy_out(t0);
                 }
-                if (!shared && half * kFp8StageCols >= N) drained();
+                if (half * kFp8StageCols >= N) drained();
             }
-            rd.advance(p.nd);
+            rd.advance(2);
         }
     }
 
@@ -711,7 +698,7 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
 // ------------------------------------------------------------------ host side
 
 struct Fp8Plan {
-    int cg, tile_cols, width, col_tiles, stages, nd, d_cols, d_step, sf_col;
+    int cg, tile_cols, width, col_tiles, stages, d_cols;
     bool resident;
     int flex, fold_log, group_rows, row_tiles, a_bytes, b_rows, z_offset;
     int workers;
@@ -734,12 +721,13 @@ static double fp8_pair_us(int rows, int n, int red, int cols, int pairs)
 
 static int fp8_pair_cols(int rows, int n, int red, int form, int pairs)
 {
-    static const int widths[] = {256, 224, 192, 160, 128, 96, 64, 32, 16, 0};  // of dw all but the last: what a CTA stages starts at a multiple of 16 columns
+    // Two accumulators and two buffers of scales fill tensor memory with 240.  Of dw multiples of 32: what a CTA stages starts at a multiple of 16 columns
+    static const int widths[] = {240, 224, 208, 192, 176, 160, 144, 128, 112, 96, 80, 64, 48, 32, 16, 0};
     int best = 0;
     double best_us = 0;
     for (int i = 0; widths[i]; ++i) {
         const int cols = widths[i];
-        if (form == kFp8Dw && cols < 32) break;
+        if (form == kFp8Dw && cols % 32) continue;
         if (best && div_up(n, div_up(n, cols)) <= widths[i + 1]) continue;  // the next narrower one holds the same tiles
         const double us = fp8_pair_us(rows, n, red, cols, pairs);
         if (!best || us < best_us) best = cols, best_us = us;
@@ -795,11 +783,6 @@ static Fp8Plan fp8_plan(int form, int rows, int n, int red, int x_type, int o_ty
         b_stage = 0;
     }
     l.stages = (int)std::min<size_t>(kFp8MaxStages, (room - fixed) / (l.a_bytes + b_stage));
-    const int tmem_cols = (l.cg == 1 ? 256 : 512) - 2 * kFp8SfCols;
-    // Two accumulators, which share the columns in the middle where two whole ones do not fit
-    l.nd = 2 * l.d_cols <= tmem_cols ? 2 : 1;
-    l.d_step = l.nd == 2 ? l.d_cols : tmem_cols - l.d_cols;
-    l.sf_col = tmem_cols;
     // the last stage's MMAs read 128 rows
     l.smem = std::max((size_t)l.stages * (l.a_bytes + b_stage) + fixed, (size_t)(l.stages - 1) * l.a_bytes + kBlockRows * 128);
     return l;
@@ -875,7 +858,7 @@ static int launch_fp8_form(int form, const Fp8Codes &a, int rows, const Fp8Codes
     p.tile_cols = l.tile_cols; p.width = l.width; p.row_tiles = l.row_tiles; p.col_tiles = l.col_tiles;
     p.rows_inner = l.row_tiles < l.col_tiles;
     p.group_rows = l.group_rows; p.groups = rows / l.group_rows; p.flex = l.flex;
-    p.a_bytes = l.a_bytes; p.b_rows = l.b_rows; p.stages = l.stages; p.nd = l.nd; p.d_cols = l.d_cols; p.d_step = l.d_step; p.sf_col = l.sf_col;
+    p.a_bytes = l.a_bytes; p.b_rows = l.b_rows; p.stages = l.stages; p.d_cols = l.d_cols;
     p.ahead = form <= kFp8GatedProduct && cols <= kFp8AheadTokens;
     p.stagger = form <= kFp8GatedProduct && !l.fold_log;
     p.x_bf16 = x_type == TUNA_BF16; p.gelu = gelu; p.z_offset = l.z_offset;
