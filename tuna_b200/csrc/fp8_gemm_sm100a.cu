@@ -50,12 +50,13 @@ __host__ __device__ constexpr int fp8_warps(int cg) { return cg == 1 ? 12 : 16; 
 constexpr int kFp8EpilogueWarp0 = 4;
 constexpr int kFp8ScaleWarp0 = 8;
 constexpr int kFp8MaxStages = 12;
-constexpr int kFp8DirectCols = 16;        // tokens up to which single CTAs take the tiles
+constexpr int kFp8Deep = 2;               // units of a stage: what a wait, a commit and the turn of the issuing warp cost is paid once for eight MMAs
+constexpr int kFp8SingleCols = 16;        // tokens up to which single CTAs may take the tiles
 constexpr int kFp8StageCols = 32;         // columns of a group's output staging buffer
 constexpr int kFp8AheadTokens = 64;       // up to here weights count as constants and are copied ahead of the dependency wait, as in mx_gemm_sm100a.cu
 constexpr int kFp8ResidentLoads = 4;      // loads in flight of a quantizing warp
 constexpr int kFp8SfCols = 16;            // tensor-memory columns of a group's scales: A's words at 0 to 3, B's at 8 to 15
-constexpr uint32_t kFp8FoldBytes = kFp8DirectCols * kBlockRows * 4;
+constexpr uint32_t kFp8SumBytes = kFp8SingleCols * kBlockRows * 4;  // where the parts of a folded tile, or a gated one's projections, meet
 constexpr int kFp8SmemMax = 225 * 1024;   // dynamic shared memory of a CTA alone on its SM (1 KB is the kernel's static part, 1 KB the system's)
 constexpr int kFp8SmemHalf = 111 * 1024;  // of one that leaves room for another
 
@@ -68,19 +69,16 @@ struct Fp8Params {
     int cols;        // of B
     int red;         // what is summed over
     int blocks;      // ceil(red / 128)
-    int units;       // stages of a tile: ceil(blocks / fold)
-    int fold_log;    // log2(fold): blocks side by side in a stage
+    int units;       // of a tile: ceil(blocks / fold), four MMAs each
+    int fold_log;    // log2(fold): blocks side by side in a unit
+    int steps;       // stages of a tile: ceil(units / kFp8Deep)
     int tile_cols;   // N
     int width;       // columns of a tile, all but the last
     int row_tiles, col_tiles;
     int rows_inner;  // tiles follow one another along the rows
-    int group_rows;  // rows of a tile come in groups of 8, gated 16: eight features
-    int groups;
-    int flex;        // row tiles of equal height: tile t has the groups t * groups / row_tiles up to the next tile's
-    int a_bytes;     // of a stage of A
-    int b_rows;      // rows of B in a stage of a CTA (MN-major: 128)
+    int a_bytes;     // of a unit of A
+    int b_rows;      // rows of B in a unit of a CTA (MN-major: 128)
     int stages;
-    int last_steps;  // MMAs of the last block: 32 each
     int d_cols;      // tensor-memory columns of each of the two accumulators: columns of a tile times fold
     int ahead;       // A is there before the dependency wait
     int x_bf16;      // RESIDENT: type of the tokens
@@ -103,18 +101,20 @@ struct Fp8Tiles {
         next_tile += step;
         return true;
     }
-    // Stages come in groups of four (one word of scales); a tile starts with this one and goes round.
+    // Units come in groups of four (one word of scales); a tile starts with this one and goes round.
     __device__ int first_group(const Fp8Params &p, int groups) const { return p.stagger ? rt % groups : 0; }
     __device__ int total(const Fp8Params &p) const { const int n = p.row_tiles * p.col_tiles; return next_tile < n ? (n - 1 - next_tile) / step + 1 : 0; }
 };
 
-// The stages of a tile in order.
+// The stages of a tile in order: `c` is a stage's first unit, and it has those before `end`.
 struct Fp8Stages {
     int c, units;
     __device__ Fp8Stages(const Fp8Params &p, int first_group) : c(4 * first_group), units(p.units) {}
+    __device__ int end() const { return min(c + kFp8Deep, units); }
     __device__ void advance()
     {
-        if (++c == units) c = 0;
+        c += kFp8Deep;
+        if (c >= units) c = 0;
     }
 };
 
@@ -151,11 +151,13 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map
                  : "memory");
 }
 
-// First row of row block b (a CTA's share of a tile).
-__device__ __forceinline__ int fp8_row(const Fp8Params &p, int b) { return p.flex ? p.group_rows * (int)((long long)b * p.groups / p.row_tiles) : b * kBlockRows; }
+// First row of row block b (a CTA's share of a tile).  Single CTAs: blocks of equal height, a multiple of four rows.  Gated: twice the first feature.
+template <int CG>
+__device__ __forceinline__ int fp8_row(const Fp8Params &p, int b) { return CG == 1 ? 4 * (int)((long long)b * (p.rows / 4) / p.row_tiles) : b * kBlockRows; }
 
-// Quantizes the tokens' numbers, all of K: warp `w` of `warps` takes every warps-th (two blocks, token).  Codes as TMA would have put them (128-byte
-// swizzle); scale bytes in words [group of four stages][64 columns: token of a block of the stage].
+// Quantizes the tokens' numbers, all of K: warp `w` of `warps` takes every warps-th (two blocks, token).  Codes by 16 bytes, [block][piece of 16 columns][token]: the MMAs
+// read eight tokens from there, of which those behind the last are the next pieces' and give columns that nobody reads, so that a token takes no more room than its
+// codes.  Scale bytes in words [group of four units][64 columns: token of a block of the unit].
 template <typename T>
 __device__ __forceinline__ void fp8_quantize_resident(const Fp8Params &p, int w, int warps, int lane, uint32_t codes_at, uint32_t words_at)
 {
@@ -184,9 +186,7 @@ __device__ __forceinline__ void fp8_quantize_resident(const Fp8Params &p, int w,
             uint32_t lo = fp8_encode4(f[0], f[1], f[2], f[3]), hi = fp8_encode4(f[4], f[5], f[6], f[7]);
             if (e == 255u) lo = hi = 0;
             if (b >= limit) continue;
-            // 16-byte piece (lane % 16) / 2 of the token's 128 bytes, XORed with the token's number mod 8
-            const uint32_t piece = (((uint32_t)lane >> 1) & 7u) ^ ((uint32_t)t & 7u);
-            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(codes_at + ((uint32_t)b * (uint32_t)p.b_rows + (uint32_t)t) * 128u + (piece << 4) + ((uint32_t)lane & 1u) * 8u),
+            asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(codes_at + ((uint32_t)(8 * b + ((lane >> 1) & 7)) * (uint32_t)p.cols + (uint32_t)t) * 16u + ((uint32_t)lane & 1u) * 8u),
                          "r"(lo), "r"(hi)
                          : "memory");
             const int unit = b >> p.fold_log, at = (b - (unit << p.fold_log)) * p.b_rows + t;
@@ -216,9 +216,9 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
     const int N = p.tile_cols, S = p.stages;
     // [stages of A][of B][words of the resident tokens' scales][staging buffer]; the MMAs read 128 rows of A, in low tiles past their stage's end.
     // RESIDENT: of B, all of a tile's stages.
-    const int b_stages = RESIDENT ? p.units : S, groups = (p.units + 3) >> 2;
-    const uint32_t base = smem_u32(smem), a_bytes = (uint32_t)p.a_bytes, b_bytes = (uint32_t)(p.b_rows << p.fold_log) * 128u;
-    const uint32_t b_ring = base + (uint32_t)S * a_bytes, words_at = b_ring + (uint32_t)b_stages * b_bytes, staging = words_at + (RESIDENT ? 256u * (uint32_t)groups : 0u);
+    const int b_units = RESIDENT ? p.units : S * kFp8Deep, groups = (p.units + 3) >> 2;
+    const uint32_t base = smem_u32(smem), a_bytes = (uint32_t)p.a_bytes, b_bytes = (uint32_t)((RESIDENT ? p.cols : p.b_rows) << p.fold_log) * 128u;  // of a unit
+    const uint32_t b_ring = base + (uint32_t)(S * kFp8Deep) * a_bytes, words_at = b_ring + (uint32_t)b_units * b_bytes, staging = words_at + (RESIDENT ? 256u * (uint32_t)groups : 0u);
 
     const uint32_t landed = smem_u32(&bars[0]), full = CG == 1 ? landed : landed + 8 * kFp8MaxStages, empty = landed + 16 * kFp8MaxStages;
     const uint32_t d_full = empty + 8 * kFp8MaxStages, d_empty = d_full + 16, sf_full = d_empty + 16, sf_empty = sf_full + 16;
@@ -260,7 +260,7 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
     const int fold = 1 << p.fold_log, part = kBlockRows >> p.fold_log;  // rows of a part
     Fp8Tiles tile;
     tile.init(worker, workers);
-    const int tiles = tile.total(p), total = tiles * p.units;
+    const int tiles = tile.total(p), total = tiles * p.steps;
     auto mma_cols = [&] {  // that the tile's MMAs cover; a half's first column is a multiple of 16 where it is a coordinate of bytes
         constexpr int kUnit = kAcrossB ? 32 : 8 * CG;
         return (tile.valid + kUnit - 1) & -kUnit;
@@ -284,28 +284,35 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
             // Rows, or along the sum for what is read across, by eights 1024 bytes apart, version 1, 128-byte swizzle.  Read across, an MMA's 32 are 32
             // staged rows of 128 bytes, otherwise 32 of a row's 128 bytes.
             constexpr uint64_t sw128 = ((uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29))) << 32;
-            constexpr uint64_t kStepA = (kAcrossA ? 32 * 128 : 32) >> 4, kStepB = (kAcrossB ? 32 * 128 : 32) >> 4;
+            constexpr uint64_t kStepA = (kAcrossA ? 32 * 128 : 32) >> 4;
+            // Resident tokens: not swizzled, pieces of 16 columns 16 bytes a token apart, the eight rows of the next block a block's bytes.
+            const uint64_t kStepB = RESIDENT ? 2 * (uint64_t)p.cols : (kAcrossB ? 32 * 128 : 32) >> 4;
+            const uint64_t b_form = RESIDENT ? ((uint64_t)p.cols << 16) | ((uint64_t)(8u * (uint32_t)p.cols | (1u << 14)) << 32) : sw128;
             while (ok && tile.next(p)) {
                 const uint32_t idesc = fp8_idesc<CG>(p.fold_log ? p.d_cols : mma_cols(), kAcrossA, kAcrossB);
                 ok = mbar_wait_warp(d_empty + 8 * rd.idx, rd.phase ^ 1, abort_flag, p.status, 303);
                 const uint32_t d = tmem + (uint32_t)(rd.idx * p.d_cols);
                 Fp8Stages st(p, tile.first_group(p, groups));
-                for (int i = 0; ok && i < p.units; ++i, st.advance()) {
-                    const int c = st.c;
-                    if (i == 0 || (c & 3) == 0) ok = mbar_wait_warp(sf_full + 8 * rs.idx, rs.phase, abort_flag, p.status, 304);
+                for (int i = 0; ok && i < p.steps; ++i, st.advance()) {
+                    if ((st.c & 3) == 0) ok = mbar_wait_warp(sf_full + 8 * rs.idx, rs.phase, abort_flag, p.status, 304);
                     ok = ok && mbar_wait_warp(full + 8 * ru.idx, ru.phase, abort_flag, p.status, 305);
                     if (!ok) break;
                     tc_fence_after();
-                    const bool last = i + 1 == p.units, group_ends = c + 1 == p.units || (c & 3) == 3;
+                    const int end = st.end();
+                    const bool last = i + 1 == p.steps, group_ends = end == p.units || (end & 3) == 0;
                     if (elect_one_sync()) {
-                        const uint64_t a = sw128 | (uint64_t)(((base + (uint32_t)ru.idx * a_bytes) & 0x3FFFFu) >> 4);
-                        const uint64_t b = sw128 | (uint64_t)(((b_ring + (uint32_t)(RESIDENT ? c : ru.idx) * b_bytes) & 0x3FFFFu) >> 4);
                         const uint32_t sfa = tmem + kSfCol + (uint32_t)(rs.idx * kFp8SfCols), sfb = sfa + 8;
-                        const int steps = c + 1 == p.units && !p.fold_log ? p.last_steps : 4;
-                        const uint32_t id = idesc | ((uint32_t)(c & 3) << 29) | ((uint32_t)(c & 3) << 4);
+                        const uint64_t a = sw128 | (uint64_t)(((base + (uint32_t)(ru.idx * kFp8Deep) * a_bytes) & 0x3FFFFu) >> 4);
+                        const uint64_t b = b_form | (uint64_t)(((b_ring + (uint32_t)(RESIDENT ? st.c : ru.idx * kFp8Deep) * b_bytes) & 0x3FFFFu) >> 4);
+                        const uint32_t id = idesc | ((uint32_t)(st.c & 3) << 29) | ((uint32_t)(st.c & 3) << 4);
+                        // what lies behind the last block's columns is zeros, and multiplied like the rest
 #pragma unroll
-                        for (int kk = 0; kk < 4; ++kk)
-                            if (kk < steps) tc_mma_fp8<CG>(d, a + kStepA * kk, b + kStepB * kk, id, sfa, sfb, i == 0 && kk == 0 ? 0u : 1u);
+                        for (int u = 0; u < kFp8Deep; ++u)
+                            if (u == 0 || st.c + u < end)
+#pragma unroll
+                                for (int kk = 0; kk < 4; ++kk)
+                                    tc_mma_fp8<CG>(d, a + u * (a_bytes >> 4) + kStepA * kk, b + u * (b_bytes >> 4) + kStepB * kk, id + u * ((1u << 29) | (1u << 4)), sfa, sfb,
+                                                   i == 0 && u == 0 && kk == 0 ? 0u : 1u);
                         if (CG == 1) {
                             tc_commit(empty + 8 * ru.idx);
                             if (group_ends) tc_commit(sf_empty + 8 * rs.idx);
@@ -330,23 +337,27 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
         int issued = 0;
         if (!p.ahead) depend();
         while (ok && tile.next(p)) {
-            const int block = CG * tile.rt + rank, row = fp8_row(p, block), rows = p.flex ? fp8_row(p, block + 1) - row : kBlockRows;
-            const CUtensorMap *map = !p.flex || rows == p.group_rows * div_up(p.groups, p.row_tiles) ? &tmap_a : &tmap_a2;  // boxes of the taller and of the lower tiles
+            const int block = CG * tile.rt + rank, row = fp8_row<CG>(p, block), rows = CG == 1 ? fp8_row<CG>(p, block + 1) - row : kBlockRows;
+            const CUtensorMap *map = CG == 2 || rows == 4 * div_up(p.rows / 4, p.row_tiles) ? &tmap_a : &tmap_a2;  // boxes of the taller and of the lower tiles
             Fp8Stages st(p, tile.first_group(p, groups));
-            for (int i = 0; i < p.units; ++i, st.advance(), ru.advance(S)) {
-                const int c = st.c;
+            for (int i = 0; i < p.steps; ++i, st.advance(), ru.advance(S)) {
                 if (issued++ == S) depend();
                 ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 300);
                 if (!ok) break;
                 if (elect_one_sync()) {
                     const uint32_t bar = landed + 8 * ru.idx;
-                    mbar_expect_tx(bar, (uint32_t)(rows << p.fold_log) * 128u);
-                    for (int f = 0; f < fold; ++f) {  // what lies behind the last block reads as zeros
-                        const int at = ((c << p.fold_log) + f) * kFp8Block;
-                        const uint32_t to = base + (uint32_t)ru.idx * a_bytes + (uint32_t)(f * part) * 128u;
-                        if constexpr (kGated) tma_load_4d(to, map, at, 0, 0, row >> 4, bar);
-                        else if constexpr (kAcrossA) tma_load_2d(to, map, row, at, bar);
-                        else tma_load_2d(to, map, at, row, bar);
+                    const int end = st.end();
+                    mbar_expect_tx(bar, (uint32_t)((end - st.c) * (rows << p.fold_log)) * 128u);
+                    for (int c = st.c; c < end; ++c) {
+                        const uint32_t unit = base + (uint32_t)(ru.idx * kFp8Deep + c - st.c) * a_bytes;
+                        for (int f = 0; f < fold; ++f) {  // what lies behind the last block reads as zeros
+                            const int at = ((c << p.fold_log) + f) * kFp8Block;
+                            const uint32_t to = unit + (uint32_t)(f * part) * 128u;
+                            if constexpr (kGated && CG == 1) tma_load_3d(to, map, at, row >> 1, 0, bar);
+                            else if constexpr (kGated) tma_load_4d(to, map, at, 0, 0, row >> 4, bar);
+                            else if constexpr (kAcrossA) tma_load_2d(to, map, row, at, bar);
+                            else tma_load_2d(to, map, at, row, bar);
+                        }
                     }
                 }
                 __syncwarp();
@@ -364,18 +375,21 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
         while (ok && tile.next(p)) {
             const int col = tile.col0 + rank * (mma_cols() / CG);
             Fp8Stages st(p, tile.first_group(p, groups));
-            for (int i = 0; i < p.units; ++i, st.advance(), ru.advance(S)) {
-                const int c = st.c;
+            for (int i = 0; i < p.steps; ++i, st.advance(), ru.advance(S)) {
                 ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 301);
                 if (!ok) break;
                 if (elect_one_sync()) {
                     const uint32_t bar = landed + 8 * ru.idx;
-                    mbar_expect_tx(bar, b_bytes);
-                    for (int f = 0; f < fold; ++f) {
-                        const int at = ((c << p.fold_log) + f) * kFp8Block;
-                        const uint32_t to = b_ring + (uint32_t)ru.idx * b_bytes + (uint32_t)(f * p.b_rows) * 128u;
-                        if constexpr (kAcrossB) tma_load_2d(to, &tmap_b, col, at, bar);
-                        else tma_load_2d(to, &tmap_b, at, col, bar);
+                    const int end = st.end();
+                    mbar_expect_tx(bar, (uint32_t)(end - st.c) * b_bytes);
+                    for (int c = st.c; c < end; ++c) {
+                        const uint32_t unit = b_ring + (uint32_t)(ru.idx * kFp8Deep + c - st.c) * b_bytes;
+                        for (int f = 0; f < fold; ++f) {
+                            const int at = ((c << p.fold_log) + f) * kFp8Block;
+                            const uint32_t to = unit + (uint32_t)(f * p.b_rows) * 128u;
+                            if constexpr (kAcrossB) tma_load_2d(to, &tmap_b, col, at, bar);
+                            else tma_load_2d(to, &tmap_b, at, col, bar);
+                        }
                     }
                 }
                 __syncwarp();
@@ -396,58 +410,107 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
         const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + kSfCol;
         const uint32_t leader_full = CG == 1 ? sf_full : map_to_rank(sf_full, 0);
         const int a_blocks = div_up(p.rows, kFp8Block);
-        // Of a group, as loaded: A's words (dw) or, spread over the lanes, its bytes; B's words or (folded) bytes of two.  They are put together when the group
-        // before has been written, so that nothing waits for the loads before that.
+        // Some groups ahead are on their way, as loaded: A's words (dw) or, spread over the lanes, its bytes; B's words, those of a folded tile spread over the lanes too.  They
+        // are put together when their turn comes.  One group ahead the loads' latency, 1.5 us while the weights stream, was what single CTAs took for four stages (gated
+        // 14336x4096 at 1 token 28.1 us).
         constexpr bool kWordsA = FORM == kFp8Dw;
-        uint32_t raw_a[4] = {0, 0, 0, 0}, raw_b[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) raw_b[i] = 0;
+        constexpr int kAhead = 2;
+        struct Group {
+            int g, row0, features, col0, valid;  // its number, its tile's rows and columns
+            uint32_t a[kWordsA ? 4 : 2], b[CG == 1 ? 2 : 8];
+        } ring[kAhead];
         // Square scales: a tile's rows are of one block or two, gated of as many for each projection.  A group has 4 * fold bytes of each, which lie side by side: byte
         // `pos` of slot `slot` is lane (slot * 4 * fold + pos) % 32's.  (A byte for every row, loaded by all lanes, made one line of L2 what all SMs waited for:
         // 8192x8192 at 4096 tokens 205 -> 290 us.)
         const int fold_log = CG == 1 ? p.fold_log : 0;
-        auto block_of = [&](int slot, int row0) {
-            if (FORM == kFp8Dx) return row0 / kFp8Block;
-            if (kGated) return min(((slot >> 1) * (p.rows / 2) + (row0 >> 1)) / kFp8Block + (slot & 1), a_blocks - 1);
-            return min(row0 / kFp8Block + (slot & 1), a_blocks - 1);
+        bool more = tile.next(p);
+        int g = more ? tile.first_group(p, groups) : 0, left = groups;
+        auto take = [&](Group &r) {  // the next group
+            r.g = g;
+            r.row0 = fp8_row<CG>(p, CG * tile.rt + rank);
+            r.features = CG == 1 && kGated ? (fp8_row<CG>(p, tile.rt + 1) - r.row0) >> 1 : 8;
+            r.col0 = tile.col0;
+            r.valid = tile.valid;
+            if (++g == groups) g = 0;
+            if (--left == 0) {
+                left = groups;
+                more = tile.next(p);
+                if (more) g = tile.first_group(p, groups);
+            }
         };
-        // Group g of the tile: stages 4g .. 4g + 3.  What lies behind the last block or column is any of them: nothing is multiplied with it.
-        auto fetch_a = [&](int g) {
-            const int row0 = fp8_row(p, CG * tile.rt + rank);
+        // Group r.g of the tile: stages 4 r.g .. 4 r.g + 3.  What lies behind the last block or column is any of them: nothing is multiplied with it.
+        auto fetch_a = [&](Group &r) {
             if constexpr (kWordsA) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) raw_a[i] = __ldcg(reinterpret_cast<const uint32_t *>(p.as) + (size_t)g * p.rows + min(row0 + 32 * i + lane, p.rows - 1));
+                for (int i = 0; i < 4; ++i) r.a[i] = __ldcg(reinterpret_cast<const uint32_t *>(p.as) + (size_t)r.g * p.rows + min(r.row0 + 32 * i + lane, p.rows - 1));
             } else {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int idx = 32 * i + lane, slot = idx >> (2 + fold_log), kb = min((4 * g << fold_log) + (idx & ((4 << fold_log) - 1)), p.blocks - 1);
+                for (int i = 0; i < (CG == 1 ? 2 : 1); ++i) {
+                    const int idx = 32 * i + lane, slot = idx >> (2 + fold_log), kb = min((4 * r.g << fold_log) + (idx & ((4 << fold_log) - 1)), p.blocks - 1);
                     if (slot < (FORM == kFp8Dx ? 1 : kGated ? 4 : 2)) {
-                        const int block = block_of(slot, row0);
-                        raw_a[i] = __ldcg(p.as + (FORM == kFp8Dx ? (size_t)kb * a_blocks + block : (size_t)block * p.blocks + kb));
+                        const int first = kGated ? (slot >> 1) * (p.rows / 2) + (r.row0 >> 1) : r.row0;
+                        const int block = FORM == kFp8Dx ? first / kFp8Block : min(first / kFp8Block + (slot & 1), a_blocks - 1);
+                        r.a[i] = __ldcg(p.as + (FORM == kFp8Dx ? (size_t)kb * a_blocks + block : (size_t)block * p.blocks + kb));
                     }
                 }
             }
         };
-        // MMA row 32 i + lane is row `of` of part f
-        auto word_a = [&](int i) {
-            if constexpr (kWordsA) {
-                return raw_a[i];
+        auto fetch_b = [&](Group &r) {
+            if constexpr (RESIDENT) {
+            } else if (CG == 1 && fold_log) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {  // word w, of `fold` that a group has of a token, of token t: at w * b_rows + t, of 64 at most
+                    const int idx = 32 * i + lane, w = idx / p.b_rows, t = min(idx - w * p.b_rows, r.valid - 1), at = min((r.g << fold_log) + w, (p.blocks + 3) / 4 - 1);
+                    r.b[i] = __ldcg(reinterpret_cast<const uint32_t *>(p.bs) + (size_t)at * p.cols + r.col0 + t);
+                }
             } else {
-                const int row0 = fp8_row(p, CG * tile.rt + rank), r = 32 * i + lane, f = r >> (7 - fold_log), of = r & ((kBlockRows >> fold_log) - 1);
+#pragma unroll
+                for (int j = 0; j < (CG == 1 ? 2 : 8); ++j)
+                    if (32 * j < r.valid) r.b[j] = __ldcg(reinterpret_cast<const uint32_t *>(p.bs) + (size_t)r.g * p.cols + r.col0 + min(32 * j + lane, r.valid - 1));
+            }
+        };
+        // MMA column 32 j + lane is column t of block f of a unit
+        auto word_b = [&](const Group &r, int j) {
+            if constexpr (RESIDENT) {
+                uint32_t w;
+                asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(words_at + 256u * (uint32_t)r.g + 128u * j + 4u * lane));
+                return w;
+            } else if (CG == 1 && fold_log) {
+                const int at = 32 * j + lane, f = at / p.b_rows, t = at - f * p.b_rows;
+                uint32_t w = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int block = (i << fold_log) + f, idx = (block >> 2) * p.b_rows + t;  // of the group
+                    const uint32_t w0 = __shfl_sync(0xffffffffu, r.b[0], idx & 31), w1 = __shfl_sync(0xffffffffu, r.b[1], idx & 31);
+                    w |= (((idx < 32 ? w0 : w1) >> (8 * (block & 3))) & 255u) << (8 * i);
+                }
+                return w;
+            } else {
+                return r.b[j];
+            }
+        };
+        // MMA row 32 i + lane is row `of` of part f
+        auto word_a = [&](const Group &r, int i) {
+            if constexpr (kWordsA) {
+                return r.a[i];
+            } else {
+                const int m = 32 * i + lane, f = m >> (7 - fold_log), of = m & ((kBlockRows >> fold_log) - 1);
                 int slot = 0;
                 if constexpr (kGated) {
-                    const int base = (of & 8) ? p.rows / 2 : 0, first = row0 >> 1, feature = min(first + ((of >> 4) << 3) + (of & 7), p.rows / 2 - 1);
-                    slot = ((of & 8) >> 2) + (base + feature) / kFp8Block - (base + first) / kFp8Block;
+                    // pairs: eight rows of either projection in turn; single CTAs: one's, then the other's
+                    const bool up = CG == 1 ? of >= r.features : (of & 8) != 0;
+                    const int base = up ? p.rows / 2 : 0, first = r.row0 >> 1, at = CG == 1 ? (up ? of - r.features : of) : ((of >> 4) << 3) + (of & 7);
+                    slot = (up ? 2 : 0) + (base + min(first + at, p.rows / 2 - 1)) / kFp8Block - (base + first) / kFp8Block;
                 } else if (FORM == kFp8Product) {
-                    slot = min(row0 + of, p.rows - 1) / kFp8Block - row0 / kFp8Block;
+                    slot = min(r.row0 + of, p.rows - 1) / kFp8Block - r.row0 / kFp8Block;
                 }
                 uint32_t w = 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int idx = (slot << (2 + fold_log)) + (j << fold_log) + f;
-                    uint32_t b = __shfl_sync(0xffffffffu, raw_a[0], idx & 31);
+                    uint32_t b = __shfl_sync(0xffffffffu, r.a[0], idx & 31);
                     if (CG == 1) {
-                        const uint32_t b2 = __shfl_sync(0xffffffffu, raw_a[1], idx & 31);
+                        const uint32_t b2 = __shfl_sync(0xffffffffu, r.a[1], idx & 31);
                         if (idx >= 32) b = b2;
                     }
                     w |= b << (8 * j);
@@ -455,67 +518,55 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
                 return w;
             }
         };
-        auto fetch_b = [&](int g) {
-            if constexpr (RESIDENT) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(raw_b[j]) : "r"(words_at + 256u * (uint32_t)g + 128u * j + 4u * lane));
-            } else if (CG == 1 && p.fold_log) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {  // column t of block f of a stage
-                    const int at = 32 * j + lane, f = at / p.b_rows, t = min(at - f * p.b_rows, tile.valid - 1);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int kb = min(((4 * g + i) << p.fold_log) + f, p.blocks - 1);
-                        raw_b[4 * j + i] = __ldcg(p.bs + ((size_t)(kb >> 2) * p.cols + tile.col0 + t) * 4 + (kb & 3));
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < (CG == 1 ? 1 : 8); ++j)
-                    if (32 * j < tile.valid) raw_b[j] = __ldcg(reinterpret_cast<const uint32_t *>(p.bs) + (size_t)g * p.cols + tile.col0 + min(32 * j + lane, tile.valid - 1));
-            }
-        };
-        auto word = [](const uint32_t *b) { return b[0] | (b[1] << 8) | (b[2] << 16) | (b[3] << 24); };
+        const int total_groups = tiles * groups;
+        int taken = 0, written = 0;
         Ring rs;
         bool ok = true;
         if (!p.ahead) depend();
-        bool more = tile.next(p);
-        int g = more ? tile.first_group(p, groups) : 0, left = groups;
-        if (more) fetch_a(g);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            for (uint32_t &w : ring[k].a) w = 0;
+            for (uint32_t &w : ring[k].b) w = 0;
+            if (taken < total_groups) {
+                take(ring[k]);
+                fetch_a(ring[k]);
+                ++taken;
+            }
+        }
         depend();
-        if (more) fetch_b(g);
-        const int total_groups = tiles * groups;
-        while (more) {
-            uint32_t v[kFp8SfCols];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = word_a(i);
+        for (int k = 0; k < kAhead; ++k)
+            if (k < taken) fetch_b(ring[k]);
+        while (ok && written < total_groups) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[8 + i] = CG == 2 || i < 2 ? raw_b[i] : 0u;
-            if (CG == 1 && !RESIDENT && p.fold_log) v[8] = word(raw_b), v[9] = word(raw_b + 4);
+            for (int k = 0; k < kAhead; ++k) {
+                if (!ok || written >= total_groups) break;
+                Group &r = ring[k];
+                uint32_t v[kFp8SfCols];
 #pragma unroll
-            for (int i = 4; i < 8; ++i) v[i] = 0;
-            if (++g == groups) g = 0;
-            if (--left == 0) {
-                left = groups;
-                more = tile.next(p);
-                if (more) g = tile.first_group(p, groups);
+                for (int i = 0; i < 4; ++i) v[i] = word_a(r, i), v[4 + i] = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[8 + i] = CG == 2 || i < 2 ? word_b(r, CG == 2 ? i : i & 1) : 0u;
+                if (taken < total_groups) {
+                    take(r);
+                    fetch_a(r);
+                    fetch_b(r);
+                    ++taken;
+                }
+                ok = mbar_wait_warp(sf_empty + 8 * rs.idx, rs.phase ^ 1, abort_flag, p.status, 306);
+                if (!ok) break;
+                tc_fence_after();
+                tc_st_x16(lanes + (uint32_t)(rs.idx * kFp8SfCols), v);
+                asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (CG == 1) mbar_arrive(sf_full + 8 * rs.idx);
+                    else mbar_arrive_cluster(leader_full + 8 * rs.idx);
+                }
+                rs.advance(2);
+                ++written;
             }
-            if (more) {  // on their way while the group before is waited for
-                fetch_a(g);
-                fetch_b(g);
-            }
-            ok = mbar_wait_warp(sf_empty + 8 * rs.idx, rs.phase ^ 1, abort_flag, p.status, 306);
-            if (!ok) break;
-            tc_fence_after();
-            tc_st_x16(lanes + (uint32_t)(rs.idx * kFp8SfCols), v);
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) {
-                if (CG == 1) mbar_arrive(sf_full + 8 * rs.idx);
-                else mbar_arrive_cluster(leader_full + 8 * rs.idx);
-            }
-            rs.advance(2);
         }
         // the commits for the last two groups have arrived before the CTA leaves
         if (total_groups == 1) rs = Ring();
@@ -627,25 +678,25 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
             if (bar_any(1 + 2 * half, 128, !ok)) break;  // the group's four warps go on together or not at all
             tc_fence_after();
             const uint32_t d = tmem_q + (uint32_t)(rd.idx * p.d_cols);
-            row0 = fp8_row(p, CG * tile.rt + rank);
-            rows = max(0, min(p.flex ? fp8_row(p, CG * tile.rt + rank + 1) : row0 + kBlockRows, p.rows) - row0);
+            row0 = fp8_row<CG>(p, CG * tile.rt + rank);
+            rows = max(0, min(CG == 1 ? fp8_row<CG>(p, tile.rt + 1) : row0 + kBlockRows, p.rows) - row0);
             if constexpr (CG == 1) {
-                float v[16];
-                const int f = thread >> (7 - p.fold_log);
+                const int f = thread >> (7 - p.fold_log), features = rows >> 1;
+                float *sums = reinterpret_cast<float *>(smem + (staging - base));
+                float v[kFp8SingleCols];
                 tc_ld_x16(d + f * p.b_rows, v);
                 drained();
                 if (!kGated && p.fold_log == 0) {
-                    OT *to = o + (size_t)tile.col0 * out + row0 + thread;
+                    OT *to = o + row0 + thread;
                     if (thread < rows) {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
+                        for (int i = 0; i < kFp8SingleCols; ++i)
                             if (i < tile.valid) to[(size_t)i * out] = mx_convert<OT>(v[i]);
                     }
                 } else {
                     // Part f's sums of row i are lane part * f + i, columns b_rows * f ..: added up in the order of the parts.
-                    float *sums = reinterpret_cast<float *>(smem + (staging - base));
 #pragma unroll
-                    for (int t = 0; t < 16; ++t)
+                    for (int t = 0; t < kFp8SingleCols; ++t)
                         if (t < tile.valid) sums[t * kBlockRows + thread] = v[t];
                     meet();
                     auto sum = [&](int t, int i) {
@@ -654,19 +705,19 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
                         return s;
                     };
                     if constexpr (kGated) {
-                        const int i = thread & 63, at = 2 * (i & ~7) + (i & 7);
-                        for (int t = thread >> 6; t < tile.valid && i < rows / 2; t += 2) {
-                            const float g = sum(t, at), u = sum(t, at + 8);
-                            o[(size_t)(tile.col0 + t) * out + row0 / 2 + i] = mx_convert<OT>(fp8_activation(g, u, p.gelu));
+                        const int i = thread & 63;
+                        for (int t = thread >> 6; t < tile.valid && i < features; t += 2) {
+                            const float g = sum(t, i), u = sum(t, features + i);
+                            o[(size_t)t * out + row0 / 2 + i] = mx_convert<OT>(fp8_activation(g, u, p.gelu));
                             if (z) {
-                                OT *to = z + (size_t)(tile.col0 + t) * p.rows + row0 / 2 + i;
+                                OT *to = z + (size_t)t * p.rows + row0 / 2 + i;
                                 to[0] = mx_convert<OT>(g);
                                 to[out] = mx_convert<OT>(u);
                             }
                         }
                     } else {
                         const int i = thread & (part - 1);
-                        for (int t = f; t < tile.valid && i < rows; t += fold) o[(size_t)(tile.col0 + t) * out + row0 + i] = mx_convert<OT>(sum(t, i));
+                        for (int t = f; t < tile.valid && i < rows; t += fold) o[(size_t)t * out + row0 + i] = mx_convert<OT>(sum(t, i));
                     }
                     meet();  // they have been read
                 }
@@ -700,7 +751,7 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
 struct Fp8Plan {
     int cg, tile_cols, width, col_tiles, stages, d_cols;
     bool resident;
-    int flex, fold_log, group_rows, row_tiles, a_bytes, b_rows, z_offset;
+    int fold_log, row_tiles, a_bytes, b_rows, z_offset;
     int workers;
     size_t smem;
 };
@@ -723,75 +774,92 @@ static int fp8_pair_cols(int rows, int n, int red, int form, int pairs)
 {
     // Two accumulators and two buffers of scales fill tensor memory with 240.  Of dw multiples of 32: what a CTA stages starts at a multiple of 16 columns
     static const int widths[] = {240, 224, 208, 192, 176, 160, 144, 128, 112, 96, 80, 64, 48, 32, 16, 0};
+    const int unit = form == kFp8Dw ? 32 : 16;
     int best = 0;
     double best_us = 0;
     for (int i = 0; widths[i]; ++i) {
         const int cols = widths[i];
-        if (form == kFp8Dw && cols % 32) continue;
-        if (best && div_up(n, div_up(n, cols)) <= widths[i + 1]) continue;  // the next narrower one holds the same tiles
+        int narrower = 0;
+        for (int j = i + 1; widths[j] && !narrower; ++j)
+            if (widths[j] % unit == 0) narrower = widths[j];
+        if (cols % unit || div_up(n, div_up(n, cols)) <= narrower) continue;  // the next narrower one holds the same tiles
         const double us = fp8_pair_us(rows, n, red, cols, pairs);
         if (!best || us < best_us) best = cols, best_us = us;
     }
     return best;
 }
 
-// rows x red of A, n columns.  x_type: TUNA_FP8, or what B is before it is quantized.
-static Fp8Plan fp8_plan(int form, int rows, int n, int red, int x_type, int o_type, bool with_z, int sm_count)
+// Shared memory: `fixed` bytes, and as many stages as `room` has place for.
+static void fp8_stages(Fp8Plan &l, size_t room, size_t fixed, size_t b_unit)
+{
+    const size_t unit = l.a_bytes + b_unit;
+    l.stages = (int)std::min<size_t>(kFp8MaxStages, (room - fixed) / (kFp8Deep * unit));
+    // the last unit's MMAs read 128 rows
+    l.smem = std::max((size_t)(l.stages * kFp8Deep) * unit + fixed, (size_t)(l.stages * kFp8Deep - 1) * l.a_bytes + kBlockRows * 128);
+}
+
+static Fp8Plan fp8_plan_single(bool gated, int rows, int n, int red, int x_type, int sm_count)
+{
+    Fp8Plan l = {};
+    const int blocks = div_up(red, kFp8Block);
+    l.cg = 1;
+    l.workers = sm_count;
+    l.tile_cols = l.width = l.b_rows = div_up(n, 8) * 8;
+    l.col_tiles = 1;
+    l.row_tiles = (int)std::min<long long>(rows / 4, div_up_ll(rows, (long long)kBlockRows * sm_count) * sm_count);
+    const int height = 4 * div_up(rows / 4, l.row_tiles);
+    l.fold_log = height <= 32 ? 2 : height <= 64 ? 1 : 0;
+    l.a_bytes = (l.fold_log ? kBlockRows : div_up(height, 8) * 8) * 128;
+    const int fold = 1 << l.fold_log, units = div_up(blocks, fold);
+    l.d_cols = l.b_rows * fold;
+    const size_t fixed = l.fold_log || gated ? kFp8SumBytes : 0;
+    // Tokens that the CTAs quantize themselves: one round of the quantizing warps, and shared memory left for stages enough.
+    const size_t resident = (size_t)units * fold * n * 128 + 256 * (size_t)div_up(units, 4);
+    l.resident = x_type != TUNA_FP8 && n <= 8 && (long long)div_up(units * fold, 2) * n <= kFp8ResidentLoads * (fp8_warps(1) - 1) && resident + 4 * (size_t)l.a_bytes + fixed <= kFp8SmemHalf;
+    if (l.resident) fp8_stages(l, kFp8SmemHalf, fixed + resident, 0);
+    else fp8_stages(l, kFp8SmemHalf, fixed, (size_t)l.b_rows * fold * 128);
+    return l;
+}
+
+static Fp8Plan fp8_plan_pairs(int form, int rows, int n, int red, int o_type, bool with_z, int sm_count)
 {
     Fp8Plan l = {};
     const bool gated = form == kFp8GatedProduct;
-    const int blocks = div_up(red, kFp8Block), o_bytes = o_type == TUNA_FP32 ? 4 : 2;
-    l.cg = form <= kFp8GatedProduct && n <= kFp8DirectCols ? 1 : 2;
-    l.workers = sm_count / l.cg;
-    l.group_rows = gated ? 16 : 8;
-    const int groups = rows / l.group_rows;
-    size_t fixed;
-    if (l.cg == 1) {
-        l.flex = 1;
-        l.tile_cols = l.width = kFp8DirectCols;
-        l.row_tiles = (int)std::min<long long>(groups, div_up_ll(rows, (long long)kBlockRows * sm_count) * sm_count);
-        const int height = l.group_rows * div_up(groups, l.row_tiles);
-        l.fold_log = height <= 32 ? 2 : height <= 64 ? 1 : 0;
-        l.a_bytes = (l.fold_log ? kBlockRows : height) * 128;
-        l.b_rows = l.fold_log ? div_up(n, 8) * 8 : kFp8DirectCols;
-        fixed = l.fold_log || gated ? kFp8FoldBytes : 0;
-    } else {
-        l.tile_cols = fp8_pair_cols(rows, n, red, form, l.workers);
-        const int unit = form == kFp8Dw ? 32 : 16;
-        l.width = div_up(div_up(n, div_up(n, l.tile_cols)), unit) * unit;
-        l.row_tiles = div_up(rows, 2 * kBlockRows);
-        l.a_bytes = kBlockRows * 128;
-        l.b_rows = form == kFp8Dw ? kBlockRows : l.tile_cols / 2;
-        const size_t pitch = gated ? 64 * o_bytes + 16 : kBlockRows * o_bytes + (o_bytes == 2 ? 16 : 0);
-        fixed = 2 * kFp8StageCols * pitch;
-        l.z_offset = (int)fixed;
-        if (with_z) fixed += 2 * kFp8StageCols * (kBlockRows * 2 + 16);
-    }
+    const int o_bytes = o_type == TUNA_FP32 ? 4 : 2, unit = form == kFp8Dw ? 32 : 16;
+    l.cg = 2;
+    l.workers = sm_count / 2;
+    l.tile_cols = l.d_cols = fp8_pair_cols(rows, n, red, form, l.workers);
+    l.width = div_up(div_up(n, div_up(n, l.tile_cols)), unit) * unit;
     l.col_tiles = div_up(n, l.width);
-    const int fold = 1 << l.fold_log, units = div_up(blocks, fold);
-    l.d_cols = l.fold_log ? l.b_rows * fold : l.tile_cols;
-    const size_t room = l.cg == 1 ? kFp8SmemHalf : kFp8SmemMax;
-    size_t b_stage = (size_t)l.b_rows * fold * 128;
-    // Tokens that the CTAs quantize themselves: one round of the quantizing warps, and shared memory left for stages enough.
-    const int rows8 = div_up(n, 8) * 8;
-    const size_t resident = (size_t)units * rows8 * fold * 128 + 256 * (size_t)div_up(units, 4);
-    l.resident = l.cg == 1 && x_type != TUNA_FP8 && (long long)div_up(units * fold, 2) * n <= kFp8ResidentLoads * (fp8_warps(1) - 1) && resident + 4 * (size_t)l.a_bytes + fixed <= room;
-    if (l.resident) {
-        l.b_rows = rows8;
-        if (l.fold_log) l.d_cols = rows8 * fold;
-        fixed += resident;
-        b_stage = 0;
-    }
-    l.stages = (int)std::min<size_t>(kFp8MaxStages, (room - fixed) / (l.a_bytes + b_stage));
-    // the last stage's MMAs read 128 rows
-    l.smem = std::max((size_t)l.stages * (l.a_bytes + b_stage) + fixed, (size_t)(l.stages - 1) * l.a_bytes + kBlockRows * 128);
+    l.row_tiles = div_up(rows, 2 * kBlockRows);
+    // Rows in tiles of 256, also where that leaves the last round of tiles short: tiles of equal height that fill it are no faster (us, 256 / equal: 28672x4096 at 43 tokens
+    // 21.7 / 22.3, 11024x4112 at 43 13.5 / 13.3, 57344x8192 at 64 78.9 / 77.4, 4096x14336 at 64 22.5 / 25.4).
+    l.a_bytes = kBlockRows * 128;
+    l.b_rows = form == kFp8Dw ? kBlockRows : l.tile_cols / 2;
+    const size_t pitch = gated ? 64 * o_bytes + 16 : kBlockRows * o_bytes + (o_bytes == 2 ? 16 : 0);
+    size_t fixed = 2 * kFp8StageCols * pitch;
+    l.z_offset = (int)fixed;
+    if (with_z) fixed += 2 * kFp8StageCols * (kBlockRows * 2 + 16);
+    fp8_stages(l, kFp8SmemMax, fixed, (size_t)l.b_rows * 128);
     return l;
+}
+
+// rows x red of A, n columns.  x_type: TUNA_FP8, or what B is before it is quantized.
+static Fp8Plan fp8_plan(int form, int rows, int n, int red, int x_type, int o_type, bool with_z, int sm_count)
+{
+    // Single CTAs take what they quantize themselves, and few rows of long sums, which their tiles of any height share evenly and fold (us, single / pairs, codes: 4096x4096
+    // at 16 tokens 7.1 / 8.5, 4096x14336 at 1 14.5 / 21.5, 10240x8192 at 1 16.8 / 18.1; 1024x1024 at 8 4.5 / 4.0, 28672x4096 at 16 22.1 / 20.5).
+    if (form <= kFp8GatedProduct && n <= kFp8SingleCols) {
+        const Fp8Plan l = fp8_plan_single(form == kFp8GatedProduct, rows, n, red, x_type, sm_count);
+        if (l.resident || (rows <= sm_count * kBlockRows && red >= 2048)) return l;
+    }
+    return fp8_plan_pairs(form, rows, n, red, o_type, with_z, sm_count);
 }
 
 bool fp8_gemm_takes(bool gated, int rows, int n, int red, int x_type, int sm_count)
 {
     if (x_type == TUNA_FP8) return true;
-    return n <= kFp8DirectCols && fp8_plan(gated ? kFp8GatedProduct : kFp8Product, rows, n, red, x_type, TUNA_FP16, false, sm_count).resident;
+    return fp8_plan(gated ? kFp8GatedProduct : kFp8Product, rows, n, red, x_type, TUNA_FP16, false, sm_count).resident;
 }
 
 struct Fp8Maps {
@@ -853,11 +921,9 @@ static int launch_fp8_form(int form, const Fp8Codes &a, int rows, const Fp8Codes
     p.as = (const uint8_t *)a.s; p.bs = (const uint8_t *)b.s; p.o = o; p.z = z; p.x = numbers;
     p.rows = rows; p.cols = cols; p.red = red;
     p.blocks = div_up(red, kFp8Block);
-    p.fold_log = l.fold_log; p.units = div_up(p.blocks, 1 << l.fold_log);
-    p.last_steps = div_up(red - (p.blocks - 1) * kFp8Block, 32);
+    p.fold_log = l.fold_log; p.units = div_up(p.blocks, 1 << l.fold_log); p.steps = div_up(p.units, kFp8Deep);
     p.tile_cols = l.tile_cols; p.width = l.width; p.row_tiles = l.row_tiles; p.col_tiles = l.col_tiles;
     p.rows_inner = l.row_tiles < l.col_tiles;
-    p.group_rows = l.group_rows; p.groups = rows / l.group_rows; p.flex = l.flex;
     p.a_bytes = l.a_bytes; p.b_rows = l.b_rows; p.stages = l.stages; p.d_cols = l.d_cols;
     p.ahead = form <= kFp8GatedProduct && cols <= kFp8AheadTokens;
     p.stagger = form <= kFp8GatedProduct && !l.fold_log;
@@ -875,14 +941,17 @@ static int launch_fp8_form(int form, const Fp8Codes &a, int rows, const Fp8Codes
     auto weights = [&](CUtensorMap *map, int height) {
         if (form == kFp8Product) return matrix(map, a.q, red, rows, height);
         if (form != kFp8GatedProduct) return matrix(map, a.q, rows, red, kFp8Block);
-        const uint64_t k = (uint64_t)red, f = (uint64_t)rows / 2;  // [features by eight][gate or other][eight][k]
+        const uint64_t k = (uint64_t)red, f = (uint64_t)rows / 2;
+        if (l.cg == 1)  // [gate or other][features][k]
+            return make_tensor_map_3d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.q, k, f, 2, k, f * k, kFp8Block, (uint32_t)height / 2, 2, CU_TENSOR_MAP_SWIZZLE_128B);
+        // [features by eight][gate or other][eight][k]
         const uint64_t dims[4] = {k, 8, 2, f / 8}, strides[3] = {k, f * k, 8 * k};
         const uint32_t box[4] = {kFp8Block, 8, 2, (uint32_t)height / 16};
         return make_tensor_map_nd(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, a.q, 4, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     };
-    if (!weights(&maps.a, l.flex ? l.group_rows * div_up(p.groups, p.row_tiles) : kBlockRows)) return TUNA_ERR_NO_DEVICE;
+    if (!weights(&maps.a, l.cg == 1 ? 4 * div_up(rows / 4, l.row_tiles) : kBlockRows)) return TUNA_ERR_NO_DEVICE;
     maps.a2 = maps.b = maps.a;
-    if (l.flex && p.groups % p.row_tiles && !weights(&maps.a2, l.group_rows * (p.groups / p.row_tiles))) return TUNA_ERR_NO_DEVICE;
+    if (l.cg == 1 && rows / 4 % l.row_tiles && !weights(&maps.a2, 4 * (rows / 4 / l.row_tiles))) return TUNA_ERR_NO_DEVICE;
     if (!l.resident && !(form == kFp8Dw ? matrix(&maps.b, b.q, cols, red, kFp8Block) : matrix(&maps.b, b.q, red, cols, l.b_rows))) return TUNA_ERR_NO_DEVICE;
     if (numbers && b.q && launch_fp8_quantize_rows(numbers, x_type, red, b.q, b.s, cols, red, true, stream) != cudaSuccess) return TUNA_ERR_LAUNCH;
     switch (o_type) {
