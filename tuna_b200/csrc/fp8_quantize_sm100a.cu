@@ -99,25 +99,39 @@ constexpr int kFp8LaneRows = kFp8TileRows / 2;
 
 __device__ __forceinline__ uint32_t fp8_magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }  // compare as the numbers do, NaN above infinity
 
+// Rows' maxima over the 16 lanes that have them: in every step a lane keeps half of the rows and sends the other half, so that in the end lanes 2 r and 2 r + 1 have
+// that of row r.  30 instructions for eight rows, where every lane taking part in every row's would be 64, and one scale a lane to work out instead of eight.
+template <typename V, typename Max>
+__device__ __forceinline__ V fp8_rows_max(V (&v)[kFp8LaneRows], int lane, Max largest)
+{
+#pragma unroll
+    for (int half = kFp8LaneRows / 2; half >= 1; half >>= 1) {
+        const int d = 2 * half;
+        const bool upper = lane & d;
+#pragma unroll
+        for (int r = 0; r < half; ++r) {
+            const V keep = upper ? v[r + half] : v[r], give = upper ? v[r] : v[r + half];
+            v[r] = largest(keep, __shfl_xor_sync(0xffffffffu, give, d));
+        }
+    }
+    return largest(v[0], __shfl_xor_sync(0xffffffffu, v[0], 1));
+}
+
 // A lane's numbers as they were loaded, the bits (fp32) of their largest magnitudes, and their values.
 template <typename T>
 struct Fp8Raw {  // 16 bits: maxima in pairs
     Mx8<T> v[kFp8LaneRows];
     using Pair = decltype(v[0].pair(0));
-    __device__ __forceinline__ static Pair largest(Pair a, Pair b) { return __hmax2_nan(a, __habs2(b)); }
-    __device__ __forceinline__ static uint32_t bits(Pair p)
-    {
-        const float2 f = widen(p);
-        return max(fp8_magnitude(f.x), fp8_magnitude(f.y));
-    }
+    __device__ __forceinline__ static Pair with(Pair a, Pair b) { return __hmax2_nan(a, __habs2(b)); }
     __device__ __forceinline__ static float2 widen(__half2 p) { return __half22float2(p); }
     __device__ __forceinline__ static float2 widen(__nv_bfloat162 p) { return __bfloat1622float2(p); }
-    __device__ __forceinline__ uint32_t row_max(int r) const
+    __device__ __forceinline__ uint32_t row_max(int lane) const  // of row (lane / 2) % 8 of the lane's
     {
-        Pair m = largest(largest(__habs2(v[r].pair(0)), v[r].pair(1)), __hmax2_nan(__habs2(v[r].pair(2)), __habs2(v[r].pair(3))));
+        Pair m[kFp8LaneRows];
 #pragma unroll
-        for (int d = 1; d < 16; d <<= 1) m = __hmax2_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
-        return bits(m);
+        for (int r = 0; r < kFp8LaneRows; ++r) m[r] = with(with(__habs2(v[r].pair(0)), v[r].pair(1)), __hmax2_nan(__habs2(v[r].pair(2)), __habs2(v[r].pair(3))));
+        const float2 f = widen(fp8_rows_max(m, lane, [](Pair a, Pair b) { return __hmax2_nan(a, b); }));
+        return max(fp8_magnitude(f.x), fp8_magnitude(f.y));
     }
     __device__ __forceinline__ void col_max(uint32_t (&m)[8]) const  // of the warp's 16 rows
     {
@@ -125,25 +139,37 @@ struct Fp8Raw {  // 16 bits: maxima in pairs
         for (int i = 0; i < 4; ++i) {
             Pair p = __habs2(v[0].pair(i));
 #pragma unroll
-            for (int r = 1; r < kFp8LaneRows; ++r) p = largest(p, v[r].pair(i));
+            for (int r = 1; r < kFp8LaneRows; ++r) p = with(p, v[r].pair(i));
             p = __hmax2_nan(p, __shfl_xor_sync(0xffffffffu, p, 16));
             const float2 f = widen(p);
             m[2 * i] = fp8_magnitude(f.x);
             m[2 * i + 1] = fp8_magnitude(f.y);
         }
     }
+    __device__ __forceinline__ uint32_t lane_max() const
+    {
+        Pair m = __habs2(v[0].pair(0));
+#pragma unroll
+        for (int r = 0; r < kFp8LaneRows; ++r)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m = with(m, v[r].pair(i));
+        const float2 f = widen(m);
+        return max(fp8_magnitude(f.x), fp8_magnitude(f.y));
+    }
     __device__ __forceinline__ void values(int r, float (&f)[8]) const { v[r].values(f); }
 };
 struct Fp8RawFloat {
     float v[kFp8LaneRows][8];
-    __device__ __forceinline__ uint32_t row_max(int r) const
+    __device__ __forceinline__ uint32_t row_max(int lane) const
     {
-        uint32_t m = 0;
+        uint32_t m[kFp8LaneRows];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, fp8_magnitude(v[r][i]));
+        for (int r = 0; r < kFp8LaneRows; ++r) {
+            m[r] = fp8_magnitude(v[r][0]);
 #pragma unroll
-        for (int d = 1; d < 16; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-        return m;
+            for (int i = 1; i < 8; ++i) m[r] = max(m[r], fp8_magnitude(v[r][i]));
+        }
+        return fp8_rows_max(m, lane, [](uint32_t a, uint32_t b) { return max(a, b); });
     }
     __device__ __forceinline__ void col_max(uint32_t (&m)[8]) const
     {
@@ -154,6 +180,15 @@ struct Fp8RawFloat {
             for (int r = 0; r < kFp8LaneRows; ++r) m[i] = max(m[i], fp8_magnitude(v[r][i]));
             m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], 16));
         }
+    }
+    __device__ __forceinline__ uint32_t lane_max() const
+    {
+        uint32_t m = 0;
+#pragma unroll
+        for (int r = 0; r < kFp8LaneRows; ++r)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = max(m, fp8_magnitude(v[r][i]));
+        return m;
     }
     __device__ __forceinline__ void values(int r, float (&f)[8]) const
     {
@@ -233,12 +268,14 @@ struct Fp8Gated {
 };
 
 template <int WAYS, typename Source>  // WAYS: 1 << kFp8Row | 1 << kFp8Column, one of them, or 1 << kFp8Square
-__global__ void __launch_bounds__(32 * kFp8TileWarps, sizeof(typename Source::Raw) <= 128 ? 3 : 2)
+__global__ void __launch_bounds__(32 * kFp8TileWarps, sizeof(typename Source::Raw) > 128 ? 2 : WAYS & (WAYS - 1) ? 3 : 4)
 fp8_quantize_tile_kernel(const Source src, uint8_t *q, uint8_t *s, uint8_t *q2, uint8_t *s2, int rows, int cols, bool two_halves, bool chained)
 {
     constexpr bool kRows = WAYS & (1 << kFp8Row), kCols = WAYS & (1 << kFp8Column), kSquare = WAYS & (1 << kFp8Square);
-    __shared__ uint4 s_max[kFp8TileWarps][32];   // of a warp's rows, column by column
-    __shared__ uint32_t s_scale[kFp8Block];
+    __shared__ uint4 s_max[kFp8TileWarps][32];  // of a warp's rows, column by column
+    __shared__ __align__(16) float s_inverse[kFp8Block];
+    __shared__ uint32_t s_square[kFp8TileWarps];
+    __shared__ int s_none;  // a column's block is NaN
     if (chained) {
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -248,90 +285,101 @@ fp8_quantize_tile_kernel(const Source src, uint8_t *q, uint8_t *s, uint8_t *q2, 
     // Halves of the columns that read the same: tile t of the one and of the other follow one another, so that L2 has it.
     const int ct = !two_halves ? blockIdx.x : (blockIdx.x & 1) ? (col_tiles + 1) / 2 + (blockIdx.x >> 1) : blockIdx.x >> 1;
     const int col = ct * kFp8Block + (lane & 15) * 8;
+    const size_t step = 2 * (size_t)cols;
     for (int rt = blockIdx.y; rt < row_tiles; rt += gridDim.y) {
         const long long row0 = (long long)rt * kFp8Block + warp * kFp8TileRows + (lane >> 4);
         typename Source::Raw raw;
         src.load(raw, row0, col, rows, cols);
-        auto write = [&](uint8_t *to, int r, uint32_t lo, uint32_t hi) {
-            if (col < cols && row0 + 2 * r < rows) *reinterpret_cast<uint2 *>(to + (row0 + 2 * r) * cols + col) = make_uint2(lo, hi);
+        const int have = col < cols ? (int)min((long long)rows - row0, 2ll * kFp8LaneRows) : 0;  // of the rows from row0 on
+        // Codes of row r; MASKED: zeros where a bit of `none` says so.  Two ways and no test in the common one: with it square blocks of 28672x4096 in bf16 took 73 us, so 55.
+        auto write = [&](auto masked, uint8_t *to, int r, const float (&inverse)[8], uint32_t none) {
+            float f[8];
+            raw.values(r, f);
+            uint2 w = make_uint2(fp8_encode4(f[0] * inverse[0], f[1] * inverse[1], f[2] * inverse[2], f[3] * inverse[3]),
+                                 fp8_encode4(f[4] * inverse[4], f[5] * inverse[5], f[6] * inverse[6], f[7] * inverse[7]));
+            if constexpr (decltype(masked)::value)
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (none >> i & 1) (i < 4 ? w.x : w.y) &= ~(0xffu << (8 * (i & 3)));
+            if (2 * r < have) *reinterpret_cast<uint2 *>(to + r * step) = w;
         };
         if constexpr (kRows) {
-            uint32_t mine = 0;  // of row lane % 16 of the lane's
+            const uint32_t e = fp8_scale(raw.row_max(lane));  // of the lane's row (lane / 2) % 8
+            const float mine = fp8_inverse(e);
+            uint8_t *to = q + (size_t)row0 * cols + col;
+            auto rows_of = [&](auto masked) {
 #pragma unroll
-            for (int r = 0; r < kFp8LaneRows; ++r) {
-                const uint32_t e = fp8_scale(raw.row_max(r));
-                const float i = fp8_inverse(e);
-                float f[8];
-                raw.values(r, f);
-                const uint32_t lo = fp8_encode4(f[0] * i, f[1] * i, f[2] * i, f[3] * i), hi = fp8_encode4(f[4] * i, f[5] * i, f[6] * i, f[7] * i);
-                write(q, r, e == 255u ? 0u : lo, e == 255u ? 0u : hi);
-                if ((lane & 15) == r) mine = e;
-            }
-            const long long row = row0 + 2 * (lane & 15);
-            if ((lane & 15) < kFp8LaneRows && row < rows) {
+                for (int r = 0; r < kFp8LaneRows; ++r) {
+                    const float i = __shfl_sync(0xffffffffu, mine, (lane & 16) + 2 * r);
+                    const uint32_t none = decltype(masked)::value && __shfl_sync(0xffffffffu, e, (lane & 16) + 2 * r) == 255u ? 255u : 0u;
+                    write(masked, to, r, {i, i, i, i, i, i, i, i}, none);
+                }
+            };
+            if (__any_sync(0xffffffffu, e == 255u)) rows_of(Int<1>());
+            else rows_of(Int<0>());
+            const long long row = row0 + 2 * ((lane >> 1) & 7);
+            if ((lane & 1) == 0 && row < rows) {
                 uint8_t *at = s + ((long long)(ct >> 2) * rows + row) * 4 + (ct & 3);
-                *at = (uint8_t)mine;
+                *at = (uint8_t)e;
                 if (ct + 1 == col_tiles)
                     for (int i = 1; i < 4 - (ct & 3); ++i) at[i] = 0;
             }
         }
         if constexpr (kCols || kSquare) {
-            uint32_t m[8];
-            raw.col_max(m);
-            if constexpr (kSquare) {
-                m[0] = max(max(max(m[0], m[1]), max(m[2], m[3])), max(max(m[4], m[5]), max(m[6], m[7])));
-                m[0] = __reduce_max_sync(0xffffffffu, m[0]);
-            }
             if (rt != (int)blockIdx.y) __syncthreads();  // what was there before has been read
+            uint8_t *to = (kRows ? q2 : q) + (size_t)row0 * cols + col, *words = kRows ? s2 : s;
+            float inverse[8];
+            uint32_t none = 0;
             if constexpr (kSquare) {
-                if (lane == 0) s_scale[warp] = m[0];
-            } else if (lane < 16) {
-                s_max[warp][2 * lane] = make_uint4(m[0], m[1], m[2], m[3]);
-                s_max[warp][2 * lane + 1] = make_uint4(m[4], m[5], m[6], m[7]);
-            }
-            __syncthreads();
-            uint8_t *to = kRows ? q2 : q, *words = kRows ? s2 : s;
-            uint32_t e[8];
-            if constexpr (kSquare) {
+                uint32_t m = raw.lane_max();
 #pragma unroll
-                for (int w = 0; w < kFp8TileWarps; ++w) m[0] = max(m[0], s_scale[w]);
+                for (int d = 1; d < 32; d <<= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+                if (lane == 0) s_square[warp] = m;
+                __syncthreads();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) e[i] = fp8_scale(m[0]);
-                if (threadIdx.x == 0) words[(long long)rt * col_tiles + ct] = (uint8_t)e[0];
+                for (int w = 0; w < kFp8TileWarps; ++w) m = max(m, s_square[w]);
+                const uint32_t e = fp8_scale(m);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) inverse[i] = fp8_inverse(e);
+                none = e == 255u ? 255u : 0u;
+                if (threadIdx.x == 0) words[(long long)rt * col_tiles + ct] = (uint8_t)e;
             } else {
+                uint32_t m[8];
+                raw.col_max(m);
+                if (lane < 16) {
+                    s_max[warp][2 * lane] = make_uint4(m[0], m[1], m[2], m[3]);
+                    s_max[warp][2 * lane + 1] = make_uint4(m[4], m[5], m[6], m[7]);
+                }
+                if (threadIdx.x == 0) s_none = 0;
+                __syncthreads();
                 if (threadIdx.x < kFp8Block) {  // one column each
-                    uint32_t c = 0;
+                    uint32_t e = 0;
 #pragma unroll
-                    for (int w = 0; w < kFp8TileWarps; ++w) c = max(c, reinterpret_cast<const uint32_t *>(s_max[w])[threadIdx.x]);
-                    c = fp8_scale(c);
-                    s_scale[threadIdx.x] = c;
+                    for (int w = 0; w < kFp8TileWarps; ++w) e = max(e, reinterpret_cast<const uint32_t *>(s_max[w])[threadIdx.x]);
+                    e = fp8_scale(e);
+                    s_inverse[threadIdx.x] = e == 255u ? 0.0f : fp8_inverse(e);
+                    if (e == 255u) s_none = 1;
                     const int at_col = ct * kFp8Block + threadIdx.x;
                     if (at_col < cols) {
                         uint8_t *at = words + ((long long)(rt >> 2) * cols + at_col) * 4 + (rt & 3);
-                        *at = (uint8_t)c;
+                        *at = (uint8_t)e;
                         if (rt + 1 == row_tiles)
                             for (int j = 1; j < 4 - (rt & 3); ++j) at[j] = 0;
                     }
                 }
                 __syncthreads();
-                const uint4 a = *reinterpret_cast<const uint4 *>(s_scale + 8 * (lane & 15)), b = *reinterpret_cast<const uint4 *>(s_scale + 8 * (lane & 15) + 4);
-                e[0] = a.x; e[1] = a.y; e[2] = a.z; e[3] = a.w;
-                e[4] = b.x; e[5] = b.y; e[6] = b.z; e[7] = b.w;
-            }
-            float inverse[8];
-            uint32_t keep[2] = {0xffffffffu, 0xffffffffu};
+                *reinterpret_cast<float4 *>(inverse) = *reinterpret_cast<const float4 *>(s_inverse + 8 * (lane & 15));
+                *reinterpret_cast<float4 *>(inverse + 4) = *reinterpret_cast<const float4 *>(s_inverse + 8 * (lane & 15) + 4);
+                if (s_none)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                inverse[i] = fp8_inverse(e[i]);
-                if (e[i] == 255u) keep[i >> 2] &= ~(0xffu << (8 * (i & 3)));
+                    for (int i = 0; i < 8; ++i) none |= inverse[i] == 0.0f ? 1u << i : 0u;
             }
+            auto rows_of = [&](auto masked) {
 #pragma unroll
-            for (int r = 0; r < kFp8LaneRows; ++r) {
-                float f[8];
-                raw.values(r, f);
-                write(to, r, fp8_encode4(f[0] * inverse[0], f[1] * inverse[1], f[2] * inverse[2], f[3] * inverse[3]) & keep[0],
-                      fp8_encode4(f[4] * inverse[4], f[5] * inverse[5], f[6] * inverse[6], f[7] * inverse[7]) & keep[1]);
-            }
+                for (int r = 0; r < kFp8LaneRows; ++r) write(masked, to, r, inverse, none);
+            };
+            if (__any_sync(0xffffffffu, none != 0u)) rows_of(Int<1>());
+            else rows_of(Int<0>());
         }
     }
 }
@@ -391,73 +439,76 @@ cudaError_t launch_fp8_gated_gradient(const void *z, const void *dh, int type, i
 
 // ---- the inverse
 
-__device__ __forceinline__ void fp8_store8(float *p, const float (&v)[8])
+__device__ __forceinline__ void fp8_store(float *p, const float (&v)[4]) { *reinterpret_cast<float4 *>(p) = make_float4(v[0], v[1], v[2], v[3]); }
+template <typename T>
+__device__ __forceinline__ void fp8_store(T *p, const float (&v)[8])
 {
-    reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-}
-__device__ __forceinline__ void fp8_store8(__half *p, const float (&v)[8])
-{
-    *reinterpret_cast<uint4 *>(p) = make_uint4(pack_half2(v[0], v[1]), pack_half2(v[2], v[3]), pack_half2(v[4], v[5]), pack_half2(v[6], v[7]));
-}
-__device__ __forceinline__ void fp8_store8(__nv_bfloat16 *p, const float (&v)[8])
-{
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-        w[i] = *reinterpret_cast<const uint32_t *>(&h);
-    }
-    *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4 *>(p) = make_uint4(mx_pack2<T>(v[0], v[1]), mx_pack2<T>(v[2], v[3]), mx_pack2<T>(v[4], v[5]), mx_pack2<T>(v[6], v[7]));
 }
 
-// o = code * scale in fp32 (exact: four significant bits; below fp32's range it rounds), rounded once to T.  A thread has eight columns of ROWS rows, grid (columns, rows).
+// o = code * scale in fp32 (exact: four significant bits; below fp32's range it rounds), rounded once to T.  A thread has 16 bytes of the result, COLS columns, of ROWS rows;
+// grid (columns, rows).
 template <typename T, int BLOCKS, int ROWS>
 __global__ void __launch_bounds__(128)
 fp8_dequant_kernel(const uint8_t *q, const uint8_t *s, T *o, int rows, int k)
 {
-    const int col = (blockIdx.x * 128 + threadIdx.x) * 8;
+    constexpr int COLS = 16 / sizeof(T);
+    const int col = (blockIdx.x * 128 + threadIdx.x) * COLS;
     if (col >= k) return;
     for (long long row0 = (long long)blockIdx.y * ROWS; row0 < rows; row0 += (long long)gridDim.y * ROWS) {
-        uint2 codes[ROWS];
+        uint32_t codes[ROWS][COLS / 4];
+        const int have = (int)min((long long)rows - row0, (long long)ROWS);
 #pragma unroll
-        for (int r = 0; r < ROWS; ++r) codes[r] = row0 + r < rows ? __ldcg(reinterpret_cast<const uint2 *>(q + (row0 + r) * k + col)) : make_uint2(0, 0);
-        uint32_t byte[BLOCKS == kFp8Column ? 8 : ROWS];
-        if constexpr (BLOCKS == kFp8Column) {  // ROWS divides 128: the rows are of one block
-#pragma unroll
-            for (int i = 0; i < 8; ++i) byte[i] = __ldcg(s + ((row0 >> 9) * k + col + i) * 4 + ((row0 >> 7) & 3));
-        } else {
-#pragma unroll
-            for (int r = 0; r < ROWS; ++r) {
-                const long long row = min(row0 + r, (long long)rows - 1);
-                byte[r] = BLOCKS == kFp8Row ? __ldcg(s + ((long long)(col >> 9) * rows + row) * 4 + ((col >> 7) & 3)) : __ldcg(s + (row >> 7) * div_up(k, kFp8Block) + (col >> 7));
+        for (int r = 0; r < ROWS; ++r) {
+            const uint8_t *at = q + (row0 + min(r, have - 1)) * k + col;
+            if constexpr (COLS == 4) {
+                codes[r][0] = __ldcg(reinterpret_cast<const uint32_t *>(at));
+            } else {
+                const uint2 w = __ldcg(reinterpret_cast<const uint2 *>(at));
+                codes[r][0] = w.x;
+                codes[r][1] = w.y;
             }
+        }
+        uint32_t byte[BLOCKS == kFp8Column ? COLS : BLOCKS == kFp8Row ? ROWS : 1];  // ROWS divides 128: the rows are of one block
+        if constexpr (BLOCKS == kFp8Column) {
+#pragma unroll
+            for (int i = 0; i < COLS; ++i) byte[i] = __ldcg(s + ((row0 >> 9) * k + col + i) * 4 + ((row0 >> 7) & 3));
+        } else if constexpr (BLOCKS == kFp8Row) {
+#pragma unroll
+            for (int r = 0; r < ROWS; ++r) byte[r] = __ldcg(s + ((long long)(col >> 9) * rows + row0 + min(r, have - 1)) * 4 + ((col >> 7) & 3));
+        } else {
+            byte[0] = s[(row0 >> 7) * div_up(k, kFp8Block) + (col >> 7)];  // by way of L1: few bytes, which everybody reads
         }
 #pragma unroll
         for (int r = 0; r < ROWS; ++r) {
-            if (row0 + r >= rows) continue;
-            uint32_t h[4];
-            fp8_decode4(codes[r].x, *reinterpret_cast<uint32_t(*)[2]>(h));
-            fp8_decode4(codes[r].y, *reinterpret_cast<uint32_t(*)[2]>(h + 2));
-            float v[8];
+            if (r >= have) break;
+            float v[COLS];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&h[i]));
-                v[2 * i] = f.x * mx_scale_value(byte[BLOCKS == kFp8Column ? 2 * i : r]);
-                v[2 * i + 1] = f.y * mx_scale_value(byte[BLOCKS == kFp8Column ? 2 * i + 1 : r]);
+            for (int i = 0; i < COLS; i += 4) {
+                uint32_t h[2];
+                fp8_decode4(codes[r][i / 4], h);
+                const float2 a = __half22float2(*reinterpret_cast<const __half2 *>(&h[0])), b = __half22float2(*reinterpret_cast<const __half2 *>(&h[1]));
+                const float n[4] = {a.x, a.y, b.x, b.y};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[i + j] = n[j] * mx_scale_value(byte[BLOCKS == kFp8Column ? i + j : BLOCKS == kFp8Row ? r : 0]);
             }
-            fp8_store8(o + (row0 + r) * k + col, v);
+            fp8_store(o + (row0 + r) * k + col, v);
         }
     }
+}
+
+template <typename T, int BLOCKS, int ROWS>
+static cudaError_t dequant_rows(const void *q, const void *s, void *o, int rows, int k, cudaStream_t stream)
+{
+    const dim3 grid((unsigned)div_up(k, 16 / (int)sizeof(T) * 128), (unsigned)std::min(div_up(rows, ROWS), 65535));
+    fp8_dequant_kernel<T, BLOCKS, ROWS><<<grid, 128, 0, stream>>>((const uint8_t *)q, (const uint8_t *)s, (T *)o, rows, k);
+    return cudaGetLastError();
 }
 
 template <typename T, int BLOCKS>
 static cudaError_t dequant_as(const void *q, const void *s, void *o, int rows, int k, cudaStream_t stream)
 {
-    constexpr int kRows = 4;
-    const dim3 grid((unsigned)div_up(k, 8 * 128), (unsigned)std::min(div_up(rows, kRows), 65535));
-    fp8_dequant_kernel<T, BLOCKS, kRows><<<grid, 128, 0, stream>>>((const uint8_t *)q, (const uint8_t *)s, (T *)o, rows, k);
-    return cudaGetLastError();
+    return (long long)rows * k <= 1 << 20 ? dequant_rows<T, BLOCKS, 2>(q, s, o, rows, k, stream) : dequant_rows<T, BLOCKS, 8>(q, s, o, rows, k, stream);
 }
 
 template <typename T>
