@@ -91,18 +91,13 @@ static int backward(const void *dy, const void *z, int dy_type, const void *x, i
     Fp8Codes by_row = {nullptr, nullptr}, by_column = {nullptr, nullptr}, xt = {const_cast<void *>(x), const_cast<void *>(xs)};
     if (dx) by_row = place(workspace, at, (size_t)n * m, word_bytes(m, n));
     if (dw) by_column = place(workspace, at, (size_t)n * m, word_bytes(n, m));
-    cudaError_t e;
-    if (z) e = launch_fp8_gated_gradient(z, dy, dy_type, activation == TUNA_GELU, by_row, by_column, n, m / 2, stream);
-    else if (dx && dw) e = launch_fp8_quantize_tiles(dy, dy_type, m, kFp8Both, by_row, by_column, n, m, true, stream);
-    else if (dx) e = launch_fp8_quantize_rows(dy, dy_type, m, by_row.q, by_row.s, n, m, true, stream);
-    else e = launch_fp8_quantize_tiles(dy, dy_type, m, kFp8Column, by_column, by_column, n, m, true, stream);
-    if (e != cudaSuccess) return TUNA_ERR_LAUNCH;
-    if (dw && !packed) {
-        xt = place(workspace, at, (size_t)n * k, word_bytes(n, k));
-        if (launch_fp8_quantize_tiles(x, x_type, k, kFp8Column, xt, xt, n, k, true, stream) != cudaSuccess) return TUNA_ERR_LAUNCH;
-    }
+    Fp8GradientArgs g;
+    g.dy = dy; g.z = z; g.x = x; g.type = dy_type; g.x_type = x_type; g.gelu = activation == TUNA_GELU; g.rows = n; g.cols = m; g.x_cols = k;
+    g.by_row = by_row; g.by_column = by_column; g.x_to = {nullptr, nullptr}; g.stream = stream;
+    if (dw && !packed) g.x_to = xt = place(workspace, at, (size_t)n * k, word_bytes(n, k));
+    if (launch_fp8_gradient(g) != cudaSuccess) return TUNA_ERR_LAUNCH;
     if (dx) st = launch_fp8_dx({const_cast<void *>(q), const_cast<void *>(s)}, by_row, dx, dx_type, m, n, k, sms, stream);
-    if (dw && st == TUNA_OK) st = launch_fp8_dw(xt, by_column, dw, dw_type, m, n, k, sms, stream);
+    if (dw && st == TUNA_OK) st = launch_fp8_dw(xt, by_column, dw, dw_type, m, n, k, dx != nullptr, sms, stream);
     return st;
 }
 
@@ -119,7 +114,7 @@ extern "C" int tuna_fp8_quantize(const void *x, int x_type, long long row_stride
     if (!aligned_to(x, 16) || (row_stride * (x_type == TUNA_FP32 ? 4 : 2)) % 16 || !aligned_to(q, 16) || !aligned_to(q2, 16)) return TUNA_ERR_MISALIGNED;
     if (blocks != TUNA_FP8_SQUARE && (!aligned_to(s, 4) || !aligned_to(s2, 4))) return TUNA_ERR_MISALIGNED;
     const cudaError_t e = blocks == TUNA_FP8_ROW ? launch_fp8_quantize_rows(x, x_type, row_stride, q, s, rows, k, false, (cudaStream_t)stream)
-                                                 : launch_fp8_quantize_tiles(x, x_type, row_stride, blocks, {q, s}, {q2, s2}, rows, k, false, (cudaStream_t)stream);
+                                                 : launch_fp8_quantize_tiles(x, x_type, row_stride, blocks, {q, s}, {q2, s2}, rows, k, (cudaStream_t)stream);
     return e == cudaSuccess ? TUNA_OK : TUNA_ERR_LAUNCH;
 }
 

@@ -81,6 +81,7 @@ struct Fp8Params {
     int stages;
     int d_cols;      // tensor-memory columns of each of the two accumulators: columns of a tile times fold
     int ahead;       // A is there before the dependency wait
+    int beside;      // dw: launched right behind the dx of its call
     int x_bf16;      // RESIDENT: type of the tokens
     const void *x;   // RESIDENT: the tokens [cols][red]
     int stagger;     // row tiles start their sums at different groups
@@ -224,7 +225,7 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
     const uint32_t d_full = empty + 8 * kFp8MaxStages, d_empty = d_full + 16, sf_full = d_empty + 16, sf_empty = sf_full + 16;
     volatile int *abort_flag = &s_abort;
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (FORM != kFp8Dx) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 1) {
         auto count = [&](int i) {
             if (i < kFp8MaxStages) return RESIDENT ? 1 : 2;       // landed: the producers
@@ -251,11 +252,18 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
             asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
         }
     }
-    auto depend = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
+    // dw beside dx started when the kernels before dx were done (below), and reads nothing of dx's.  It waits for dx only in the end, for those who wait for it.
+    auto depend = [&] {
+        if (FORM != kFp8Dw || !p.beside) asm volatile("griddepcontrol.wait;" ::: "memory");
+    };
     tc_fence_before();
     __syncthreads();
     if (CG == 2) cluster_sync_all();  // the other CTA's barriers are there
     tc_fence_after();
+    if (FORM == kFp8Dx) {  // what dw reads is there as well
+        depend();
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    }
     const uint32_t tmem = s_tmem_base;
     const int fold = 1 << p.fold_log, part = kBlockRows >> p.fold_log;  // rows of a part
     Fp8Tiles tile;
@@ -736,6 +744,7 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
     }
 
     __syncwarp();
+    if (FORM == kFp8Dw && p.beside) asm volatile("griddepcontrol.wait;" ::: "memory");
     tc_fence_before();
     __syncthreads();
     if (CG == 2) cluster_sync_all();
@@ -913,7 +922,7 @@ static int launch_fp8_as(int form, const Fp8Plan &l, const Fp8Params &p, const F
 }
 
 static int launch_fp8_form(int form, const Fp8Codes &a, int rows, const Fp8Codes &b, int cols, int red, const void *numbers, int x_type, void *o, int o_type, void *z, int gelu,
-                           int sm_count, cudaStream_t stream)
+                           bool beside, int sm_count, cudaStream_t stream)
 {
     const Fp8Plan l = fp8_plan(form, rows, cols, red, numbers && !b.q ? x_type : TUNA_FP8, o_type, z != nullptr, sm_count);
     Fp8Params p;
@@ -925,6 +934,7 @@ static int launch_fp8_form(int form, const Fp8Codes &a, int rows, const Fp8Codes
     p.tile_cols = l.tile_cols; p.width = l.width; p.row_tiles = l.row_tiles; p.col_tiles = l.col_tiles;
     p.rows_inner = l.row_tiles < l.col_tiles;
     p.a_bytes = l.a_bytes; p.b_rows = l.b_rows; p.stages = l.stages; p.d_cols = l.d_cols;
+    p.beside = beside;
     p.ahead = form <= kFp8GatedProduct && cols <= kFp8AheadTokens;
     p.stagger = form <= kFp8GatedProduct && !l.fold_log;
     p.x_bf16 = x_type == TUNA_BF16; p.gelu = gelu; p.z_offset = l.z_offset;
@@ -963,17 +973,17 @@ static int launch_fp8_form(int form, const Fp8Codes &a, int rows, const Fp8Codes
 
 int launch_fp8_product(const Fp8ProductArgs &a)
 {
-    return launch_fp8_form(a.gated ? kFp8GatedProduct : kFp8Product, a.w, a.m, a.x, a.n, a.k, a.numbers, a.x_type, a.o, a.o_type, a.z, a.gelu, a.sm_count, a.stream);
+    return launch_fp8_form(a.gated ? kFp8GatedProduct : kFp8Product, a.w, a.m, a.x, a.n, a.k, a.numbers, a.x_type, a.o, a.o_type, a.z, a.gelu, false, a.sm_count, a.stream);
 }
 
 int launch_fp8_dx(const Fp8Codes &w, const Fp8Codes &dy, void *dx, int type, int m, int n, int k, int sm_count, cudaStream_t stream)
 {
-    return launch_fp8_form(kFp8Dx, w, k, dy, n, m, nullptr, TUNA_FP8, dx, type, nullptr, 0, sm_count, stream);
+    return launch_fp8_form(kFp8Dx, w, k, dy, n, m, nullptr, TUNA_FP8, dx, type, nullptr, 0, false, sm_count, stream);
 }
 
-int launch_fp8_dw(const Fp8Codes &x, const Fp8Codes &dy, void *dw, int type, int m, int n, int k, int sm_count, cudaStream_t stream)
+int launch_fp8_dw(const Fp8Codes &x, const Fp8Codes &dy, void *dw, int type, int m, int n, int k, bool beside, int sm_count, cudaStream_t stream)
 {
-    return launch_fp8_form(kFp8Dw, x, k, dy, m, n, nullptr, TUNA_FP8, dw, type, nullptr, 0, sm_count, stream);
+    return launch_fp8_form(kFp8Dw, x, k, dy, m, n, nullptr, TUNA_FP8, dw, type, nullptr, 0, beside, sm_count, stream);
 }
 
 }  // namespace tuna

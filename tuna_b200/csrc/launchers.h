@@ -123,10 +123,16 @@ struct Fp8Codes {
 // `chained`: part of a call whose next launch may start with this one, and waits for it before it reads what this one writes
 cudaError_t launch_fp8_quantize_rows(const void *x, int type, long long row_stride, void *q, void *s, int rows, int k, bool chained, cudaStream_t stream);
 // Column, square, or both: `to` by row and `to2` by column
-cudaError_t launch_fp8_quantize_tiles(const void *x, int type, long long row_stride, int blocks, const Fp8Codes &to, const Fp8Codes &to2, int rows, int k, bool chained,
-                                      cudaStream_t stream);
-// The gradients of a gated block's two projections, [rows, 2f], by row and by column (one of which may have null pointers: it is not wanted)
-cudaError_t launch_fp8_gated_gradient(const void *z, const void *dh, int type, int gelu, const Fp8Codes &by_row, const Fp8Codes &by_column, int rows, int f, cudaStream_t stream);
+cudaError_t launch_fp8_quantize_tiles(const void *x, int type, long long row_stride, int blocks, const Fp8Codes &to, const Fp8Codes &to2, int rows, int k, cudaStream_t stream);
+// What the products of a gradient's call multiply: dy [rows, cols], or the gradients of a gated block's two projections that z and dy = dh say, by row and by
+// column (null codes: not wanted), and x [rows, x_cols] by column (null codes: it is there).  The next launch may start with this one, and waits for it before it reads.
+struct Fp8GradientArgs {
+    const void *dy, *z, *x;
+    int type, x_type, gelu, rows, cols, x_cols;
+    Fp8Codes by_row, by_column, x_to;
+    cudaStream_t stream;
+};
+cudaError_t launch_fp8_gradient(const Fp8GradientArgs &a);
 cudaError_t launch_fp8_dequant(const void *q, const void *s, int blocks, void *o, int type, int rows, int k, cudaStream_t stream);
 
 struct Fp8ProductArgs {
@@ -138,8 +144,9 @@ struct Fp8ProductArgs {
     int sm_count;
 };
 int launch_fp8_product(const Fp8ProductArgs &a);
+// dx lets the next launch start when those before it are done; dw may be that launch (`beside`), and then runs beside it.
 int launch_fp8_dx(const Fp8Codes &w, const Fp8Codes &dy, void *dx, int type, int m, int n, int k, int sm_count, cudaStream_t stream);
-int launch_fp8_dw(const Fp8Codes &x, const Fp8Codes &dy, void *dw, int type, int m, int n, int k, int sm_count, cudaStream_t stream);
+int launch_fp8_dw(const Fp8Codes &x, const Fp8Codes &dy, void *dw, int type, int m, int n, int k, bool beside, int sm_count, cudaStream_t stream);
 // Whether the product takes tokens of this type as they are; otherwise it wants their codes and scales.
 bool fp8_gemm_takes(bool gated, int rows, int n, int red, int x_type, int sm_count);
 
