@@ -135,6 +135,31 @@ def test_gradients(f, n, k, kind):
     backward(f, n, k, kind, seed=f + n)
 
 
+@pytest.mark.parametrize("f,n,kind,dtype", [(2048, 2500, "silu", torch.bfloat16), (12800, 385, "gelu", torch.float16)])
+def test_gradients_of_many_tiles(f, n, kind, dtype):
+    """As many as stream through: more than two of 128 x 128 for every SM, and rows that end inside one."""
+    backward(f, n, 16, kind, seed=n, dtype=dtype)
+
+
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("f,n", [(2048, 2500), (256, 300), (144, 300)])
+def test_gradients_that_are_no_numbers_spoil_their_own_blocks(f, n, bad):
+    """Of dx the rows of tokens, of dw the rows of features, that have one."""
+    k = 16
+    (q, s), _ = weights(f, k, 3)
+    x, z, dh = (torch.randn(n, c, device="cuda", dtype=torch.bfloat16) for c in (k, 2 * f, f))
+    dh[7, 3] = dh[n - 1, f - 1] = bad
+    dx, dw = torch.empty(n, k, device="cuda"), torch.empty(2 * f, k, device="cuda")
+    tuna_b200.fp8_gated_backward(dh, z, x, None, q, s, dx, dw, f, n, k)
+    finish()
+    rows = torch.zeros(n, dtype=torch.bool, device="cuda")
+    rows[[7, n - 1]] = True
+    assert torch.equal(torch.isnan(dx), rows[:, None].expand(n, k))
+    rows = torch.zeros(2 * f, dtype=torch.bool, device="cuda")
+    rows[[3, f - 1, f + 3, 2 * f - 1]] = True
+    assert torch.equal(torch.isnan(dw), rows[:, None].expand(2 * f, k))
+
+
 @pytest.mark.parametrize("types", [(torch.float16, torch.float16, torch.float32), (torch.bfloat16, torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32, torch.float16)], ids=str)
 @pytest.mark.parametrize("codes", [False, True])
 def test_types_of_the_gradients(types, codes):

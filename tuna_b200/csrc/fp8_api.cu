@@ -93,7 +93,7 @@ static int backward(const void *dy, const void *z, int dy_type, const void *x, i
     if (dw) by_column = place(workspace, at, (size_t)n * m, word_bytes(n, m));
     Fp8GradientArgs g;
     g.dy = dy; g.z = z; g.x = x; g.type = dy_type; g.x_type = x_type; g.gelu = activation == TUNA_GELU; g.rows = n; g.cols = m; g.x_cols = k;
-    g.by_row = by_row; g.by_column = by_column; g.x_to = {nullptr, nullptr}; g.stream = stream;
+    g.by_row = by_row; g.by_column = by_column; g.x_to = {nullptr, nullptr}; g.stream = stream; g.sm_count = sms;
     if (dw && !packed) g.x_to = xt = place(workspace, at, (size_t)n * k, word_bytes(n, k));
     if (launch_fp8_gradient(g) != cudaSuccess) return TUNA_ERR_LAUNCH;
     if (dx) st = launch_fp8_dx({const_cast<void *>(q), const_cast<void *>(s)}, by_row, dx, dx_type, m, n, k, sms, stream);

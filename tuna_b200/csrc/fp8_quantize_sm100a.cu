@@ -1,7 +1,9 @@
 // Quantizers of the 8-bit block-scaled format (fp8_format.cuh), their inverse, and the quantizer of a gated block's gradients.
 #include <algorithm>
+#include <mutex>
 #include "launchers.h"
 #include "fp8_format.cuh"
+#include "sm100_ptx.cuh"
 
 namespace tuna {
 
@@ -234,6 +236,31 @@ struct Fp8Plain {
         }
     }
 };
+// Eight columns of a gated block's gradients: of the gate, dh u act'(g), and of the other projection, dh act(g); or of one of them.
+template <typename T, bool GELU>
+__device__ __forceinline__ void fp8_gated_row(const Mx8<T> &g, const Mx8<T> &u, const Mx8<T> &d, float (&of_gate)[8], float (&of_other)[8])
+{
+    float gv[8], uv[8], dv[8];
+    g.values(gv);
+    u.values(uv);
+    d.values(dv);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float sigma = fp8_gate<GELU>(gv[i]);
+        of_gate[i] = dv[i] * uv[i] * fp8_gate_slope<GELU>(gv[i], sigma);
+        of_other[i] = dv[i] * (gv[i] * sigma);
+    }
+}
+template <typename T, bool GELU>
+__device__ __forceinline__ void fp8_gated_row(const Mx8<T> &g, const Mx8<T> &u, const Mx8<T> &d, bool gate, float (&to)[8])
+{
+    float of_other[8];
+    fp8_gated_row<T, GELU>(g, u, d, to, of_other);
+    if (!gate)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) to[i] = of_other[i];
+}
+
 // Columns 0 .. f - 1: the gradient of a gated block's gate, dh u act'(g); f .. 2f - 1: of the other projection, dh act(g).  z = [g | u].  What bounds it is the
 // logistic function (two instructions of 16 lanes a clock and SM): where blocks end between the projections two parts share it, otherwise a tile is of either.
 template <typename T, bool GELU, int PARTS>
@@ -270,20 +297,8 @@ struct Fp8Gated {
             }
 #pragma unroll
             for (int r = 0; r < kBatch; ++r) {
-                float gv[8], uv[8], dv[8];
-                g[r].values(gv);
-                u[r].values(uv);
-                d[r].values(dv);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float sigma = fp8_gate<GELU>(gv[i]), of_gate = dv[i] * uv[i] * fp8_gate_slope<GELU>(gv[i], sigma), of_other = dv[i] * (gv[i] * sigma);
-                    if constexpr (PARTS == 2) {
-                        to.v[r0 + r][i] = of_gate;
-                        to.v[kLaneRows + r0 + r][i] = of_other;
-                    } else {
-                        to.v[r0 + r][i] = gate ? of_gate : of_other;
-                    }
-                }
+                if constexpr (PARTS == 2) fp8_gated_row<T, GELU>(g[r], u[r], d[r], to.v[r0 + r], to.v[kLaneRows + r0 + r]);
+                else fp8_gated_row<T, GELU>(g[r], u[r], d[r], gate, to.v[r0 + r]);
             }
         }
     }
@@ -297,18 +312,18 @@ struct Fp8TileShared {
     int none;  // a column's block is NaN
 };
 
-// One column of tiles; `at` of `tiles` of them.
+// The tile of columns kFp8Block ct .. and rows kFp8Block rt ..; `again`: `shared` was in use for another one.
 template <int WAYS, typename Source>  // WAYS: 1 << kFp8Row | 1 << kFp8Column, one of them, or 1 << kFp8Square
-__device__ __forceinline__ void fp8_quantize_tiles(const Source &src, uint8_t *q, uint8_t *s, uint8_t *q2, uint8_t *s2, int rows, int cols, int at_tile, int tiles,
-                                                   Fp8TileShared<Source::kParts> &shared)
+__device__ __forceinline__ void fp8_quantize_tile(Source &src, uint8_t *q, uint8_t *s, uint8_t *q2, uint8_t *s2, int rows, int cols, int ct, int rt, bool again,
+                                                  Fp8TileShared<Source::kParts> &shared)
 {
     constexpr bool kRows = WAYS & (1 << kFp8Row), kCols = WAYS & (1 << kFp8Column), kSquare = WAYS & (1 << kFp8Square);
     constexpr int kParts = Source::kParts, kWarps = Fp8Tile<kParts>::kWarps, kLaneRows = Fp8Tile<kParts>::kLaneRows;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row_tiles = div_up(rows, kFp8Block), col_blocks = div_up(cols, kFp8Block);
-    const int ct = src.column_tile(at_tile, tiles), col = ct * kFp8Block + (lane & 15) * 8, part_cols = src.part_cols();
+    const int col = ct * kFp8Block + (lane & 15) * 8, part_cols = src.part_cols();
     const size_t step = 2 * (size_t)cols;
-    for (int rt = blockIdx.y; rt < row_tiles; rt += gridDim.y) {
+    {
         const long long row0 = (long long)rt * kFp8Block + warp * Fp8Tile<kParts>::kRows + (lane >> 4);
         typename Source::Raw raw;
         src.load(raw, row0, col, rows, cols);
@@ -350,7 +365,7 @@ __device__ __forceinline__ void fp8_quantize_tiles(const Source &src, uint8_t *q
             }
         }
         if constexpr (kCols || kSquare) {
-            if (rt != (int)blockIdx.y) __syncthreads();  // what was there before has been read
+            if (again) __syncthreads();  // what was there before has been read
             uint8_t *to = (kRows ? q2 : q) + (size_t)row0 * cols + col, *words = kRows ? s2 : s;
             float inverse[kParts][8];
             uint32_t none[kParts] = {};
@@ -421,6 +436,14 @@ __device__ __forceinline__ void fp8_quantize_tiles(const Source &src, uint8_t *q
     }
 }
 
+// One column of tiles, number `at` of `tiles`.
+template <int WAYS, typename Source>
+__device__ __forceinline__ void fp8_quantize_tiles(Source src, uint8_t *q, uint8_t *s, uint8_t *q2, uint8_t *s2, int rows, int cols, int at, int tiles, Fp8TileShared<Source::kParts> &shared)
+{
+    const int ct = src.column_tile(at, tiles);
+    for (int rt = blockIdx.y; rt < div_up(rows, kFp8Block); rt += gridDim.y) fp8_quantize_tile<WAYS>(src, q, s, q2, s2, rows, cols, ct, rt, rt != (int)blockIdx.y, shared);
+}
+
 template <typename Source>
 __host__ __device__ constexpr int fp8_tile_ctas(int ways)  // of an SM: what registers there are for
 {
@@ -450,6 +473,102 @@ fp8_quantize_two_kernel(const Source src, uint8_t *q, uint8_t *s, uint8_t *q2, u
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if ((int)blockIdx.x < tiles) fp8_quantize_tiles<WAYS>(src, q, s, q2, s2, rows, cols, blockIdx.x, tiles, shared);
     else fp8_quantize_tiles<1 << kFp8Column>(x, xq, xs, xq, xs, rows, x_cols, blockIdx.x - tiles, gridDim.x - tiles, shared);
+}
+
+// ---- a gated block's gradients, streamed
+
+// The same numbers as Fp8Gated's of two parts, for many tiles: one CTA an SM walks through them, and TMA has the next tile's three boxes of 32 KB under way while one is worked
+// on.  Loaded by the lanes themselves, one tile a CTA, 14336 features of 2048 tokens took 115 us, most of it waiting: 512 threads of 128 registers leave no room for another
+// CTA that would work meanwhile.
+constexpr int kFp8BoxBytes = kFp8Block * kFp8Block * 2, kFp8StreamBytes = 2 * 3 * kFp8BoxBytes;
+
+template <typename T, bool GELU>
+struct Fp8GatedStaged {
+    int f, col_tiles, tiles, stride, next;  // the tile that is copied next, and how far apart the CTA's are
+    uint32_t box, bar;                      // of the tile that is loaded
+    const CUtensorMap *z, *dh;
+    using Raw = Fp8RawFloat;
+    static constexpr int kParts = 2;
+    __device__ __forceinline__ int part_cols() const { return f; }
+    __device__ __forceinline__ void copy()  // into the boxes at `box`
+    {
+        if (next >= tiles || threadIdx.x) return;
+        const int rt = next / col_tiles, c = (next - rt * col_tiles) * kFp8Block;
+        mbar_expect_tx(bar, 3 * kFp8BoxBytes);
+        tma_load_2d(box, z, c, rt * kFp8Block, bar);
+        tma_load_2d(box + kFp8BoxBytes, z, f + c, rt * kFp8Block, bar);
+        tma_load_2d(box + 2 * kFp8BoxBytes, dh, c, rt * kFp8Block, bar);
+    }
+    __device__ __forceinline__ void load(Raw &to, long long, int, int, int)
+    {
+        constexpr int kLaneRows = Fp8Tile<2>::kLaneRows;
+        const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+        auto piece = [](uint32_t at) {
+            Mx8<T> v;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.r.x), "=r"(v.r.y), "=r"(v.r.z), "=r"(v.r.w) : "r"(at) : "memory");
+            return v;
+        };
+#pragma unroll
+        for (int r = 0; r < kLaneRows; ++r) {
+            const uint32_t at = box + (uint32_t)(warp * Fp8Tile<2>::kRows + 2 * r + (lane >> 4)) * (2 * kFp8Block) + (uint32_t)(lane & 15) * 16u;
+            fp8_gated_row<T, GELU>(piece(at), piece(at + kFp8BoxBytes), piece(at + 2 * kFp8BoxBytes), to.v[r], to.v[kLaneRows + r]);
+        }
+        __syncthreads();  // everybody has read the boxes
+        copy();
+        next += stride;
+    }
+};
+
+template <typename T, bool GELU, int WAYS>
+__global__ void __launch_bounds__(512, 1)
+fp8_gated_stream_kernel(const __grid_constant__ CUtensorMap tmap_z, const __grid_constant__ CUtensorMap tmap_dh, uint8_t *q, uint8_t *s, uint8_t *q2, uint8_t *s2, int rows, int f,
+                        DeviceStatus *status)
+{
+    extern __shared__ __align__(128) uint8_t boxes[];
+    __shared__ __align__(16) Fp8TileShared<2> shared;
+    __shared__ __align__(8) uint64_t bars[2];
+    __shared__ int s_abort;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (threadIdx.x == 0) {
+        s_abort = 0;
+        mbar_init(smem_u32(&bars[0]), 1);
+        mbar_init(smem_u32(&bars[1]), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_map(&tmap_z);
+        prefetch_map(&tmap_dh);
+    }
+    __syncthreads();
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    Fp8GatedStaged<T, GELU> src;
+    src.f = f;
+    src.col_tiles = f / kFp8Block;
+    src.tiles = src.col_tiles * div_up(rows, kFp8Block);
+    src.stride = gridDim.x;
+    src.next = blockIdx.x;
+    src.z = &tmap_z;
+    src.dh = &tmap_dh;
+    auto turn = [&](int b) {
+        src.box = smem_u32(boxes) + (uint32_t)(b * 3 * kFp8BoxBytes);
+        src.bar = smem_u32(&bars[b]);
+    };
+    for (int b = 0; b < 2; ++b) {
+        turn(b);
+        src.copy();
+        src.next += src.stride;
+    }
+    int turns = 0;
+    for (int t = blockIdx.x; t < src.tiles; t += gridDim.x, ++turns) {
+        turn(turns & 1);
+        const bool ok = mbar_wait(src.bar, (uint32_t)(turns >> 1) & 1u, &s_abort, status, 320);
+        if (__syncthreads_or(!ok)) {  // given up: no copy may land in what is no longer this CTA's
+            if (threadIdx.x == 0)
+                for (int i = 0; i < 2; ++i)
+                    for (const long long t0 = clock64(); !mbar_try_wait(smem_u32(&bars[(turns + i) & 1]), (uint32_t)((turns + i) >> 1) & 1u) && t + i * (int)gridDim.x < src.tiles && clock64() - t0 < kWaitCycles;) {}
+            return;
+        }
+        const int rt = t / src.col_tiles;
+        fp8_quantize_tile<WAYS>(src, q, s, q2, s2, rows, 2 * f, t - rt * src.col_tiles, rt, turns > 0, shared);
+    }
 }
 
 // What a launch quantizes beside its own matrix: nothing where q is null.
@@ -518,10 +637,55 @@ cudaError_t launch_fp8_quantize_tiles(const void *x, int type, long long row_str
     }
 }
 
+template <typename T>
+static cudaError_t second_alone(const Fp8Second &x, int rows, cudaStream_t stream)
+{
+    return tile_launch<1 << kFp8Column>(Fp8Plain<T, 1>{(const T *)x.x, x.cols}, div_up(x.cols, kFp8Block), x.to, x.to, rows, x.cols, true, stream);
+}
+
+template <typename T, bool GELU, int WAYS>
+static cudaError_t stream_launch(const Fp8GradientArgs &a, const Fp8Codes &to, const Fp8Codes &to2)
+{
+    static bool attr_set[64] = {false};
+    static std::mutex mu;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || dev < 0 || dev >= 64) return e != cudaSuccess ? e : cudaErrorInvalidDevice;
+    {
+        std::lock_guard<std::mutex> lock(mu);
+        if (!attr_set[dev]) {
+            e = cudaFuncSetAttribute(fp8_gated_stream_kernel<T, GELU, WAYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp8StreamBytes);
+            if (e != cudaSuccess) return e;
+            attr_set[dev] = true;
+        }
+    }
+    const int f = a.cols / 2;
+    CUtensorMap z, dh;
+    const CUtensorMapDataType type = sizeof(T) == 2 && a.type == TUNA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    DeviceStatus *status = device_status_word();
+    if (!status || !make_tensor_map_2d(&z, type, a.z, (uint64_t)a.cols, (uint64_t)a.rows, (uint64_t)a.cols * 2, kFp8Block, kFp8Block, CU_TENSOR_MAP_SWIZZLE_NONE) ||
+        !make_tensor_map_2d(&dh, type, a.dy, (uint64_t)f, (uint64_t)a.rows, (uint64_t)f * 2, kFp8Block, kFp8Block, CU_TENSOR_MAP_SWIZZLE_NONE))
+        return cudaErrorUnknown;
+    cudaLaunchAttribute attr;
+    cudaLaunchConfig_t lc = tile_config(a.sm_count, 1, 512, true, attr, a.stream);
+    lc.dynamicSmemBytes = kFp8StreamBytes;
+    return cudaLaunchKernelEx(&lc, fp8_gated_stream_kernel<T, GELU, WAYS>, z, dh, (uint8_t *)to.q, (uint8_t *)to.s, (uint8_t *)to2.q, (uint8_t *)to2.s, a.rows, f, status);
+}
+
 template <typename T, bool GELU>
 static cudaError_t gated_gradient(const Fp8GradientArgs &a, const Fp8Second &x)
 {
     const int f = a.cols / 2;
+    const long long tiles = (long long)(f / kFp8Block) * div_up(a.rows, kFp8Block);
+    if (f % kFp8Block == 0 && tiles >= 2 * a.sm_count && tiles < 1 << 30) {
+        if (x.to.q) {
+            const cudaError_t e = second_alone<T>(x, a.rows, a.stream);
+            if (e != cudaSuccess) return e;
+        }
+        if (a.by_row.q && a.by_column.q) return stream_launch<T, GELU, 1 << kFp8Row | 1 << kFp8Column>(a, a.by_row, a.by_column);
+        if (a.by_row.q) return stream_launch<T, GELU, 1 << kFp8Row>(a, a.by_row, a.by_row);
+        return stream_launch<T, GELU, 1 << kFp8Column>(a, a.by_column, a.by_column);
+    }
     if (f % kFp8Block == 0)
         return gradient_ways<T>(Fp8Gated<T, GELU, 2>{(const T *)a.z, (const T *)a.dy, f}, f / kFp8Block, a.by_row, a.by_column, a.rows, a.cols, x, a.stream);
     return gradient_ways<T>(Fp8Gated<T, GELU, 1>{(const T *)a.z, (const T *)a.dy, f}, div_up(a.cols, kFp8Block), a.by_row, a.by_column, a.rows, a.cols, x, a.stream);
@@ -533,12 +697,6 @@ static cudaError_t gradient_of(const Fp8GradientArgs &a, const Fp8Second &x)
     if (a.z) return a.gelu ? gated_gradient<T, true>(a, x) : gated_gradient<T, false>(a, x);
     if (!a.by_column.q) return launch_fp8_quantize_rows(a.dy, a.type, a.cols, a.by_row.q, a.by_row.s, a.rows, a.cols, true, a.stream);
     return gradient_ways<T>(Fp8Plain<T, 1>{(const T *)a.dy, a.cols}, div_up(a.cols, kFp8Block), a.by_row, a.by_column, a.rows, a.cols, x, a.stream);
-}
-
-template <typename T>
-static cudaError_t second_alone(const Fp8Second &x, int rows, cudaStream_t stream)
-{
-    return tile_launch<1 << kFp8Column>(Fp8Plain<T, 1>{(const T *)x.x, x.cols}, div_up(x.cols, kFp8Block), x.to, x.to, rows, x.cols, true, stream);
 }
 
 cudaError_t launch_fp8_gradient(const Fp8GradientArgs &a)

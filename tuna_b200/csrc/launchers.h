@@ -131,6 +131,7 @@ struct Fp8GradientArgs {
     int type, x_type, gelu, rows, cols, x_cols;
     Fp8Codes by_row, by_column, x_to;
     cudaStream_t stream;
+    int sm_count;
 };
 cudaError_t launch_fp8_gradient(const Fp8GradientArgs &a);
 cudaError_t launch_fp8_dequant(const void *q, const void *s, int blocks, void *o, int type, int rows, int k, cudaStream_t stream);
