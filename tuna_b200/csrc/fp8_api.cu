@@ -76,7 +76,7 @@ static int backward(const void *dy, const void *z, int dy_type, const void *x, i
 {
     const bool packed = x_type == TUNA_FP8;
     if (!dy || (!dx && !dw) || (dx && (!q || !s)) || (dw && (!x || (packed && !xs)))) return TUNA_ERR_NULL_POINTER;
-    int st = check_sizes(m, n, k);
+    const int st = check_sizes(m, n, k);
     if (st != TUNA_OK) return st;
     if (!is_16bit(dy_type) || (dx && !is_number_type(dx_type)) || (dw && (!is_number_type(dw_type) || (!packed && !is_16bit(x_type)))) ||
         (activation != TUNA_SILU && activation != TUNA_GELU))
@@ -86,19 +86,19 @@ static int backward(const void *dy, const void *z, int dy_type, const void *x, i
         return TUNA_ERR_MISALIGNED;
     const size_t need = backward_workspace(dx, dw, m, n, k, x_type);
     if (need > 0 && (!workspace || workspace_bytes < need)) return TUNA_ERR_WORKSPACE;
-    const int sms = device_sm_count();
     size_t at = 0;
     Fp8Codes by_row = {nullptr, nullptr}, by_column = {nullptr, nullptr}, xt = {const_cast<void *>(x), const_cast<void *>(xs)};
     if (dx) by_row = place(workspace, at, (size_t)n * m, word_bytes(m, n));
     if (dw) by_column = place(workspace, at, (size_t)n * m, word_bytes(n, m));
-    Fp8GradientArgs g;
+    Fp8BackwardArgs a;
+    Fp8GradientArgs &g = a.operands;
     g.dy = dy; g.z = z; g.x = x; g.type = dy_type; g.x_type = x_type; g.gelu = activation == TUNA_GELU; g.rows = n; g.cols = m; g.x_cols = k;
-    g.by_row = by_row; g.by_column = by_column; g.x_to = {nullptr, nullptr}; g.stream = stream; g.sm_count = sms;
+    g.by_row = by_row; g.by_column = by_column; g.x_to = {nullptr, nullptr}; g.stream = stream; g.sm_count = device_sm_count();
     if (dw && !packed) g.x_to = xt = place(workspace, at, (size_t)n * k, word_bytes(n, k));
-    if (launch_fp8_gradient(g) != cudaSuccess) return TUNA_ERR_LAUNCH;
-    if (dx) st = launch_fp8_dx({const_cast<void *>(q), const_cast<void *>(s)}, by_row, dx, dx_type, m, n, k, sms, stream);
-    if (dw && st == TUNA_OK) st = launch_fp8_dw(xt, by_column, dw, dw_type, m, n, k, dx != nullptr, sms, stream);
-    return st;
+    a.w = {const_cast<void *>(q), const_cast<void *>(s)};
+    a.x = xt;
+    a.dx = dx; a.dw = dw; a.dx_type = dx_type; a.dw_type = dw_type;
+    return launch_fp8_backward(a);
 }
 
 }  // namespace tuna

@@ -81,7 +81,7 @@ struct Fp8Params {
     int stages;
     int d_cols;      // tensor-memory columns of each of the two accumulators: columns of a tile times fold
     int ahead;       // A is there before the dependency wait
-    int beside;      // dw: launched right behind the dx of its call
+    int beside;      // dx and dw of one call: dw is launched right behind dx
     int x_bf16;      // RESIDENT: type of the tokens
     const void *x;   // RESIDENT: the tokens [cols][red]
     int stagger;     // row tiles start their sums at different groups
@@ -200,8 +200,7 @@ __device__ __forceinline__ float fp8_activation(float g, float u, int gelu) { re
 
 // CG: CTAs of a worker (1 or 2).  Single CTAs leave room for a second one on the SM: that of the next launch, which copies its first weights meanwhile.
 template <int CG, int FORM, bool RESIDENT, typename OT>
-__global__ void __launch_bounds__(32 * fp8_warps(CG), CG == 1 ? 2 : 1)
-fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a2, const __grid_constant__ CUtensorMap tmap_b)
+__device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &tmap_a, const CUtensorMap &tmap_a2, const CUtensorMap &tmap_b, int worker, int workers)
 {
     extern __shared__ __align__(1024) uint8_t smem[];
     // landed, full, empty: of the stages; d_full, d_empty, sf_full, sf_empty: two each
@@ -213,7 +212,6 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
     constexpr uint32_t kTmemCols = CG == 1 ? 256 : 512, kSfCol = kTmemCols - 2 * kFp8SfCols;  // two accumulators below
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = CG == 1 ? 0 : (int)cluster_ctarank();
-    const int worker = blockIdx.x / CG, workers = gridDim.x / CG;
     const int N = p.tile_cols, S = p.stages;
     // [stages of A][of B][words of the resident tokens' scales][staging buffer]; the MMAs read 128 rows of A, in low tiles past their stage's end.
     // RESIDENT: of B, all of a tile's stages.
@@ -225,7 +223,7 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
     const uint32_t d_full = empty + 8 * kFp8MaxStages, d_empty = d_full + 16, sf_full = d_empty + 16, sf_empty = sf_full + 16;
     volatile int *abort_flag = &s_abort;
 
-    if (FORM != kFp8Dx) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (FORM != kFp8Dx || !p.beside) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (warp == 1) {
         auto count = [&](int i) {
             if (i < kFp8MaxStages) return RESIDENT ? 1 : 2;       // landed: the producers
@@ -260,7 +258,7 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
     __syncthreads();
     if (CG == 2) cluster_sync_all();  // the other CTA's barriers are there
     tc_fence_after();
-    if (FORM == kFp8Dx) {  // what dw reads is there as well
+    if (FORM == kFp8Dx && p.beside) {  // what dw reads is there as well
         depend();
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     }
@@ -755,6 +753,24 @@ fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUt
     }
 }
 
+template <int CG, int FORM, bool RESIDENT, typename OT>
+__global__ void __launch_bounds__(32 * fp8_warps(CG), CG == 1 ? 2 : 1)
+fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a2, const __grid_constant__ CUtensorMap tmap_b)
+{
+    fp8_gemm<CG, FORM, RESIDENT, OT>(p, tmap_a, tmap_a2, tmap_b, blockIdx.x / CG, gridDim.x / CG);
+}
+
+// dx and dw in one launch, the first `dx_pairs` pairs and the others: where neither fills the device.
+template <typename XT, typename WT>
+__global__ void __launch_bounds__(32 * fp8_warps(2), 1)
+fp8_gradients_kernel(const __grid_constant__ Fp8Params dx, const __grid_constant__ CUtensorMap dx_a, const __grid_constant__ CUtensorMap dx_b, const __grid_constant__ Fp8Params dw,
+                     const __grid_constant__ CUtensorMap dw_a, const __grid_constant__ CUtensorMap dw_b, int dx_pairs)
+{
+    const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
+    if (pair < dx_pairs) fp8_gemm<2, kFp8Dx, false, XT>(dx, dx_a, dx_a, dx_b, pair, dx_pairs);
+    else fp8_gemm<2, kFp8Dw, false, WT>(dw, dw_a, dw_a, dw_b, pair - dx_pairs, pairs - dx_pairs);
+}
+
 // ------------------------------------------------------------------ host side
 
 struct Fp8Plan {
@@ -875,20 +891,10 @@ struct Fp8Maps {
     CUtensorMap a, a2, b;
 };
 
-template <int CG, int FORM, bool RESIDENT, typename OT>
-static int launch_fp8(const Fp8Params &p, const Fp8Maps &maps, int ctas, size_t smem, cudaStream_t stream)
+// Launches a kernel on `ctas` CTAs, CG of a cluster.
+template <int CG, typename... Params, typename... Args>
+static int launch_fp8_kernel(void (*kernel)(Params...), int ctas, size_t smem, cudaStream_t stream, const Args &...args)
 {
-    static bool attr_set[64] = {false};
-    static std::mutex mu;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TUNA_ERR_NO_DEVICE;
-    {
-        std::lock_guard<std::mutex> lock(mu);
-        if (!attr_set[dev]) {
-            if (cudaFuncSetAttribute(fp8_gemm_kernel<CG, FORM, RESIDENT, OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp8SmemMax) != cudaSuccess) return TUNA_ERR_NO_DEVICE;
-            attr_set[dev] = true;
-        }
-    }
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3((unsigned)ctas);
     lc.blockDim = dim3(32 * fp8_warps(CG));
@@ -902,30 +908,73 @@ static int launch_fp8(const Fp8Params &p, const Fp8Maps &maps, int ctas, size_t 
     attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     lc.attrs = attr;
     lc.numAttrs = CG == 1 ? 1 : 2;
-    return cudaLaunchKernelEx(&lc, fp8_gemm_kernel<CG, FORM, RESIDENT, OT>, p, maps.a, maps.a2, maps.b) == cudaSuccess ? TUNA_OK : TUNA_ERR_LAUNCH;
+    return cudaLaunchKernelEx(&lc, kernel, args...) == cudaSuccess ? TUNA_OK : TUNA_ERR_LAUNCH;
 }
+
+// Once a device: the kernel may have as much shared memory as it asks for.
+struct Fp8Allowed {
+    bool set[64] = {false};
+    std::mutex mu;
+    int allow(const void *kernel)
+    {
+        int dev = 0;
+        if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TUNA_ERR_NO_DEVICE;
+        std::lock_guard<std::mutex> lock(mu);
+        if (!set[dev] && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp8SmemMax) != cudaSuccess) return TUNA_ERR_NO_DEVICE;
+        set[dev] = true;
+        return TUNA_OK;
+    }
+};
+
+template <int CG, int FORM, bool RESIDENT, typename OT>
+static int launch_fp8(const Fp8Params &p, const Fp8Maps &maps, int ctas, size_t smem, cudaStream_t stream)
+{
+    static Fp8Allowed allowed;
+    const int st = allowed.allow((const void *)fp8_gemm_kernel<CG, FORM, RESIDENT, OT>);
+    return st != TUNA_OK ? st : launch_fp8_kernel<CG>(fp8_gemm_kernel<CG, FORM, RESIDENT, OT>, ctas, smem, stream, p, maps.a, maps.a2, maps.b);
+}
+
+// A launch: plan, parameters and tensor maps.
+struct Fp8Launch {
+    int form, o_type;
+    Fp8Plan l;
+    Fp8Params p;
+    Fp8Maps maps;
+    int pairs() const { return (int)std::min<long long>((long long)l.row_tiles * l.col_tiles, l.workers); }  // or single CTAs
+};
 
 template <typename OT>
-static int launch_fp8_as(int form, const Fp8Plan &l, const Fp8Params &p, const Fp8Maps &maps, cudaStream_t stream)
+static int launch_fp8_as(const Fp8Launch &a, cudaStream_t stream)
 {
-    const int ctas = l.workers * l.cg;
+    const Fp8Plan &l = a.l;
+    const int ctas = a.pairs() * l.cg;
     if (l.cg == 1) {
-        if (form == kFp8Product) return l.resident ? launch_fp8<1, kFp8Product, true, OT>(p, maps, ctas, l.smem, stream) : launch_fp8<1, kFp8Product, false, OT>(p, maps, ctas, l.smem, stream);
-        return l.resident ? launch_fp8<1, kFp8GatedProduct, true, OT>(p, maps, ctas, l.smem, stream) : launch_fp8<1, kFp8GatedProduct, false, OT>(p, maps, ctas, l.smem, stream);
+        if (a.form == kFp8Product) return l.resident ? launch_fp8<1, kFp8Product, true, OT>(a.p, a.maps, ctas, l.smem, stream) : launch_fp8<1, kFp8Product, false, OT>(a.p, a.maps, ctas, l.smem, stream);
+        return l.resident ? launch_fp8<1, kFp8GatedProduct, true, OT>(a.p, a.maps, ctas, l.smem, stream) : launch_fp8<1, kFp8GatedProduct, false, OT>(a.p, a.maps, ctas, l.smem, stream);
     }
-    switch (form) {
-        case kFp8Product: return launch_fp8<2, kFp8Product, false, OT>(p, maps, ctas, l.smem, stream);
-        case kFp8GatedProduct: return launch_fp8<2, kFp8GatedProduct, false, OT>(p, maps, ctas, l.smem, stream);
-        case kFp8Dx: return launch_fp8<2, kFp8Dx, false, OT>(p, maps, ctas, l.smem, stream);
-        default: return launch_fp8<2, kFp8Dw, false, OT>(p, maps, ctas, l.smem, stream);
+    switch (a.form) {
+        case kFp8Product: return launch_fp8<2, kFp8Product, false, OT>(a.p, a.maps, ctas, l.smem, stream);
+        case kFp8GatedProduct: return launch_fp8<2, kFp8GatedProduct, false, OT>(a.p, a.maps, ctas, l.smem, stream);
+        case kFp8Dx: return launch_fp8<2, kFp8Dx, false, OT>(a.p, a.maps, ctas, l.smem, stream);
+        default: return launch_fp8<2, kFp8Dw, false, OT>(a.p, a.maps, ctas, l.smem, stream);
     }
 }
 
-static int launch_fp8_form(int form, const Fp8Codes &a, int rows, const Fp8Codes &b, int cols, int red, const void *numbers, int x_type, void *o, int o_type, void *z, int gelu,
-                           bool beside, int sm_count, cudaStream_t stream)
+static int launch_fp8_any(const Fp8Launch &a, cudaStream_t stream)
+{
+    switch (a.o_type) {
+        case TUNA_FP16: return launch_fp8_as<__half>(a, stream);
+        case TUNA_BF16: return launch_fp8_as<__nv_bfloat16>(a, stream);
+        default: return launch_fp8_as<float>(a, stream);
+    }
+}
+
+// x_type: of tokens that the product takes as they are, otherwise TUNA_FP8
+static int prepare_fp8(Fp8Launch &out, int form, const Fp8Codes &a, int rows, const Fp8Codes &b, int cols, int red, const void *numbers, int x_type, void *o, int o_type, void *z, int gelu,
+                       int sm_count)
 {
     const Fp8Plan l = fp8_plan(form, rows, cols, red, numbers && !b.q ? x_type : TUNA_FP8, o_type, z != nullptr, sm_count);
-    Fp8Params p;
+    Fp8Params &p = out.p;
     std::memset(&p, 0, sizeof(p));
     p.as = (const uint8_t *)a.s; p.bs = (const uint8_t *)b.s; p.o = o; p.z = z; p.x = numbers;
     p.rows = rows; p.cols = cols; p.red = red;
@@ -934,7 +983,6 @@ static int launch_fp8_form(int form, const Fp8Codes &a, int rows, const Fp8Codes
     p.tile_cols = l.tile_cols; p.width = l.width; p.row_tiles = l.row_tiles; p.col_tiles = l.col_tiles;
     p.rows_inner = l.row_tiles < l.col_tiles;
     p.a_bytes = l.a_bytes; p.b_rows = l.b_rows; p.stages = l.stages; p.d_cols = l.d_cols;
-    p.beside = beside;
     p.ahead = form <= kFp8GatedProduct && cols <= kFp8AheadTokens;
     p.stagger = form <= kFp8GatedProduct && !l.fold_log;
     p.x_bf16 = x_type == TUNA_BF16; p.gelu = gelu; p.z_offset = l.z_offset;
@@ -944,7 +992,7 @@ static int launch_fp8_form(int form, const Fp8Codes &a, int rows, const Fp8Codes
     const long long tiles = (long long)p.row_tiles * p.col_tiles;
     if (tiles >= 1ll << 30 || (tiles / l.workers + 2) * p.units >= 1ll << 30) return TUNA_ERR_TOO_LARGE;
 
-    Fp8Maps maps;
+    Fp8Maps &maps = out.maps;
     auto matrix = [](CUtensorMap *map, const void *at, int inner, int outer, int box_outer) {  // row by row; boxes of 128 columns
         return make_tensor_map_2d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, at, (uint64_t)inner, (uint64_t)outer, (uint64_t)inner, kFp8Block, (uint32_t)box_outer, CU_TENSOR_MAP_SWIZZLE_128B);
     };
@@ -963,27 +1011,68 @@ static int launch_fp8_form(int form, const Fp8Codes &a, int rows, const Fp8Codes
     maps.a2 = maps.b = maps.a;
     if (l.cg == 1 && rows / 4 % l.row_tiles && !weights(&maps.a2, 4 * (rows / 4 / l.row_tiles))) return TUNA_ERR_NO_DEVICE;
     if (!l.resident && !(form == kFp8Dw ? matrix(&maps.b, b.q, cols, red, kFp8Block) : matrix(&maps.b, b.q, red, cols, l.b_rows))) return TUNA_ERR_NO_DEVICE;
-    if (numbers && b.q && launch_fp8_quantize_rows(numbers, x_type, red, b.q, b.s, cols, red, true, stream) != cudaSuccess) return TUNA_ERR_LAUNCH;
-    switch (o_type) {
-        case TUNA_FP16: return launch_fp8_as<__half>(form, l, p, maps, stream);
-        case TUNA_BF16: return launch_fp8_as<__nv_bfloat16>(form, l, p, maps, stream);
-        default: return launch_fp8_as<float>(form, l, p, maps, stream);
-    }
+    out.form = form;
+    out.o_type = o_type;
+    out.l = l;
+    return TUNA_OK;
 }
 
 int launch_fp8_product(const Fp8ProductArgs &a)
 {
-    return launch_fp8_form(a.gated ? kFp8GatedProduct : kFp8Product, a.w, a.m, a.x, a.n, a.k, a.numbers, a.x_type, a.o, a.o_type, a.z, a.gelu, false, a.sm_count, a.stream);
+    Fp8Launch launch;
+    const int st = prepare_fp8(launch, a.gated ? kFp8GatedProduct : kFp8Product, a.w, a.m, a.x, a.n, a.k, a.numbers, a.x_type, a.o, a.o_type, a.z, a.gelu, a.sm_count);
+    if (st != TUNA_OK) return st;
+    if (a.numbers && a.x.q && launch_fp8_quantize_rows(a.numbers, a.x_type, a.k, a.x.q, a.x.s, a.n, a.k, true, a.stream) != cudaSuccess) return TUNA_ERR_LAUNCH;
+    return launch_fp8_any(launch, a.stream);
 }
 
-int launch_fp8_dx(const Fp8Codes &w, const Fp8Codes &dy, void *dx, int type, int m, int n, int k, int sm_count, cudaStream_t stream)
+template <typename XT, typename WT>
+static int launch_fp8_both(const Fp8Launch &dx, const Fp8Launch &dw, cudaStream_t stream)
 {
-    return launch_fp8_form(kFp8Dx, w, k, dy, n, m, nullptr, TUNA_FP8, dx, type, nullptr, 0, false, sm_count, stream);
+    static Fp8Allowed allowed;
+    const int st = allowed.allow((const void *)fp8_gradients_kernel<XT, WT>), dx_pairs = dx.pairs();
+    return st != TUNA_OK ? st : launch_fp8_kernel<2>(fp8_gradients_kernel<XT, WT>, 2 * (dx_pairs + dw.pairs()), std::max(dx.l.smem, dw.l.smem), stream, dx.p, dx.maps.a, dx.maps.b, dw.p,
+                                                     dw.maps.a, dw.maps.b, dx_pairs);
+}
+template <typename XT>
+static int launch_fp8_both_as(const Fp8Launch &dx, const Fp8Launch &dw, cudaStream_t stream)
+{
+    switch (dw.o_type) {
+        case TUNA_FP16: return launch_fp8_both<XT, __half>(dx, dw, stream);
+        case TUNA_BF16: return launch_fp8_both<XT, __nv_bfloat16>(dx, dw, stream);
+        default: return launch_fp8_both<XT, float>(dx, dw, stream);
+    }
 }
 
-int launch_fp8_dw(const Fp8Codes &x, const Fp8Codes &dy, void *dw, int type, int m, int n, int k, bool beside, int sm_count, cudaStream_t stream)
+int launch_fp8_backward(const Fp8BackwardArgs &a)
 {
-    return launch_fp8_form(kFp8Dw, x, k, dy, m, n, nullptr, TUNA_FP8, dw, type, nullptr, 0, beside, sm_count, stream);
+    const Fp8GradientArgs &g = a.operands;
+    const int m = g.cols, n = g.rows, k = g.x_cols;
+    Fp8Launch dx, dw;
+    auto plan = [&](int sms) {
+        int st = a.dx ? prepare_fp8(dx, kFp8Dx, a.w, k, g.by_row, n, m, nullptr, TUNA_FP8, a.dx, a.dx_type, nullptr, 0, sms) : TUNA_OK;
+        if (st == TUNA_OK && a.dw) st = prepare_fp8(dw, kFp8Dw, a.x, k, g.by_column, m, n, nullptr, TUNA_FP8, a.dw, a.dw_type, nullptr, 0, sms);
+        return st;
+    };
+    int st = plan(g.sm_count);
+    if (st != TUNA_OK) return st;
+    // Up to 2^35 products side by side in one launch, half of the pairs each; above, dw behind dx, and beside it where that leaves pairs idle (us, one launch / two:
+    // 1552x1040 at 301 tokens 14.7 / 19.5, 2048x2048 at 256 17.2 / 22.9, at 1024 23.5 / 27.6, 6144x4096 at 300 41.4 / 40.7, at 1024 61.2 / 64.5, at 4096 195 / 190, 28672x4096 at 2048
+    // 547 / 450 to 490).
+    const bool together = a.dx && a.dw && (double)m * n * k <= (double)(1ll << 35);
+    if (together && (st = plan(g.sm_count / 2)) != TUNA_OK) return st;
+    if (launch_fp8_gradient(g) != cudaSuccess) return TUNA_ERR_LAUNCH;
+    if (!a.dx || !a.dw) return launch_fp8_any(a.dx ? dx : dw, g.stream);
+    if (together) {
+        switch (a.dx_type) {
+            case TUNA_FP16: return launch_fp8_both_as<__half>(dx, dw, g.stream);
+            case TUNA_BF16: return launch_fp8_both_as<__nv_bfloat16>(dx, dw, g.stream);
+            default: return launch_fp8_both_as<float>(dx, dw, g.stream);
+        }
+    }
+    dx.p.beside = dw.p.beside = 1;
+    st = launch_fp8_any(dx, g.stream);
+    return st != TUNA_OK ? st : launch_fp8_any(dw, g.stream);
 }
 
 }  // namespace tuna

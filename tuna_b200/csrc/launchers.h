@@ -145,9 +145,13 @@ struct Fp8ProductArgs {
     int sm_count;
 };
 int launch_fp8_product(const Fp8ProductArgs &a);
-// dx lets the next launch start when those before it are done; dw may be that launch (`beside`), and then runs beside it.
-int launch_fp8_dx(const Fp8Codes &w, const Fp8Codes &dy, void *dx, int type, int m, int n, int k, int sm_count, cudaStream_t stream);
-int launch_fp8_dw(const Fp8Codes &x, const Fp8Codes &dy, void *dw, int type, int m, int n, int k, bool beside, int sm_count, cudaStream_t stream);
+struct Fp8BackwardArgs {
+    Fp8GradientArgs operands;
+    Fp8Codes w, x;  // w for dx; x by column, for dw
+    void *dx, *dw;  // null: not wanted
+    int dx_type, dw_type;
+};
+int launch_fp8_backward(const Fp8BackwardArgs &a);
 // Whether the product takes tokens of this type as they are; otherwise it wants their codes and scales.
 bool fp8_gemm_takes(bool gated, int rows, int n, int red, int x_type, int sm_count);
 
