@@ -16,20 +16,26 @@
 // gated: a tile's rows are, by a four-dimensional tensor map, eight of the gate and the eight of the other projection that belong to them in turn.  So
 // the fragments that a thread takes out of tensor memory (lanes i and i + 8) hold both factors, and the product is made in its registers.
 //
-// Persistent CTAs (up to 16 tokens), or pairs of CTAs (cta_group::2: 256 rows of A, every CTA stages its own 128 and half of B), of 12 warps:
+// Persistent CTAs (12 warps), or pairs of CTAs (cta_group::2, 16 warps: 256 rows of A, every CTA stages its own 128 and half of B):
 //   warp 0     MMA issue (one elected lane; in a pair the first CTA's)
 //   warp 1, 2  TMA producers of A and of B
 //   warp 3     tensor-memory allocation; in a pair, tells the first CTA that a stage has landed
 //   warps 4-7  epilogue: tensor memory -> registers -> output type -> shared memory, where rows become contiguous -> memory; in a pair 12-15 too
-//   warps 8-11 scales, one warp per lane quarter: global memory -> registers, a group of four stages ahead -> tensor memory, the word of row r at lane r % 32,
+//   warps 8-11 scales, one warp per lane quarter: global memory -> registers, two groups of four units ahead -> tensor memory, the word of row r at lane r % 32,
 //              column r / 32, in every quarter
 // RESIDENT: a few tokens in 16 bits are quantized by the CTA itself before its first MMA, all of K, and stay in shared memory.
 //
-// Work split.  No sum is cut.  Up to 16 tokens the weights are cut into row tiles of equal height, a whole number of them for every CTA: the MMAs compute 128
+// Work split.  No sum is cut.  Up to 16 tokens weights of few rows are cut into row tiles of equal height, a whole number of them for every CTA: the MMAs compute 128
 // rows whatever the height, which costs nothing where the weights' bytes are the bound.  Where a tile has at most 64 (32) of the
 // 128 rows, two (four) blocks of K lie side by side in it ("folded"): the MMA's rows are those of the tile for each block in turn, its columns the tokens
 // for each block, and the epilogue adds up what belongs together.  Everything else goes in tiles of 256 rows on pairs, of as many columns as an estimate says.
 //
+// What bounds it (graph replay, weights of 0.4 GB in turn; 6.55 TB/s is the measured copy rate, 3.39 PFLOP/s twice the measured bf16 burst, 2.79 twice the sustained rate):
+//   weights' bytes    57344x8192 at 1 token 74 us = 6.3 TB/s, 28672x4096 21.5 = 5.5 (17.9 of bytes and what is left of a launch's chain of 4 us)
+//   a launch's chain  4096x4096 at 1 token 6.5 us: end of the kernel before, the tokens' copy and scales, the last stages, epilogue
+//   steps in a row    4096x14336 at 43 tokens 22 us: 16 tiles on 74 pairs, each 112 units of 0.17 us one after another
+//   tensor pipe       28672x4096 at 2048 tokens 175 us = 2.75 PFLOP/s (gated 170 to 185), active for 77 to 80 % of the time, at the power cap; dx of the same the same
+//   stores            dw of the same, 235 MB of results in bf16, 205 us without them and 235 with them
 // Every wait is bounded, as in the other pipeline kernels.
 #include <algorithm>
 #include <cmath>
@@ -44,13 +50,13 @@ namespace tuna {
 
 enum Fp8Form { kFp8Product, kFp8GatedProduct, kFp8Dx, kFp8Dw };
 
-// Warps of a CTA: pairs have eight for the epilogue, two groups of four that take turns on 32 columns.  With four, gated tiles of 256 columns waited for them (4096 features
-// of K: 14336x4096 at 2048 tokens 206 us, with z 233).
+// Warps of a CTA: pairs have eight for the epilogue, two groups of four that take turns on 32 columns.  With four, gated tiles waited for them (14336x4096 at 2048 tokens 206 -> 185
+// us, with z 233 -> 200).
 __host__ __device__ constexpr int fp8_warps(int cg) { return cg == 1 ? 12 : 16; }
 constexpr int kFp8EpilogueWarp0 = 4;
 constexpr int kFp8ScaleWarp0 = 8;
 constexpr int kFp8MaxStages = 12;
-constexpr int kFp8Deep = 2;               // units of a stage: what a wait, a commit and the turn of the issuing warp cost is paid once for eight MMAs
+constexpr int kFp8Deep = 2;               // units of a stage: what a wait, a commit and the turn of the issuing warp cost is paid once for eight MMAs (one unit: 4096x14336 at 43 tokens 28 us, so 22)
 constexpr int kFp8SingleCols = 16;        // tokens up to which single CTAs may take the tiles
 constexpr int kFp8StageCols = 32;         // columns of a group's output staging buffer
 constexpr int kFp8AheadTokens = 64;       // up to here weights count as constants and are copied ahead of the dependency wait, as in mx_gemm_sm100a.cu
@@ -782,7 +788,9 @@ struct Fp8Plan {
 };
 
 // Microseconds that tiles of 256 rows and `cols` columns take on `pairs` pairs, beside what a launch costs: rounds of tiles, each with its steps of 128 (the
-// tensor pipe's four MMAs, which take hardly less for few columns) and what of a wide tile's epilogue nothing hides; what all tiles copy, from L2; A, from HBM.
+// tensor pipe's four MMAs, which take hardly less for few columns) and what of a wide tile's epilogue nothing hides; what all tiles copy, from L2; A, from HBM.  Compared with 2400
+// launches (16 matrices from 512x4096 to 57344x8192, plain and gated, 1 to 4096 tokens, every width): what it chooses takes 1.4 % longer than the fastest width in the mean,
+// 18 % at worst (2720x784, gated, at 2000 tokens); constants fitted to these launches choose no better.
 static double fp8_pair_us(int rows, int n, int red, int cols, int pairs)
 {
     const int row_tiles = div_up(rows, 2 * kBlockRows), blocks = div_up(red, kFp8Block);

@@ -1,4 +1,12 @@
 // Quantizers of the 8-bit block-scaled format (fp8_format.cuh), their inverse, and the quantizer of a gated block's gradients.
+//
+// A block's scale is a power of two, so dividing by it is exact and the only rounding is that of the code.  A block by row is 16 lanes of a warp, one by column or a square one
+// a tile of 128 x 128 that a CTA holds in registers: its numbers are read once, whatever is made of them.  Nothing is transposed: blocks by column are codes in the
+// same place, with other scales.
+//
+// HBM bounds them (6.55 TB/s is the measured copy rate): 28672x4096 in fp32, square 88 us = 6.7 TB/s, by row 92, back 89; in bf16 square 58 and back 56 = 6.3, by row 59; 2048x28672 in
+// bf16 by row and by column at once 45 us = 5.2 TB/s, where half of the issue slots are busy and a tile's loads, maxima and stores follow one another.  A gated block's
+// gradients, 14336 features of 2048 tokens both ways, 66 us for 290 MB: the issue slots (62 % busy), the logistic function a third of it.
 #include <algorithm>
 #include <mutex>
 #include "launchers.h"
@@ -462,7 +470,8 @@ fp8_quantize_tile_kernel(const Source src, uint8_t *q, uint8_t *s, uint8_t *q2, 
     fp8_quantize_tiles<WAYS>(src, q, s, q2, s2, rows, cols, blockIdx.x, gridDim.x, shared);
 }
 
-// The same, and the columns of a second matrix of as many rows, its blocks by column: what a weight's gradient multiplies.  One launch: 1552x1040 at 301 tokens takes 3 us less.
+// The same, and the columns of a second matrix of as many rows, its blocks by column: what a weight's gradient multiplies, in one launch (gradients of 1552x1040 at 301 tokens
+// 22.7 -> 21.3 us).
 template <int WAYS, typename Source, typename T>
 __global__ void __launch_bounds__(256 * Source::kParts, fp8_tile_ctas<Source>(WAYS))
 fp8_quantize_two_kernel(const Source src, uint8_t *q, uint8_t *s, uint8_t *q2, uint8_t *s2, int rows, int cols, int tiles, const Fp8Plain<T, Source::kParts> x, uint8_t *xq, uint8_t *xs,
