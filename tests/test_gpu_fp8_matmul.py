@@ -364,6 +364,47 @@ def test_calls_on_two_streams_at_once():
         check_product(o, fo.numbers(numpy64(x), "row"), w.T)
 
 
+def test_gradients_on_two_streams_at_once():
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    cases = []
+    for i, (m, n, k) in enumerate([(1040, 300, 528), (4096, 1500, 6144)]):  # dx and dw in one launch, and in two
+        gen = torch.Generator(device="cuda").manual_seed(i)
+        dy, x, w = (torch.randint(-3, 4, s, generator=gen, device="cuda").float() for s in ((n, m), (n, k), (m, k)))  # whole numbers, sums below 2^24
+        cases.append((dy, x, w, dy.half(), x.half(), tuna_b200.fp8_quantize(w, "square"), torch.empty(n, k, device="cuda"), torch.empty(m, k, device="cuda"), (m, n, k)))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for (_, _, _, dy, x, weights, dx, dw, sizes), s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                tuna_b200.fp8_matmul_backward(dy, x, None, *weights, dx, dw, *sizes)
+    finish()
+    for dy, x, w, _, _, _, dx, dw, _ in cases:
+        assert torch.equal(dx, dy @ w) and torch.equal(dw, dy.T @ x)
+
+
+@pytest.mark.parametrize("k", [16, 144, 2064, 2576, 4112])
+@pytest.mark.parametrize("n", [1, 5, 16, 40])
+@pytest.mark.parametrize("m", [272, 9472, 18944])
+def test_what_the_last_scale_word_has_behind_the_last_block_is_not_used(m, n, k):
+    (wq, ws), _ = random_matrix(m, k, "square", 1)
+    x = torch.randn(n, k, device="cuda", dtype=torch.float16)
+    outs = []
+    for fill in (0, 255):
+        xq, xs = tuna_b200.fp8_quantize(x)
+        xs[-1, :, -(-k // 128) % 4 or 4:] = fill
+        o = torch.empty(n, m, device="cuda")
+        tuna_b200.fp8_matmul(xq, xs, wq, ws, o, m, n, k)
+        outs.append(o)
+    dy = torch.randn(n, m, device="cuda", dtype=torch.float16)
+    for fill in (0, 255):
+        xq, xs = tuna_b200.fp8_quantize(x, "column")
+        xs[-1, :, -(-n // 128) % 4 or 4:] = fill
+        dw = torch.empty(m, k, device="cuda")
+        tuna_b200.fp8_matmul_backward(dy, xq, xs, None, None, None, dw, m, n, k)
+        outs.append(dw)
+    finish()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[2], outs[3])
+
+
 @pytest.mark.parametrize("n", [4, 90])
 def test_a_chain_of_layers_follows_stream_order(n):
     """Every layer's output is the next one's input, without anything in between; small whole numbers, so that the chain is exact."""

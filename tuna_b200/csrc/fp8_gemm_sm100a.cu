@@ -481,6 +481,14 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
                     if (32 * j < r.valid) r.b[j] = __ldcg(reinterpret_cast<const uint32_t *>(p.bs) + (size_t)r.g * p.cols + r.col0 + min(32 * j + lane, r.valid - 1));
             }
         };
+        // The last unit's blocks behind the last one are multiplied, zeros that they are: their scales must be numbers, whatever the last words have there.
+        uint32_t there[2] = {~0u, ~0u};
+        if (CG == 1 && !RESIDENT && fold_log)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int blocks = p.blocks - (4 * (groups - 1) << fold_log) - (32 * j + lane) / p.b_rows, bytes = (blocks + fold - 1) >> fold_log;  // of a column's word
+                there[j] = bytes >= 4 ? ~0u : (1u << (8 * max(bytes, 0))) - 1u;
+            }
         // MMA column 32 j + lane is column t of block f of a unit
         auto word_b = [&](const Group &r, int j) {
             if constexpr (RESIDENT) {
@@ -496,7 +504,7 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
                     const uint32_t w0 = __shfl_sync(0xffffffffu, r.b[0], idx & 31), w1 = __shfl_sync(0xffffffffu, r.b[1], idx & 31);
                     w |= (((idx < 32 ? w0 : w1) >> (8 * (block & 3))) & 255u) << (8 * i);
                 }
-                return w;
+                return r.g + 1 == groups ? w & there[j] : w;
             } else {
                 return r.b[j];
             }
