@@ -1,5 +1,7 @@
 """The gated block of 8-bit block-scaled matrices and its gradients on the GPU, against 64 bits with the bounds that fp8_util derives."""
 
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -158,6 +160,34 @@ def test_gradients_that_are_no_numbers_spoil_their_own_blocks(f, n, bad):
     rows = torch.zeros(2 * f, dtype=torch.bool, device="cuda")
     rows[[3, f - 1, f + 3, 2 * f - 1]] = True
     assert torch.equal(torch.isnan(dw), rows[:, None].expand(2 * f, k))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("f,n", [(144, 300), (256, 300), (2048, 2500)])
+def test_the_gradient_is_that_of_elementary_operations_in_32_bits(f, n, dtype, kind):
+    """Bit for bit, before it is quantized: so its codes are those of the same formula written with torch, in every form of the quantizer."""
+    gen = torch.Generator(device="cuda").manual_seed(f)
+    z = (torch.randn(n, 2 * f, generator=gen, device="cuda") * 3).to(dtype)
+    z[0, :f] = torch.linspace(-200, 200, f).to(dtype)
+    dh = torch.randn(n, f, generator=gen, device="cuda").to(dtype)
+    k = -(-n // 16) * 16
+    x = torch.eye(n, k, device="cuda", dtype=dtype)  # picks the numbers one by one
+    dw = torch.empty(2 * f, k, device="cuda")
+    tuna_b200.fp8_gated_backward(dh, z, x, None, None, None, None, dw, f, n, k, kind)
+    finish()
+    g, u = z.float().split(f, 1)
+    p, slope = g, torch.ones_like(g)
+    if kind == "gelu":
+        c = 2 * math.sqrt(2 / math.pi)
+        p, slope = c * (g + 0.044715 * (g * g * g)), c * (1 + 3 * 0.044715 * (g * g))
+    sigma = 1 / (1 + torch.exp(-p))
+    d = dh.float()
+    dy = torch.cat((d * u * (sigma + g * sigma * (1 - sigma) * slope), d * g * sigma), 1)
+    q, s = tuna_b200.fp8_quantize(dy, "column")
+    want = torch.empty(n, 2 * f, device="cuda")
+    tuna_b200.fp8_dequant(q, s, want, n, 2 * f, "column")
+    assert torch.equal(dw[:, :n].T, want)
 
 
 @pytest.mark.parametrize("types", [(torch.float16, torch.float16, torch.float32), (torch.bfloat16, torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32, torch.float16)], ids=str)

@@ -253,10 +253,13 @@ __device__ __forceinline__ void fp8_gated_row(const Mx8<T> &g, const Mx8<T> &u, 
     u.values(uv);
     d.values(dv);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float sigma = fp8_gate<GELU>(gv[i]);
-        of_gate[i] = dv[i] * uv[i] * fp8_gate_slope<GELU>(gv[i], sigma);
-        of_other[i] = dv[i] * (gv[i] * sigma);
+    for (int i = 0; i < 8; i += 2) {
+        const Fp8Two gate(gv[i], gv[i + 1]), dh(dv[i], dv[i + 1]);
+        Fp8Two sigma, derivative;
+        fp8_gate_and_slope<GELU>(gate, sigma, derivative);
+        const float2 a = (dh * Fp8Two(uv[i], uv[i + 1]) * derivative).both(), b = (dh * gate * sigma).both();
+        of_gate[i] = a.x, of_gate[i + 1] = a.y;
+        of_other[i] = b.x, of_other[i + 1] = b.y;
     }
 }
 template <typename T, bool GELU>
