@@ -335,7 +335,7 @@ typedef enum tuna_activation { TUNA_SILU = 0, TUNA_GELU = 1 } tuna_activation;
  * Quantizer: x [rows, k] of x_type (fp16, bf16 or fp32), rows row_stride elements apart -> q and s; TUNA_FP8_BOTH: by row into q and s, by column into
  * q2 and s2, which the others do not use.  The scale of a block is the smallest power of two over which its largest magnitude is not above 448,
  * not below 2^-127; codes are its numbers over the scale, rounded to nearest with ties to even.  A block that holds an infinity or
- * NaN gets scale byte 255.  Scale bytes of blocks that the last word does not have are zero.
+ * NaN gets scale byte 255.  Scale bytes of blocks that the last word does not have are zero; the calls below take any.
  */
 int tuna_fp8_quantize(const void *x, int x_type, long long row_stride, int blocks, void *q, void *s, void *q2, void *s2, int rows, int k, void *stream);
 

@@ -6,7 +6,7 @@
 //
 // HBM bounds them (6.55 TB/s is the measured copy rate): 28672x4096 in fp32, square 88 us = 6.7 TB/s, by row 92, back 89; in bf16 square 58 and back 56 = 6.3, by row 59; 2048x28672 in
 // bf16 by row and by column at once 45 us = 5.2 TB/s, where half of the issue slots are busy and a tile's loads, maxima and stores follow one another.  A gated block's
-// gradients, 14336 features of 2048 tokens both ways, 66 us for 290 MB: the issue slots (62 % busy), the logistic function a third of it.
+// gradients, 14336 features of 2048 tokens both ways, 79 us for 290 MB (GELU 88): the issue slots (62 % busy).
 #include <algorithm>
 #include <mutex>
 #include "launchers.h"
@@ -273,7 +273,7 @@ __device__ __forceinline__ void fp8_gated_row(const Mx8<T> &g, const Mx8<T> &u, 
 }
 
 // Columns 0 .. f - 1: the gradient of a gated block's gate, dh u act'(g); f .. 2f - 1: of the other projection, dh act(g).  z = [g | u].  What bounds it is the
-// logistic function (two instructions of 16 lanes a clock and SM): where blocks end between the projections two parts share it, otherwise a tile is of either.
+// activation's arithmetic: where blocks end between the projections two parts share it, otherwise a tile is of either.
 template <typename T, bool GELU, int PARTS>
 struct Fp8Gated {
     const T *z, *dh;
@@ -490,7 +490,8 @@ fp8_quantize_two_kernel(const Source src, uint8_t *q, uint8_t *s, uint8_t *q2, u
 // ---- a gated block's gradients, streamed
 
 // The same numbers as Fp8Gated's of two parts, for many tiles: one CTA an SM walks through them, and TMA has the next tile's three boxes of 32 KB under way while one is worked
-// on.  Loaded by the lanes themselves, one tile a CTA, 14336 features of 2048 tokens took 115 us, most of it waiting: 512 threads of 128 registers leave no room for another
+// on.  Loaded by the lanes themselves, one tile a CTA, 14336 features of 2048 tokens took 115 us where this took 66 (the activation by
+// fast approximations in both), most of it waiting: 512 threads of 128 registers leave no room for another
 // CTA that would work meanwhile.
 constexpr int kFp8BoxBytes = kFp8Block * kFp8Block * 2, kFp8StreamBytes = 2 * 3 * kFp8BoxBytes;
 
