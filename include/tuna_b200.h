@@ -343,8 +343,9 @@ int tuna_fp8_quantize(const void *x, int x_type, long long row_stride, int block
 int tuna_fp8_dequant(const void *q, const void *s, int blocks, void *o, int o_type, int rows, int k, void *stream);
 
 /*
- * o[n, m] (fp16, bf16 or fp32) = x[n, k] * w[m, k]^T, w given by q and s (square), fp32 accumulation, one rounding; results are bit-identical from
- * run to run.  x_type TUNA_FP8: x and xs are codes and scales of the tokens, by row.  TUNA_FP16 or TUNA_BF16: x is [n, k] of that
+ * o[n, m] (fp16, bf16 or fp32) = x[n, k] * w[m, k]^T, w given by q and s (square), fp32 accumulation, one rounding (the
+ * accumulators cut off below their last bit: sums of 28672 random numbers are 2e-6 off, of 4096 2e-7); results are bit-identical from run to
+ * run.  x_type TUNA_FP8: x and xs are codes and scales of the tokens, by row.  TUNA_FP16 or TUNA_BF16: x is [n, k] of that
  * type, xs is not read, and the call quantizes x as tuna_fp8_quantize does.
  * Workspace, here and below: tuna_fp8_workspace_bytes bytes, written before they are read; null where that is 0.  Calls that overlap on the device
  * need separate ones.

@@ -233,7 +233,8 @@ def fp8_gated(x, xs, q, s, h, f: int, n: int, k: int, activation: str = "silu", 
 
 def fp8_gated_backward(dh, z, x, xs, q, s, dx, dw, f: int, n: int, k: int, activation: str = "silu", *, workspace=None) -> None:
     """The gradients of `fp8_gated` given dh `[n, f]` and z `[n, 2f]` (fp16 or bf16, one type): those of `fp8_matmul_backward`, dw `[2f, k]`, for
-    dy = [dh u activation'(g) | dh activation(g)], which is made and quantized in one pass and never stored in 16 bits."""
+    dy = [dh u activation'(g) | dh activation(g)], which is made and quantized in one pass and never stored in 16 bits: in fp32, as elementary operations
+    one after the other give it.  Both gradients are those of z as it was kept, rounded."""
     act = _choice(activation, "activation", _ACTIVATIONS)
     if workspace is None and _launched(_front().fp8_gated_backward(dh, z, x, xs, q, s, dx, dw, f, n, k, act)):
         return
