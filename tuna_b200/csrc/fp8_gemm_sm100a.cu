@@ -44,6 +44,7 @@
 #include <mutex>
 #include "launchers.h"
 #include "fp8_format.cuh"
+#include "fp8_scales.h"
 #include "sm100_ptx.cuh"
 #include "tcgen05.cuh"
 
@@ -422,7 +423,6 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
         const int quarter = warp - kFp8ScaleWarp0;
         const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + kSfCol;
         const uint32_t leader_full = CG == 1 ? sf_full : map_to_rank(sf_full, 0);
-        const int a_blocks = div_up(p.rows, kFp8Block);
         // Some groups ahead are on their way, as loaded: A's words (dw) or, spread over the lanes, its bytes; B's words, those of a folded tile spread over the lanes too.  They
         // are put together when their turn comes.  One group ahead the loads' latency, 1.5 us while the weights stream, was what single CTAs took for four stages (gated
         // 14336x4096 at 1 token 28.1 us).
@@ -459,12 +459,8 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
             } else {
 #pragma unroll
                 for (int i = 0; i < (CG == 1 ? 2 : 1); ++i) {
-                    const int idx = 32 * i + lane, slot = idx >> (2 + fold_log), kb = min((4 * r.g << fold_log) + (idx & ((4 << fold_log) - 1)), p.blocks - 1);
-                    if (slot < (FORM == kFp8Dx ? 1 : kGated ? 4 : 2)) {
-                        const int first = kGated ? (slot >> 1) * (p.rows / 2) + (r.row0 >> 1) : r.row0;
-                        const int block = FORM == kFp8Dx ? first / kFp8Block : min(first / kFp8Block + (slot & 1), a_blocks - 1);
-                        r.a[i] = __ldcg(p.as + (FORM == kFp8Dx ? (size_t)kb * a_blocks + block : (size_t)block * p.blocks + kb));
-                    }
+                    const int idx = 32 * i + lane, slot = idx >> (2 + fold_log), kb = (4 * r.g << fold_log) + (idx & ((4 << fold_log) - 1));
+                    if (slot < (FORM == kFp8Dx ? 1 : kGated ? 4 : 2)) r.a[i] = __ldcg(p.as + fp8_square_scale(FORM == kFp8Dx, kGated, r.row0, slot, kb, p.rows, p.blocks));
                 }
             }
         };
