@@ -343,9 +343,10 @@ int tuna_fp8_quantize(const void *x, int x_type, long long row_stride, int block
 int tuna_fp8_dequant(const void *q, const void *s, int blocks, void *o, int o_type, int rows, int k, void *stream);
 
 /*
- * o[n, m] (fp16, bf16 or fp32) = x[n, k] * w[m, k]^T, w given by q and s (square), fp32 accumulation, one rounding (the
- * accumulators cut off below their last bit: sums of 28672 random numbers are 2e-6 off, of 4096 2e-7); results are bit-identical from run to
- * run.  x_type TUNA_FP8: x and xs are codes and scales of the tokens, by row.  TUNA_FP16 or TUNA_BF16: x is [n, k] of that
+ * o[n, m] (fp16, bf16 or fp32) = x[n, k] * w[m, k]^T, w given by q and s (square), fp32 accumulation, one rounding; results are
+ * bit-identical from run to run.  An accumulator cuts off below its last bit, here and in the gradients: all of one sign, or random, a sum of 28672 ends up
+ * 2e-6 nearer to zero, of 4096 2e-7, which in 16 bits is below a hundredth of a rounding.  Sums for results in 32 bits, and for z below, are therefore made of
+ * parts of up to 2048 addends, which are added to nearest: 1e-7 off, as sums in fp32 are.  x_type TUNA_FP8: x and xs are codes and scales of the tokens, by row.  TUNA_FP16 or TUNA_BF16: x is [n, k] of that
  * type, xs is not read, and the call quantizes x as tuna_fp8_quantize does.
  * Workspace, here and below: tuna_fp8_workspace_bytes bytes, written before they are read; null where that is 0.  Calls that overlap on the device
  * need separate ones.
@@ -360,7 +361,7 @@ int tuna_fp8_matmul(const void *x, int x_type, const void *xs, const void *q, co
  *   dx[n, k] = dy * w    dy quantized by row
  *   dw[m, k] = dy^T * x  dy and x quantized by column; the gradient of the numbers that q and s stand for
  * Either of dx and dw (fp16, bf16 or fp32) may be null, and what only it reads (q and s; x and xs) too.  x_type TUNA_FP8: x and xs are codes and
- * scales by COLUMN.  What is quantized has the quantizer's rounding: dx and dw are the exact sums of these, in fp32, rounded once.
+ * scales by COLUMN.  What is quantized has the quantizer's rounding: dx and dw are the sums of these in fp32, with the error above, rounded once.
  */
 int tuna_fp8_matmul_backward(const void *dy, int dy_type, const void *x, int x_type, const void *xs, const void *q, const void *s, void *dx, int dx_type, void *dw,
                              int dw_type, int m, int n, int k, void *workspace, size_t workspace_bytes, void *stream);
@@ -368,7 +369,8 @@ int tuna_fp8_matmul_backward(const void *dy, int dy_type, const void *x, int x_t
 /*
  * The first half of a gated feed-forward block in one launch: h[n, f] (fp16, bf16 or fp32) = activation(g) * u, where g[n, f] and u[n, f] are x
  * times the transposed first and last f rows of w[2f, k].  x as in tuna_fp8_matmul.  z (null, or [n, 2f] of h_type, which is fp16 or bf16 then)
- * keeps g and u side by side for the gradients; h is made of g and u before they are rounded.
+ * keeps g and u side by side for the gradients; h is made of g and u before they are rounded.  With z sums of more than 1024 columns are more exact
+ * (above), so that h may differ from the one without it by a rounding.
  */
 int tuna_fp8_gated(const void *x, int x_type, const void *xs, const void *q, const void *s, void *h, int h_type, void *z, int f, int n, int k, int activation,
                    void *workspace, size_t workspace_bytes, void *stream);

@@ -36,7 +36,11 @@
 //   steps in a row    4096x14336 at 43 tokens 22 us: 16 tiles on 74 pairs, each 112 units of 0.17 us one after another
 //   tensor pipe       28672x4096 at 2048 tokens 175 us = 2.75 PFLOP/s (gated 170 to 185), active for 77 to 80 % of the time, at the power cap; dx of the same the same
 //   stores            dw of the same, 235 MB of results in bf16, 205 us without them and 235 with them
-// The accumulators are fp32, and what an addition has below their last bit is cut off: sums of 28672 columns end up 2e-6 of their size nearer to zero, of 4096 2e-7 (64 tokens, random numbers).
+// Sums of parts.  The accumulators are fp32, and what an addition has below their last bit is cut off, so a long sum in one of them ends up nearer to zero: 2.5e-6 off for 28672 columns, 2.1e-7 for
+// 4096 (2-norm against 64 bits, 64 tokens, random numbers; sums in fp32 that round are 1e-7 and 0.6e-7 off).  Where that can be seen - results in 32 bits, and z, which in 16 bits decides on which side
+// of a border a gradient's code falls - the tensor cores add up at most 1024 columns (2048 in tiles of more than 128 columns, whose epilogue two parts have to cover: gated 4096x2048 at 2048 tokens with z
+// 47 us in parts of 1536, 41 in parts of 2048), and the epilogue the parts, to nearest, in its registers: 1.2e-7 and 0.7e-7.  It costs what reading an accumulator does: 28672x4096 at 43
+// tokens in 32 bits 23.1 -> 23.4 us, 4096x14336 at 43 (14 parts) 22.6 -> 23.8, 6144x4096 with gradients in 32 bits at 4096 204 -> 208.  Results in 16 bits are a hundredth of a rounding off without.
 // Every wait is bounded, as in the other pipeline kernels.
 #include <algorithm>
 #include <cmath>
@@ -57,12 +61,18 @@ enum Fp8Form { kFp8Product, kFp8GatedProduct, kFp8Dx, kFp8Dw };
 __host__ __device__ constexpr int fp8_warps(int cg) { return cg == 1 ? 12 : 16; }
 constexpr int kFp8EpilogueWarp0 = 4;
 constexpr int kFp8ScaleWarp0 = 8;
+// Registers of a thread where the parts of a wide tile's sums are added up: the epilogue's hold the sums, 128 of theirs, and the four groups of four warps share what the CTA was launched with.
+constexpr int kFp8LaunchRegs = 128, kFp8IssueRegs = 40, kFp8ScaleRegs = 72, kFp8EpilogueRegs = 200;
+static_assert(kFp8IssueRegs + kFp8ScaleRegs + 2 * kFp8EpilogueRegs <= 4 * kFp8LaunchRegs, "a group would wait for registers that nobody gives back");
 constexpr int kFp8MaxStages = 12;
 constexpr int kFp8Deep = 2;               // units of a stage: what a wait, a commit and the turn of the issuing warp cost is paid once for eight MMAs (one unit: 4096x14336 at 43 tokens 28 us, so 22)
 constexpr int kFp8SingleCols = 16;        // tokens up to which single CTAs may take the tiles
 constexpr int kFp8StageCols = 32;         // columns of a group's output staging buffer
+constexpr int kFp8NarrowCols = 128;      // tiles whose sums every warp has registers for
+constexpr int kFp8WideSlices = 4, kFp8NarrowSlices = 2;  // staging buffers of columns that an epilogue group has of a tile at most: of 240 columns, and of 128
 constexpr int kFp8AheadTokens = 64;       // up to here weights count as constants and are copied ahead of the dependency wait, as in mx_gemm_sm100a.cu
 constexpr int kFp8ResidentLoads = 4;      // loads in flight of a quantizing warp
+constexpr int kFp8PartSteps = 4, kFp8WidePartSteps = 8;  // stages of a part of a sum at most, and of wide tiles: 1024 columns (folded: for each block of a unit), 2048
 constexpr int kFp8SfCols = 16;            // tensor-memory columns of a group's scales: A's words at 0 to 3, B's at 8 to 15
 constexpr uint32_t kFp8SumBytes = kFp8SingleCols * kBlockRows * 4;  // where the parts of a folded tile, or a gated one's projections, meet
 constexpr int kFp8SmemMax = 225 * 1024;   // dynamic shared memory of a CTA alone on its SM (1 KB is the kernel's static part, 1 KB the system's)
@@ -80,6 +90,8 @@ struct Fp8Params {
     int units;       // of a tile: ceil(blocks / fold), four MMAs each
     int fold_log;    // log2(fold): blocks side by side in a unit
     int steps;       // stages of a tile: ceil(units / kFp8Deep)
+    int part_steps;  // stages of a part of the sum: the tensor cores add these up, the epilogue the parts
+    int parts;       // ceil(steps / part_steps)
     int tile_cols;   // N
     int width;       // columns of a tile, all but the last
     int row_tiles, col_tiles;
@@ -206,8 +218,8 @@ __device__ __forceinline__ void fp8_quantize_resident(const Fp8Params &p, int w,
 
 __device__ __forceinline__ float fp8_activation(float g, float u, int gelu) { return gelu ? g * fp8_gate<true>(g) * u : g * fp8_gate<false>(g) * u; }
 
-// CG: CTAs of a worker (1 or 2).  Single CTAs leave room for a second one on the SM: that of the next launch, which copies its first weights meanwhile.
-template <int CG, int FORM, bool RESIDENT, typename OT>
+// CG: CTAs of a worker (1 or 2).  SLICES: of a pair's tile the slices of columns whose sums an epilogue group adds up of parts, 0 where sums have one part.  Single CTAs leave room for a second one on the SM: that of the next launch, which copies its first weights meanwhile.
+template <int CG, int FORM, bool RESIDENT, int SLICES, typename OT>
 __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &tmap_a, const CUtensorMap &tmap_a2, const CUtensorMap &tmap_b, int worker, int workers)
 {
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -216,11 +228,12 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
     __shared__ uint32_t s_tmem_base;
     __shared__ int s_abort;
 
+    constexpr bool kParts = CG == 2 && SLICES > 0, kShares = SLICES > kFp8NarrowSlices;
     constexpr bool kGated = FORM == kFp8GatedProduct, kAcrossA = FORM >= kFp8Dx, kAcrossB = FORM == kFp8Dw;
     constexpr uint32_t kTmemCols = CG == 1 ? 256 : 512, kSfCol = kTmemCols - 2 * kFp8SfCols;  // two accumulators below
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const int rank = CG == 1 ? 0 : (int)cluster_ctarank();
-    const int N = p.tile_cols, S = p.stages;
+    const int S = p.stages;
     // [stages of A][of B][words of the resident tokens' scales][staging buffer]; the MMAs read 128 rows of A, in low tiles past their stage's end.
     // RESIDENT: of B, all of a tile's stages.
     const int b_units = RESIDENT ? p.units : S * kFp8Deep, groups = (p.units + 3) >> 2;
@@ -289,7 +302,7 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
         asm volatile("bar.sync 2, %0;" ::"n"(32 * (fp8_warps(CG) - 1)) : "memory");
     }
     // Whoever makes a bounded wait that ends only after the kernels before this one waits for those first.
-    if (warp == 0) {
+    auto issue = [&] {
         if (CG == 1 || rank == 0) {
             depend();
             Ring ru, rd, rs;
@@ -304,16 +317,20 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
             const uint64_t b_form = RESIDENT ? ((uint64_t)p.cols << 16) | ((uint64_t)(8u * (uint32_t)p.cols | (1u << 14)) << 32) : sw128;
             while (ok && tile.next(p)) {
                 const uint32_t idesc = fp8_idesc<CG>(p.fold_log ? p.d_cols : mma_cols(), kAcrossA, kAcrossB);
-                ok = mbar_wait_warp(d_empty + 8 * rd.idx, rd.phase ^ 1, abort_flag, p.status, 303);
-                const uint32_t d = tmem + (uint32_t)(rd.idx * p.d_cols);
+                const int part_steps = CG == 2 && !kParts ? p.steps : p.part_steps;
+                uint32_t d = 0;
                 Fp8Stages st(p, tile.first_group(p, groups));
-                for (int i = 0; ok && i < p.steps; ++i, st.advance()) {
-                    if ((st.c & 3) == 0) ok = mbar_wait_warp(sf_full + 8 * rs.idx, rs.phase, abort_flag, p.status, 304);
-                    ok = ok && mbar_wait_warp(full + 8 * ru.idx, ru.phase, abort_flag, p.status, 305);
+                for (int i = 0, of_part = 0; ok && i < p.steps; ++i, st.advance()) {
+                    if (of_part == 0) {
+                        ok = mbar_wait_warp<!kShares>(d_empty + 8 * rd.idx, rd.phase ^ 1, abort_flag, p.status, 303);
+                        d = tmem + (uint32_t)(rd.idx * p.d_cols);
+                    }
+                    if (ok && (st.c & 3) == 0) ok = mbar_wait_warp<!kShares>(sf_full + 8 * rs.idx, rs.phase, abort_flag, p.status, 304);
+                    ok = ok && mbar_wait_warp<!kShares>(full + 8 * ru.idx, ru.phase, abort_flag, p.status, 305);
                     if (!ok) break;
                     tc_fence_after();
                     const int end = st.end();
-                    const bool last = i + 1 == p.steps, group_ends = end == p.units || (end & 3) == 0;
+                    const bool last = i + 1 == p.steps || of_part + 1 == part_steps, group_ends = end == p.units || (end & 3) == 0;
                     if (elect_one_sync()) {
                         const uint32_t sfa = tmem + kSfCol + (uint32_t)(rs.idx * kFp8SfCols), sfb = sfa + 8;
                         const uint64_t a = sw128 | (uint64_t)(((base + (uint32_t)(ru.idx * kFp8Deep) * a_bytes) & 0x3FFFFu) >> 4);
@@ -326,7 +343,7 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
 #pragma unroll
                                 for (int kk = 0; kk < 4; ++kk)
                                     tc_mma_fp8<CG>(d, a + u * (a_bytes >> 4) + kStepA * kk, b + u * (b_bytes >> 4) + kStepB * kk, id + u * ((1u << 29) | (1u << 4)), sfa, sfb,
-                                                   i == 0 && u == 0 && kk == 0 ? 0u : 1u);
+                                                   of_part == 0 && u == 0 && kk == 0 ? 0u : 1u);
                         if (CG == 1) {
                             tc_commit(empty + 8 * ru.idx);
                             if (group_ends) tc_commit(sf_empty + 8 * rs.idx);
@@ -340,11 +357,16 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
                     __syncwarp();
                     ru.advance(S);
                     if (group_ends) rs.advance(2);
+                    ++of_part;
+                    if (last) {
+                        rd.advance(2);
+                        of_part = 0;
+                    }
                 }
-                rd.advance(2);
             }
         }
-    } else if (warp == 1) {
+    };
+    auto copy_a = [&] {
         // ------------------------------------------------------------------ A
         Ring ru;
         bool ok = true;
@@ -356,7 +378,7 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
             Fp8Stages st(p, tile.first_group(p, groups));
             for (int i = 0; i < p.steps; ++i, st.advance(), ru.advance(S)) {
                 if (issued++ == S) depend();
-                ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 300);
+                ok = mbar_wait_warp<!kShares>(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 300);
                 if (!ok) break;
                 if (elect_one_sync()) {
                     const uint32_t bar = landed + 8 * ru.idx;
@@ -380,8 +402,9 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
         // The MMAs' commits have arrived at every stage in use before the CTA leaves.
         depend();
         if (total < S) ru = Ring();
-        for (int i = min(S, total); ok && i > 0; --i, ru.advance(S)) ok = mbar_wait_warp(empty + 8 * ru.idx, total < S ? 0u : ru.phase ^ 1, abort_flag, p.status, 310);
-    } else if (warp == 2 && !RESIDENT) {
+        for (int i = min(S, total); ok && i > 0; --i, ru.advance(S)) ok = mbar_wait_warp<!kShares>(empty + 8 * ru.idx, total < S ? 0u : ru.phase ^ 1, abort_flag, p.status, 310);
+    };
+    auto copy_b = [&] {
         // ------------------------------------------------------------------ B
         Ring ru;
         bool ok = true;
@@ -390,7 +413,7 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
             const int col = tile.col0 + rank * (mma_cols() / CG);
             Fp8Stages st(p, tile.first_group(p, groups));
             for (int i = 0; i < p.steps; ++i, st.advance(), ru.advance(S)) {
-                ok = mbar_wait_warp(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 301);
+                ok = mbar_wait_warp<!kShares>(empty + 8 * ru.idx, ru.phase ^ 1, abort_flag, p.status, 301);
                 if (!ok) break;
                 if (elect_one_sync()) {
                     const uint32_t bar = landed + 8 * ru.idx;
@@ -409,16 +432,18 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
                 __syncwarp();
             }
         }
-    } else if (warp == 3 && CG == 2) {
+    };
+    auto landed_here = [&] {
         // ------------------------------------------------------------------ a stage has landed
         const uint32_t leader_full = map_to_rank(full, 0);
         Ring ru;
         depend();
         for (int i = 0; i < total; ++i, ru.advance(S)) {
-            if (!mbar_wait_warp(landed + 8 * ru.idx, ru.phase, abort_flag, p.status, 302)) break;
+            if (!mbar_wait_warp<!kShares>(landed + 8 * ru.idx, ru.phase, abort_flag, p.status, 302)) break;
             if (lane == 0) mbar_arrive_cluster(leader_full + 8 * ru.idx);
         }
-    } else if (warp >= kFp8ScaleWarp0 && warp < kFp8ScaleWarp0 + 4) {
+    };
+    auto scales = [&] {
         // ------------------------------------------------------------------ scales to tensor memory
         const int quarter = warp - kFp8ScaleWarp0;
         const uint32_t lanes = tmem + ((uint32_t)(32 * quarter) << 16) + kSfCol;
@@ -570,7 +595,7 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
                     fetch_b(r);
                     ++taken;
                 }
-                ok = mbar_wait_warp(sf_empty + 8 * rs.idx, rs.phase ^ 1, abort_flag, p.status, 306);
+                ok = mbar_wait_warp<!kShares>(sf_empty + 8 * rs.idx, rs.phase ^ 1, abort_flag, p.status, 306);
                 if (!ok) break;
                 tc_fence_after();
                 tc_st_x16(lanes + (uint32_t)(rs.idx * kFp8SfCols), v);
@@ -587,8 +612,9 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
         }
         // the commits for the last two groups have arrived before the CTA leaves
         if (total_groups == 1) rs = Ring();
-        for (int i = min(2, total_groups); ok && i > 0; --i, rs.advance(2)) ok = mbar_wait_warp(sf_empty + 8 * rs.idx, total_groups == 1 ? 0u : rs.phase ^ 1, abort_flag, p.status, 311);
-    } else if (warp >= kFp8EpilogueWarp0) {
+        for (int i = min(2, total_groups); ok && i > 0; --i, rs.advance(2)) ok = mbar_wait_warp<!kShares>(sf_empty + 8 * rs.idx, total_groups == 1 ? 0u : rs.phase ^ 1, abort_flag, p.status, 311);
+    };
+    auto epilogue = [&] {
         // ------------------------------------------------------------------ epilogue
         const int quarter = warp & 3, thread = threadIdx.x & 127, half = warp / (kFp8ScaleWarp0 + 4);  // which group
         const uint32_t tmem_q = tmem + ((uint32_t)(32 * quarter) << 16);
@@ -641,34 +667,51 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
                 }
             }
         };
-        // 32 columns of the accumulator at `d`, from t on, to the group's staging buffer.
-        auto fill_from = [&](uint32_t d, int t) {
-            const uint32_t to = out_staging;
-            auto f32 = [](uint32_t v) { return __uint_as_float(v); };
-            if constexpr (kGated || sizeof(OT) == 2) {
+        // 32 columns of the accumulator at `d`, from t on.  16 bits and gated: lo, then hi halves of the lanes in fragments of 8 x 8; otherwise a lane a thread.
+        constexpr bool kFragments = kGated || sizeof(OT) == 2;
+        auto load = [&](uint32_t d, int t, auto &&take) {
+            if constexpr (kFragments) {
                 uint32_t lo[16], hi[16];
                 tc_ld_16x256b_x4(d + t, lo);
                 tc_ld_16x256b_x4(d + (16u << 16) + t, hi);
                 asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+                for (int i = 0; i < 16; ++i) take(i, __uint_as_float(lo[i])), take(16 + i, __uint_as_float(hi[i]));
+            } else {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float r[16];
+                    tc_ld_x16(d + t + 16 * h, r);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) take(16 * h + i, r[i]);
+                }
+            }
+        };
+        // 32 columns' sums to the group's staging buffer.
+        auto fill_from = [&](const float (&v)[32]) {
+            const uint32_t to = out_staging;
+            if constexpr (kFragments) {
+                auto lo = [&](int i) { return v[i]; };
+                auto hi = [&](int i) { return v[16 + i]; };
                 // Fragments of 8 rows x 8 columns, packed, are written transposed (stmatrix): 16 bytes = 8 rows of one column.
                 auto rows_of_8 = [&](uint32_t at_, uint32_t pitch) {
                     if constexpr (sizeof(OT) == 2) {
                         const uint32_t dst = at_ + (uint32_t)(lane & 7) * pitch + (uint32_t)(4 * quarter + (lane >> 3)) * 16u;
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
-                            stmatrix_x4_trans(dst + 8u * i * pitch, mx_pack2<OT>(f32(lo[4 * i]), f32(lo[4 * i + 1])), mx_pack2<OT>(f32(lo[4 * i + 2]), f32(lo[4 * i + 3])),
-                                              mx_pack2<OT>(f32(hi[4 * i]), f32(hi[4 * i + 1])), mx_pack2<OT>(f32(hi[4 * i + 2]), f32(hi[4 * i + 3])));
+                            stmatrix_x4_trans(dst + 8u * i * pitch, mx_pack2<OT>(lo(4 * i), lo(4 * i + 1)), mx_pack2<OT>(lo(4 * i + 2), lo(4 * i + 3)), mx_pack2<OT>(hi(4 * i), hi(4 * i + 1)),
+                                              mx_pack2<OT>(hi(4 * i + 2), hi(4 * i + 3)));
                     }
                 };
                 if constexpr (!kGated) {
                     rows_of_8(to, kPitch);
                 } else {
                     if (z) rows_of_8(z_staging, kPitchZ);
-                    auto act = [&](uint32_t g, uint32_t u) { return fp8_activation(f32(g), f32(u), p.gelu); };
+                    auto act = [&](float g, float u) { return fp8_activation(g, u, p.gelu); };
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {  // lanes i and i + 8 of a half: gate and other projection of one feature, two columns
-                        const float l0 = act(lo[4 * i], lo[4 * i + 2]), l1 = act(lo[4 * i + 1], lo[4 * i + 3]);
-                        const float h0 = act(hi[4 * i], hi[4 * i + 2]), h1 = act(hi[4 * i + 1], hi[4 * i + 3]);
+                        const float l0 = act(lo(4 * i), lo(4 * i + 2)), l1 = act(lo(4 * i + 1), lo(4 * i + 3));
+                        const float h0 = act(hi(4 * i), hi(4 * i + 2)), h1 = act(hi(4 * i + 1), hi(4 * i + 3));
                         if constexpr (sizeof(OT) == 2) {
                             stmatrix_x2_trans(to + (uint32_t)(8 * i + (lane & 7)) * kPitch + (uint32_t)(2 * quarter + ((lane >> 3) & 1)) * 16u, mx_pack2<OT>(l0, l1), mx_pack2<OT>(h0, h1));
                         } else {
@@ -682,27 +725,40 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
                 }
             } else {
 #pragma unroll
-                for (int h = 0; h < 32; h += 16) {
-                    float v[16];
-                    tc_ld_x16(d + t + h, v);
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + (uint32_t)(h + i) * kPitch + (uint32_t)thread * 4u), "f"(v[i]) : "memory");
-                }
+                for (int i = 0; i < 32; ++i) asm volatile("st.shared.f32 [%0], %1;" ::"r"(to + (uint32_t)i * kPitch + (uint32_t)thread * 4u), "f"(v[i]) : "memory");
             }
         };
-        while (tile.next(p)) {
-            const bool ok = mbar_wait_warp(d_full + 8 * rd.idx, rd.phase, abort_flag, p.status, 307);
-            if (bar_any(1 + 2 * half, 128, !ok)) break;  // the group's four warps go on together or not at all
+        auto next_part = [&] {  // the group's four warps go on together or not at all
+            const bool ok = mbar_wait_warp<!kShares>(d_full + 8 * rd.idx, rd.phase, abort_flag, p.status, 307);
+            if (bar_any(1 + 2 * half, 128, !ok)) return false;
             tc_fence_after();
-            const uint32_t d = tmem_q + (uint32_t)(rd.idx * p.d_cols);
+            return true;
+        };
+        // The parts of a tile's sum in order: `take` what the accumulator at `d` has.
+        auto each_part = [&](auto &&take) {
+            for (int i = 0; i < p.parts; ++i, rd.advance(2)) {
+                if (!next_part()) return false;
+                take(tmem_q + (uint32_t)(rd.idx * p.d_cols));
+                drained();
+            }
+            return true;
+        };
+        while (tile.next(p)) {
             row0 = fp8_row<CG>(p, CG * tile.rt + rank);
             rows = max(0, min(CG == 1 ? fp8_row<CG>(p, tile.rt + 1) : row0 + kBlockRows, p.rows) - row0);
             if constexpr (CG == 1) {
                 const int f = thread >> (7 - p.fold_log), features = rows >> 1;
                 float *sums = reinterpret_cast<float *>(smem + (staging - base));
                 float v[kFp8SingleCols];
-                tc_ld_x16(d + f * p.b_rows, v);
-                drained();
+#pragma unroll
+                for (int c = 0; c < kFp8SingleCols; ++c) v[c] = -0.0f;  // as below
+                if (!each_part([&](uint32_t d) {
+                        float w[kFp8SingleCols];
+                        tc_ld_x16(d + f * p.b_rows, w);
+#pragma unroll
+                        for (int c = 0; c < kFp8SingleCols; ++c) v[c] += w[c];
+                    }))
+                    break;
                 if (!kGated && p.fold_log == 0) {
                     OT *to = o + row0 + thread;
                     if (thread < rows) {
@@ -738,18 +794,71 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
                     }
                     meet();  // they have been read
                 }
-            } else {
-                for (int t0 = half * kFp8StageCols; t0 < N; t0 += 2 * kFp8StageCols) {
+            } else if constexpr (!kParts) {
+                if (!next_part()) break;
+                const uint32_t d = tmem_q + (uint32_t)(rd.idx * p.d_cols);
+                for (int t0 = half * kFp8StageCols; t0 < p.tile_cols; t0 += 2 * kFp8StageCols) {
                     meet();  // what was staged before has been copied
-                    if (t0 < tile.valid) fill_from(d, t0);
-                    if (t0 + 2 * kFp8StageCols >= N) drained();
+                    if (t0 < tile.valid) {
+                        float v[kFp8StageCols];
+                        load(d, t0, [&](int c, float w) { v[c] = w; });
+                        fill_from(v);
+                    }
+                    if (t0 + 2 * kFp8StageCols >= p.tile_cols) drained();
                     meet();
                     copy_out(t0);
                 }
-                if (half * kFp8StageCols >= N) drained();
+                if (half * kFp8StageCols >= p.tile_cols) drained();
+                rd.advance(2);
+            } else {
+                float v[SLICES][kFp8StageCols];  // columns 32 half + 64 j on
+#pragma unroll
+                for (int j = 0; j < SLICES; ++j)
+#pragma unroll
+                    for (int c = 0; c < kFp8StageCols; ++c) v[j][c] = -0.0f;  // any number that is added to it stays as it is
+                if (!each_part([&](uint32_t d) {
+#pragma unroll
+                        for (int j = 0; j < SLICES; ++j)
+                            if ((half + 2 * j) * kFp8StageCols < tile.valid) load(d, (half + 2 * j) * kFp8StageCols, [&](int c, float w) { v[j][c] += w; });
+                    }))
+                    break;
+                // One copy of what follows, whose first run by a CTA waits for its instructions: the sums move down instead of being indexed (unrolled, gated 14336x4096 at 43 tokens
+                // 34 us, so 30).
+#pragma unroll 1
+                for (int t0 = half * kFp8StageCols; t0 < tile.valid; t0 += 2 * kFp8StageCols) {
+                    meet();  // what was staged before has been copied
+                    fill_from(v[0]);
+#pragma unroll
+                    for (int j = 0; j + 1 < SLICES; ++j)
+#pragma unroll
+                        for (int c = 0; c < kFp8StageCols; ++c) v[j][c] = v[j + 1][c];
+                    meet();
+                    copy_out(t0);
+                }
             }
-            rd.advance(2);
         }
+    };
+    if constexpr (kShares) {  // four groups of four warps: each takes its share of the registers
+        if (warp < kFp8EpilogueWarp0) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFp8IssueRegs));
+            if (warp == 0) issue();
+            else if (warp == 1) copy_a();
+            else if (warp == 2) copy_b();
+            else landed_here();
+        } else if (warp >= kFp8ScaleWarp0 && warp < kFp8ScaleWarp0 + 4) {
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFp8ScaleRegs));
+            scales();
+        } else {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kFp8EpilogueRegs));
+            epilogue();
+        }
+    } else {  // one choice after the other: nested as above a launch of few tokens takes 0.5 us longer
+        if (warp == 0) issue();
+        else if (warp == 1) copy_a();
+        else if (warp == 2 && !RESIDENT) copy_b();
+        else if (warp == 3 && CG == 2) landed_here();
+        else if (warp >= kFp8ScaleWarp0 && warp < kFp8ScaleWarp0 + 4) scales();
+        else if (warp >= kFp8EpilogueWarp0) epilogue();
     }
 
     __syncwarp();
@@ -764,22 +873,22 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
     }
 }
 
-template <int CG, int FORM, bool RESIDENT, typename OT>
+template <int CG, int FORM, bool RESIDENT, int SLICES, typename OT>
 __global__ void __launch_bounds__(32 * fp8_warps(CG), CG == 1 ? 2 : 1)
 fp8_gemm_kernel(const __grid_constant__ Fp8Params p, const __grid_constant__ CUtensorMap tmap_a, const __grid_constant__ CUtensorMap tmap_a2, const __grid_constant__ CUtensorMap tmap_b)
 {
-    fp8_gemm<CG, FORM, RESIDENT, OT>(p, tmap_a, tmap_a2, tmap_b, blockIdx.x / CG, gridDim.x / CG);
+    fp8_gemm<CG, FORM, RESIDENT, SLICES, OT>(p, tmap_a, tmap_a2, tmap_b, blockIdx.x / CG, gridDim.x / CG);
 }
 
 // dx and dw in one launch, the first `dx_pairs` pairs and the others: where neither fills the device.
-template <typename XT, typename WT>
+template <int SLICES, typename XT, typename WT>
 __global__ void __launch_bounds__(32 * fp8_warps(2), 1)
 fp8_gradients_kernel(const __grid_constant__ Fp8Params dx, const __grid_constant__ CUtensorMap dx_a, const __grid_constant__ CUtensorMap dx_b, const __grid_constant__ Fp8Params dw,
                      const __grid_constant__ CUtensorMap dw_a, const __grid_constant__ CUtensorMap dw_b, int dx_pairs)
 {
     const int pair = blockIdx.x / 2, pairs = gridDim.x / 2;
-    if (pair < dx_pairs) fp8_gemm<2, kFp8Dx, false, XT>(dx, dx_a, dx_a, dx_b, pair, dx_pairs);
-    else fp8_gemm<2, kFp8Dw, false, WT>(dw, dw_a, dw_a, dw_b, pair - dx_pairs, pairs - dx_pairs);
+    if (pair < dx_pairs) fp8_gemm<2, kFp8Dx, false, sizeof(XT) == 4 ? SLICES : 0, XT>(dx, dx_a, dx_a, dx_b, pair, dx_pairs);
+    else fp8_gemm<2, kFp8Dw, false, sizeof(WT) == 4 ? SLICES : 0, WT>(dw, dw_a, dw_a, dw_b, pair - dx_pairs, pairs - dx_pairs);
 }
 
 // ------------------------------------------------------------------ host side
@@ -924,27 +1033,31 @@ static int launch_fp8_kernel(void (*kernel)(Params...), int ctas, size_t smem, c
     return cudaLaunchKernelEx(&lc, kernel, args...) == cudaSuccess ? TUNA_OK : TUNA_ERR_LAUNCH;
 }
 
-// Once a device: the kernel may have as much shared memory as it asks for.
+// Once a device: the kernel may have as much shared memory as it asks for, and, if its warps share their registers out, was built to be launched with what they share (with
+// fewer, those who ask for more would wait for good).
 struct Fp8Allowed {
     bool set[64] = {false};
     std::mutex mu;
-    int allow(const void *kernel)
+    int allow(const void *kernel, bool shares)
     {
         int dev = 0;
         if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return TUNA_ERR_NO_DEVICE;
         std::lock_guard<std::mutex> lock(mu);
-        if (!set[dev] && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp8SmemMax) != cudaSuccess) return TUNA_ERR_NO_DEVICE;
+        if (set[dev]) return TUNA_OK;
+        cudaFuncAttributes has;
+        if (cudaFuncGetAttributes(&has, kernel) != cudaSuccess || (shares && has.numRegs < kFp8LaunchRegs)) return TUNA_ERR_NO_DEVICE;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kFp8SmemMax) != cudaSuccess) return TUNA_ERR_NO_DEVICE;
         set[dev] = true;
         return TUNA_OK;
     }
 };
 
-template <int CG, int FORM, bool RESIDENT, typename OT>
+template <int CG, int FORM, bool RESIDENT, int SLICES, typename OT>
 static int launch_fp8(const Fp8Params &p, const Fp8Maps &maps, int ctas, size_t smem, cudaStream_t stream)
 {
     static Fp8Allowed allowed;
-    const int st = allowed.allow((const void *)fp8_gemm_kernel<CG, FORM, RESIDENT, OT>);
-    return st != TUNA_OK ? st : launch_fp8_kernel<CG>(fp8_gemm_kernel<CG, FORM, RESIDENT, OT>, ctas, smem, stream, p, maps.a, maps.a2, maps.b);
+    const int st = allowed.allow((const void *)fp8_gemm_kernel<CG, FORM, RESIDENT, SLICES, OT>, SLICES > kFp8NarrowSlices);
+    return st != TUNA_OK ? st : launch_fp8_kernel<CG>(fp8_gemm_kernel<CG, FORM, RESIDENT, SLICES, OT>, ctas, smem, stream, p, maps.a, maps.a2, maps.b);
 }
 
 // A launch: plan, parameters and tensor maps.
@@ -956,21 +1069,30 @@ struct Fp8Launch {
     int pairs() const { return (int)std::min<long long>((long long)l.row_tiles * l.col_tiles, l.workers); }  // or single CTAs
 };
 
+template <int SLICES, typename OT>
+static int launch_fp8_pairs(const Fp8Launch &a, cudaStream_t stream)
+{
+    const int ctas = 2 * a.pairs();
+    if (a.form == kFp8GatedProduct) return launch_fp8<2, kFp8GatedProduct, false, SLICES, OT>(a.p, a.maps, ctas, a.l.smem, stream);
+    constexpr int kSlices = sizeof(OT) == 4 ? SLICES : 0;
+    switch (a.form) {
+        case kFp8Product: return launch_fp8<2, kFp8Product, false, kSlices, OT>(a.p, a.maps, ctas, a.l.smem, stream);
+        case kFp8Dx: return launch_fp8<2, kFp8Dx, false, kSlices, OT>(a.p, a.maps, ctas, a.l.smem, stream);
+        default: return launch_fp8<2, kFp8Dw, false, kSlices, OT>(a.p, a.maps, ctas, a.l.smem, stream);
+    }
+}
+
 template <typename OT>
 static int launch_fp8_as(const Fp8Launch &a, cudaStream_t stream)
 {
     const Fp8Plan &l = a.l;
-    const int ctas = a.pairs() * l.cg;
+    const int ctas = a.pairs();
     if (l.cg == 1) {
-        if (a.form == kFp8Product) return l.resident ? launch_fp8<1, kFp8Product, true, OT>(a.p, a.maps, ctas, l.smem, stream) : launch_fp8<1, kFp8Product, false, OT>(a.p, a.maps, ctas, l.smem, stream);
-        return l.resident ? launch_fp8<1, kFp8GatedProduct, true, OT>(a.p, a.maps, ctas, l.smem, stream) : launch_fp8<1, kFp8GatedProduct, false, OT>(a.p, a.maps, ctas, l.smem, stream);
+        if (a.form == kFp8Product) return l.resident ? launch_fp8<1, kFp8Product, true, 0, OT>(a.p, a.maps, ctas, l.smem, stream) : launch_fp8<1, kFp8Product, false, 0, OT>(a.p, a.maps, ctas, l.smem, stream);
+        return l.resident ? launch_fp8<1, kFp8GatedProduct, true, 0, OT>(a.p, a.maps, ctas, l.smem, stream) : launch_fp8<1, kFp8GatedProduct, false, 0, OT>(a.p, a.maps, ctas, l.smem, stream);
     }
-    switch (a.form) {
-        case kFp8Product: return launch_fp8<2, kFp8Product, false, OT>(a.p, a.maps, ctas, l.smem, stream);
-        case kFp8GatedProduct: return launch_fp8<2, kFp8GatedProduct, false, OT>(a.p, a.maps, ctas, l.smem, stream);
-        case kFp8Dx: return launch_fp8<2, kFp8Dx, false, OT>(a.p, a.maps, ctas, l.smem, stream);
-        default: return launch_fp8<2, kFp8Dw, false, OT>(a.p, a.maps, ctas, l.smem, stream);
-    }
+    if (a.p.parts == 1) return launch_fp8_pairs<0, OT>(a, stream);
+    return l.tile_cols <= kFp8NarrowCols ? launch_fp8_pairs<kFp8NarrowSlices, OT>(a, stream) : launch_fp8_pairs<kFp8WideSlices, OT>(a, stream);
 }
 
 static int launch_fp8_any(const Fp8Launch &a, cudaStream_t stream)
@@ -993,6 +1115,8 @@ static int prepare_fp8(Fp8Launch &out, int form, const Fp8Codes &a, int rows, co
     p.rows = rows; p.cols = cols; p.red = red;
     p.blocks = div_up(red, kFp8Block);
     p.fold_log = l.fold_log; p.units = div_up(p.blocks, 1 << l.fold_log); p.steps = div_up(p.units, kFp8Deep);
+    p.parts = o_type == TUNA_FP32 || z ? div_up(p.steps, l.tile_cols <= kFp8NarrowCols ? kFp8PartSteps : kFp8WidePartSteps) : 1;
+    p.part_steps = div_up(p.steps, p.parts); p.parts = div_up(p.steps, p.part_steps);
     p.tile_cols = l.tile_cols; p.width = l.width; p.row_tiles = l.row_tiles; p.col_tiles = l.col_tiles;
     p.rows_inner = l.row_tiles < l.col_tiles;
     p.a_bytes = l.a_bytes; p.b_rows = l.b_rows; p.stages = l.stages; p.d_cols = l.d_cols;
@@ -1039,13 +1163,21 @@ int launch_fp8_product(const Fp8ProductArgs &a)
     return launch_fp8_any(launch, a.stream);
 }
 
+template <int SLICES, typename XT, typename WT>
+static int launch_fp8_both_of(const Fp8Launch &dx, const Fp8Launch &dw, cudaStream_t stream)
+{
+    static Fp8Allowed allowed;
+    const int st = allowed.allow((const void *)fp8_gradients_kernel<SLICES, XT, WT>, SLICES > kFp8NarrowSlices), dx_pairs = dx.pairs();
+    return st != TUNA_OK ? st : launch_fp8_kernel<2>(fp8_gradients_kernel<SLICES, XT, WT>, 2 * (dx_pairs + dw.pairs()), std::max(dx.l.smem, dw.l.smem), stream, dx.p, dx.maps.a, dx.maps.b, dw.p,
+                                                     dw.maps.a, dw.maps.b, dx_pairs);
+}
 template <typename XT, typename WT>
 static int launch_fp8_both(const Fp8Launch &dx, const Fp8Launch &dw, cudaStream_t stream)
 {
-    static Fp8Allowed allowed;
-    const int st = allowed.allow((const void *)fp8_gradients_kernel<XT, WT>), dx_pairs = dx.pairs();
-    return st != TUNA_OK ? st : launch_fp8_kernel<2>(fp8_gradients_kernel<XT, WT>, 2 * (dx_pairs + dw.pairs()), std::max(dx.l.smem, dw.l.smem), stream, dx.p, dx.maps.a, dx.maps.b, dw.p,
-                                                     dw.maps.a, dw.maps.b, dx_pairs);
+    if constexpr (sizeof(XT) == 4 || sizeof(WT) == 4)
+        if (dx.p.parts > 1 || dw.p.parts > 1)
+            return std::max(dx.l.tile_cols, dw.l.tile_cols) <= kFp8NarrowCols ? launch_fp8_both_of<kFp8NarrowSlices, XT, WT>(dx, dw, stream) : launch_fp8_both_of<kFp8WideSlices, XT, WT>(dx, dw, stream);
+    return launch_fp8_both_of<0, XT, WT>(dx, dw, stream);
 }
 template <typename XT>
 static int launch_fp8_both_as(const Fp8Launch &dx, const Fp8Launch &dw, cudaStream_t stream)

@@ -45,8 +45,8 @@ __device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity)
 
 // Bounded wait.  Returns false when the time limit ran out or another role raised the abort
 // flag; the caller unwinds.
-static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int *abort_flag,
-                                            DeviceStatus *status, int where, long long limit = kWaitCycles)
+__device__ __forceinline__ bool mbar_wait_loop(uint32_t bar, uint32_t parity, volatile int *abort_flag,
+                                               DeviceStatus *status, int where, long long limit)
 {
     const long long t0 = clock64();
     for (;;) {
@@ -65,18 +65,29 @@ static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity
     }
 }
 
+// Out of the way of what waits rarely.
+static __device__ __noinline__ bool mbar_wait_slow(uint32_t bar, uint32_t parity, volatile int *abort_flag,
+                                            DeviceStatus *status, int where, long long limit = kWaitCycles)
+{
+    return mbar_wait_loop(bar, parity, abort_flag, status, where, limit);
+}
+
+// CALL false: no call, for kernels whose warps share their registers out among themselves (setmaxnreg): a callee's would have to
+// be in every share.
+template <bool CALL = true>
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *abort_flag,
                                           DeviceStatus *status, int where)
 {
     if (mbar_try_wait(bar, parity)) return true;
-    return mbar_wait_slow(bar, parity, abort_flag, status, where);
+    return CALL ? mbar_wait_slow(bar, parity, abort_flag, status, where) : mbar_wait_loop(bar, parity, abort_flag, status, where, kWaitCycles);
 }
 
 // The same wait executed by a whole converged warp, with one answer for all its lanes.
+template <bool CALL = true>
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile int *abort_flag,
                                                DeviceStatus *status, int where)
 {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, where)) != 0;
+    return __all_sync(0xffffffffu, mbar_wait<CALL>(bar, parity, abort_flag, status, where)) != 0;
 }
 
 // ---- CTA pairs: barriers that the other CTA of the cluster arrives at

@@ -159,7 +159,7 @@ def fp8_dequant(q, s, o, m: int, k: int, blocks: str = "square") -> None:
 
 def fp8_matmul(x, xs, q, s, o, m: int, n: int, k: int, *, workspace=None) -> None:
     """o `[n, m]` (fp16, bf16 or fp32, overwritten) = x `[n, k]` times the transposed matrix of `(q, s)` `[m, k]` (square blocks), fp32 accumulation,
-    one rounding.  x is codes with their scales `xs` (row blocks), or fp16 or bf16 with `xs=None`: the call quantizes it as `fp8_quantize` does.
+    one rounding; for o in fp32 long sums are made of parts, so that they are as exact as sums in fp32 that round.  x is codes with their scales `xs` (row blocks), or fp16 or bf16 with `xs=None`: the call quantizes it as `fp8_quantize` does.
     m and k multiples of 16.  Enqueued on the current stream of x's device, in whose order it reads and writes; only q and s, up to 64 tokens, count
     as constants and are read while the kernel before still drains, as in `mx_matmul`."""
     if workspace is None and _launched(_front().fp8_matmul(x, xs, q, s, o, m, n, k)):
@@ -215,7 +215,7 @@ def fp8_gated(x, xs, q, s, h, f: int, n: int, k: int, activation: str = "silu", 
     `[n, f]` being x `[n, k]` times the transposed first and last f rows of the matrix of `(q, s)` `[2f, k]` (square blocks): gate and up projection,
     one over the other.  x as in `fp8_matmul`, and so are the order of reading and the constants.  activation: `"silu"`, or `"gelu"` in its tanh
     form.  z `[n, 2f]` of h's type (fp16 or bf16) keeps g and u, side by side, for `fp8_gated_backward`; h is made of g and u before they are
-    rounded.  f and k multiples of 16."""
+    rounded; long sums are made of parts then, and h may be a rounding off from the one without z.  f and k multiples of 16."""
     act = _choice(activation, "activation", _ACTIVATIONS)
     if workspace is None and _launched(_front().fp8_gated(x, xs, q, s, h, f, n, k, act, z)):
         return
