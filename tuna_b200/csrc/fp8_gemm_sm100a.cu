@@ -216,7 +216,14 @@ __device__ __forceinline__ void fp8_quantize_resident(const Fp8Params &p, int w,
     }
 }
 
-__device__ __forceinline__ float fp8_activation(float g, float u, int gelu) { return gelu ? g * fp8_gate<true>(g) * u : g * fp8_gate<false>(g) * u; }
+// activation(g) u of two numbers of the output's type
+template <typename OT>
+__device__ __forceinline__ float2 fp8_activation(float g0, float u0, float g1, float u1, int gelu)
+{
+    constexpr bool kExact = sizeof(OT) == 4;
+    const float2 s = (gelu ? fp8_gate<true, kExact>(g0, g1) : fp8_gate<false, kExact>(g0, g1)).both();
+    return make_float2(g0 * s.x * u0, g1 * s.y * u1);
+}
 
 // CG: CTAs of a worker (1 or 2).  SLICES: of a pair's tile the slices of columns whose sums an epilogue group adds up of parts, 0 where sums have one part.  Single CTAs leave room for a second one on the SM: that of the next launch, which copies its first weights meanwhile.
 template <int CG, int FORM, bool RESIDENT, int SLICES, typename OT>
@@ -707,19 +714,18 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
                     rows_of_8(to, kPitch);
                 } else {
                     if (z) rows_of_8(z_staging, kPitchZ);
-                    auto act = [&](float g, float u) { return fp8_activation(g, u, p.gelu); };
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {  // lanes i and i + 8 of a half: gate and other projection of one feature, two columns
-                        const float l0 = act(lo(4 * i), lo(4 * i + 2)), l1 = act(lo(4 * i + 1), lo(4 * i + 3));
-                        const float h0 = act(hi(4 * i), hi(4 * i + 2)), h1 = act(hi(4 * i + 1), hi(4 * i + 3));
+                        const float2 l = fp8_activation<OT>(lo(4 * i), lo(4 * i + 2), lo(4 * i + 1), lo(4 * i + 3), p.gelu);
+                        const float2 h = fp8_activation<OT>(hi(4 * i), hi(4 * i + 2), hi(4 * i + 1), hi(4 * i + 3), p.gelu);
                         if constexpr (sizeof(OT) == 2) {
-                            stmatrix_x2_trans(to + (uint32_t)(8 * i + (lane & 7)) * kPitch + (uint32_t)(2 * quarter + ((lane >> 3) & 1)) * 16u, mx_pack2<OT>(l0, l1), mx_pack2<OT>(h0, h1));
+                            stmatrix_x2_trans(to + (uint32_t)(8 * i + (lane & 7)) * kPitch + (uint32_t)(2 * quarter + ((lane >> 3) & 1)) * 16u, mx_pack2<OT>(l.x, l.y), mx_pack2<OT>(h.x, h.y));
                         } else {
                             const uint32_t dst = to + (uint32_t)(8 * i + 2 * (lane & 3)) * kPitch + (uint32_t)(16 * quarter + (lane >> 2)) * 4u;
-                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst), "f"(l0) : "memory");
-                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + kPitch), "f"(l1) : "memory");
-                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + 32u), "f"(h0) : "memory");
-                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + kPitch + 32u), "f"(h1) : "memory");
+                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst), "f"(l.x) : "memory");
+                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + kPitch), "f"(l.y) : "memory");
+                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + 32u), "f"(h.x) : "memory");
+                            asm volatile("st.shared.f32 [%0], %1;" ::"r"(dst + kPitch + 32u), "f"(h.y) : "memory");
                         }
                     }
                 }
@@ -781,7 +787,7 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
                         const int i = thread & 63;
                         for (int t = thread >> 6; t < tile.valid && i < features; t += 2) {
                             const float g = sum(t, i), u = sum(t, features + i);
-                            o[(size_t)t * out + row0 / 2 + i] = mx_convert<OT>(fp8_activation(g, u, p.gelu));
+                            o[(size_t)t * out + row0 / 2 + i] = mx_convert<OT>(fp8_activation<OT>(g, u, g, u, p.gelu).x);
                             if (z) {
                                 OT *to = z + (size_t)t * p.rows + row0 / 2 + i;
                                 to[0] = mx_convert<OT>(g);
