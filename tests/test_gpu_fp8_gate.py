@@ -1,4 +1,7 @@
-"""The activations of the 8-bit gated block, step by step: results in 32 bits, and results in 16 bits far down."""
+"""The activations of the 8-bit gated block, step by step: results in 32 bits, results in 16 bits far down, and the reciprocal that the gradients divide by."""
+
+import re
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -6,7 +9,7 @@ import torch
 
 import tuna_b200
 from tests.fp8_util import numpy64
-from tuna_b200 import _lib
+from tuna_b200 import _lib, build
 
 pytestmark = pytest.mark.gpu
 STEP = 2.0 ** -23
@@ -75,3 +78,49 @@ def test_results_in_16_bits_are_right_to_the_last_that_there_are(n, kind, dtype)
     if dtype == torch.bfloat16:
         assert (got != 0)[(argument(g, kind) > -87) & (g != 0)].all()
 
+
+PROGRAM = """
+typedef unsigned int uint32_t;
+typedef unsigned long long uint64_t;
+%s
+// out[0]: how many reciprocals of the numbers 2^e (1 + m 2^-23) are not the nearest, out[1]: the bits of one of them
+extern "C" __global__ void reciprocals(int e, unsigned int *out)
+{
+    const unsigned int m = blockIdx.x * blockDim.x + threadIdx.x;
+    const float x = __uint_as_float((unsigned int)(e + 127) << 23 | m), y = __uint_as_float((unsigned int)(e + 127) << 23 | (m * 2654435761u & 0x7fffffu));
+    const float2 r = tuna::fp8_reciprocal(tuna::Fp8Two(x, y)).both();
+    if (r.x != 1.0f / x || r.y != 1.0f / y) {
+        atomicAdd(out, 1u);
+        out[1] = __float_as_uint(r.x != 1.0f / x ? x : y);
+    }
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def reciprocals():
+    text = re.sub(r"^\s*#pragma once.*$", "", (Path(build.CSRC) / "fp8_gate.cuh").read_text(), flags=re.M)
+    assert "#include" not in text
+    return torch.cuda._compile_kernel(PROGRAM % text, "reciprocals")
+
+
+@pytest.mark.parametrize("e", [0, 1, 2, 24, 63, 100, 124, 125])
+def test_the_reciprocal_is_the_nearest_number(reciprocals, e):
+    """Of every significand: the quotient that torch's division gives."""
+    out = torch.zeros(2, dtype=torch.int32, device="cuda")
+    reciprocals(grid=(1 << 15, 1, 1), block=(256, 1, 1), args=[e, out])
+    count, bits = out.tolist()
+    assert count == 0, f"{count} of 2^24, among them {bits:#x}"
+
+
+def test_the_reciprocals_ends(reciprocals):
+    """From 2^126 on the nearest number is not normal: the estimate stands."""
+    source = PROGRAM.replace("extern", """extern "C" __global__ void at(const float *x, float *r, int n) { for (int i = 0; i < n; ++i) r[i] = tuna::fp8_reciprocal(tuna::Fp8Two(x[i])).both().x; }
+extern""", 1)
+    text = re.sub(r"^\s*#pragma once.*$", "", (Path(build.CSRC) / "fp8_gate.cuh").read_text(), flags=re.M)
+    run = torch.cuda._compile_kernel(source % text, "at")
+    x = torch.tensor([1.0, 2.0 ** 126, 2.0 ** 126 * 1.5, 2.0 ** 127 * 1.99, float("inf"), 2 - 2.0 ** -23], device="cuda")
+    r = torch.empty_like(x)
+    run(grid=(1, 1, 1), block=(1, 1, 1), args=[x, r, x.numel()])
+    want = 1 / x.double()
+    assert ((r.double() - want).abs() <= 2.0 ** -24 * want + 2.0 ** -148).all()

@@ -46,7 +46,8 @@ __device__ __forceinline__ Fp8Two fp8_rounded_product(Fp8Two a, Fp8Two b)
     return fp8_fma(a, b, Fp8Two(__uint_as_float(0x80000000u | sm >> 20)));
 }
 
-// 1 / x for x >= 1: a Newton step with fused multiply-adds (Markstein, 1990) from the hardware's estimate, which leaves the number nearest to it where that is normal.
+// 1 / x for x >= 1, the number nearest to it where that is normal: a Newton step with fused multiply-adds (Markstein, 1990) from the hardware's estimate.  The theorem leaves out divisors whose
+// significand is all ones, for which it depends on the estimate; compared with the quotient for every significand, they are right as well.
 __device__ __forceinline__ Fp8Two fp8_reciprocal(Fp8Two x)
 {
     const float2 f = x.both();
