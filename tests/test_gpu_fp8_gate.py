@@ -124,3 +124,29 @@ extern""", 1)
     run(grid=(1, 1, 1), block=(1, 1, 1), args=[x, r, x.numel()])
     want = 1 / x.double()
     assert ((r.double() - want).abs() <= 2.0 ** -24 * want + 2.0 ** -148).all()
+
+
+ROUNDED = """
+typedef unsigned int uint32_t;
+typedef unsigned long long uint64_t;
+%s
+// out: how many of c + a b are not rounded twice, and how many of them a fused step would give
+extern "C" __global__ void rounded(const float *a, const float *b, const float *c, double minus_zero, int *out)
+{
+    const int i = blockIdx.x * blockDim.x + threadIdx.x;
+    const tuna::Fp8Two sum = tuna::Fp8Two(c[i]) + tuna::fp8_rounded_product(tuna::Fp8Two(a[i]), tuna::Fp8Two(b[i]), (float)minus_zero);
+    if (sum.both().x != __fadd_rn(c[i], __fmul_rn(a[i], b[i]))) atomicAdd(out, 1);
+    if (__fmaf_rn(a[i], b[i], c[i]) != __fadd_rn(c[i], __fmul_rn(a[i], b[i]))) atomicAdd(out + 1, 1);
+}
+"""
+
+
+def test_a_product_that_is_added_is_rounded_first():
+    text = re.sub(r"^\s*#pragma once.*$", "", (Path(build.CSRC) / "fp8_gate.cuh").read_text(), flags=re.M)
+    run = torch.cuda._compile_kernel(ROUNDED % text, "rounded")
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    a, b, c = (torch.randn(1 << 20, generator=gen, device="cuda") for _ in range(3))
+    out = torch.zeros(2, dtype=torch.int32, device="cuda")
+    run(grid=(1 << 12, 1, 1), block=(256, 1, 1), args=[a, b, c, -0.0, out])
+    wrong, fused = out.tolist()
+    assert wrong == 0 and fused > 1 << 16  # these numbers tell one from the other

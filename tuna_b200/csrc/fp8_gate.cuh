@@ -38,13 +38,9 @@ __device__ __forceinline__ Fp8Two operator*(Fp8Two a, Fp8Two b)
     return r;
 }
 // The product of what is to be added to something.  A product of two at once is made one step with a sum that follows by the compiler, although both say that they round; so it is
-// the sum with a -0 that the compiler cannot know for one (gradients of 1360 features and 333 tokens 22.0 us; 22.9 with two single products, which it leaves apart and which are as fast for SiLU's one).
-__device__ __forceinline__ Fp8Two fp8_rounded_product(Fp8Two a, Fp8Two b)
-{
-    uint32_t sm;
-    asm("mov.u32 %0, %%smid;" : "=r"(sm));
-    return fp8_fma(a, b, Fp8Two(__uint_as_float(0x80000000u | sm >> 20)));
-}
+// the sum with a -0 that the compiler does not know for one: an argument of the launch (gradients of 1360 features and 333 tokens 22.0 us; 22.9 with two single products, which it leaves apart
+// and which are as fast for SiLU's one).
+__device__ __forceinline__ Fp8Two fp8_rounded_product(Fp8Two a, Fp8Two b, float minus_zero) { return fp8_fma(a, b, Fp8Two(minus_zero)); }
 
 // 1 / x for x >= 1, the number nearest to it where that is normal: a Newton step with fused multiply-adds (Markstein, 1990) from the hardware's estimate.  The theorem leaves out divisors whose
 // significand is all ones, for which it depends on the estimate; compared with the quotient for every significand, they are right as well.
@@ -73,16 +69,16 @@ __device__ __forceinline__ Fp8Two fp8_gate(float g0, float g1)
 // sigma, and the derivative of g sigma: sigma + g sigma (1 - sigma) p'.  What is made of these is quantized to three bits, where an error of 2^-22 turns one number of 2^18 into its neighbour, a
 // sixteenth away; so, unlike above, every step is rounded to nearest, in the order in which the formula stands, as elementary operations in 32 bits do it.
 template <bool GELU>
-__device__ __forceinline__ void fp8_gate_and_slope(Fp8Two g, Fp8Two &sigma, Fp8Two &derivative)
+__device__ __forceinline__ void fp8_gate_and_slope(Fp8Two g, float minus_zero, Fp8Two &sigma, Fp8Two &derivative)
 {
     const Fp8Two one(1.0f), square = g * g;
-    const float2 p = (GELU ? Fp8Two(kGeluA) * (g + fp8_rounded_product(Fp8Two(kGeluB), square * g)) : g).both();
+    const float2 p = (GELU ? Fp8Two(kGeluA) * (g + fp8_rounded_product(Fp8Two(kGeluB), square * g, minus_zero)) : g).both();
     sigma = fp8_reciprocal(one + Fp8Two(expf(-p.x), expf(-p.y)));
     const Fp8Two a = g * sigma, b = fp8_fma(sigma, Fp8Two(-1.0f), one);
     Fp8Two rest;
     if (GELU) {  // where sigma has become 0 or 1 rest is 0, whatever p' is
         rest = a * b;
-        const float2 r = rest.both(), slope = (rest * (Fp8Two(kGeluA) * (one + fp8_rounded_product(Fp8Two(kGeluB3), square)))).both();
+        const float2 r = rest.both(), slope = (rest * (Fp8Two(kGeluA) * (one + fp8_rounded_product(Fp8Two(kGeluB3), square, minus_zero)))).both();
         rest = {r.x == 0.0f ? r.x : slope.x, r.y == 0.0f ? r.y : slope.y};
     } else {
         const float2 l = a.both(), r = b.both();

@@ -246,7 +246,7 @@ struct Fp8Plain {
 };
 // Eight columns of a gated block's gradients: of the gate, dh u act'(g), and of the other projection, dh act(g); or of one of them.
 template <typename T, bool GELU>
-__device__ __forceinline__ void fp8_gated_row(const Mx8<T> &g, const Mx8<T> &u, const Mx8<T> &d, float (&of_gate)[8], float (&of_other)[8])
+__device__ __forceinline__ void fp8_gated_row(const Mx8<T> &g, const Mx8<T> &u, const Mx8<T> &d, float minus_zero, float (&of_gate)[8], float (&of_other)[8])
 {
     float gv[8], uv[8], dv[8];
     g.values(gv);
@@ -256,17 +256,17 @@ __device__ __forceinline__ void fp8_gated_row(const Mx8<T> &g, const Mx8<T> &u, 
     for (int i = 0; i < 8; i += 2) {
         const Fp8Two gate(gv[i], gv[i + 1]), dh(dv[i], dv[i + 1]);
         Fp8Two sigma, derivative;
-        fp8_gate_and_slope<GELU>(gate, sigma, derivative);
+        fp8_gate_and_slope<GELU>(gate, minus_zero, sigma, derivative);
         const float2 a = (dh * Fp8Two(uv[i], uv[i + 1]) * derivative).both(), b = (dh * gate * sigma).both();
         of_gate[i] = a.x, of_gate[i + 1] = a.y;
         of_other[i] = b.x, of_other[i + 1] = b.y;
     }
 }
 template <typename T, bool GELU>
-__device__ __forceinline__ void fp8_gated_row(const Mx8<T> &g, const Mx8<T> &u, const Mx8<T> &d, bool gate, float (&to)[8])
+__device__ __forceinline__ void fp8_gated_row(const Mx8<T> &g, const Mx8<T> &u, const Mx8<T> &d, float minus_zero, bool gate, float (&to)[8])
 {
     float of_other[8];
-    fp8_gated_row<T, GELU>(g, u, d, to, of_other);
+    fp8_gated_row<T, GELU>(g, u, d, minus_zero, to, of_other);
     if (!gate)
 #pragma unroll
         for (int i = 0; i < 8; ++i) to[i] = of_other[i];
@@ -278,6 +278,7 @@ template <typename T, bool GELU, int PARTS>
 struct Fp8Gated {
     const T *z, *dh;
     int f;
+    float minus_zero = -0.0f;
     using Raw = Fp8RawFloat;
     static constexpr int kParts = PARTS;
     __device__ __forceinline__ int part_cols() const { return f; }
@@ -308,8 +309,8 @@ struct Fp8Gated {
             }
 #pragma unroll
             for (int r = 0; r < kBatch; ++r) {
-                if constexpr (PARTS == 2) fp8_gated_row<T, GELU>(g[r], u[r], d[r], to.v[r0 + r], to.v[kLaneRows + r0 + r]);
-                else fp8_gated_row<T, GELU>(g[r], u[r], d[r], gate, to.v[r0 + r]);
+                if constexpr (PARTS == 2) fp8_gated_row<T, GELU>(g[r], u[r], d[r], minus_zero, to.v[r0 + r], to.v[kLaneRows + r0 + r]);
+                else fp8_gated_row<T, GELU>(g[r], u[r], d[r], minus_zero, gate, to.v[r0 + r]);
             }
         }
     }
@@ -499,6 +500,7 @@ template <typename T, bool GELU>
 struct Fp8GatedStaged {
     int f, col_tiles, tiles, stride, next;  // the tile that is copied next, and how far apart the CTA's are
     uint32_t box, bar;                      // of the tile that is loaded
+    float minus_zero;
     const CUtensorMap *z, *dh;
     using Raw = Fp8RawFloat;
     static constexpr int kParts = 2;
@@ -524,7 +526,7 @@ struct Fp8GatedStaged {
 #pragma unroll
         for (int r = 0; r < kLaneRows; ++r) {
             const uint32_t at = box + (uint32_t)(warp * Fp8Tile<2>::kRows + 2 * r + (lane >> 4)) * (2 * kFp8Block) + (uint32_t)(lane & 15) * 16u;
-            fp8_gated_row<T, GELU>(piece(at), piece(at + kFp8BoxBytes), piece(at + 2 * kFp8BoxBytes), to.v[r], to.v[kLaneRows + r]);
+            fp8_gated_row<T, GELU>(piece(at), piece(at + kFp8BoxBytes), piece(at + 2 * kFp8BoxBytes), minus_zero, to.v[r], to.v[kLaneRows + r]);
         }
         __syncthreads();  // everybody has read the boxes
         copy();
@@ -535,7 +537,7 @@ struct Fp8GatedStaged {
 template <typename T, bool GELU, int WAYS>
 __global__ void __launch_bounds__(512, 1)
 fp8_gated_stream_kernel(const __grid_constant__ CUtensorMap tmap_z, const __grid_constant__ CUtensorMap tmap_dh, uint8_t *q, uint8_t *s, uint8_t *q2, uint8_t *s2, int rows, int f,
-                        DeviceStatus *status)
+                        float minus_zero, DeviceStatus *status)
 {
     extern __shared__ __align__(128) uint8_t boxes[];
     __shared__ __align__(16) Fp8TileShared<2> shared;
@@ -554,6 +556,7 @@ fp8_gated_stream_kernel(const __grid_constant__ CUtensorMap tmap_z, const __grid
     asm volatile("griddepcontrol.wait;" ::: "memory");
     Fp8GatedStaged<T, GELU> src;
     src.f = f;
+    src.minus_zero = minus_zero;
     src.col_tiles = f / kFp8Block;
     src.tiles = src.col_tiles * div_up(rows, kFp8Block);
     src.stride = gridDim.x;
@@ -682,7 +685,7 @@ static cudaError_t stream_launch(const Fp8GradientArgs &a, const Fp8Codes &to, c
     cudaLaunchAttribute attr;
     cudaLaunchConfig_t lc = tile_config(a.sm_count, 1, 512, true, attr, a.stream);
     lc.dynamicSmemBytes = kFp8StreamBytes;
-    return cudaLaunchKernelEx(&lc, fp8_gated_stream_kernel<T, GELU, WAYS>, z, dh, (uint8_t *)to.q, (uint8_t *)to.s, (uint8_t *)to2.q, (uint8_t *)to2.s, a.rows, f, status);
+    return cudaLaunchKernelEx(&lc, fp8_gated_stream_kernel<T, GELU, WAYS>, z, dh, (uint8_t *)to.q, (uint8_t *)to.s, (uint8_t *)to2.q, (uint8_t *)to2.s, a.rows, f, -0.0f, status);
 }
 
 template <typename T, bool GELU>
