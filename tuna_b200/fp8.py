@@ -251,13 +251,28 @@ def fp8_gated_backward(dh, z, x, xs, q, s, dx, dw, f: int, n: int, k: int, activ
 
 def fp8_pack(codes, scales):
     """A checkpoint's matrix with fp32 scales, codes `torch.float8_e4m3fn` `[rows, k]` and scales fp32 `[ceil(rows/128), ceil(k/128)]` of any value, in
-    this package's form: `(q, s)` with square blocks.  Blocks whose scale is a power of two keep their numbers; the others are quantized again, each
-    number off by at most half a step of e4m3.  On any device."""
+    this package's form: `(q, s)` with square blocks.  Blocks whose scale is a power of two, 2^-127 or above, keep their numbers; the others are quantized
+    again, each number off by at most half a step of e4m3 (steps do not go below 2^-136).  A block with an infinity or NaN, or a number above fp32's, is
+    NaN.  On any device, a few million numbers at a time."""
     if not isinstance(codes, torch.Tensor) or codes.dtype != _CODES or codes.dim() != 2:
         raise ValueError("codes must be a torch.float8_e4m3fn [rows, k] tensor")
     rows, k = codes.shape
     if not isinstance(scales, torch.Tensor) or scales.dtype != torch.float32 or tuple(scales.shape) != _scale_shape(rows, k, "square"):
         raise ValueError(f"scales must be a torch.float32 {list(_scale_shape(rows, k, 'square'))} tensor")
+    q = torch.empty((rows, k), dtype=_CODES, device=codes.device)
+    s = torch.empty(_scale_shape(rows, k, "square"), dtype=torch.uint8, device=codes.device)
+    blocks = max(1, _PACK_NUMBERS // (128 * max(k, 1)))  # of rows
+    for b in range(0, s.shape[0], blocks):
+        at = slice(128 * b, 128 * (b + blocks))
+        q[at], s[b:b + blocks] = _pack_blocks(codes[at], scales[b:b + blocks])
+    return q, s
+
+
+_PACK_NUMBERS = 1 << 22  # of 64 bits and some of their kind at once: a third of a gigabyte
+
+
+def _pack_blocks(codes, scales):
+    rows, k = codes.shape
     # in 64 bits: the product of a code and a scale is exact, and so is what it becomes over a power of two
     blocks = torch.nn.functional.pad(codes.double(), (0, -k % 128, 0, -rows % 128)).unflatten(0, (-1, 128)).unflatten(2, (-1, 128)) * scales.double()[:, None, :, None]
     largest = blocks.abs().amax((1, 3))
