@@ -1,0 +1,17 @@
+"""What the 8-bit calls say where they refuse."""
+
+import pytest
+import torch
+
+import tuna_b200
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("z_type", [torch.float16, torch.bfloat16, torch.float32], ids=str)
+def test_z_beside_results_in_32_bits(z_type):
+    f, n, k = 32, 4, 64
+    q, s = tuna_b200.fp8_quantize(torch.zeros(2 * f, k, device="cuda"), "square")
+    x, h = torch.zeros(n, k, device="cuda", dtype=torch.float16), torch.zeros(n, f, device="cuda")
+    with pytest.raises(TypeError, match="h must be torch.float16 or torch.bfloat16"):
+        tuna_b200.fp8_gated(x, None, q, s, h, f, n, k, z=torch.zeros(n, 2 * f, device="cuda", dtype=z_type))

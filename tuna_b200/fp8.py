@@ -225,6 +225,8 @@ def fp8_gated(x, xs, q, s, h, f: int, n: int, k: int, activation: str = "silu", 
     _expect_codes(q, s, ("q", "s"), 2 * f, k, "square", dev)
     _expect_output(h, n * f, dev)
     if z is not None:
+        if h.dtype == torch.float32:
+            raise TypeError("with z h must be torch.float16 or torch.bfloat16, got torch.float32")
         _expect_16bit(z, "z", n * 2 * f, dev, h.dtype)
     with _on_device(dev):
         _keep, ws = _workspace(workspace, dev, _GATED, 2 * f, n, k, kind)
