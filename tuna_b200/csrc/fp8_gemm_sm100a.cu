@@ -225,7 +225,7 @@ __device__ __forceinline__ float2 fp8_activation(float g0, float u0, float g1, f
     return make_float2(g0 * s.x * u0, g1 * s.y * u1);
 }
 
-// CG: CTAs of a worker (1 or 2).  SLICES: of a pair's tile the slices of columns whose sums an epilogue group adds up of parts, 0 where sums have one part.  Single CTAs leave room for a second one on the SM: that of the next launch, which copies its first weights meanwhile.
+// CG: CTAs of a worker (1 or 2).  SLICES: 0 where sums have one part; otherwise the slices of a tile's columns whose parts an epilogue group adds up.  Single CTAs leave room for a second one on the SM: that of the next launch, which copies its first weights meanwhile.
 template <int CG, int FORM, bool RESIDENT, int SLICES, typename OT>
 __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &tmap_a, const CUtensorMap &tmap_a2, const CUtensorMap &tmap_b, int worker, int workers)
 {
@@ -235,7 +235,7 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
     __shared__ uint32_t s_tmem_base;
     __shared__ int s_abort;
 
-    constexpr bool kParts = CG == 2 && SLICES > 0, kShares = SLICES > kFp8NarrowSlices;
+    constexpr bool kParts = SLICES > 0, kShares = SLICES > kFp8NarrowSlices;
     constexpr bool kGated = FORM == kFp8GatedProduct, kAcrossA = FORM >= kFp8Dx, kAcrossB = FORM == kFp8Dw;
     constexpr uint32_t kTmemCols = CG == 1 ? 256 : 512, kSfCol = kTmemCols - 2 * kFp8SfCols;  // two accumulators below
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -324,20 +324,21 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
             const uint64_t b_form = RESIDENT ? ((uint64_t)p.cols << 16) | ((uint64_t)(8u * (uint32_t)p.cols | (1u << 14)) << 32) : sw128;
             while (ok && tile.next(p)) {
                 const uint32_t idesc = fp8_idesc<CG>(p.fold_log ? p.d_cols : mma_cols(), kAcrossA, kAcrossB);
-                const int part_steps = CG == 2 && !kParts ? p.steps : p.part_steps;
                 uint32_t d = 0;
+                auto next_accumulator = [&] {
+                    ok = mbar_wait_warp<!kShares>(d_empty + 8 * rd.idx, rd.phase ^ 1, abort_flag, p.status, 303);
+                    d = tmem + (uint32_t)(rd.idx * p.d_cols);
+                };
+                if (!kParts) next_accumulator();
                 Fp8Stages st(p, tile.first_group(p, groups));
                 for (int i = 0, of_part = 0; ok && i < p.steps; ++i, st.advance()) {
-                    if (of_part == 0) {
-                        ok = mbar_wait_warp<!kShares>(d_empty + 8 * rd.idx, rd.phase ^ 1, abort_flag, p.status, 303);
-                        d = tmem + (uint32_t)(rd.idx * p.d_cols);
-                    }
+                    if (kParts && of_part == 0) next_accumulator();
                     if (ok && (st.c & 3) == 0) ok = mbar_wait_warp<!kShares>(sf_full + 8 * rs.idx, rs.phase, abort_flag, p.status, 304);
                     ok = ok && mbar_wait_warp<!kShares>(full + 8 * ru.idx, ru.phase, abort_flag, p.status, 305);
                     if (!ok) break;
                     tc_fence_after();
                     const int end = st.end();
-                    const bool last = i + 1 == p.steps || of_part + 1 == part_steps, group_ends = end == p.units || (end & 3) == 0;
+                    const bool last = i + 1 == p.steps || (kParts && of_part + 1 == p.part_steps), group_ends = end == p.units || (end & 3) == 0;
                     if (elect_one_sync()) {
                         const uint32_t sfa = tmem + kSfCol + (uint32_t)(rs.idx * kFp8SfCols), sfb = sfa + 8;
                         const uint64_t a = sw128 | (uint64_t)(((base + (uint32_t)(ru.idx * kFp8Deep) * a_bytes) & 0x3FFFFu) >> 4);
@@ -350,7 +351,7 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
 #pragma unroll
                                 for (int kk = 0; kk < 4; ++kk)
                                     tc_mma_fp8<CG>(d, a + u * (a_bytes >> 4) + kStepA * kk, b + u * (b_bytes >> 4) + kStepB * kk, id + u * ((1u << 29) | (1u << 4)), sfa, sfb,
-                                                   of_part == 0 && u == 0 && kk == 0 ? 0u : 1u);
+                                                   (kParts ? of_part : i) == 0 && u == 0 && kk == 0 ? 0u : 1u);
                         if (CG == 1) {
                             tc_commit(empty + 8 * ru.idx);
                             if (group_ends) tc_commit(sf_empty + 8 * rs.idx);
@@ -365,11 +366,12 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
                     ru.advance(S);
                     if (group_ends) rs.advance(2);
                     ++of_part;
-                    if (last) {
+                    if (kParts && last) {
                         rd.advance(2);
                         of_part = 0;
                     }
                 }
+                if (!kParts) rd.advance(2);
             }
         }
     };
@@ -756,15 +758,22 @@ __device__ __forceinline__ void fp8_gemm(const Fp8Params &p, const CUtensorMap &
                 const int f = thread >> (7 - p.fold_log), features = rows >> 1;
                 float *sums = reinterpret_cast<float *>(smem + (staging - base));
                 float v[kFp8SingleCols];
+                if constexpr (kParts) {
 #pragma unroll
-                for (int c = 0; c < kFp8SingleCols; ++c) v[c] = -0.0f;  // as below
-                if (!each_part([&](uint32_t d) {
-                        float w[kFp8SingleCols];
-                        tc_ld_x16(d + f * p.b_rows, w);
+                    for (int c = 0; c < kFp8SingleCols; ++c) v[c] = -0.0f;  // as below
+                    if (!each_part([&](uint32_t d) {
+                            float w[kFp8SingleCols];
+                            tc_ld_x16(d + f * p.b_rows, w);
 #pragma unroll
-                        for (int c = 0; c < kFp8SingleCols; ++c) v[c] += w[c];
-                    }))
-                    break;
+                            for (int c = 0; c < kFp8SingleCols; ++c) v[c] += w[c];
+                        }))
+                        break;
+                } else {
+                    if (!next_part()) break;
+                    tc_ld_x16(tmem_q + (uint32_t)(rd.idx * p.d_cols) + f * p.b_rows, v);
+                    drained();
+                    rd.advance(2);
+                }
                 if (!kGated && p.fold_log == 0) {
                     OT *to = o + row0 + thread;
                     if (thread < rows) {
@@ -1088,15 +1097,21 @@ static int launch_fp8_pairs(const Fp8Launch &a, cudaStream_t stream)
     }
 }
 
+template <int SLICES, typename OT>
+static int launch_fp8_singles(const Fp8Launch &a, cudaStream_t stream)
+{
+    const int ctas = a.pairs();
+    if (a.form == kFp8GatedProduct)
+        return a.l.resident ? launch_fp8<1, kFp8GatedProduct, true, SLICES, OT>(a.p, a.maps, ctas, a.l.smem, stream) : launch_fp8<1, kFp8GatedProduct, false, SLICES, OT>(a.p, a.maps, ctas, a.l.smem, stream);
+    constexpr int kSlices = sizeof(OT) == 4 ? SLICES : 0;
+    return a.l.resident ? launch_fp8<1, kFp8Product, true, kSlices, OT>(a.p, a.maps, ctas, a.l.smem, stream) : launch_fp8<1, kFp8Product, false, kSlices, OT>(a.p, a.maps, ctas, a.l.smem, stream);
+}
+
 template <typename OT>
 static int launch_fp8_as(const Fp8Launch &a, cudaStream_t stream)
 {
     const Fp8Plan &l = a.l;
-    const int ctas = a.pairs();
-    if (l.cg == 1) {
-        if (a.form == kFp8Product) return l.resident ? launch_fp8<1, kFp8Product, true, 0, OT>(a.p, a.maps, ctas, l.smem, stream) : launch_fp8<1, kFp8Product, false, 0, OT>(a.p, a.maps, ctas, l.smem, stream);
-        return l.resident ? launch_fp8<1, kFp8GatedProduct, true, 0, OT>(a.p, a.maps, ctas, l.smem, stream) : launch_fp8<1, kFp8GatedProduct, false, 0, OT>(a.p, a.maps, ctas, l.smem, stream);
-    }
+    if (l.cg == 1) return a.p.parts == 1 ? launch_fp8_singles<0, OT>(a, stream) : launch_fp8_singles<1, OT>(a, stream);
     if (a.p.parts == 1) return launch_fp8_pairs<0, OT>(a, stream);
     return l.tile_cols <= kFp8NarrowCols ? launch_fp8_pairs<kFp8NarrowSlices, OT>(a, stream) : launch_fp8_pairs<kFp8WideSlices, OT>(a, stream);
 }
