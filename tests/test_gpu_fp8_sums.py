@@ -6,6 +6,10 @@ themselves do at worst, so relative to the sum's size it is a part's - and of th
 any sign together are sqrt(P) 2^-24 of the sum's size.  What a part is off by is measured here with sums of one part, of the same kind of numbers."""
 
 import math
+import os
+import subprocess
+import sys
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -137,3 +141,33 @@ def test_a_gated_step_of_long_sums(n, f, k, kind):
     ref, sum_off = sums(b.T, fo.numbers(numpy64(x), "column"), b_off.T)
     check(dw, ref, rounded(ref, sum_off, dw.dtype))
     assert np.isfinite(ref).all()
+
+
+FIRST_CALL_CAPTURED = """
+import torch, tuna_b200 as t
+f, n, k = 512, 200, 8192
+x, dh = (torch.randn(n, c, device="cuda", dtype=torch.bfloat16) for c in (k, f))
+w = torch.randn(2 * f, k, device="cuda") * k ** -0.5
+h, z = (torch.empty(n, c, device="cuda", dtype=torch.bfloat16) for c in (f, 2 * f))
+o, dx, dw = (torch.empty(s, device="cuda") for s in ((n, 2 * f), (n, k), (2 * f, k)))
+def step():
+    q, s = t.fp8_quantize(w, "square")
+    t.fp8_gated(x, None, q, s, h, f, n, k, z=z)
+    t.fp8_matmul(x, None, q, s, o, 2 * f, n, k)
+    t.fp8_gated_backward(dh, z, x, None, q, s, dx, dw, f, n, k)
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    step()
+g.replay()
+torch.cuda.synchronize()
+first = [v.clone() for v in (h, z, o, dx, dw)]
+step()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) and a.isfinite().all() for a, b in zip(first, (h, z, o, dx, dw)))
+print("captured")
+"""
+
+
+def test_first_calls_of_long_sums_can_be_captured():
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL_CAPTURED], capture_output=True, text=True, timeout=300, cwd=Path(__file__).resolve().parents[1], env=dict(os.environ))
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr

@@ -32,7 +32,7 @@
 //
 // What bounds it (graph replay, weights of 0.4 GB in turn; 6.55 TB/s is the measured copy rate, 3.39 PFLOP/s twice the measured bf16 burst, 2.79 twice the sustained rate):
 //   weights' bytes    57344x8192 at 1 token 74 us = 6.3 TB/s, 28672x4096 21.5 = 5.5 (17.9 of bytes and what is left of a launch's chain of 4 us)
-//   a launch's chain  4096x4096 at 1 token 6.5 us: end of the kernel before, the tokens' copy and scales, the last stages, epilogue
+//   a launch's chain  4096x4096 at 1 token 6.1 us: end of the kernel before, the tokens' copy and scales, the last stages, epilogue
 //   steps in a row    4096x14336 at 43 tokens 22 us: 16 tiles on 74 pairs, each 112 units of 0.17 us one after another
 //   tensor pipe       28672x4096 at 2048 tokens 175 us = 2.75 PFLOP/s (gated 170 to 185), active for 77 to 80 % of the time, at the power cap; dx of the same the same
 //   stores            dw of the same, 235 MB of results in bf16, 205 us without them and 235 with them
